@@ -179,6 +179,153 @@ int yk_decode_nms_static(const YkLevel* levels, int nlevels, int batch, int nc, 
                          float iou, int max_out, float* outdets, int* outidx, int* outcnt,
                          int* rawcnt, yk_stream_t st);
 
+// ---------------------------------------------------------------------------------------
+// Text decoder (no counterpart in the reference): the operators of one step of a decoder that
+// answers about a frame or its detections, over ragged batches of requests.  Lengths, tables
+// and slots are device arrays, nothing is read back and nothing is allocated, so a whole step
+// is one CUDA graph.  8-bit values are e4m3 codes (1 sign, 4 exponent, 3 fraction bits, largest
+// 448, no infinity); a value is code * scale.  A refused call (YK_EINVAL, YK_EUNSUP) launches
+// nothing and says why in yk_last_cuda_error().
+#define YK_F16 0
+#define YK_BF16 1
+#define YK_E4M3 2
+
+// Key/value cache in 8 bits: a pool of blocks of `tokens` tokens, one scale for each (block,
+// head).  Channel d of token t of head h in block b is code b*block_stride + (h*tokens + t)*dim
+// + d of k and v, its scale entry b*scale_stride + h of kscale and vscale.  Slot s of the pool
+// is token s % tokens of block s / tokens.
+typedef struct {
+  void* k;                 // e4m3 codes, 16-byte aligned
+  void* v;
+  float* kscale;           // positive
+  float* vscale;
+  long long block_stride;  // codes from block to block, >= heads*tokens*dim, multiple of 16
+  long long scale_stride;  // scales from block to block, >= heads
+  int blocks;              // blocks of the pool (blocks * tokens < 2^31)
+  int heads;               // key/value heads
+  int tokens;              // tokens of a block: 16, 32, 64 or 128
+  int dim;                 // channels of a head: 64, 128 or 256
+} YkKvCache;
+
+// Block tables and slots of a step from the requests' lengths.  Request r holds past[r] tokens
+// in the blocks table[r][0 .. ceil(past/tokens)) and adds fresh[r].  In request order, each
+// takes the blocks it needs more from free_blocks (from entry *free_head on, when given) and
+// appends them to its table row.  Row n of the step is token past + j of its request r, with
+// n = cu[r] + j: pos[n] is that position and slots[n] its place in the pool.
+// A request is refused, and takes no block, when the free blocks that earlier requests left do
+// not suffice (one that needs none still goes on), when its tokens pass max_blocks blocks, when
+// its rows pass `rows`, or when a length is negative (a negative fresh counts as no rows).  Its
+// kv_lens stays past and its rows' slots are -1; so are the slots of rows past the last
+// request's (their pos too), and of tokens whose table entry lies outside the pool.
+typedef struct {
+  const int* past;         // [requests]
+  const int* fresh;        // [requests]
+  const int* free_blocks;  // [free_count] block ids
+  int* free_head;          // NULL (0), or in/out: the first free entry; moved past those taken
+  int* table;              // in/out [requests][table_stride]; only the new entries are written
+  int* kv_lens;            // out [requests]: past + fresh, or past if refused; may be `past`
+  int* cu;                 // out [requests + 1]: rows before each request (at most `rows`)
+  int* slots;              // out [rows]
+  int* pos;                // out [rows], or NULL
+  int* counts;             // out [4]: blocks taken, rows placed, requests refused, rows; or NULL
+  long long table_stride;  // >= max_blocks
+  int requests;            // 1 .. 16384
+  int rows;                // rows of slots and pos
+  int free_count;
+  int blocks;              // blocks of the pool
+  int max_blocks;          // table entries of a request
+  int tokens;              // tokens of a block: 16, 32, 64 or 128
+} YkKvPlan;
+int yk_kv_plan(const YkKvPlan* p, yk_stream_t st);
+
+// New keys and values, one row a token: head h of row n at n*k_row + h*k_head.
+typedef struct {
+  const void* k;           // fp16 or bf16, 16-byte aligned
+  const void* v;
+  const int* slots;        // [rows]; a row whose slot lies outside the pool is left out
+  long long k_row, v_row, k_head, v_head;   // elements, multiples of 8
+  int rows;
+  int dtype;               // YK_F16 or YK_BF16
+} YkKvRows;
+// Quantises rows into the cache.  The rows of one block are consecutive and ascend (as
+// yk_kv_plan's slots do); tokens before them in the block are kept, tokens after them are not
+// used.  Each (block, head) gets the smallest power-of-two scale that holds its finite new
+// values (at least 2^-126), or keeps its scale where that is larger and the block has earlier
+// tokens; those are rounded to the new scale where it grew.  Infinite values become +-448, NaN
+// stays NaN.
+int yk_kv_append(const YkKvCache* c, const YkKvRows* x, yk_stream_t st);
+
+// Attention of a step's rows over the cache: rows cu[r] .. cu[r+1]-1 are request r's last
+// tokens, query head h reads key/value head h / (heads / c->heads).  causal: row i of a request
+// of q rows sees keys j <= kv_lens[r] - q + i, with a window w > 0 only j > kv_lens[r] - q + i
+// - w; else every key.  A row that sees no key gives zeros (lse -inf); keys in blocks outside
+// the pool are not seen.  What the cache holds past kv_lens is never used.
+typedef struct {
+  const void* q;           // head h of row n at n*q_row + h*dim; fp16 or bf16, 16-byte aligned
+  void* out;               // likewise, with out_row
+  float* lse;              // [rows][heads]: log of the sum of the weights, or NULL
+  const int* cu;           // [requests + 1]
+  const int* kv_lens;      // [requests]
+  const int* table;        // [requests][table_stride] block ids
+  void* ws;                // yk_attn_kv8_workspace_bytes, 16-byte aligned, zeroed before its first
+  size_t ws_bytes;         // use (each call leaves it so); calls that overlap need one each
+  long long q_row, out_row;   // elements, multiples of 8
+  long long table_stride;
+  int max_blocks;          // table entries of a request
+  int requests;            // 1 .. 16384
+  int rows;
+  int heads;               // query heads, a multiple of c->heads
+  int dtype;               // YK_F16 or YK_BF16 (q and out)
+  int causal;
+  int window;              // 0: none
+  float scale;             // of the products; 0: 1 / sqrt(dim)
+} YkAttnKv8;
+size_t yk_attn_kv8_workspace_bytes(int requests, int rows, int heads, int kv_heads, int dim);
+int yk_attn_kv8(const YkKvCache* c, const YkAttnKv8* a, yk_stream_t st);
+
+// h = x + add, y = h / sqrt(mean(h^2) + eps) * weight over each row, in 32 bits; sum = h and
+// out = y rounded to dtype, codes = y / scale rounded to e4m3 with one scale for each `group`
+// columns: the largest finite |y| / 448 (at least 2^-126).  sum may be x or add itself.
+typedef struct {
+  const void* x;
+  const void* add;         // or NULL
+  void* sum;               // or NULL
+  const void* weight;      // [cols]
+  void* out;               // or NULL
+  void* codes;             // e4m3, or NULL
+  float* scales;           // [rows][scales_row], with codes
+  long long x_row, add_row, sum_row, out_row, codes_row, scales_row;   // elements
+  int rows, cols;          // cols up to 32768
+  int group;               // columns of a scale, at least 16 (the last group may be shorter); 0: the
+                           // whole row
+  int dtype;               // YK_F16 or YK_BF16: x, add, sum, weight, out
+  float eps;
+} YkRmsNorm8;
+int yk_rmsnorm8(const YkRmsNorm8* p, yk_stream_t st);
+
+// y[m][j] = sum_k x[m][k] * (q[j][k] - zero) * scale + bias[j] for up to 64 rows: 4-bit weights
+// q (0..15), byte i of a row holds column 2i in its low and 2i+1 in its high half; scale and zero
+// for each `group` columns.  x is fp16 / bf16, or e4m3 codes with a scale for each xgroup columns
+// (yk_rmsnorm8's output).  32-bit sums, one rounding to dtype.
+typedef struct {
+  const void* x;
+  const float* xscale;     // e4m3: [rows][xscale_row]
+  const void* w;           // [n][w_row bytes], 16-byte aligned
+  const void* wscale;      // [n][group_row] of dtype
+  const void* wzero;       // [n][group_row] bytes 0..15, or NULL (8)
+  const float* bias;       // [n] or NULL
+  void* y;                 // [rows][y_row]
+  long long x_row, xscale_row, w_row, group_row, y_row;   // elements; w_row: bytes, multiple of 16
+  int rows;                // 1 .. 64
+  int n;                   // outputs
+  int k;                   // columns, a multiple of group
+  int group;               // 32, 64 or 128
+  int xgroup;              // e4m3: a multiple of group, or 0: one scale a row
+  int xtype;               // dtype, or YK_E4M3
+  int dtype;               // YK_F16 or YK_BF16: wscale, y (and x)
+} YkGemv4;
+int yk_gemv4(const YkGemv4* p, yk_stream_t st);
+
 // Device error word (bounded-wait timeouts) of the current device; cleared by the call.
 int yk_fetch_device_error(void);
 // Test hook for the bounded-wait failure path (no counterpart in the reference, which has no

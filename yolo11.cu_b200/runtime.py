@@ -50,6 +50,58 @@ class YoloOptions(C.Structure):
                 ("max_det", C.c_int), ("autotune", C.c_int), ("fuse", C.c_int)]
 
 
+YK_F16, YK_BF16, YK_E4M3 = 0, 1, 2
+
+
+class YkKvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("kscale", C.c_void_p),
+                ("vscale", C.c_void_p), ("block_stride", C.c_longlong),
+                ("scale_stride", C.c_longlong), ("blocks", C.c_int), ("heads", C.c_int),
+                ("tokens", C.c_int), ("dim", C.c_int)]
+
+
+class YkKvPlan(C.Structure):
+    _fields_ = [("past", C.c_void_p), ("fresh", C.c_void_p), ("free_blocks", C.c_void_p),
+                ("free_head", C.c_void_p), ("table", C.c_void_p), ("kv_lens", C.c_void_p),
+                ("cu", C.c_void_p), ("slots", C.c_void_p), ("pos", C.c_void_p),
+                ("counts", C.c_void_p), ("table_stride", C.c_longlong), ("requests", C.c_int),
+                ("rows", C.c_int), ("free_count", C.c_int), ("blocks", C.c_int),
+                ("max_blocks", C.c_int), ("tokens", C.c_int)]
+
+
+class YkKvRows(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("slots", C.c_void_p),
+                ("k_row", C.c_longlong), ("v_row", C.c_longlong), ("k_head", C.c_longlong),
+                ("v_head", C.c_longlong), ("rows", C.c_int), ("dtype", C.c_int)]
+
+
+class YkAttnKv8(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("cu", C.c_void_p),
+                ("kv_lens", C.c_void_p), ("table", C.c_void_p), ("ws", C.c_void_p),
+                ("ws_bytes", C.c_size_t), ("q_row", C.c_longlong), ("out_row", C.c_longlong),
+                ("table_stride", C.c_longlong), ("max_blocks", C.c_int), ("requests", C.c_int),
+                ("rows", C.c_int), ("heads", C.c_int), ("dtype", C.c_int), ("causal", C.c_int),
+                ("window", C.c_int), ("scale", C.c_float)]
+
+
+class YkRmsNorm8(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("add", C.c_void_p), ("sum", C.c_void_p),
+                ("weight", C.c_void_p), ("out", C.c_void_p), ("codes", C.c_void_p),
+                ("scales", C.c_void_p), ("x_row", C.c_longlong), ("add_row", C.c_longlong),
+                ("sum_row", C.c_longlong), ("out_row", C.c_longlong), ("codes_row", C.c_longlong),
+                ("scales_row", C.c_longlong), ("rows", C.c_int), ("cols", C.c_int),
+                ("group", C.c_int), ("dtype", C.c_int), ("eps", C.c_float)]
+
+
+class YkGemv4(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("xscale", C.c_void_p), ("w", C.c_void_p),
+                ("wscale", C.c_void_p), ("wzero", C.c_void_p), ("bias", C.c_void_p),
+                ("y", C.c_void_p), ("x_row", C.c_longlong), ("xscale_row", C.c_longlong),
+                ("w_row", C.c_longlong), ("group_row", C.c_longlong), ("y_row", C.c_longlong),
+                ("rows", C.c_int), ("n", C.c_int), ("k", C.c_int), ("group", C.c_int),
+                ("xgroup", C.c_int), ("xtype", C.c_int), ("dtype", C.c_int)]
+
+
 _P = C.POINTER
 _SIGS = {
     # kernel ABI (include/yk.h)
@@ -85,6 +137,12 @@ _SIGS = {
     "yk_decode_nms_static": (C.c_int, [_P(YkLevel), C.c_int, C.c_int, C.c_int, C.c_float,
                                        C.c_float, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
                                        C.c_void_p, C.c_void_p]),
+    "yk_kv_plan": (C.c_int, [_P(YkKvPlan), C.c_void_p]),
+    "yk_kv_append": (C.c_int, [_P(YkKvCache), _P(YkKvRows), C.c_void_p]),
+    "yk_attn_kv8_workspace_bytes": (C.c_size_t, [C.c_int] * 5),
+    "yk_attn_kv8": (C.c_int, [_P(YkKvCache), _P(YkAttnKv8), C.c_void_p]),
+    "yk_rmsnorm8": (C.c_int, [_P(YkRmsNorm8), C.c_void_p]),
+    "yk_gemv4": (C.c_int, [_P(YkGemv4), C.c_void_p]),
     "yk_fetch_device_error": (C.c_int, []),
     "yk_test_inject": (C.c_int, [C.c_int, C.c_ulonglong]),
     "yk_test_nms_cluster": (C.c_int, [C.c_int]),
