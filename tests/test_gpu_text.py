@@ -26,7 +26,8 @@ def within(got, want, bound, dt):
         fine = np.abs(got - want) <= bound
     inf = got == np.copysign(np.inf, want)
     over, under = np.abs(want) - bound >= top, np.abs(want) + bound < top
-    return np.where(over, inf, np.where(under, fine, fine | inf))
+    good = np.where(over, inf, np.where(under, fine, fine | inf))
+    return np.where(np.isnan(want), np.isnan(got), good)
 
 
 def i32(v):
@@ -271,7 +272,7 @@ def test_append_special_values(lib, cuda):
 
 def run_attention(lib, rt, kind, heads, kv_heads, D, T, lens, causal=1, window=0, scale=0.0,
                   qscale=1.0, pad=0, joint=False, lse=True, spoil=True, vspread=0.5, bad_block=None,
-                  repeat=2, seed=0):
+                  repeat=2, seed=0, nan=()):
     """lens: (kv, q) of each request; pad: rows of no request at the end."""
     dt, code, u = TYPES[kind]
     rng = random.Random(seed)
@@ -291,6 +292,8 @@ def run_attention(lib, rt, kind, heads, kv_heads, D, T, lens, causal=1, window=0
         for (kv, _), row in zip(lens, table):
             if kv % T and 0 <= row[kv // T] < blocks:
                 view[row[kv // T], :, :, kv % T:] = 127
+    for r, j, part, ch in nan:     # NaN in the middle: seen by the rows from token j on
+        view[table[r][j // T], part, :, j % T, ch] = 255
     cu = np.cumsum([0] + [q for _, q in lens]).tolist()
     n = cu[-1] + pad
     g = torch.Generator(device="cuda").manual_seed(seed + 1)
@@ -326,8 +329,9 @@ def run_attention(lib, rt, kind, heads, kv_heads, D, T, lens, causal=1, window=0
     assert (f64(out[cu[-1]:]) == 9).all() and (f64(out[:, heads]) == 9).all()
     if lse:
         gl, l = f64(ls)[:cu[-1]], l[:cu[-1]]
-        empty = np.isinf(l)
-        assert (gl[empty] == -np.inf).all()
+        assert np.array_equal(np.isnan(gl), np.isnan(l))
+        empty = np.isinf(l) | np.isnan(l)
+        assert (gl[np.isinf(l)] == -np.inf).all()
         lb = ds[:cu[-1], :, 0] + 2.0 ** -20 * (1 + np.abs(np.where(empty, 0, l)))
         assert (np.abs(gl[~empty] - l[~empty]) <= lb[~empty]).all()
     return got
@@ -386,6 +390,19 @@ def test_attention_block_outside_pool(lib, cuda, bad, q):
     """Keys of a block id outside the pool are not seen; nothing is read for them."""
     from yolo11_cu_b200 import runtime as rt
     run_attention(lib, rt, "f16", 4, 2, 64, 32, [(100, q), (129, q)], bad_block=bad)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 9])
+@pytest.mark.parametrize("lens", [[(40, 20), (90, 6)], [(300, 150), (31, 1)]])
+def test_attention_nan_is_seen_only_where_visible(lib, cuda, D, window, lens):
+    """A NaN value reaches its channel in the rows that see its token, a NaN key those rows whole;
+    rows that do not see the token are as without it."""
+    from yolo11_cu_b200 import runtime as rt
+    run_attention(lib, rt, "f16", 4, 2, D, 32, lens, window=window,
+                  nan=[(0, 35, 1, 3), (0, 33, 1, D - 1), (1, 20, 1, 7)])
+    run_attention(lib, rt, "bf16", 3, 1, D, 32, lens, window=window,
+                  nan=[(0, 37, 0, 3), (0, 26, 1, 9), (1, 30, 1, 0)])
 
 
 def test_attention_offsets_past_32_bits(lib, cuda):
