@@ -7,7 +7,8 @@ struct Attn8Args {
   YkKvCache c;
   YkAttnKv8 a;
   float scale_log2;   // a.scale * log2(e): weights are powers of two
-  int min_part;       // granules a CTA takes at least
+  int lead;           // cost of starting an item, in granules
+  int min_part;       // cost that a CTA takes on at least
 };
 
 // ---------------- few rows: split along the keys ----------------
@@ -33,19 +34,28 @@ struct Attn8Args {
 //    the weights, whose 16-bit form is taken relative to the largest weight * scale so far (M
 //    below, kept beside the softmax's m), so blocks of very different loudness keep their bits.
 constexpr int kDecWarps = 4;
-constexpr int kDecGran = 16 * kDecWarps;   // tokens of a granule
+constexpr int kDecSub = 2 * kDecWarps;     // 16-token subtiles of a granule: two for each warp
+constexpr int kDecGran = 16 * kDecSub;     // tokens of a granule
+// Cost of starting an item and the least share of a CTA, in granules (measured, 64 requests of 64
+// to 8192 keys, 32 / 8 heads of 128: lead 0, 1, 2, 3, 4 give 93, 75, 64, 65, 68 us; one request of
+// 431 keys: least share 3, 6 give 10.0, 8.5 us).
+constexpr int kDecLead = 2, kDecMin = 6;
 constexpr int kDecCtas = 148 * 2;
+constexpr int kAtOnce = 8;                 // parts that a join reads at a time
 
 template <int D>
 struct Dec {
   static constexpr int kStage = 32 * D;                      // bytes of a warp's stage (K and V)
-  static constexpr int kStages = D == 64 ? 8 : D == 128 ? 5 : 3;
+  static constexpr int kStages = D == 64 ? 8 : 4;
+  static constexpr int kPairs = kStages / 2;                 // a warp's iteration takes two stages
   static constexpr int kWarpBytes = kStages * kStage;
-  static constexpr int kSmem = kDecWarps * kWarpBytes;
   static constexpr int kKC = D / 64;                         // 16-byte key chunks a lane and token
   static constexpr int kVC = D == 256 ? 2 : 1;               // value chunks a lane and token
   static constexpr int kVB = D == 64 ? 8 : 16;               // bytes of a value chunk
-  static constexpr int kRow = D + 8;                         // floats of a row when states meet
+  static constexpr int kCol = D / 8 + 1, kRow = 8 * kCol;    // floats of an MMA column, of a row, when states meet
+  static constexpr int kMeet = D == 256 ? 1 : 2;
+  static constexpr int kQRow = 2 * D + 16, kQBytes = 16 * kQRow;
+  static constexpr int kSmem = kDecWarps * kWarpBytes + 2 * kQBytes + kMeet * 16 * kRow * (int)sizeof(float);
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -53,6 +63,7 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// B bytes into shared memory; without `ok`, zeros and no read.
 template <int B>
 __device__ __forceinline__ void cp_async_lane(uint32_t dst, const void* src, bool ok) {
   if (B == 16) {
@@ -60,6 +71,11 @@ __device__ __forceinline__ void cp_async_lane(uint32_t dst, const void* src, boo
   } else {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
   }
+}
+template <int B>
+__device__ __forceinline__ void cp_async_lane(uint32_t dst, const void* src) {
+  if (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
@@ -72,19 +88,23 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   return v;
 }
 
-// o += p (16 rows x 16 tokens) * v: words v[j] hold 4 channels a word of the lane's token j (of
-// 2t, 2t + 1, 2t + 8, 2t + 9); bytes of a token pair interleave into the B operand.
+// o += p (16 rows x 16 tokens) * v for two subtiles: words v[u][j] hold 4 channels a word of the
+// lane's token j (of 2t, 2t + 1, 2t + 8, 2t + 9); bytes of a token pair interleave into the B operand.
 template <int W>
-__device__ __forceinline__ void pv_mma(float (*o)[4], const uint32_t (&pa)[4], const uint32_t (&v)[4][W]) {
+__device__ __forceinline__ void pv_mma(float (*o)[4], const uint32_t (&pa)[2][4], const uint32_t (&v)[2][4][W]) {
 #pragma unroll
-  for (int w = 0; w < W; w++) {
-    const uint32_t lo01 = __byte_perm(v[0][w], v[1][w], 0x5140), lo23 = __byte_perm(v[0][w], v[1][w], 0x7362);
-    const uint32_t hi01 = __byte_perm(v[2][w], v[3][w], 0x5140), hi23 = __byte_perm(v[2][w], v[3][w], 0x7362);
-    mma16816(o[4 * w], pa, e4m3x2_to_half2(lo01), e4m3x2_to_half2(hi01));
-    mma16816(o[4 * w + 1], pa, e4m3x2_to_half2(lo01 >> 16), e4m3x2_to_half2(hi01 >> 16));
-    mma16816(o[4 * w + 2], pa, e4m3x2_to_half2(lo23), e4m3x2_to_half2(hi23));
-    mma16816(o[4 * w + 3], pa, e4m3x2_to_half2(lo23 >> 16), e4m3x2_to_half2(hi23 >> 16));
-  }
+  for (int w = 0; w < W; w++)
+#pragma unroll
+    for (int half = 0; half < 2; half++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const uint32_t sel = half ? 0x7362 : 0x5140;
+        uint32_t a0, a1, b0, b1;
+        e4m3x4_to_half2x2(__byte_perm(v[u][0][w], v[u][1][w], sel), a0, a1);
+        e4m3x4_to_half2x2(__byte_perm(v[u][2][w], v[u][3][w], sel), b0, b1);
+        mma16816(o[4 * w + 2 * half], pa[u], a0, b0);
+        mma16816(o[4 * w + 2 * half + 1], pa[u], a1, b1);
+      }
 }
 
 // The first key that a row at position `pos` sees.
@@ -105,134 +125,199 @@ __device__ __forceinline__ Req attn_req(const YkKvCache& c, const YkAttnKv8& a, 
   return o;
 }
 
+// What a CTA does next: granules g0 .. g1 of the n of item (key head kh, row tile) of request r.
+struct Seg {
+  int r, kh, tile, row_n;        // row_n: rows of the tile
+  int q0, q, kv;                 // the request's first row, rows, keys
+  int g0, g1, n, cost;           // none (g0 == g1) where the CTA's share ends in the item's lead
+  int s_lo, s_hi;                // 16-token subtiles [s_lo, s_hi) that the tile needs of them
+  int tile_hi;                   // keys that any of its rows sees end here
+};
+
 template <bool BF16, int D>
-__global__ void __launch_bounds__(32 * kDecWarps, 2) attn8_split_kernel(const __grid_constant__ Attn8Args p) {
-  pdl_wait();
-  pdl_trigger();
+__global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_kernel(const __grid_constant__ Attn8Args p) {
   using L = Dec<D>;
-  extern __shared__ __align__(128) uint8_t dec_sm[];
+  extern __shared__ __align__(128) uint8_t dec_sm[];    // rings, then q rows (two), then meeting rows
   __shared__ long long part[32], pre[32 * kDecWarps];
-  __shared__ float wm[kDecWarps][16], wl[kDecWarps][16];
+  __shared__ float wm[kDecWarps][16], wl[kDecWarps][16], row_m[16], row_l[16];
   __shared__ uint4 qsm[D == 256 ? D / 16 : 1][32];   // q fragments (registers below 256 channels)
   __shared__ int arrived;
   const YkAttnKv8& a = p.a;
   const YkKvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int G = a.heads / c.heads, T = c.tokens;
+  const int G = a.heads / c.heads, T = c.tokens, lead = p.lead;
+  pdl_wait();
+  pdl_trigger();
 
   // granules of a request: (items) x (granules of an item, at least one: empty rows are written)
   const auto item_gran = [&](const Req& q) { return max(1, (q.kv - (q.lo & ~15) + kDecGran - 1) / kDecGran); };
   const auto row_tiles = [&](const Req& q) { return (int)(((long long)q.q * G + 15) / 16); };
-  const auto req_gran = [&](const Req& q) { return q.q ? (long long)item_gran(q) * row_tiles(q) * c.heads : 0ll; };
+  const auto req_cost = [&](const Req& q) { return q.q ? (long long)(item_gran(q) + lead) * row_tiles(q) * c.heads : 0ll; };
   const int per_thread = (a.requests + 32 * kDecWarps - 1) / (32 * kDecWarps);
   long long sum = 0, total;
-  for (int r = tid * per_thread; r < min(a.requests, (tid + 1) * per_thread); r++) sum += req_gran(attn_req(c, a, r));
+  for (int r = tid * per_thread; r < min(a.requests, (tid + 1) * per_thread); r++) sum += req_cost(attn_req(c, a, r));
   pre[tid] = block_exclusive(sum, part, &total);
   __syncthreads();
   const long long per = max((total + gridDim.x - 1) / gridDim.x, (long long)p.min_part);
   long long f = blockIdx.x * per;
   const long long f_end = min(total, f + per);
   if (f >= f_end) return;
-  int lo = 0, hi = 32 * kDecWarps;
-  while (hi - lo > 1) {
-    const int m = (lo + hi) >> 1;
-    if (pre[m] <= f) lo = m; else hi = m;
+  int at_r;
+  long long base;                  // granules before request at_r
+  {
+    int lo = 0, hi = 32 * kDecWarps;
+    while (hi - lo > 1) {
+      const int m = (lo + hi) >> 1;
+      if (pre[m] <= f) lo = m; else hi = m;
+    }
+    at_r = lo * per_thread;
+    base = pre[lo];
   }
-  int r = lo * per_thread;
-  long long base = pre[lo];        // granules before request r
-  Req q = attn_req(c, a, r);
-  long long rg = req_gran(q);
+  Req rq = attn_req(c, a, at_r);
+  long long rg = req_cost(rq);
+  // the segment at f, of which there is one; moves the cursor (at_r, base, rq, rg) to its request
+  const auto segment_at = [&](long long f) -> Seg {
+    while (f >= base + rg) {
+      base += rg;
+      rq = attn_req(c, a, ++at_r);
+      rg = req_cost(rq);
+    }
+    Seg s;
+    s.r = at_r; s.q0 = rq.q0; s.q = rq.q; s.kv = rq.kv;
+    s.n = item_gran(rq);
+    const long long item = (f - base) / (s.n + lead);
+    const int at = (int)(f - base - item * (s.n + lead));
+    s.cost = (int)min((long long)(s.n + lead - at), f_end - f);
+    s.g0 = max(0, at - lead);
+    s.g1 = max(0, at + s.cost - lead);
+    const int tiles = row_tiles(rq);
+    s.kh = (int)(item / tiles);
+    s.tile = (int)(item - (long long)s.kh * tiles);
+    s.row_n = min(16, rq.q * G - s.tile * 16);
+    const int t0 = s.tile * 16 / G, t1 = (s.tile * 16 + s.row_n - 1) / G;   // the tile's tokens
+    s.tile_hi = a.causal ? max(0, rq.kv - rq.q + t1 + 1) : rq.kv;
+    const int tile_lo = a.causal ? first_key(rq.kv - rq.q + t0, a.window) : 0;
+    s.s_lo = max((rq.lo >> 4) + s.g0 * kDecSub, tile_lo >> 4);
+    s.s_hi = min((rq.lo >> 4) + s.g1 * kDecSub, (s.tile_hi + 15) >> 4);
+    return s;
+  };
 
   const uint32_t ring = smem_u32(dec_sm) + warp * L::kWarpBytes;
-  while (f < f_end) {
-    while (f >= base + rg) {       // f < total: some later request holds it
-      base += rg;
-      q = attn_req(c, a, ++r);
-      rg = req_gran(q);
+  uint8_t* const q_sm = dec_sm + kDecWarps * L::kWarpBytes;
+  float* const meet = (float*)(q_sm + 2 * L::kQBytes);
+  // rows of a segment's q into buffer b (each thread its own 16-byte chunks)
+  const auto load_q = [&](const Seg& s, int b) {
+    for (int i = tid; i < 16 * D / 8; i += 32 * kDecWarps) {
+      const int rr = s.tile * 16 + min(i / (D / 8), s.row_n - 1), tok = rr / G;
+      cp_async_lane<16>(smem_u32(q_sm) + b * L::kQBytes + i / (D / 8) * L::kQRow + i % (D / 8) * 16,
+                        (const uint16_t*)a.q + (long long)(s.q0 + tok) * a.q_row + (long long)(s.kh * G + rr - tok * G) * D + i % (D / 8) * 8);
     }
-    const int n = item_gran(q);
-    const long long item = (f - base) / n;
-    const int g0 = (int)(f - base - item * n);
-    const int g1 = (int)min((long long)n, g0 + (f_end - f));
-    const int tiles = row_tiles(q), kh = (int)(item / tiles), tile = (int)(item - (long long)kh * tiles);
+  };
 
-    // rows g and g + 8 of this lane: row in a.q, head, and the keys it sees [first, last]
-    int row_tok[2], row_head[2], first[2], last[2];
-    const int row_n = min(16, q.q * G - tile * 16);
-    int tile_lo = q.kv, tile_hi = 0;      // keys that any row of the tile sees
+  // ---- the ring: block ids and scales of 32 subtiles at a time, one a lane ----
+  int count;                               // subtiles of this warp
+  const int* table;
+  const uint8_t *kcodes, *vcodes;
+  int s_first, tile_hi;
+  const auto sub_at = [&](int i) { return s_first + (i >> 1) * kDecSub + (i & 1); };   // this warp's i-th subtile
+  const auto block_at = [&](int i) -> int {   // of this warp's i-th subtile; -1: none
+    if (i >= count) return -1;
+    const int b = table[sub_at(i) * 16 / T];
+    return (unsigned)b < (unsigned)c.blocks ? b : -1;
+  };
+  int id_i = -1, id_n = -1, kh_i = 0;
+  float ks_i = 0.f, vs_i = 0.f;
+  uint32_t fill = ring;                       // the stage that the next copy fills
+  const auto open = [&](const Seg& s) {       // from here on issue() copies segment s
+    s_first = s.s_lo + 2 * warp;
+    const int left = max(0, s.s_hi - s_first);
+    count = left / kDecSub * 2 + min(2, left % kDecSub);
+    table = a.table + s.r * a.table_stride;
+    kh_i = s.kh;
+    tile_hi = s.tile_hi;
+    kcodes = (const uint8_t*)c.k + (long long)kh_i * T * D + g * D + t * 16;
+    vcodes = (const uint8_t*)c.v + (long long)kh_i * T * D + 2 * t * D + g * L::kVB;
+    id_n = block_at(lane);
+  };
+  const auto issue = [&](int i) {
+    if ((i & 31) == 0) {
+      id_i = id_n;
+      ks_i = id_i < 0 ? 0.f : c.kscale[id_i * c.scale_stride + kh_i];
+      vs_i = id_i < 0 ? 0.f : c.vscale[id_i * c.scale_stride + kh_i];
+      id_n = block_at(i + 32 + lane);
+    }
+    const int id = __shfl_sync(~0u, id_i, i & 31);
+    const int tok0 = sub_at(i) * 16;
+    const long long at = max(id, 0) * c.block_stride + (tok0 & (T - 1)) * D;
+    const uint8_t *kp = kcodes + at, *vp = vcodes + at;
+    const uint32_t kd = fill + lane * 16, vd = fill + 2 * L::kKC * 512 + lane * L::kVB;
+    const int left = id < 0 ? 0 : tile_hi - tok0;   // tokens past what the tile sees read as zero
+    if (left >= 16) {
+#pragma unroll
+      for (int j = 0; j < 2 * L::kKC; j++)
+        cp_async_lane<16>(kd + j * 512, kp + 8 * (j / L::kKC) * D + (j % L::kKC) * 64);
+#pragma unroll
+      for (int j = 0; j < 4 * L::kVC; j++)
+        cp_async_lane<L::kVB>(vd + j * 32 * L::kVB, vp + ((j / L::kVC & 1) + 8 * (j / L::kVC >> 1)) * D + (j % L::kVC) * 128);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2 * L::kKC; j++)
+        cp_async_lane<16>(kd + j * 512, kp + 8 * (j / L::kKC) * D + (j % L::kKC) * 64, 8 * (j / L::kKC) + g < left);
+#pragma unroll
+      for (int j = 0; j < 4 * L::kVC; j++) {
+        const int tok = (j / L::kVC & 1) + 8 * (j / L::kVC >> 1);
+        cp_async_lane<L::kVB>(vd + j * 32 * L::kVB, vp + tok * D + (j % L::kVC) * 128, 2 * t + tok < left);
+      }
+    }
+    fill += L::kStage;
+    if (fill == ring + L::kWarpBytes) fill = ring;
+  };
+  // Subtiles go in pairs (a warp's iteration), each pair a group of its own; one past the end
+  // reads as zero.
+  const auto issue_pair = [&](int i) {
+    if (i < count) {
+      issue(i);
+      issue(i + 1);
+    }
+    cp_async_commit();
+  };
+  const auto prologue = [&] {
+#pragma unroll
+    for (int i = 0; i < L::kPairs - 1; i++) issue_pair(2 * i);
+  };
+
+  // The next segment's q rows are copied, and its first block ids read, while this one runs; its
+  // first stages are under way while the warps' states of this one meet.
+  Seg cur = segment_at(f);
+  if (cur.g0 == cur.g1) return;
+  load_q(cur, 0);
+  cp_async_commit();
+  open(cur);
+  prologue();
+  uint32_t src = ring;
+  cp_async_wait<L::kPairs - 1>();
+  __syncthreads();                 // q is there
+  for (int turn = 0;; turn ^= 1) {
+    const long long f_next = f + cur.cost;
+
+    // rows g and g + 8 of this lane: the keys they see, [first, last]
+    int first[2], last[2], all_lo = 0, all_hi = cur.kv;    // [all_lo, all_hi): keys that every row sees
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const int rr = tile * 16 + min(g + 8 * i, row_n - 1);
-      row_tok[i] = rr / G;
-      row_head[i] = kh * G + rr - row_tok[i] * G;
-      last[i] = a.causal ? min(q.kv - 1, q.kv - q.q + row_tok[i]) : q.kv - 1;
-      first[i] = a.causal ? first_key(q.kv - q.q + row_tok[i], a.window) : 0;
+      const int pos = cur.kv - cur.q + (cur.tile * 16 + min(g + 8 * i, cur.row_n - 1)) / G;
+      last[i] = a.causal ? min(cur.kv - 1, pos) : cur.kv - 1;
+      first[i] = a.causal ? first_key(pos, a.window) : 0;
     }
-    {
-      const int t0 = tile * 16 / G, t1 = (tile * 16 + row_n - 1) / G;   // the tile's tokens
-      tile_hi = a.causal ? max(0, q.kv - q.q + t1 + 1) : q.kv;
-      tile_lo = a.causal ? first_key(q.kv - q.q + t0, a.window) : 0;
-    }
-    // 16-token subtiles of the segment that the tile needs
-    const int s_base = (q.lo >> 4);
-    const int s_lo = max(s_base + g0 * kDecWarps, tile_lo >> 4);
-    const int s_hi = min(s_base + g1 * kDecWarps, (tile_hi + 15) >> 4);
-    const int count = s_hi > s_lo + warp ? (s_hi - s_lo - warp + kDecWarps - 1) / kDecWarps : 0;
-
-    // ---- the ring: block ids and scales of 32 subtiles at a time, one a lane ----
-    const int* table = a.table + r * a.table_stride;
-    const auto block_at = [&](int i) -> int {   // of this warp's i-th subtile; -1: none
-      if (i >= count) return -1;
-      const int b = table[(s_lo + warp + i * kDecWarps) * 16 / T];
-      return (unsigned)b < (unsigned)c.blocks ? b : -1;
-    };
-    int id_i = -1, id_n = block_at(lane), id_c = -1;
-    float ks_i = 0.f, vs_i = 0.f, ks_c = 0.f, vs_c = 0.f;
-    const uint8_t* kcodes = (const uint8_t*)c.k + (long long)kh * T * D;
-    const uint8_t* vcodes = (const uint8_t*)c.v + (long long)kh * T * D;
-    const auto issue = [&](int i) {
-      if ((i & 31) == 0) {
-        id_i = id_n;
-        if (id_i >= 0) {
-          ks_i = c.kscale[id_i * c.scale_stride + kh];
-          vs_i = c.vscale[id_i * c.scale_stride + kh];
-        }
-        id_n = block_at(i + 32 + lane);
-      }
-      const int id = __shfl_sync(~0u, id_i, i & 31);
-      const int tok0 = (s_lo + warp + i * kDecWarps) * 16;
-      const long long at = max(id, 0) * c.block_stride + (long long)(tok0 & (T - 1)) * D;
-      const uint32_t dst = ring + (i % L::kStages) * L::kStage;
-      const int left = id < 0 ? 0 : tile_hi - tok0;   // tokens past what the tile sees read as zero
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (int h = 0; h < L::kKC; h++)
-          cp_async_lane<16>(dst + (j * L::kKC + h) * 512 + lane * 16,
-                            kcodes + at + (8 * j + g) * D + (t + 4 * h) * 16, 8 * j + g < left);
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
-#pragma unroll
-        for (int h = 0; h < L::kVC; h++)
-          cp_async_lane<L::kVB>(dst + 2 * L::kKC * 512 + (j * L::kVC + h) * (32 * L::kVB) + lane * L::kVB,
-                                vcodes + at + tok * D + h * 128 + g * L::kVB, tok < left);
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < L::kStages - 1; i++) {
-      if (i < count) issue(i);
-      cp_async_commit();
+    if (a.causal) {
+      all_hi = cur.kv - cur.q + cur.tile * 16 / G + 1;
+      all_lo = first_key(cur.kv - cur.q + (cur.tile * 16 + cur.row_n - 1) / G, a.window);
     }
 
     // ---- q fragments: chunk h, part i: channels (t + 4 h) * 16 + 4 i + {0, 1 | 2, 3} ----
     uint32_t qf[D == 256 ? 1 : D / 16][4];
     float fac[2];      // score factor of the row: scale * log2 e * the power of two taken out of q
     {
-      const uint16_t* qp[2];
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-        qp[i] = (const uint16_t*)a.q + (long long)(q.q0 + row_tok[i]) * a.q_row + (long long)row_head[i] * D;
+      const uint8_t* qp[2] = {q_sm + turn * L::kQBytes + g * L::kQRow, q_sm + turn * L::kQBytes + (g + 8) * L::kQRow};
       float up[2] = {1.f, 1.f};
       fac[0] = fac[1] = p.scale_log2;
       if (BF16) {
@@ -241,7 +326,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) attn8_split_kernel(const __
           float m = 0.f;
 #pragma unroll
           for (int h = 0; h < 2 * L::kKC; h++) {
-            const uint4 v = *(const uint4*)(qp[i] + (t + 4 * (h >> 1)) * 16 + (h & 1) * 8);
+            const uint4 v = *(const uint4*)(qp[i] + (t + 4 * (h >> 1)) * 32 + (h & 1) * 16);
             const uint32_t* u = (const uint32_t*)&v;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -263,7 +348,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) attn8_split_kernel(const __
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
-          for (int e = 0; e < 2; e++) v[i][e] = *(const uint4*)(qp[i] + (t + 4 * h) * 16 + e * 8);
+          for (int e = 0; e < 2; e++) v[i][e] = *(const uint4*)(qp[i] + (t + 4 * h) * 32 + e * 16);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           uint32_t w[4];
@@ -287,137 +372,173 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) attn8_split_kernel(const __
       }
       if (D == 256) __syncthreads();
     }
+    Seg next = cur;
+    bool more = f_next < f_end;
+    if (more) {
+      next = segment_at(f_next);
+      more = next.g0 < next.g1;
+      if (more) load_q(next, turn ^ 1);      // joins the next group that is committed
+    }
 
     // ---- the subtiles ----
     float o[D / 8][4];
 #pragma unroll
     for (int j = 0; j < D / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    // m: reference of the weights (2^(score - m)), M: of weight * value scale; both follow the
+    // running maximum only when it passes them by more than 2^kSlack, so the sums are rescaled
+    // a few times a segment, and weights stay below 2^kSlack (fp16 holds 2^15)
+    constexpr float kNone = -1e30f, kSlack = 6.f;
+    float m[2] = {kNone, kNone}, M[2] = {kNone, kNone}, gain[2] = {1.f, 1.f}, l[2] = {0.f, 0.f};
+    int tok0 = s_first * 16, id_c = -1;
+    float ks_c = 0.f, vs_c = 0.f;
 #pragma unroll 1
-    for (int i = 0; i < count; i++) {
-      if (i + L::kStages - 1 < count) issue(i + L::kStages - 1);
-      cp_async_commit();
-      cp_async_wait<L::kStages - 1>();
+    for (int i = 0; i < count; i += 2, tok0 += kDecGran, src = src + 2 * L::kStage == ring + L::kWarpBytes ? ring : src + 2 * L::kStage) {
+      issue_pair(i + 2 * (L::kPairs - 1));
+      cp_async_wait<L::kPairs - 1>();
       if ((i & 31) == 0) { id_c = id_i; ks_c = ks_i; vs_c = vs_i; }   // issue() is in the same 32
-      const int id = __shfl_sync(~0u, id_c, i & 31);
-      const float ks = __shfl_sync(~0u, ks_c, i & 31), vs = __shfl_sync(~0u, vs_c, i & 31);
-      if (id < 0) continue;
-      const int tok0 = (s_lo + warp + i * kDecWarps) * 16;
-      const uint32_t src = ring + (i % L::kStages) * L::kStage;
-      float s[2][4];
+      float s[2][2][4];          // of subtile u, token octet j
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int h = 0; h < L::kKC; h++) {
-          const uint4 kw = lds128(src + (j * L::kKC + h) * 512 + lane * 16);
-          const uint32_t* w = (const uint32_t*)&kw;
+        for (int j = 0; j < 2; j++) s[u][j][0] = s[u][j][1] = s[u][j][2] = s[u][j][3] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const uint32_t b0 = e4m3x2_to_half2(w[e]), b1 = e4m3x2_to_half2(w[e] >> 16);
-            if (D == 256) {
-              const uint4 qv = qsm[h * 4 + e][lane];
-              const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
-              mma16816(s[j], qa, b0, b1);
-            } else {
-              mma16816(s[j], qf[D == 256 ? 0 : h * 4 + e], b0, b1);
+      for (int h = 0; h < L::kKC; h++) {
+        uint4 kw[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) kw[u][j] = lds128(src + u * L::kStage + (j * L::kKC + h) * 512 + lane * 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t qa[4];
+          if (D == 256) {
+            const uint4 qv = qsm[h * 4 + e][lane];
+            qa[0] = qv.x; qa[1] = qv.y; qa[2] = qv.z; qa[3] = qv.w;
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; x++) qa[x] = qf[D == 256 ? 0 : h * 4 + e][x];
+          }
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              uint32_t b0, b1;
+              e4m3x4_to_half2x2(((const uint32_t*)&kw[u][j])[e], b0, b1);
+              mma16816(s[u][j], qa, b0, b1);
             }
+        }
+      }
+      float k[2][2], vs[2], lv[2], top[2] = {-INFINITY, -INFINITY}, top_v[2] = {-INFINITY, -INFINITY};
+      bool edge[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int id = __shfl_sync(~0u, id_c, (i & 31) + u);
+        const float ks = __shfl_sync(~0u, ks_c, (i & 31) + u);
+        vs[u] = __shfl_sync(~0u, vs_c, (i & 31) + u);
+        lv[u] = __log2f(vs[u]);
+        const int at = tok0 + 16 * u;
+        edge[u] = id < 0 || at < all_lo || at + 16 > all_hi;   // some row does not see some token
+#pragma unroll
+        for (int r2 = 0; r2 < 2; r2++) {
+          k[u][r2] = fmaxf(ks * fac[r2], 1e-38f);   // above 0: masked scores stay -inf
+          if (edge[u]) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const int tok = at + 8 * j + 2 * t + e;
+                if (id < 0 || tok < first[r2] || tok > last[r2]) s[u][j][2 * r2 + e] = -INFINITY;
+              }
+          }
+          const float x = fmaxf(fmaxf(s[u][0][2 * r2], s[u][0][2 * r2 + 1]), fmaxf(s[u][1][2 * r2], s[u][1][2 * r2 + 1])) * k[u][r2];
+          top[r2] = fmaxf(top[r2], x);
+          top_v[r2] = fmaxf(top_v[r2], x + lv[u]);
+        }
+      }
+      const bool grew = top[0] > m[0] + kSlack || top[1] > m[1] + kSlack ||
+                        top_v[0] > M[0] + kSlack || top_v[1] > M[1] + kSlack;
+      if (__any_sync(~0u, grew)) {
+#pragma unroll
+        for (int r2 = 0; r2 < 2; r2++) {
+          float x = top[r2], y = top_v[r2];
+          x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+          y = fmaxf(y, __shfl_xor_sync(~0u, y, 1));
+          y = fmaxf(y, __shfl_xor_sync(~0u, y, 2));
+          const float mn = fmaxf(m[r2], x), Mn = fmaxf(M[r2], y);
+          l[r2] *= ex2(m[r2] - mn);
+          const float corr = ex2(M[r2] - Mn);
+          m[r2] = mn;
+          M[r2] = Mn;
+          gain[r2] = ex2(mn - Mn);
+#pragma unroll
+          for (int j = 0; j < D / 8; j++) {
+            o[j][2 * r2] *= corr;
+            o[j][2 * r2 + 1] *= corr;
           }
         }
       }
-      const float lv = __log2f(vs);
-      const bool edge = tok0 < first[0] || tok0 < first[1] || tok0 + 15 > last[0] || tok0 + 15 > last[1];
-      const bool any_edge = __any_sync(~0u, edge);
-      float corr[2], corr_o[2], f_v[2];
+      uint32_t pa[2][4];
 #pragma unroll
-      for (int i2 = 0; i2 < 2; i2++) {
-        const float k = ks * fac[i2];
-        float top = -INFINITY;
+      for (int u = 0; u < 2; u++) {
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int r2 = 0; r2 < 2; r2++) {
+          const float f_v = vs[u] * gain[r2];
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float& x = s[j][2 * i2 + e];
-            x *= k;
-            if (any_edge) {
-              const int tok = tok0 + 8 * j + 2 * t + e;
-              if (tok < first[i2] || tok > last[i2]) x = -INFINITY;
-            }
-            top = fmaxf(top, x);
+          for (int j = 0; j < 2; j++) {
+            const float x0 = ex2(fmaf(s[u][j][2 * r2], k[u][r2], -m[r2]));
+            const float x1 = ex2(fmaf(s[u][j][2 * r2 + 1], k[u][r2], -m[r2]));
+            l[r2] += x0 + x1;
+            pa[u][2 * j + r2] = pack_half2(x0 * f_v, x1 * f_v);
           }
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        const float mn = fmaxf(m[i2], top);
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        corr[i2] = ex2(m[i2] - ref);
-        m[i2] = mn;
-        const float Mn = fmaxf(M[i2], top + lv);
-        const float Mref = Mn == -INFINITY ? 0.f : Mn;
-        corr_o[i2] = exp2f(M[i2] - Mref);
-        M[i2] = Mn;
-        f_v[i2] = Mn == -INFINITY || lv == -INFINITY ? 0.f : vs * exp2f(ref - Mref);
-        l[i2] *= corr[i2];
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float& x = s[j][2 * i2 + e];
-            x = ex2(x - ref);
-            l[i2] += x;
-            x *= f_v[i2];
-          }
-      }
-      if (__any_sync(~0u, corr_o[0] != 1.f || corr_o[1] != 1.f)) {
-#pragma unroll
-        for (int j = 0; j < D / 8; j++) {
-          o[j][0] *= corr_o[0];
-          o[j][1] *= corr_o[0];
-          o[j][2] *= corr_o[1];
-          o[j][3] *= corr_o[1];
         }
       }
-      const uint32_t pa[4] = {pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]),
-                              pack_half2(s[1][0], s[1][1]), pack_half2(s[1][2], s[1][3])};
 #pragma unroll
       for (int h = 0; h < L::kVC; h++) {
-        uint32_t v[4][L::kVB / 4];
+        uint32_t v[2][4][L::kVB / 4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint32_t at = src + 2 * L::kKC * 512 + (j * L::kVC + h) * (32 * L::kVB) + lane * L::kVB;
-          if (L::kVB == 16) {
-            const uint4 x = lds128(at);
-            v[j][0] = x.x; v[j][1] = x.y; v[j][L::kVB / 4 - 2] = x.z; v[j][L::kVB / 4 - 1] = x.w;
-          } else {
-            const uint2 x = lds64(at);
-            v[j][0] = x.x; v[j][1] = x.y;
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const uint32_t at = src + u * L::kStage + 2 * L::kKC * 512 + (j * L::kVC + h) * (32 * L::kVB) + lane * L::kVB;
+            if (L::kVB == 16) {
+              const uint4 x = lds128(at);
+              v[u][j][0] = x.x; v[u][j][1] = x.y; v[u][j][L::kVB / 4 - 2] = x.z; v[u][j][L::kVB / 4 - 1] = x.w;
+            } else {
+              const uint2 x = lds64(at);
+              v[u][j][0] = x.x; v[u][j][1] = x.y;
+            }
           }
-        }
         // 0 * NaN: a NaN code that only some rows of the tile see must not reach the others, so
         // each row then goes through the MMA by itself, without the tokens that it does not see
         bool nan = false;
-        if (any_edge) {
+        if (edge[0] || edge[1]) {
 #pragma unroll
-          for (int j = 0; j < 4; j++)
+          for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int w = 0; w < L::kVB / 4; w++) nan |= (((v[j][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+              for (int w = 0; w < L::kVB / 4; w++) nan |= (((v[u][j][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
           nan = __any_sync(~0u, nan);
         }
         if (!nan) {
           pv_mma<L::kVB / 4>(o + h * 16, pa, v);
         } else {
 #pragma unroll 1
-          for (int i2 = 0; i2 < 16; i2++) {
-            const int src_lane = (i2 & 7) * 4;
+          for (int r16 = 0; r16 < 16; r16++) {
+            const int src_lane = (r16 & 7) * 4;
             const int f0 = __shfl_sync(~0u, first[0], src_lane), f1 = __shfl_sync(~0u, first[1], src_lane);
             const int l0 = __shfl_sync(~0u, last[0], src_lane), l1 = __shfl_sync(~0u, last[1], src_lane);
-            uint32_t seen[4][L::kVB / 4];
+            uint32_t seen[2][4][L::kVB / 4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const int tok = tok0 + 2 * t + (j & 1) + 8 * (j >> 1);
-              const bool see = tok >= (i2 < 8 ? f0 : f1) && tok <= (i2 < 8 ? l0 : l1);
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-              for (int w = 0; w < L::kVB / 4; w++) seen[j][w] = see ? v[j][w] : 0;
-            }
+              for (int j = 0; j < 4; j++) {
+                const int tok = tok0 + 16 * u + 2 * t + (j & 1) + 8 * (j >> 1);
+                const bool see = tok >= (r16 < 8 ? f0 : f1) && tok <= (r16 < 8 ? l0 : l1);
+#pragma unroll
+                for (int w = 0; w < L::kVB / 4; w++) seen[u][j][w] = see ? v[u][j][w] : 0;
+              }
             float one[L::kVB][4];
 #pragma unroll
             for (int j = 0; j < L::kVB; j++) one[j][0] = one[j][1] = one[j][2] = one[j][3] = 0.f;
@@ -426,116 +547,206 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) attn8_split_kernel(const __
             for (int j = 0; j < L::kVB; j++)
 #pragma unroll
               for (int e = 0; e < 4; e++)
-                if (g == (i2 & 7) && (e >> 1) == (i2 >> 3)) o[h * 16 + j][e] += one[j][e];
+                if (g == (r16 & 7) && (e >> 1) == (r16 >> 3)) o[h * 16 + j][e] += one[j][e];
           }
         }
       }
     }
-    cp_async_wait<0>();
+
+    // ---- the next segment's first stages ----
+    cp_async_commit();
+    cp_async_wait<0>();            // the next q too
+    if (more) {
+      open(next);
+      fill = src = ring;
+      prologue();
+    }
 
     // ---- the warps' states meet: o relative to the common m ----
+    // kMeet warps at a time leave their rows in shared memory or add them to what is there.
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       l[i] += __shfl_xor_sync(~0u, l[i], 1);
       l[i] += __shfl_xor_sync(~0u, l[i], 2);
+      if (m[i] == kNone) m[i] = -INFINITY;
       if (t == 0) { wm[warp][g + 8 * i] = m[i]; wl[warp][g + 8 * i] = l[i]; }
     }
     __syncthreads();
-    float* mine = (float*)(dec_sm + warp * L::kWarpBytes);
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      float top = wm[0][g + 8 * i];
+      float top = wm[0][g + 8 * i], sum = 0.f;
 #pragma unroll
       for (int w = 1; w < kDecWarps; w++) top = fmaxf(top, wm[w][g + 8 * i]);
-      const float k = M[i] == -INFINITY ? 0.f : exp2f(M[i] - top);
-#pragma unroll
-      for (int j = 0; j < D / 8; j++)
-        *(float2*)(mine + (g + 8 * i) * L::kRow + j * 8 + 2 * t) = make_float2(o[j][2 * i] * k, o[j][2 * i + 1] * k);
-    }
-    __syncthreads();
-    // thread (row, column n of the MMA tiles): channels n * kVB .. of each 128 (64)
-    const int row = tid >> 3, col = tid & 7;
-    float top = wm[0][row], lsum = 0.f;
-#pragma unroll
-    for (int w = 1; w < kDecWarps; w++) top = fmaxf(top, wm[w][row]);
-#pragma unroll
-    for (int w = 0; w < kDecWarps; w++) lsum = fmaf(wl[w][row], wm[w][row] == -INFINITY ? 0.f : exp2f(wm[w][row] - top), lsum);
-    float acc[D / 8];
-#pragma unroll
-    for (int j = 0; j < D / 8; j++) {
-      acc[j] = 0.f;
 #pragma unroll
       for (int w = 0; w < kDecWarps; w++)
-        acc[j] += ((const float*)(dec_sm + w * L::kWarpBytes))[row * L::kRow + j * 8 + col];
+        sum = fmaf(wl[w][g + 8 * i], wm[w][g + 8 * i] == -INFINITY ? 0.f : ex2(wm[w][g + 8 * i] - top), sum);
+      if (warp == 0 && t == 0) { row_m[g + 8 * i] = top; row_l[g + 8 * i] = sum; }
+      const float k = m[i] == -INFINITY ? 0.f : ex2(M[i] - top);
+#pragma unroll
+      for (int j = 0; j < D / 8; j++) {
+        o[j][2 * i] *= k;
+        o[j][2 * i + 1] *= k;
+      }
+    }
+    float* mine = meet + warp % L::kMeet * (16 * L::kRow) + g * L::kRow + 2 * t * L::kCol;
+#pragma unroll
+    for (int round = 0; round < kDecWarps / L::kMeet; round++) {
+      if (warp / L::kMeet == round) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int j = 0; j < D / 8; j++) {
+            float *p0 = mine + 8 * i * L::kRow + j, *p1 = p0 + L::kCol;
+            *p0 = (round ? *p0 : 0.f) + o[j][2 * i];
+            *p1 = (round ? *p1 : 0.f) + o[j][2 * i + 1];
+          }
+      }
+      __syncthreads();
+    }
+    // From here on thread `tid` holds the quads tid, tid + 128, ... of the rows x D outputs: quad
+    // e is row e / (D / 4), MMA column (e / (D / 32)) % 8, four of its D / 8 channels.
+    constexpr int kQuads = D / 32;
+    const int quads = cur.row_n * (D / 4);
+    float4 acc[kQuads];
+    float row_top[kQuads], row_sum[kQuads];     // m and l of the quads' rows
+#pragma unroll
+    for (int x = 0; x < kQuads; x++) {
+      const int e = tid + x * 32 * kDecWarps;
+      const float* p4 = meet + e / (D / 4) * L::kRow + e / kQuads % 8 * L::kCol + e % kQuads * 4;
+      acc[x] = make_float4(p4[0], p4[1], p4[2], p4[3]);
+      if (L::kMeet == 2) {
+        const float* p5 = p4 + 16 * L::kRow;
+        acc[x] = make_float4(acc[x].x + p5[0], acc[x].y + p5[1], acc[x].z + p5[2], acc[x].w + p5[3]);
+      }
+      row_top[x] = row_m[e / (D / 4)];
+      row_sum[x] = row_l[e / (D / 4)];
     }
     // ---- a whole item is written out; a part goes to the workspace ----
+    // Parts join in two steps, groups of about the square root of their number first, so that no
+    // CTA has many to read; the last to arrive does it, in the order of the parts.
     bool write = true;
-    if (g0 > 0 || g1 < n) {
-      const long long fs = f - g0;
-      const int ca = (int)(fs / per), cb = (int)((fs + n - 1) / per);   // the CTAs of this item
-      float* ws = (float*)((uint8_t*)a.ws + kDecCtas * sizeof(int));
-      constexpr int kPart = 16 * D + 32;     // floats of a part: o, then m and l of each row
-      int* counter = (int*)a.ws + ca;
-      const bool starts = (int)blockIdx.x == ca;
-      float* slot = ws + ((long long)blockIdx.x * 2 + (starts ? 1 : 0)) * kPart;
-      if (row < row_n) {
+    if (cur.g0 > 0 || cur.g1 < cur.n) {
+      const long long f0 = f + cur.cost - cur.g1;       // the item's first granule
+      const int ca = (int)(f0 / per), cb = (int)((f0 + cur.n - 1) / per);   // the CTAs of this item
+      const int parts = cb - ca + 1;
+      int size = kAtOnce;
+      while (size * size < parts) size++;
+      const int me = (int)blockIdx.x - ca, head_g = me - me % size, count_g = min(size, parts - head_g);
+      // counters and parts of CTA b: 1 where an item begins that goes on, 0 where one continues
+      const auto at_of = [&](int i) { return (ca + i) * 2 + (i == 0 ? 1 : 0); };
+      int* counters = (int*)a.ws;
+      const auto part_of = [&](int i) {
+        return (float*)((uint8_t*)a.ws + kDecCtas * 3 * sizeof(int)) + (long long)at_of(i) * (16 * D + 32);
+      };
+      const auto put = [&](float* slot) {
 #pragma unroll
-        for (int j = 0; j < D / 8; j += 4)
-          *(float4*)(slot + (row * 8 + col) * (D / 8) + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-        if (col == 0) { slot[16 * D + row] = top; slot[16 * D + 16 + row] = lsum; }
-      }
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) arrived = atomicAdd(counter, 1);
-      __syncthreads();
-      write = arrived == cb - ca;
-      if (write) {
-        __threadfence();
-        if (tid == 0) *counter = 0;          // as the next call expects it
-        if (row < row_n) {
-          const auto part_of = [&](int b) { return ws + ((long long)b * 2 + (b == ca ? 1 : 0)) * kPart; };
-          top = -INFINITY;
-          for (int b = ca; b <= cb; b++) top = fmaxf(top, __ldcg(part_of(b) + 16 * D + row));
-          lsum = 0.f;
-#pragma unroll
-          for (int j = 0; j < D / 8; j++) acc[j] = 0.f;
-          for (int b = ca; b <= cb; b++) {
-            const float* s = part_of(b);
-            const float pm = __ldcg(s + 16 * D + row);
-            const float k = pm == -INFINITY ? 0.f : exp2f(pm - top);
-            lsum = fmaf(k, __ldcg(s + 16 * D + 16 + row), lsum);
-#pragma unroll
-            for (int j = 0; j < D / 8; j += 4) {
-              const float4 v = __ldcg((const float4*)(s + (row * 8 + col) * (D / 8) + j));
-              acc[j] = fmaf(k, v.x, acc[j]);
-              acc[j + 1] = fmaf(k, v.y, acc[j + 1]);
-              acc[j + 2] = fmaf(k, v.z, acc[j + 2]);
-              acc[j + 3] = fmaf(k, v.w, acc[j + 3]);
-            }
+        for (int x = 0; x < kQuads; x++) {
+          const int e = tid + x * 32 * kDecWarps;
+          if (e < quads) {
+            __stcg((float4*)slot + e, acc[x]);
+            if (e % (D / 4) == 0) __stcg((float2*)(slot + 16 * D) + e / (D / 4), make_float2(row_top[x], row_sum[x]));
           }
         }
+      };
+      const auto last_of = [&](int* counter, int n_parts) {
+        __syncthreads();                                  // every thread's part is written
+        if (tid == 0) {
+          __threadfence();
+          arrived = atomicAdd(counter, 1);
+          if (arrived == n_parts - 1) *counter = 0;      // as the next call expects it
+          __threadfence();
+        }
+        __syncthreads();
+        return arrived == n_parts - 1;
+      };
+      const auto join = [&](int from, int step, int n_parts) {   // parts from, from + step, ...
+#pragma unroll
+        for (int x0 = 0; x0 < kQuads; x0 += 2) {        // two quads of up to kAtOnce parts in flight
+          if (tid + x0 * 32 * kDecWarps >= quads) break;
+          float4 sum4[2] = {};
+          float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+#pragma unroll 1
+          for (int i0 = 0; i0 < n_parts; i0 += kAtOnce) {
+            float4 v[kAtOnce][2];
+            float2 ml[kAtOnce][2];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++)
+#pragma unroll
+              for (int x = 0; x < 2; x++) {
+                const int e = min(tid + (x0 + x) * 32 * kDecWarps, quads - 1);
+                const float* s = part_of(from + min(i0 + i, n_parts - 1) * step);
+                v[i][x] = __ldcg((const float4*)s + e);
+                ml[i][x] = __ldcg((const float2*)(s + 16 * D) + e / (D / 4));
+              }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              float mn = top[x];
+#pragma unroll
+              for (int i = 0; i < kAtOnce; i++) {
+                if (i0 + i >= n_parts) ml[i][x] = make_float2(-INFINITY, 0.f);
+                mn = fmaxf(mn, ml[i][x].x);
+              }
+              const float k0 = top[x] == -INFINITY ? 0.f : ex2(top[x] - mn);
+              top[x] = mn;
+              sum[x] *= k0;
+              sum4[x].x *= k0;
+              sum4[x].y *= k0;
+              sum4[x].z *= k0;
+              sum4[x].w *= k0;
+#pragma unroll
+              for (int i = 0; i < kAtOnce; i++) {
+                if (i0 + i >= n_parts) break;
+                const float k = ml[i][x].x == -INFINITY ? 0.f : ex2(ml[i][x].x - mn);
+                sum[x] = fmaf(k, ml[i][x].y, sum[x]);
+                sum4[x].x = fmaf(k, v[i][x].x, sum4[x].x);
+                sum4[x].y = fmaf(k, v[i][x].y, sum4[x].y);
+                sum4[x].z = fmaf(k, v[i][x].z, sum4[x].z);
+                sum4[x].w = fmaf(k, v[i][x].w, sum4[x].w);
+              }
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            acc[x0 + x] = sum4[x];
+            row_top[x0 + x] = top[x];
+            row_sum[x0 + x] = sum[x];
+          }
+        }
+      };
+      put(part_of(me));
+      write = last_of(counters + at_of(head_g), count_g);
+      if (write) {
+        join(head_g, 1, count_g);
+        if (parts > size) {
+          __syncthreads();       // all of the group's parts are read: its sum takes the first one's place
+          put(part_of(head_g));
+          const int groups = (parts + size - 1) / size;
+          write = last_of(counters + 2 * kDecCtas + ca, groups);
+          if (write) join(0, size, groups);
+        }
       }
     }
-    if (write && row < row_n) {
-      const int rr = tile * 16 + row, tok = rr / G, head = kh * G + rr - tok * G;
-      const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-      uint16_t* op = (uint16_t*)a.out + (long long)(q.q0 + tok) * a.out_row + (long long)head * D;
+    if (write) {
 #pragma unroll
-      for (int h = 0; h < L::kVC; h++)
-#pragma unroll
-        for (int j = 0; j < L::kVB; j += 8) {
-          uint32_t u[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            u[e] = float2_to_pair<BF16>(acc[h * 16 + j + 2 * e] * inv, acc[h * 16 + j + 2 * e + 1] * inv);
-          *(uint4*)(op + h * 128 + col * L::kVB + j) = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-      if (a.lse && col == 0)
-        a.lse[(long long)(q.q0 + tok) * a.heads + head] =
-            lsum == 0.f ? -INFINITY : (top + log2f(lsum)) * 0.6931471805599453f;
+      for (int x = 0; x < kQuads; x++) {
+        const int e = tid + x * 32 * kDecWarps;
+        if (e >= quads) break;
+        const int row = e / (D / 4), col = e / kQuads % 8, j = e % kQuads * 4;
+        const int rr = cur.tile * 16 + row, tok = rr / G, head = cur.kh * G + rr - tok * G;
+        const float inv = row_sum[x] > 0.f ? 1.f / row_sum[x] : 0.f;
+        uint16_t* op = (uint16_t*)a.out + (long long)(cur.q0 + tok) * a.out_row + (long long)head * D;
+        *(uint2*)(op + (j / L::kVB) * 128 + col * L::kVB + j % L::kVB) =
+            make_uint2(float2_to_pair<BF16>(acc[x].x * inv, acc[x].y * inv),
+                       float2_to_pair<BF16>(acc[x].z * inv, acc[x].w * inv));
+        if (a.lse && e % (D / 4) == 0)
+          a.lse[(long long)(cur.q0 + tok) * a.heads + head] =
+              row_sum[x] == 0.f ? -INFINITY : (row_top[x] + log2f(row_sum[x])) * 0.6931471805599453f;
+      }
     }
-    __syncthreads();      // the ring and the small arrays are used again
-    f += g1 - g0;
+    if (!more) break;
+    f = f_next;
+    cur = next;
+    __syncthreads();      // the next q is there; the small arrays are used again
   }
 }
 
@@ -544,9 +755,9 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) attn8_split_kernel(const __
 using namespace yk;
 
 extern "C" size_t yk_attn_kv8_workspace_bytes(int requests, int rows, int heads, int kv_heads, int dim) {
-  // a counter and two parts (o, m, l of 16 rows) for each CTA, whatever the lengths
+  // three counters and two parts (o, m, l of 16 rows) for each CTA, whatever the lengths
   (void)requests; (void)rows; (void)heads; (void)kv_heads;
-  return kDecCtas * (sizeof(int) + 2 * (16 * (size_t)std::max(dim, 0) + 32) * sizeof(float));
+  return kDecCtas * (3 * sizeof(int) + 2 * (16 * (size_t)std::max(dim, 0) + 32) * sizeof(float));
 }
 
 template <bool BF16, int D>
@@ -574,7 +785,7 @@ extern "C" int yk_attn_kv8(const YkKvCache* c, const YkAttnKv8* a, yk_stream_t s
     return refuse(YK_EINVAL, "attn_kv8: q and out need 16-byte alignment and row strides that are multiples of 8");
   if (!aligned16(a->ws) || a->ws_bytes < yk_attn_kv8_workspace_bytes(a->requests, a->rows, a->heads, c->heads, c->dim))
     return refuse(YK_EINVAL, "attn_kv8: workspace too small or not 16-byte aligned");
-  Attn8Args p{*c, *a, 0.f, 1};
+  Attn8Args p{*c, *a, 0.f, kDecLead, kDecMin};
   if (p.a.scale == 0.f) p.a.scale = 1.f / sqrtf((float)c->dim);
   p.scale_log2 = p.a.scale * 1.4426950408889634f;
   const bool bf = a->dtype == YK_BF16;

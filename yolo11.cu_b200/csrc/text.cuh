@@ -23,6 +23,11 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t codes) {
   asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(r) : "r"(codes));
   return r;
 }
+// Four codes: bytes 0, 1 and bytes 2, 3.
+__device__ __forceinline__ void e4m3x4_to_half2x2(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t codes) {
   const uint32_t h = e4m3x2_to_half2(codes & 0xffffu);
   return __half22float2(*(const __half2*)&h);
