@@ -13,8 +13,9 @@ namespace yk {
 //    warp's own ring, piece (output, 32-column block) at block * 256 + output * 16, so that lane
 //    (g, t) reads its word t of outputs g and g + 8 of a block without bank conflicts; the block's
 //    32 columns are two MMAs, in an order of columns that x follows.
-//  * Scales and zero points of the chunk travel in the same stage, as the aligned words that hold
-//    them.
+//  * Lane (g, t) reads the scales and zero points of block t of its outputs one chunk ahead; they
+//    reach the other lanes by shuffles.  (In the ring, by aligned words, they cost as many L2
+//    sectors as the codes.)
 //  * The CTA's 8 warps are WN along the outputs times WK along the columns; each warp takes R
 //    output tiles, which share the x operand.  The WK partial sums meet in shared memory.
 struct Gemv4Args {
@@ -23,6 +24,8 @@ struct Gemv4Args {
   int zero;        // there are zero points
   int bf16;        // type of scales and y
   int xgroup;      // columns of a scale of e4m3 x; 0: one a row, or none
+  int x_shift;     // its logarithm, -1: not a power of two
+  int x_inside;    // it may change inside a chunk of 128 columns
 };
 constexpr int kGemvWarps = 8;
 
@@ -50,35 +53,60 @@ __device__ __forceinline__ uint32_t bsub2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hsub2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
   return *(const uint32_t*)&r;
 }
-// The 8 codes of a word minus the zero point z: pairs (0, 4), (1, 5), (2, 6), (3, 7).
+// A zero point z as the packed operands that codes8 takes.
+struct Zero {
+  uint32_t a, b;
+};
+template <bool F16>
+__device__ __forceinline__ Zero zero_of(uint32_t z) {
+  if (F16) return {0x64006400u + z * 0x10001u, 0xd400d400u + z * 0x100010u};   // 1024 + z, -(64 + z)
+  return {0x43004300u + z * 0x10001u, 0};                                      // 128 + z
+}
+// The 8 codes of a word minus the zero point: pairs (0, 4), (1, 5), (2, 6), (3, 7).
 // fp16: 1024 + q in the low nibble's place; 1024 + 16 q a nibble higher, times 1/16.
 template <bool F16>
-__device__ __forceinline__ void codes8(uint32_t w, uint32_t z, uint32_t (&o)[4]) {
+__device__ __forceinline__ void codes8(uint32_t w, const Zero& z, uint32_t (&o)[4]) {
   if (F16) {
-    const uint32_t z0 = 0x64006400u | z * 0x10001u, z1 = 0xd400d400u + z * 0x100010u;   // 1024 + z, -(64 + z)
-    o[0] = hsub2((w & 0x000f000fu) | 0x64006400u, z0);
-    o[1] = hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z1);
+    o[0] = hsub2((w & 0x000f000fu) | 0x64006400u, z.a);
+    o[1] = hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z.b);
     w >>= 8;
-    o[2] = hsub2((w & 0x000f000fu) | 0x64006400u, z0);
-    o[3] = hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z1);
+    o[2] = hsub2((w & 0x000f000fu) | 0x64006400u, z.a);
+    o[3] = hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z.b);
   } else {
-    const uint32_t z0 = 0x43004300u | z * 0x10001u;                                     // 128 + z
 #pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = bsub2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u, z0);
+    for (int i = 0; i < 4; i++) o[i] = bsub2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u, z.a);
   }
+}
+__device__ __forceinline__ uint32_t lds_u8(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint16_t lds_u16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
 }
 
 template <int NT, int R>
 struct Gemv {
   static constexpr int kStages = R == 1 ? 5 : 4;
-  static constexpr int kTile = 1024 + 256 + 256;     // codes, scales, zero points of 16 outputs
+  // codes of 16 outputs: four blocks, 32 bytes more than 256 apart so that the pieces a warp
+  // writes at once fall into different banks
+  static constexpr int kBlock = 256 + 32, kTile = 4 * kBlock;
   static constexpr int kStage = R * kTile;
   static constexpr int kRing = kGemvWarps * kStages * kStage, kMeet = kGemvWarps * R * NT * 512;
   static constexpr int kSmem = kRing > kMeet ? kRing : kMeet;
 };
 
 // XT: type of x; the MMA is bf16 for bf16 rows and fp16 otherwise (e4m3 converts exactly).
-template <int XT, int NT, int R, int WN>
+// GB: blocks (32 columns) of a group of w.
+template <int XT, int GB, int NT, int R, int WN>
 __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel(const __grid_constant__ Gemv4Args ga) {
   using S = Gemv<NT, R>;
   constexpr bool X8 = XT == YK_E4M3, F16 = XT != YK_BF16;
@@ -90,45 +118,34 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int wn = warp % WN, wk = warp / WN;
   const int n0 = (blockIdx.x * WN + wn) * R * 16;   // this warp's first output
-  const int K = p.k, G = p.group, chunks = (K + 127) / 128;
+  const int K = p.k, chunks = (K + 127) / 128;
   const int count = n0 < p.n && chunks > wk ? (chunks - wk + WK - 1) / WK : 0;
   const uint32_t ring = smem_u32(sm) + warp * kStages * kStage;
 
-  const uint8_t* wrow[R][2];
-  const uint8_t *srow[R][2], *zrow[R][2];
+  // first codes, scales and zero points of this lane's outputs g, g + 8 of each tile
+  const uint8_t *wrow[R][2], *zrow[R][2];
+  const uint16_t* srow[R][2];
 #pragma unroll
   for (int r = 0; r < R; r++)
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const long long n = min(n0 + r * 16 + g + 8 * i, p.n - 1);
-      wrow[r][i] = (const uint8_t*)p.w + n * p.w_row + t * 16;
-      srow[r][i] = (const uint8_t*)p.wscale + n * p.group_row * 2;
-      zrow[r][i] = zero ? (const uint8_t*)p.wzero + n * p.group_row : nullptr;
+    for (int h = 0; h < 2; h++) {
+      const long long n = min(n0 + r * 16 + g + 8 * h, p.n - 1);
+      wrow[r][h] = (const uint8_t*)p.w + n * p.w_row + t * 16;
+      srow[r][h] = (const uint16_t*)p.wscale + n * p.group_row + t / GB;
+      zrow[r][h] = (const uint8_t*)p.wzero + n * p.group_row + t / GB;
     }
-  const uint8_t* s_end = (const uint8_t*)p.wscale + ((long long)(p.n - 1) * p.group_row + K / G) * 2;
-  const uint8_t* z_end = zero ? (const uint8_t*)p.wzero + (long long)(p.n - 1) * p.group_row + K / G : nullptr;
-  const int t_group = t * 32 / G;                    // group of block t in its chunk
-  // the aligned word around `a`, up to the array's end
-  const auto word = [&](uint32_t dst, const uint8_t* a, const uint8_t* end, bool ok) {
-    const uint8_t* w = (const uint8_t*)((uintptr_t)a & ~(uintptr_t)3);
-    const int bytes = ok ? (int)min((long long)4, (long long)(end - w)) : 0;
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(w), "r"(bytes) : "memory");
-  };
+  constexpr int kPer = 4 / GB;       // groups of a chunk
+  const auto x_group = [&](int k) { return ga.x_shift >= 0 ? k >> ga.x_shift : k / ga.xgroup; };
   uint32_t fill = ring;
+  const uint32_t piece = t * S::kBlock + g * 16;
   const auto issue = [&](int i) {
     if (i < count) {
       const int c = wk + i * WK;
       const bool ok = c * 128 + t * 32 < K;
-      const int gi = c * (128 / G) + t_group;
 #pragma unroll
       for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint32_t at = fill + r * kTile;
-          cp_async16(at + t * 256 + (g + 8 * h) * 16, wrow[r][h] + (ok ? c * 64ll : 0), ok ? 16 : 0);
-          word(at + 1024 + h * 128 + lane * 4, srow[r][h] + (ok ? gi * 2 : 0), s_end, ok);
-          if (zero) word(at + 1280 + h * 128 + lane * 4, zrow[r][h] + (ok ? gi : 0), z_end, ok);
-        }
+        for (int h = 0; h < 2; h++) cp_async16(fill + r * kTile + piece + h * 128, wrow[r][h] + c * 64, ok ? 16 : 0);
       fill = fill + kStage == ring + kStages * kStage ? ring : fill + kStage;
     }
     cp_async_commit();
@@ -143,101 +160,147 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
   for (int r = 0; r < R; r++)
 #pragma unroll
     for (int j = 0; j < NT; j++) tot[r][j][0] = tot[r][j][1] = tot[r][j][2] = tot[r][j][3] = 0.f;
-  // x of row j * 8 + g, columns k .. k + 7 (k < K): pairs (0, 4), (1, 5), (2, 6), (3, 7)
-  const auto load_x = [&](int j, int k, uint32_t (&o)[4]) {
-    const int m = j * 8 + g;
-    if (m >= p.rows || k >= K) {
-      o[0] = o[1] = o[2] = o[3] = 0;
-      return;
-    }
-    const long long at = (long long)m * p.x_row + k;
-    if (X8) {
-      const uint8_t* x = (const uint8_t*)p.x + at;
-      uint2 v;
-      if (ga.x_vec) {
-        v = *(const uint2*)x;
+
+  // x of rows j * 8 + g: this lane's 8 columns of a block
+  constexpr int kSize = X8 ? 1 : 2;
+  const uint8_t* xp[NT];
+#pragma unroll
+  for (int j = 0; j < NT; j++)
+    xp[j] = (const uint8_t*)p.x + ((long long)min(j * 8 + g, p.rows - 1) * p.x_row + t * 8) * kSize;
+  const auto raw_x = [&](int j, int k, uint32_t (&v)[2 * kSize]) {     // columns k + 8 t ..
+    const bool ok = j * 8 + g < p.rows && k < K;
+    const uint8_t* x = xp[j] + k * kSize;
+    if (ga.x_vec) {
+      if (X8) {
+        const uint2 u = ok ? *(const uint2*)x : make_uint2(0, 0);
+        v[0] = u.x; v[1] = u.y;
       } else {
-        v.x = x[0] | x[1] << 8 | x[2] << 16 | (uint32_t)x[3] << 24;
-        v.y = x[4] | x[5] << 8 | x[6] << 16 | (uint32_t)x[7] << 24;
+        const uint4 u = ok ? *(const uint4*)x : make_uint4(0, 0, 0, 0);
+        v[0] = u.x; v[1] = u.y; v[2 * kSize - 2] = u.z; v[2 * kSize - 1] = u.w;
       }
-      e4m3x4_to_half2x2(__byte_perm(v.x, v.y, 0x5140), o[0], o[1]);
-      e4m3x4_to_half2x2(__byte_perm(v.x, v.y, 0x7362), o[2], o[3]);
     } else {
-      const uint16_t* x = (const uint16_t*)p.x + at;
-      uint4 v;
-      if (ga.x_vec) {
-        v = *(const uint4*)x;
-      } else {
-        v = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16,
-                       x[6] | (uint32_t)x[7] << 16);
+#pragma unroll 1
+      for (int i = 0; i < 2 * kSize; i++) {
+        uint32_t u = 0;
+        if (ok)
+          u = X8 ? x[4 * i] | x[4 * i + 1] << 8 | x[4 * i + 2] << 16 | (uint32_t)x[4 * i + 3] << 24
+                 : ((const uint16_t*)x)[2 * i] | (uint32_t)((const uint16_t*)x)[2 * i + 1] << 16;
+#pragma unroll
+        for (int e = 0; e < 2 * kSize; e++) v[e] = e == i ? u : v[e];
       }
-      o[0] = __byte_perm(v.x, v.z, 0x5410);
-      o[1] = __byte_perm(v.x, v.z, 0x7632);
-      o[2] = __byte_perm(v.y, v.w, 0x5410);
-      o[3] = __byte_perm(v.y, v.w, 0x7632);
     }
   };
+  // as the B operand: pairs (0, 4), (1, 5), (2, 6), (3, 7)
+  const auto pairs_x = [&](const uint32_t (&v)[2 * kSize], uint32_t (&o)[4]) {
+    if (X8) {
+      e4m3x4_to_half2x2(__byte_perm(v[0], v[1], 0x5140), o[0], o[1]);
+      e4m3x4_to_half2x2(__byte_perm(v[0], v[1], 0x7362), o[2], o[3]);
+    } else {
+      o[0] = __byte_perm(v[0], v[2 * kSize - 2], 0x5410);
+      o[1] = __byte_perm(v[0], v[2 * kSize - 2], 0x7632);
+      o[2] = __byte_perm(v[1], v[2 * kSize - 1], 0x5410);
+      o[3] = __byte_perm(v[1], v[2 * kSize - 1], 0x7632);
+    }
+  };
+  const float* xs_row[NT][2];        // scales of the rows whose sums this lane holds
+#pragma unroll
+  for (int j = 0; j < NT; j++)
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+      xs_row[j][e] = X8 ? p.xscale + min(j * 8 + 2 * t + e, p.rows - 1) * p.xscale_row : nullptr;
+
+  // scales and zero points of the next chunk's block t
+  uint32_t s_next[R][2], z_next[R][2];
+  const auto load_scales = [&](int i) {
+    const int c = wk + i * WK;
+    const bool ok = i < count && c * 128 + t * 32 < K;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        s_next[r][h] = ok ? srow[r][h][c * kPer] : 0;
+        z_next[r][h] = zero && ok ? zrow[r][h][c * kPer] : 8;
+      }
+  };
+  load_scales(0);
 
   uint32_t src = ring;
+  constexpr int kAhead = NT <= 2 ? 4 : 1;     // blocks of x read before they are used
 #pragma unroll 1
   for (int i = 0; i < count; i++) {
+    const int c = wk + i * WK;
+    uint32_t raw[kAhead][NT][2 * kSize];
+    if (kAhead == 4) {
+#pragma unroll
+      for (int b = 0; b < kAhead; b++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) raw_x(j, c * 128 + b * 32, raw[b][j]);
+    }
+    float xs[NT][2];
+    const int xg = X8 && ga.xgroup ? x_group(c * 128) : 0;
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) xs[j][e] = X8 && ga.xgroup ? xs_row[j][e][xg] : 1.f;
+    float sw[R][2];               // of block t
+    uint32_t zw[R][2];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        sw[r][h] = XT == YK_BF16 || (X8 && ga.bf16) ? elem_to_float<true>(s_next[r][h]) : elem_to_float<false>(s_next[r][h]);
+        zw[r][h] = z_next[r][h];
+      }
     issue(i + kStages - 1);
+    load_scales(i + 1);
     cp_async_wait<kStages - 1>();
     __syncwarp();                 // every lane's pieces of this stage are there
-    const int c = wk + i * WK;
     float acc[R][NT][4];
+    Zero zp[R][2];
 #pragma unroll
     for (int b = 0; b < 4; b++) {
-      const bool starts = b * 32 % G == 0, ends = (b + 1) * 32 % G == 0;   // of a group of scales
       uint32_t x[NT][4];
 #pragma unroll
-      for (int j = 0; j < NT; j++) load_x(j, c * 128 + b * 32 + t * 8, x[j]);
+      for (int j = 0; j < NT; j++) {
+        if (kAhead != 4) raw_x(j, c * 128 + b * 32, raw[0][j]);
+        pairs_x(raw[kAhead == 4 ? b : 0][j], x[j]);
+      }
+      if (X8 && b && ga.x_inside && c * 128 + b * 32 < K) {
+        const int xb = x_group(c * 128 + b * 32);
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) xs[j][e] = xs_row[j][e][xb];
+      }
 #pragma unroll
       for (int r = 0; r < R; r++) {
-        if (starts) {
+        const uint32_t at = src + r * kTile + b * S::kBlock + g * 16 + t * 4;
+        if (b % GB == 0) {
 #pragma unroll
           for (int j = 0; j < NT; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            zp[r][h] = zero_of<F16>(zero ? __shfl_sync(~0u, zw[r][h], (lane & ~3) + b) : 8);
         }
-        const uint32_t at = src + r * kTile;
         uint32_t q[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          uint32_t z = 8;
-          if (zero) {
-            const uint32_t low = (uint32_t)(uintptr_t)(zrow[r][h] + c * (128 / G) + b * 32 / G) & 3;
-            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(at + 1280 + h * 128 + (g * 4 + b) * 4 + low));
-          }
-          uint32_t w;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at + b * 256 + (g + 8 * h) * 16 + t * 4));
-          codes8<F16>(w, z, q[h]);
-        }
+        for (int h = 0; h < 2; h++) codes8<F16>(lds_u32(at + 128 * h), zp[r][h], q[h]);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const uint32_t a[4] = {q[0][2 * e], q[1][2 * e], q[0][2 * e + 1], q[1][2 * e + 1]};
 #pragma unroll
           for (int j = 0; j < NT; j++) mma_gemv<F16>(acc[r][j], a, x[j][2 * e], x[j][2 * e + 1]);
         }
-        if (ends) {
-          float s[2];
+        if (b % GB == GB - 1) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            const uint32_t low = (uint32_t)(uintptr_t)(srow[r][h] + (c * (128 / G) + b * 32 / G) * 2) & 2;
-            uint16_t u;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(at + 1024 + h * 128 + (g * 4 + b) * 4 + low));
-            s[h] = XT == YK_BF16 || (X8 && ga.bf16) ? elem_to_float<true>(u) : elem_to_float<false>(u);
+            const float f = GB == 4 ? sw[r][h] : __shfl_sync(~0u, sw[r][h], (lane & ~3) + b);
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+              for (int e = 0; e < 2; e++)
+                tot[r][j][2 * h + e] = fmaf(acc[r][j][2 * h + e], X8 ? f * xs[j][e] : f, tot[r][j][2 * h + e]);
           }
-#pragma unroll
-          for (int j = 0; j < NT; j++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              float xs = 1.f;
-              if (X8 && ga.xgroup) {
-                const int m = min(j * 8 + 2 * t + e, p.rows - 1);
-                xs = p.xscale[m * p.xscale_row + min(c * 128 + b * 32, K - 1) / ga.xgroup];
-              }
-              tot[r][j][e] = fmaf(acc[r][j][e], s[0] * xs, tot[r][j][e]);
-              tot[r][j][2 + e] = fmaf(acc[r][j][2 + e], s[1] * xs, tot[r][j][2 + e]);
-            }
         }
       }
     }
@@ -270,22 +333,30 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
   }
 }
 
-template <int XT, int NT, int R, int WN>
+template <int XT, int GB, int NT, int R, int WN>
 static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
-  const auto kern = gemv4_kernel<XT, NT, R, WN>;
+  const auto kern = gemv4_kernel<XT, GB, NT, R, WN>;
   if (smem_attr(kern, Gemv<NT, R>::kSmem) != cudaSuccess) return check_launch("gemv4 attr");
   constexpr int outputs = WN * R * 16;
   launch_k(kern, (a.p.n + outputs - 1) / outputs, 32 * kGemvWarps, Gemv<NT, R>::kSmem, st, a);
   note_launch();
   return check_launch("gemv4");
 }
-template <int XT>
+template <int XT, int GB>
 static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
   const int m = a.p.rows, n = a.p.n;
-  if (m <= 8) return launch_gemv4<XT, 1, 1, 1>(a, st);
-  if (m <= 16) return n >= 64 * 148 ? launch_gemv4<XT, 2, 2, 2>(a, st) : launch_gemv4<XT, 2, 1, 1>(a, st);
-  if (m <= 32) return launch_gemv4<XT, 4, 1, 2>(a, st);
-  return launch_gemv4<XT, 8, 1, 2>(a, st);
+  if (m <= 8) return launch_gemv4<XT, GB, 1, 1, 1>(a, st);
+  if (m <= 16) return n >= 64 * 148 ? launch_gemv4<XT, GB, 2, 2, 4>(a, st) : launch_gemv4<XT, GB, 2, 1, 1>(a, st);
+  if (m <= 32) return launch_gemv4<XT, GB, 4, 1, 2>(a, st);
+  return launch_gemv4<XT, GB, 8, 1, 2>(a, st);
+}
+template <int XT>
+static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
+  switch (a.p.group) {
+    case 32: return launch_gemv4<XT, 1>(a, st);
+    case 64: return launch_gemv4<XT, 2>(a, st);
+    default: return launch_gemv4<XT, 4>(a, st);
+  }
 }
 
 }  // namespace yk
@@ -311,7 +382,13 @@ extern "C" int yk_gemv4(const YkGemv4* p, yk_stream_t st) {
   if (x8 && p->xscale_row < (p->xgroup ? (p->k + p->xgroup - 1) / p->xgroup : 1))
     return refuse(YK_EINVAL, "gemv4: xscale stride below its row");
   const uintptr_t at = (uintptr_t)p->x | (uintptr_t)(x8 ? p->x_row : p->x_row * 2);
-  const Gemv4Args a{*p, at % (x8 ? 8 : 16) == 0, p->wzero != nullptr, p->dtype == YK_BF16, x8 ? p->xgroup : 0};
+  Gemv4Args a{*p};
+  a.x_vec = at % (x8 ? 8 : 16) == 0;
+  a.zero = p->wzero != nullptr;
+  a.bf16 = p->dtype == YK_BF16;
+  a.xgroup = x8 ? p->xgroup : 0;
+  a.x_shift = a.xgroup && !(a.xgroup & (a.xgroup - 1)) ? __builtin_ctz(a.xgroup) : -1;
+  a.x_inside = a.xgroup % 128 != 0;
   cudaStream_t s = (cudaStream_t)st;
   return x8 ? launch_gemv4<YK_E4M3>(a, s) : a.bf16 ? launch_gemv4<YK_BF16>(a, s) : launch_gemv4<YK_F16>(a, s);
 }
