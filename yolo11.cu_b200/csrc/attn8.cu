@@ -63,31 +63,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// B bytes into shared memory; without `ok`, zeros and no read.
-template <int B>
-__device__ __forceinline__ void cp_async_lane(uint32_t dst, const void* src, bool ok) {
-  if (B == 16) {
-    cp_async16(dst, src, ok ? 16 : 0);
-  } else {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
-  }
-}
-template <int B>
-__device__ __forceinline__ void cp_async_lane(uint32_t dst, const void* src) {
-  if (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-
 // o += p (16 rows x 16 tokens) * v for two subtiles: words v[u][j] hold 4 channels a word of the
 // lane's token j (of 2t, 2t + 1, 2t + 8, 2t + 9); bytes of a token pair interleave into the B operand.
 template <int W>
@@ -209,7 +184,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
   const auto load_q = [&](const Seg& s, int b) {
     for (int i = tid; i < 16 * D / 8; i += 32 * kDecWarps) {
       const int rr = s.tile * 16 + min(i / (D / 8), s.row_n - 1), tok = rr / G;
-      cp_async_lane<16>(smem_u32(q_sm) + b * L::kQBytes + i / (D / 8) * L::kQRow + i % (D / 8) * 16,
+      cp_async_at<16>(smem_u32(q_sm) + b * L::kQBytes + i / (D / 8) * L::kQRow + i % (D / 8) * 16,
                         (const uint16_t*)a.q + (long long)(s.q0 + tok) * a.q_row + (long long)(s.kh * G + rr - tok * G) * D + i % (D / 8) * 8);
     }
   };
@@ -255,18 +230,18 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
     if (left >= 16) {
 #pragma unroll
       for (int j = 0; j < 2 * L::kKC; j++)
-        cp_async_lane<16>(kd + j * 512, kp + 8 * (j / L::kKC) * D + (j % L::kKC) * 64);
+        cp_async_at<16>(kd + j * 512, kp + 8 * (j / L::kKC) * D + (j % L::kKC) * 64);
 #pragma unroll
       for (int j = 0; j < 4 * L::kVC; j++)
-        cp_async_lane<L::kVB>(vd + j * 32 * L::kVB, vp + ((j / L::kVC & 1) + 8 * (j / L::kVC >> 1)) * D + (j % L::kVC) * 128);
+        cp_async_at<L::kVB>(vd + j * 32 * L::kVB, vp + ((j / L::kVC & 1) + 8 * (j / L::kVC >> 1)) * D + (j % L::kVC) * 128);
     } else {
 #pragma unroll
       for (int j = 0; j < 2 * L::kKC; j++)
-        cp_async_lane<16>(kd + j * 512, kp + 8 * (j / L::kKC) * D + (j % L::kKC) * 64, 8 * (j / L::kKC) + g < left);
+        cp_async_at<16>(kd + j * 512, kp + 8 * (j / L::kKC) * D + (j % L::kKC) * 64, 8 * (j / L::kKC) + g < left);
 #pragma unroll
       for (int j = 0; j < 4 * L::kVC; j++) {
         const int tok = (j / L::kVC & 1) + 8 * (j / L::kVC >> 1);
-        cp_async_lane<L::kVB>(vd + j * 32 * L::kVB, vp + tok * D + (j % L::kVC) * 128, 2 * t + tok < left);
+        cp_async_at<L::kVB>(vd + j * 32 * L::kVB, vp + tok * D + (j % L::kVC) * 128, 2 * t + tok < left);
       }
     }
     fill += L::kStage;
@@ -294,7 +269,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
   cp_async_commit();
   open(cur);
   prologue();
-  uint32_t src = ring;
+  const uint8_t* const ring_p = dec_sm + warp * L::kWarpBytes;
+  const uint8_t* src = ring_p;
   cp_async_wait<L::kPairs - 1>();
   __syncthreads();                 // q is there
   for (int turn = 0;; turn ^= 1) {
@@ -392,7 +368,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
     int tok0 = s_first * 16, id_c = -1;
     float ks_c = 0.f, vs_c = 0.f;
 #pragma unroll 1
-    for (int i = 0; i < count; i += 2, tok0 += kDecGran, src = src + 2 * L::kStage == ring + L::kWarpBytes ? ring : src + 2 * L::kStage) {
+    for (int i = 0; i < count; i += 2, tok0 += kDecGran, src = src + 2 * L::kStage == ring_p + L::kWarpBytes ? ring_p : src + 2 * L::kStage) {
+      const uint8_t *src_k = src + lane * 16, *src_v = src + 2 * L::kKC * 512 + lane * L::kVB;
       issue_pair(i + 2 * (L::kPairs - 1));
       cp_async_wait<L::kPairs - 1>();
       if ((i & 31) == 0) { id_c = id_i; ks_c = ks_i; vs_c = vs_i; }   // issue() is in the same 32
@@ -407,7 +384,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-          for (int j = 0; j < 2; j++) kw[u][j] = lds128(src + u * L::kStage + (j * L::kKC + h) * 512 + lane * 16);
+          for (int j = 0; j < 2; j++) kw[u][j] = *(const uint4*)(src_k + u * L::kStage + (j * L::kKC + h) * 512);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           uint32_t qa[4];
@@ -500,12 +477,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
         for (int u = 0; u < 2; u++)
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            const uint32_t at = src + u * L::kStage + 2 * L::kKC * 512 + (j * L::kVC + h) * (32 * L::kVB) + lane * L::kVB;
+            const uint8_t* at = src_v + u * L::kStage + (j * L::kVC + h) * (32 * L::kVB);
             if (L::kVB == 16) {
-              const uint4 x = lds128(at);
+              const uint4 x = *(const uint4*)at;
               v[u][j][0] = x.x; v[u][j][1] = x.y; v[u][j][L::kVB / 4 - 2] = x.z; v[u][j][L::kVB / 4 - 1] = x.w;
             } else {
-              const uint2 x = lds64(at);
+              const uint2 x = *(const uint2*)at;
               v[u][j][0] = x.x; v[u][j][1] = x.y;
             }
           }
@@ -558,7 +535,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
     cp_async_wait<0>();            // the next q too
     if (more) {
       open(next);
-      fill = src = ring;
+      fill = ring;
+      src = ring_p;
       prologue();
     }
 

@@ -29,16 +29,22 @@ struct Gemv4Args {
 };
 constexpr int kGemvWarps = 8;
 
+// d = a * b + (first ? 0 : d)
 template <bool F16>
-__device__ __forceinline__ void mma_gemv(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_gemv(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  const float c0 = first ? 0.f : d[0], c1 = first ? 0.f : d[1], c2 = first ? 0.f : d[2], c3 = first ? 0.f : d[3];
   if (F16) {
-    mma16816(d, a, b0, b1);
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   } else {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "{%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   }
 }
 __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
@@ -77,22 +83,6 @@ __device__ __forceinline__ void codes8(uint32_t w, const Zero& z, uint32_t (&o)[
     for (int i = 0; i < 4; i++) o[i] = bsub2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u, z.a);
   }
 }
-__device__ __forceinline__ uint32_t lds_u8(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint16_t lds_u16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds_u32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-
 template <int NT, int R>
 struct Gemv {
   static constexpr int kStages = R == 1 ? 5 : 4;
@@ -121,6 +111,7 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
   const int K = p.k, chunks = (K + 127) / 128;
   const int count = n0 < p.n && chunks > wk ? (chunks - wk + WK - 1) / WK : 0;
   const uint32_t ring = smem_u32(sm) + warp * kStages * kStage;
+  const uint8_t* const ring_p = sm + warp * kStages * kStage;
 
   // first codes, scales and zero points of this lane's outputs g, g + 8 of each tile
   const uint8_t *wrow[R][2], *zrow[R][2];
@@ -145,7 +136,7 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
 #pragma unroll
       for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) cp_async16(fill + r * kTile + piece + h * 128, wrow[r][h] + c * 64, ok ? 16 : 0);
+        for (int h = 0; h < 2; h++) cp_async_at<16>(fill + piece + r * kTile + h * 128, wrow[r][h] + c * 64, ok);
       fill = fill + kStage == ring + kStages * kStage ? ring : fill + kStage;
     }
     cp_async_commit();
@@ -161,14 +152,15 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
 #pragma unroll
     for (int j = 0; j < NT; j++) tot[r][j][0] = tot[r][j][1] = tot[r][j][2] = tot[r][j][3] = 0.f;
 
-  // x of rows j * 8 + g: this lane's 8 columns of a block
+  // x of rows j * 8 + g (past the last row that row again: its sums are not written): this lane's
+  // 8 columns of a block
   constexpr int kSize = X8 ? 1 : 2;
   const uint8_t* xp[NT];
 #pragma unroll
   for (int j = 0; j < NT; j++)
     xp[j] = (const uint8_t*)p.x + ((long long)min(j * 8 + g, p.rows - 1) * p.x_row + t * 8) * kSize;
   const auto raw_x = [&](int j, int k, uint32_t (&v)[2 * kSize]) {     // columns k + 8 t ..
-    const bool ok = j * 8 + g < p.rows && k < K;
+    const bool ok = k < K;
     const uint8_t* x = xp[j] + k * kSize;
     if (ga.x_vec) {
       if (X8) {
@@ -224,7 +216,7 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
   };
   load_scales(0);
 
-  uint32_t src = ring;
+  const uint8_t* src = ring_p + g * 16 + t * 4;      // this lane's word of output g
   constexpr int kAhead = NT <= 2 ? 4 : 1;     // blocks of x read before they are used
 #pragma unroll 1
   for (int i = 0; i < count; i++) {
@@ -274,38 +266,41 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
       }
 #pragma unroll
       for (int r = 0; r < R; r++) {
-        const uint32_t at = src + r * kTile + b * S::kBlock + g * 16 + t * 4;
+        const uint8_t* at = src + r * kTile + b * S::kBlock;
         if (b % GB == 0) {
-#pragma unroll
-          for (int j = 0; j < NT; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0.f;
 #pragma unroll
           for (int h = 0; h < 2; h++)
             zp[r][h] = zero_of<F16>(zero ? __shfl_sync(~0u, zw[r][h], (lane & ~3) + b) : 8);
         }
         uint32_t q[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; h++) codes8<F16>(lds_u32(at + 128 * h), zp[r][h], q[h]);
+        for (int h = 0; h < 2; h++) codes8<F16>(*(const uint32_t*)(at + 128 * h), zp[r][h], q[h]);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const uint32_t a[4] = {q[0][2 * e], q[1][2 * e], q[0][2 * e + 1], q[1][2 * e + 1]};
 #pragma unroll
-          for (int j = 0; j < NT; j++) mma_gemv<F16>(acc[r][j], a, x[j][2 * e], x[j][2 * e + 1]);
+          for (int j = 0; j < NT; j++) mma_gemv<F16>(acc[r][j], a, x[j][2 * e], x[j][2 * e + 1], b % GB == 0 && e == 0);
         }
         if (b % GB == GB - 1) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             const float f = GB == 4 ? sw[r][h] : __shfl_sync(~0u, sw[r][h], (lane & ~3) + b);
 #pragma unroll
-            for (int j = 0; j < NT; j++)
-#pragma unroll
-              for (int e = 0; e < 2; e++)
-                tot[r][j][2 * h + e] = fmaf(acc[r][j][2 * h + e], X8 ? f * xs[j][e] : f, tot[r][j][2 * h + e]);
+            for (int j = 0; j < NT; j++) {
+              const float2 both = X8 ? ffma2(make_float2(f, f), make_float2(xs[j][0], xs[j][1]), make_float2(0.f, 0.f))
+                                     : make_float2(f, f);
+              const float2 v = ffma2(make_float2(acc[r][j][2 * h], acc[r][j][2 * h + 1]), both,
+                                     make_float2(tot[r][j][2 * h], tot[r][j][2 * h + 1]));
+              tot[r][j][2 * h] = v.x;
+              tot[r][j][2 * h + 1] = v.y;
+            }
           }
         }
       }
     }
     __syncwarp();                 // every lane has read the stage
-    src = src + kStage == ring + kStages * kStage ? ring : src + kStage;
+    src += kStage;
+    if (src >= ring_p + kStages * kStage) src -= kStages * kStage;
   }
   cp_async_wait<0>();
   __syncthreads();

@@ -85,6 +85,18 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// cp.async of B bytes (16 or 8); without `ok`, zeros and no read.
+template <int B>
+__device__ __forceinline__ void cp_async_at(uint32_t dst, const void* src, bool ok) {
+  if (B == 16) cp_async16(dst, src, ok ? 16 : 0);
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
+}
+template <int B>
+__device__ __forceinline__ void cp_async_at(uint32_t dst, const void* src) {
+  if (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+
 static inline int check_cache(const YkKvCache* c) {
   if (!c || !c->k || !c->v || !c->kscale || !c->vscale) return refuse(YK_EINVAL, "kv cache: null pointer");
   if (c->tokens != 16 && c->tokens != 32 && c->tokens != 64 && c->tokens != 128)
