@@ -13,13 +13,15 @@ struct PlanArgs {
   YkKvPlan p;
   int finish;   // write cu, kv_lens, counts and the free head (block 0)
   int rows_too; // write slots, pos and table
+  int vec;      // slots and pos allow 16-byte stores
 };
 
-__device__ __forceinline__ int plan_last_le(const int* a, int n, int v) {   // last i < n with a[i] <= v
+// The last i < n with a[i] <= v; a negative entry stands for its complement.
+__device__ __forceinline__ int plan_last_le(const int* a, int n, int v) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
-    const int m = (lo + hi) >> 1;
-    if (a[m] <= v) lo = m; else hi = m;
+    const int m = (lo + hi) >> 1, x = a[m];
+    if ((x < 0 ? ~x : x) <= v) lo = m; else hi = m;
   }
   return lo;
 }
@@ -58,9 +60,10 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
   __shared__ long long part[32];
   __shared__ int stat[3];
   const YkKvPlan& p = a.p;
-  const int R = p.requests, T = p.tokens;
-  int* cu = plan_sm;            // [R + 1] rows before each request, at most p.rows
-  int* boff = plan_sm + R + 1;  // [R + 1] blocks taken before each request
+  const int R = p.requests, T = p.tokens, shift = 31 - __clz(T);
+  int* cu = plan_sm;              // [R + 1] rows before each request, at most p.rows
+  int* boff = cu + R + 1;         // [R] blocks needed before each request, ~ of that where it is refused
+  int* past_sm = boff + R;        // [R]
   const int per = (R + blockDim.x - 1) / blockDim.x;
   const int r0 = min(R, (int)threadIdx.x * per), r1 = min(R, r0 + per);
   const int head = p.free_head ? max(0, min(*p.free_head, p.free_count)) : 0;
@@ -78,26 +81,29 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
     return (int)((end + T - 1) / T - ((long long)past + T - 1) / T);
   };
   long long blocks = 0;
+  const long long from0 = at;
   for (int r = r0; r < r1; r++) {
-    const int f = p.fresh[r];
+    const int f = p.fresh[r], past = p.past[r];
     cu[r] = (int)min(at, (long long)p.rows);
-    blocks += max(0, need_of(p.past[r], f, at));
+    past_sm[r] = past;
+    const int need = need_of(past, f, at);
+    boff[r] = need;
+    blocks += max(0, need);
     at += max(0, f);
   }
   if (threadIdx.x == 0) cu[R] = (int)min(total, (long long)p.rows);
   const long long all_rows = total;
   long long boffs = block_exclusive(blocks, part, &total);
-  long long from = at;
-  for (int r = r1 - 1; r >= r0; r--) from -= max(0, p.fresh[r]);
   int taken = 0, placed = 0, refused = 0;
+  at = from0;
   for (int r = r0; r < r1; r++) {
-    const int f = p.fresh[r], need = need_of(p.past[r], f, from);
-    boff[r] = (int)min(boffs, 0x7fffffffll);
+    const int need = boff[r];
     const bool ok = need == 0 || (need > 0 && boffs + need <= avail);
+    const int before = (int)min(boffs, 0x7fffffffll);
+    boff[r] = ok ? before : ~before;
     if (ok && need > 0) taken = (int)(boffs + need);
-    if (ok) placed += f; else refused++;
+    if (ok) placed += p.fresh[r]; else refused++;
     boffs += max(0, need);
-    from += max(0, f);
   }
   if (taken) atomicMax(&stat[0], taken);      // whole numbers: any order gives the same
   if (placed) atomicAdd(&stat[1], placed);
@@ -106,55 +112,58 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
   const int n_taken = stat[0], n_rows = cu[R];
 
   if (a.rows_too) {
-    const int warps = gridDim.x * (blockDim.x >> 5);
-    const int gw = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    // a warp takes 128 consecutive rows; a lane's request only moves forward
-    for (long long w0 = (long long)gw * 128; w0 < p.rows; w0 += (long long)warps * 128) {
-      int r = -1, held = 0, past = 0, start = 0, base = 0;
-      bool ok = false;
+    const int threads = gridDim.x * blockDim.x, me = blockIdx.x * blockDim.x + threadIdx.x;
+    // four consecutive rows a thread: mostly of one request and block, found once
+    for (long long w0 = (long long)me * 4; w0 < p.rows; w0 += (long long)threads * 4) {
+      int slot[4], pos[4];
+      int r = -1, end = 0, past = 0, start = 0, b_off = -1, held = 0, b_have = -1, id = -1;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int n = (int)min(w0 + i * 32 + lane, (long long)p.rows);
-        if (n >= p.rows) break;
-        int slot = -1, pos = -1;
-        if (n < n_rows) {
-          int q = r < 0 ? plan_last_le(cu, R, n) : r;
-          while (cu[q + 1] <= n) q++;
-          if (q != r) {
-            r = q;
-            past = p.past[r];
-            start = cu[r];
-            const int need = need_of(past, p.fresh[r], start);
-            base = boff[r];
-            ok = need == 0 || (need > 0 && (long long)base + need <= avail);
-            held = (int)(((long long)past + T - 1) / T);
-          }
-          if (past >= 0) pos = (int)min((long long)past + (n - start), 0x7fffffffll);
-          if (ok) {
-            const int b = pos / T;
-            const int id = b < held ? p.table[(long long)r * p.table_stride + b]
-                                    : p.free_blocks[head + base + (b - held)];
-            if ((unsigned)id < (unsigned)p.blocks) slot = id * T + (pos & (T - 1));
-          }
+        const int n = (int)w0 + i;
+        slot[i] = pos[i] = -1;
+        if (w0 + i >= n_rows) continue;
+        if (n >= end) {
+          if (r < 0) r = plan_last_le(cu, R, n);
+          while (cu[r + 1] <= n) r++;
+          past = past_sm[r];
+          start = cu[r];
+          end = cu[r + 1];
+          b_off = boff[r];
+          held = (int)(((long long)past + T - 1) >> shift);
+          b_have = -1;
         }
-        p.slots[n] = slot;
-        if (p.pos) p.pos[n] = pos;
+        if (past >= 0) pos[i] = (int)min((long long)past + (n - start), 0x7fffffffll);
+        if (b_off < 0) continue;
+        const int b = pos[i] >> shift;
+        if (b != b_have) {
+          id = b < held ? p.table[(long long)r * p.table_stride + b] : p.free_blocks[head + b_off + (b - held)];
+          b_have = b;
+        }
+        if ((unsigned)id < (unsigned)p.blocks) slot[i] = id * T + (pos[i] & (T - 1));
+      }
+      if (a.vec && w0 + 4 <= p.rows) {
+        *(int4*)(p.slots + w0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        if (p.pos) *(int4*)(p.pos + w0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (w0 + i < p.rows) {
+            p.slots[w0 + i] = slot[i];
+            if (p.pos) p.pos[w0 + i] = pos[i];
+          }
       }
     }
-    const int threads = gridDim.x * blockDim.x;
-    for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < n_taken; e += threads) {
-      const int r = plan_last_le(boff, R, (int)e);
-      const int held = (int)(((long long)p.past[r] + T - 1) / T);
+    for (long long e = me; e < n_taken; e += threads) {
+      const int r = plan_last_le(boff, R, (int)e);      // the last that starts there: not refused
+      const int held = (int)(((long long)past_sm[r] + T - 1) >> shift);
       p.table[(long long)r * p.table_stride + held + (e - boff[r])] = p.free_blocks[head + e];
     }
   }
   if (!a.finish || blockIdx.x) return;
-  __syncthreads();   // kv_lens may be past: every read above comes first
-  for (int r = threadIdx.x; r < R; r += blockDim.x) {
-    const int past = p.past[r], f = p.fresh[r];
-    const int need = need_of(past, f, cu[r]);
-    const bool ok = need == 0 || (need > 0 && (long long)boff[r] + need <= avail);
-    p.kv_lens[r] = ok ? past + f : past;
+  // kv_lens may be past: each request's length is read before, by this thread
+  for (int r = r0; r < r1; r++) {
+    const int f = p.fresh[r];
+    p.kv_lens[r] = boff[r] >= 0 ? past_sm[r] + f : past_sm[r];
     p.cu[r] = cu[r];
   }
   if (threadIdx.x == 0) {
@@ -170,11 +179,12 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
 }
 
 // ---------------- append ----------------
-// A unit is the part of a block that the call fills: a run of rows with consecutive slots in one
-// block.  Its items are (key or value, head).  The rows of a run share its items out among
-// them, row j of n taking items j, j + n, ..., so one rule covers a decode step (runs of one row:
-// each row's block of threads does all heads, a warp an item) and a prompt (runs of a whole
-// block: one item a row, all threads together).
+// HBM bound.  A unit is the part of a block that the call fills: a run of rows with consecutive
+// slots in one block.  The rows of a run share its heads out among them, row j of n taking heads
+// j * heads / n .. (j + 1) * heads / n - 1, so one rule covers a decode step (runs of one row: the
+// row's CTA does all heads, a warp each) and a prompt (runs of a whole block: at most one head a row,
+// the CTA's threads together).  Keys and values of a head go together: twice the bytes under way for
+// the same two waits (maximum, scale).
 constexpr int kAppendThreads = 256;
 
 struct AppendArgs {
@@ -192,99 +202,110 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __int_as_float((k + 127) << 23);
 }
 
-// Item (head, key or value) of the run of n rows from row `first` on, whose tokens start at
-// `off` in their block, done by `size` threads of which this is number `id` (a warp, or the
-// whole CTA: then `red` is the shared reduction buffer).  The x chunks that fit stay in
-// registers between the maximum and the rounding; the rest is read again (from L2).
-template <bool BF16, bool WHOLE>
-__device__ __forceinline__ void append_item(const AppendArgs& a, int item, int first, int n, int slot,
-                                            int id, float* red) {
-  constexpr int kKeep = 8;
-  const int size = WHOLE ? kAppendThreads : 32;
-  const int T = a.c.tokens, D = a.c.dim, parts = D / 8;
-  const int h = item >> 1, second = item & 1;
+// Head h of the run of n rows from row `first` on, whose tokens start at slot `slot`, done by a warp
+// or the whole CTA (WHOLE; `red` is its reduction buffer); `id` is the thread's number among them.
+// The first KEEP chunks a thread stay in registers between the maximum and the rounding; the rest
+// is read again (from L2).
+template <bool BF16, bool WHOLE, int KEEP>
+__device__ __forceinline__ void append_head(const AppendArgs& a, int h, int first, int n, int slot, int id,
+                                            float (*red)[kAppendThreads / 32]) {
+  constexpr int size = WHOLE ? kAppendThreads : 32;
+  const int T = a.c.tokens, D = a.c.dim, shift = 31 - __clz(D / 8);    // D / 8 chunks a row: a power of two
   const int block = slot / T, off = slot & (T - 1);
-  const uint16_t* x = (const uint16_t*)(second ? a.x.v : a.x.k) +
-                      (long long)h * (second ? a.x.v_head : a.x.k_head);
-  const long long row = second ? a.x.v_row : a.x.k_row;
-  uint8_t* codes = (uint8_t*)(second ? a.c.v : a.c.k) + block * a.c.block_stride + (long long)h * T * D;
-  float* scale = (second ? a.c.vscale : a.c.kscale) + block * a.c.scale_stride + h;
-  const int chunks = n * parts;
-  const float before = off ? *scale : 0.f;
-  const auto load = [&](int c) -> uint4 {
-    const int j = c / parts;
-    return *(const uint4*)(x + (first + j) * row + (c - j * parts) * 8);
+  const int chunks = n << shift;
+  const uint16_t* x[2] = {(const uint16_t*)a.x.k + h * a.x.k_head, (const uint16_t*)a.x.v + h * a.x.v_head};
+  const long long row[2] = {a.x.k_row, a.x.v_row};
+  uint8_t* codes[2] = {(uint8_t*)a.c.k + block * a.c.block_stride + (long long)h * T * D,
+                       (uint8_t*)a.c.v + block * a.c.block_stride + (long long)h * T * D};
+  float* scale[2] = {a.c.kscale + block * a.c.scale_stride + h, a.c.vscale + block * a.c.scale_stride + h};
+  const auto load = [&](int kv, int c) -> uint4 {
+    return *(const uint4*)(x[kv] + (first + (c >> shift)) * row[kv] + (c & ((1 << shift) - 1)) * 8);
   };
-  uint4 keep[kKeep];
-  float m = 0.f;
+  uint4 keep[2][KEEP];
+  float before[2], m[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < kKeep; i++) {
-    const int c = i * size + id;
-    keep[i] = c < chunks ? load(c) : make_uint4(0, 0, 0, 0);
+  for (int kv = 0; kv < 2; kv++) {
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) {
+      const int c = i * size + id;
+      keep[kv][i] = c < chunks ? load(kv, c) : make_uint4(0, 0, 0, 0);
+    }
+    before[kv] = off ? *scale[kv] : 0.f;
   }
-  const auto amax8 = [&](const uint4& v) {
+  const auto amax8 = [&](const uint4& v, float m) {
     const uint32_t* u = (const uint32_t*)&v;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const float2 f = pair_to_float2<BF16>(u[e]);
       m = fmaxf(m, fmaxf(finite_abs(f.x), finite_abs(f.y)));
     }
+    return m;
   };
 #pragma unroll
-  for (int i = 0; i < kKeep; i++) amax8(keep[i]);
-  for (int c = kKeep * size + id; c < chunks; c += size) amax8(load(c));
-  m = warp_max(m);
-  if (WHOLE) {
-    if ((id & 31) == 0) red[id >> 5] = m;
-    __syncthreads();
-    m = red[0];
+  for (int kv = 0; kv < 2; kv++) {
 #pragma unroll
-    for (int i = 1; i < kAppendThreads / 32; i++) m = fmaxf(m, red[i]);
+    for (int i = 0; i < KEEP; i++) m[kv] = amax8(keep[kv][i], m[kv]);
+    for (int c = KEEP * size + id; c < chunks; c += size) m[kv] = amax8(load(kv, c), m[kv]);
+    m[kv] = warp_max(m[kv]);
+  }
+  if (WHOLE) {
+    if ((id & 31) == 0) {
+      red[0][id >> 5] = m[0];
+      red[1][id >> 5] = m[1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kv = 0; kv < 2; kv++)
+#pragma unroll
+      for (int i = 0; i < kAppendThreads / 32; i++) m[kv] = fmaxf(m[kv], red[kv][i]);
     __syncthreads();   // every thread has read red and `before`
   } else {
     __syncwarp();
   }
-  const float s = fmaxf(pow2_scale(m), before), inv = 1.f / s;
-  const auto store = [&](int c, const uint4& v) {
-    const uint32_t* u = (const uint32_t*)&v;
-    float2 f[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) f[e] = pair_to_float2<BF16>(u[e]);
-    uint2 q;
-    q.x = float4_to_e4m3x4(f[0].x * inv, f[0].y * inv, f[1].x * inv, f[1].y * inv);
-    q.y = float4_to_e4m3x4(f[2].x * inv, f[2].y * inv, f[3].x * inv, f[3].y * inv);
-    *(uint2*)(codes + (long long)off * D + c * 8) = q;
-  };
+  for (int kv = 0; kv < 2; kv++) {
+    const float s = fmaxf(pow2_scale(m[kv]), before[kv]), inv = 1.f / s;
+    const auto store = [&](int c, const uint4& v) {
+      const uint32_t* u = (const uint32_t*)&v;
+      float2 f[4];
 #pragma unroll
-  for (int i = 0; i < kKeep; i++) {
-    const int c = i * size + id;
-    if (c < chunks) store(c, keep[i]);
-  }
-  for (int c = kKeep * size + id; c < chunks; c += size) store(c, load(c));
-  if (off && s > before) {   // the scale grew: the earlier tokens take the new one
-    const float ratio = before / s;
-    for (int c = id; c < off * D / 16; c += size) {
-      uint4 v = *(const uint4*)(codes + c * 16);
-      uint32_t* u = (uint32_t*)&v;
+      for (int e = 0; e < 4; e++) f[e] = pair_to_float2<BF16>(u[e]);
+      uint2 q;
+      q.x = float4_to_e4m3x4(f[0].x * inv, f[0].y * inv, f[1].x * inv, f[1].y * inv);
+      q.y = float4_to_e4m3x4(f[2].x * inv, f[2].y * inv, f[3].x * inv, f[3].y * inv);
+      *(uint2*)(codes[kv] + off * D + c * 8) = q;
+    };
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float2 lo = e4m3x2_to_float2(u[e]), hi = e4m3x2_to_float2(u[e] >> 16);
-        u[e] = float4_to_e4m3x4(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
-      }
-      *(uint4*)(codes + c * 16) = v;
+    for (int i = 0; i < KEEP; i++) {
+      const int c = i * size + id;
+      if (c < chunks) store(c, keep[kv][i]);
     }
+    for (int c = KEEP * size + id; c < chunks; c += size) store(c, load(kv, c));
+    if (off && s > before[kv]) {   // the scale grew: the earlier tokens take the new one
+      const float ratio = before[kv] / s;
+      for (int c = id; c < off * D / 16; c += size) {
+        uint4 v = *(const uint4*)(codes[kv] + c * 16);
+        uint32_t* u = (uint32_t*)&v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float2 lo = e4m3x2_to_float2(u[e]), hi = e4m3x2_to_float2(u[e] >> 16);
+          u[e] = float4_to_e4m3x4(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
+        }
+        *(uint4*)(codes[kv] + c * 16) = v;
+      }
+    }
+    if (id == 0) *scale[kv] = s;
   }
-  if (id == 0) *scale = s;
 }
 
 template <bool BF16>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float red[kAppendThreads / 32];
+  __shared__ float red[2][kAppendThreads / 32];
   __shared__ int sl[3 * 128];        // slots of the window and one block's tokens to either side
   __shared__ uint32_t follows[12];   // bit i: row lo + i is the next token of row lo + i - 1's run
-  const int T = a.c.tokens, items = 2 * a.c.heads;
+  const int T = a.c.tokens, heads = a.c.heads;
   const int w0 = blockIdx.x * a.window, w1 = min(a.x.rows, w0 + a.window);
   const int lo = max(0, w0 - T), hi = min(a.x.rows, w1 + T);
   for (int i = threadIdx.x; i < 3 * 128; i += blockDim.x) {
@@ -311,7 +332,6 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
       if (got <= (j & 31)) break;
       j -= got;
     }
-    if (back >= items) continue;       // enough rows before this one share the items
     for (int j = i + 1; j < 3 * 128;) {   // and from i + 1 up
       const uint32_t w = ~(follows[j >> 5] >> (j & 31));
       const int got = min(w ? __ffs(w) - 1 : 32, 32 - (j & 31));
@@ -320,12 +340,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
       j += got;
     }
     const int n = back + ahead + 1, first = lo + i - back;
+    const int h0 = back * heads / n, h1 = (back + 1) * heads / n;
     if (n * (a.c.dim / 8) <= 64) {
-      for (int it = back + warp * n; it < items; it += n * (kAppendThreads / 32))
-        append_item<BF16, false>(a, it, first, n, s - back, threadIdx.x & 31, red);
+      for (int h = h0 + warp; h < h1; h += kAppendThreads / 32)
+        append_head<BF16, false, 2>(a, h, first, n, s - back, threadIdx.x & 31, red);
     } else {
-      for (int it = back; it < items; it += n)
-        append_item<BF16, true>(a, it, first, n, s - back, threadIdx.x, red);
+      for (int h = h0; h < h1; h++) append_head<BF16, true, 4>(a, h, first, n, s - back, threadIdx.x, red);
     }
   }
 }
@@ -345,19 +365,20 @@ extern "C" int yk_kv_plan(const YkKvPlan* p, yk_stream_t st) {
   if ((long long)p->blocks * p->tokens > 0x7fffffffll)
     return refuse(YK_EINVAL, "kv_plan: blocks * tokens must be below 2^31");
   if (p->requests > 16384) return refuse(YK_EUNSUP, "kv_plan: at most 16384 requests");
-  const size_t smem = (2 * (size_t)p->requests + 2) * sizeof(int);
+  const size_t smem = (3 * (size_t)p->requests + 1) * sizeof(int);
   if (smem_attr(kv_plan_kernel, (int)smem) != cudaSuccess) return check_launch("kv_plan attr");
-  const int threads = std::min(1024, std::max(128, (std::max(p->requests, p->rows) + 31) / 32 * 32));
-  const int grid = (int)std::max(1ll, std::min(148ll, ((long long)p->rows + 4095) / 4096));
+  const int threads = std::min(1024, std::max(64, (int)((std::max<long long>(p->requests, (p->rows + 3ll) / 4) + 31) / 32 * 32)));
+  const int grid = (int)std::max(1ll, std::min(2 * 148ll, ((long long)p->rows + 4095) / 4096));
   // With several CTAs, outputs that are inputs too (the free head, kv_lens over past) wait for a
   // launch of their own, so that no CTA reads them after they moved.
   const bool inplace = p->free_head || (p->kv_lens < p->past + p->requests && p->past < p->kv_lens + p->requests);
   const bool two = grid > 1 && inplace;
-  PlanArgs a{*p, two ? 0 : 1, 1};
+  const int vec = aligned16(p->slots) && aligned16(p->pos);
+  PlanArgs a{*p, two ? 0 : 1, 1, vec};
   launch_k(kv_plan_kernel, grid, threads, smem, (cudaStream_t)st, a);
   note_launch();
   if (two) {
-    PlanArgs b{*p, 1, 0};
+    PlanArgs b{*p, 1, 0, vec};
     launch_k(kv_plan_kernel, 1, threads, smem, (cudaStream_t)st, b);
     note_launch();
   }
@@ -373,9 +394,9 @@ extern "C" int yk_kv_append(const YkKvCache* c, const YkKvRows* x, yk_stream_t s
   if (!aligned16(x->k) || !aligned16(x->v) || x->k_row % 8 || x->v_row % 8 || x->k_head % 8 || x->v_head % 8)
     return refuse(YK_EINVAL, "kv_append: rows need 16-byte alignment and strides that are multiples of 8");
   if (x->rows == 0) return YK_OK;
-  // about eight CTAs an SM, each of at most one block's rows
+  // rows of a CTA: as many as share one head of a full block, while that leaves two CTAs an SM
   int window = 1;
-  while (window < c->tokens && x->rows / (2 * window) >= 148 * 8) window *= 2;
+  while (window * 2 * c->heads <= c->tokens && x->rows / (2 * window) >= 148 * 2) window *= 2;
   AppendArgs a{*c, *x, window};
   const int grid = (x->rows + window - 1) / window;
   if (x->dtype == YK_BF16) launch_k(kv_append_kernel<true>, grid, kAppendThreads, 0, (cudaStream_t)st, a);

@@ -3,8 +3,111 @@
 
 namespace yk {
 
-// One CTA a row, the row in shared memory as fp32 between the three passes over it (sum of
-// squares, group maxima, rounding): each element is read from and written to HBM once.
+// HBM bound: x and add are read once and every output written once; the row stays in registers
+// between the three passes over it (mean square, group maxima, rounding).
+//
+// rmsnorm8_vec_kernel: rows that allow 16-byte accesses.  A thread holds V chunks of 8 columns, chunk
+// tid + i * threads, so that a group of 8 * 2^i columns (16 .. 256) lies in neighbouring lanes and its
+// maximum takes shuffles only; one scale a row takes one block reduction.  ROWS rows share a block
+// (a warp each) when a row is short.
+template <bool BF16, int V, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : 512) rmsnorm8_vec_kernel(const __grid_constant__ YkRmsNorm8 p, int lanes) {
+  __shared__ float part[2][16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = WARP ? 1 : blockDim.x >> 5;
+  const int id = WARP ? lane : threadIdx.x, size = WARP ? 32 : blockDim.x;
+  const int chunks = p.cols / 8;
+  const long long r = WARP ? (long long)blockIdx.x * 4 + warp : blockIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  if (WARP && r >= p.rows) return;
+  const uint4* x = (const uint4*)((const uint16_t*)p.x + r * p.x_row);
+  const uint4* add = p.add ? (const uint4*)((const uint16_t*)p.add + r * p.add_row) : nullptr;
+  uint4 xv[V], av[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int c = id + i * size;
+    xv[i] = c < chunks ? __ldcs(x + c) : make_uint4(0, 0, 0, 0);
+    if (add) av[i] = c < chunks ? __ldcs(add + c) : make_uint4(0, 0, 0, 0);
+  }
+  uint4 wv[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) wv[i] = id + i * size < chunks ? ((const uint4*)p.weight)[id + i * size] : make_uint4(0, 0, 0, 0);
+  float h[V][8];
+  const float over_c = 1.f / (float)p.cols;
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const uint32_t *xu = (const uint32_t*)&xv[i], *au = (const uint32_t*)&av[i];
+    uint4 o;
+    uint32_t* ou = (uint32_t*)&o;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      float2 f = pair_to_float2<BF16>(xu[e]);
+      if (add) {
+        const float2 g = pair_to_float2<BF16>(au[e]);
+        f.x += g.x;
+        f.y += g.y;
+      }
+      h[i][2 * e] = f.x;
+      h[i][2 * e + 1] = f.y;
+      ou[e] = float2_to_pair<BF16>(f.x, f.y);
+      ss = fmaf(f.x, f.x * over_c, ss);   // the mean itself: the sum would overflow sooner
+      ss = fmaf(f.y, f.y * over_c, ss);
+    }
+    if (p.sum && id + i * size < chunks) ((uint4*)((uint16_t*)p.sum + r * p.sum_row))[id + i * size] = o;
+  }
+  ss = warp_sum(ss);
+  if (!WARP) {
+    if (lane == 0) part[0][warp] = ss;
+    __syncthreads();
+    ss = part[0][0];
+    for (int i = 1; i < warps; i++) ss += part[0][i];
+  }
+  const float inv = rsqrtf(ss + p.eps);
+  float amax[V], row_max = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const uint32_t* wu = (const uint32_t*)&wv[i];
+    uint4 o;
+    uint32_t* ou = (uint32_t*)&o;
+    amax[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float2 w = pair_to_float2<BF16>(wu[e]);
+      h[i][2 * e] *= inv * w.x;
+      h[i][2 * e + 1] *= inv * w.y;
+      ou[e] = float2_to_pair<BF16>(h[i][2 * e], h[i][2 * e + 1]);
+      amax[i] = fmaxf(amax[i], fmaxf(finite_abs(h[i][2 * e]), finite_abs(h[i][2 * e + 1])));
+    }
+    if (id + i * size >= chunks) amax[i] = 0.f;
+    else if (p.out) ((uint4*)((uint16_t*)p.out + r * p.out_row))[id + i * size] = o;
+    row_max = fmaxf(row_max, amax[i]);
+  }
+  if (!p.codes) return;
+  if (lanes == 0) {                       // one scale a row
+    row_max = warp_max(row_max);
+    if (!WARP) {
+      if (lane == 0) part[1][warp] = row_max;
+      __syncthreads();
+      row_max = part[1][0];
+      for (int i = 1; i < warps; i++) row_max = fmaxf(row_max, part[1][i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int c = id + i * size;
+    float m = lanes ? amax[i] : row_max;
+    for (int o = lanes >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const float s = fmaxf(m / kE4m3Max, kMinScale), up = 1.f / s;
+    if (c >= chunks) continue;
+    if (lanes ? c % lanes == 0 : c == 0) p.scales[r * p.scales_row + (lanes ? c / lanes : 0)] = s;
+    ((uint2*)((uint8_t*)p.codes + r * p.codes_row))[c] =
+        make_uint2(float4_to_e4m3x4(h[i][0] * up, h[i][1] * up, h[i][2] * up, h[i][3] * up),
+                   float4_to_e4m3x4(h[i][4] * up, h[i][5] * up, h[i][6] * up, h[i][7] * up));
+  }
+}
+
+// Any other columns, strides, alignment and groups: one CTA a row, the row in shared memory.
 template <bool BF16>
 __global__ void rmsnorm8_kernel(const __grid_constant__ YkRmsNorm8 p, int group, int groups) {
   pdl_wait();
@@ -75,11 +178,34 @@ extern "C" int yk_rmsnorm8(const YkRmsNorm8* p, yk_stream_t st) {
       (p->out && p->out_row < p->cols) || (p->codes && (p->codes_row < p->cols || p->scales_row < groups)))
     return refuse(YK_EINVAL, "rmsnorm8: an output's row stride is below its row, or an input's is negative");
   if (p->rows == 0) return YK_OK;
+  const bool bf = p->dtype == YK_BF16;
+  cudaStream_t s = (cudaStream_t)st;
+  const auto vec = [](const void* q, long long row) { return !q || (aligned16(q) && row % 8 == 0); };
+  int lanes = 0;                            // lanes of a group, 0: one scale a row
+  bool fits = p->cols % 8 == 0 && vec(p->x, p->x_row) && vec(p->add, p->add_row) && vec(p->sum, p->sum_row) &&
+              vec(p->out, p->out_row) && vec(p->weight, 0) && ((uintptr_t)p->codes | (uintptr_t)p->codes_row) % 8 == 0;
+  if (p->codes && groups > 1) {
+    lanes = group / 8;
+    fits = fits && group % 8 == 0 && lanes <= 32 && !(lanes & (lanes - 1));
+  }
+  if (fits) {
+    // a warp a row while its chunks are at most two a lane; else four chunks a thread (eight from
+    // 16384 columns on): fewer threads leave more rows in flight on an SM
+    const int chunks = p->cols / 8;
+    if (chunks <= 64)
+      launch_k(bf ? rmsnorm8_vec_kernel<true, 2, true> : rmsnorm8_vec_kernel<false, 2, true>, (unsigned)((p->rows + 3ll) / 4), 128, 0, s, *p, lanes);
+    else if (chunks <= 2048)
+      launch_k(bf ? rmsnorm8_vec_kernel<true, 4, false> : rmsnorm8_vec_kernel<false, 4, false>, p->rows, (chunks + 127) / 128 * 32, 0, s, *p, lanes);
+    else
+      launch_k(bf ? rmsnorm8_vec_kernel<true, 8, false> : rmsnorm8_vec_kernel<false, 8, false>, p->rows, 512, 0, s, *p, lanes);
+    note_launch();
+    return check_launch("rmsnorm8");
+  }
   const size_t smem = ((size_t)p->cols + groups) * sizeof(float);
   const int threads = p->cols <= 1024 ? 128 : p->cols <= 4096 ? 256 : 512;
-  const auto kern = p->dtype == YK_BF16 ? rmsnorm8_kernel<true> : rmsnorm8_kernel<false>;
+  const auto kern = bf ? rmsnorm8_kernel<true> : rmsnorm8_kernel<false>;
   if (smem_attr(kern, (int)smem) != cudaSuccess) return check_launch("rmsnorm8 attr");
-  launch_k(kern, p->rows, threads, smem, (cudaStream_t)st, *p, group, groups);
+  launch_k(kern, p->rows, threads, smem, s, *p, group, groups);
   note_launch();
   return check_launch("rmsnorm8");
 }
