@@ -195,11 +195,9 @@ struct AppendArgs {
 
 // The smallest power of two s >= 2^-126 with 448 * s >= amax (448 = 1.75 * 2^8).
 __device__ __forceinline__ float pow2_scale(float amax) {
-  if (!(amax > 0.f)) return kMinScale;
-  int e;
-  const float f = frexpf(amax, &e);   // amax = f * 2^e, f in [0.5, 1)
-  const int k = max(e - 9 + (f > 0.875f), -126);
-  return __int_as_float((k + 127) << 23);
+  const uint32_t u = __float_as_uint(amax);          // 1.f * 2^e: 2^(e - 8), twice that where 1.f > 1.75
+  const int k = (int)(u >> 23) - 8 + ((u & 0x7fffff) > 0x600000);
+  return __uint_as_float((uint32_t)max(k, 1) << 23);
 }
 
 // Head h of the run of n rows from row `first` on, whose tokens start at slot `slot`, done by a warp
@@ -211,7 +209,7 @@ __device__ __forceinline__ void append_head(const AppendArgs& a, int h, int firs
                                             float (*red)[kAppendThreads / 32]) {
   constexpr int size = WHOLE ? kAppendThreads : 32;
   const int T = a.c.tokens, D = a.c.dim, shift = 31 - __clz(D / 8);    // D / 8 chunks a row: a power of two
-  const int block = slot / T, off = slot & (T - 1);
+  const int block = slot >> (31 - __clz(T)), off = slot & (T - 1);
   const int chunks = n << shift;
   const uint16_t* x[2] = {(const uint16_t*)a.x.k + h * a.x.k_head, (const uint16_t*)a.x.v + h * a.x.v_head};
   const long long row[2] = {a.x.k_row, a.x.v_row};
@@ -222,7 +220,7 @@ __device__ __forceinline__ void append_head(const AppendArgs& a, int h, int firs
     return *(const uint4*)(x[kv] + (first + (c >> shift)) * row[kv] + (c & ((1 << shift) - 1)) * 8);
   };
   uint4 keep[2][KEEP];
-  float before[2], m[2] = {0.f, 0.f};
+  float before[2], m[2];
 #pragma unroll
   for (int kv = 0; kv < 2; kv++) {
 #pragma unroll
@@ -232,48 +230,65 @@ __device__ __forceinline__ void append_head(const AppendArgs& a, int h, int firs
     }
     before[kv] = off ? *scale[kv] : 0.f;
   }
-  const auto amax8 = [&](const uint4& v, float m) {
-    const uint32_t* u = (const uint32_t*)&v;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float2 f = pair_to_float2<BF16>(u[e]);
-      m = fmaxf(m, fmaxf(finite_abs(f.x), finite_abs(f.y)));
+  for (int kv = 0; kv < 2; kv++) {
+    uint32_t m2 = 0;
+    const auto amax8 = [&](const uint4& v) {
+      m2 = amax_pair<BF16>(amax_pair<BF16>(m2, v.x), v.y);
+      m2 = amax_pair<BF16>(amax_pair<BF16>(m2, v.z), v.w);
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) amax8(keep[kv][i]);
+    for (int c = KEEP * size + id; c < chunks; c += size) amax8(load(kv, c));
+    const float2 f = pair_to_float2<BF16>(m2);
+    m[kv] = warp_max(fmaxf(f.x, f.y));
+  }
+  const auto meet = [&] {              // the warps' maxima
+    if (WHOLE) {
+      if ((id & 31) == 0) {
+        red[0][id >> 5] = m[0];
+        red[1][id >> 5] = m[1];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int kv = 0; kv < 2; kv++)
+#pragma unroll
+        for (int i = 0; i < kAppendThreads / 32; i++) m[kv] = fmaxf(m[kv], red[kv][i]);
+      __syncthreads();   // every thread has read red and `before`
+    } else {
+      __syncwarp();
     }
-    return m;
   };
+  meet();
+  if (m[0] == INFINITY || m[1] == INFINITY) {       // again, without the infinities
+#pragma unroll 1
+    for (int kv = 0; kv < 2; kv++) {
+      float top = 0.f;
+      for (int c = id; c < chunks; c += size) {
+        const uint4 v = load(kv, c);
+        const uint32_t* u = (const uint32_t*)&v;
 #pragma unroll
-  for (int kv = 0; kv < 2; kv++) {
-#pragma unroll
-    for (int i = 0; i < KEEP; i++) m[kv] = amax8(keep[kv][i], m[kv]);
-    for (int c = KEEP * size + id; c < chunks; c += size) m[kv] = amax8(load(kv, c), m[kv]);
-    m[kv] = warp_max(m[kv]);
-  }
-  if (WHOLE) {
-    if ((id & 31) == 0) {
-      red[0][id >> 5] = m[0];
-      red[1][id >> 5] = m[1];
+        for (int e = 0; e < 4; e++) {
+          const float2 f = pair_to_float2<BF16>(u[e]);
+          top = fmaxf(top, fmaxf(finite_abs(f.x), finite_abs(f.y)));
+        }
+      }
+      m[kv] = warp_max(top);
     }
-    __syncthreads();
-#pragma unroll
-    for (int kv = 0; kv < 2; kv++)
-#pragma unroll
-      for (int i = 0; i < kAppendThreads / 32; i++) m[kv] = fmaxf(m[kv], red[kv][i]);
-    __syncthreads();   // every thread has read red and `before`
-  } else {
-    __syncwarp();
+    meet();
   }
 #pragma unroll
   for (int kv = 0; kv < 2; kv++) {
-    const float s = fmaxf(pow2_scale(m[kv]), before[kv]), inv = 1.f / s;
+    const float s = fmaxf(pow2_scale(m[kv]), before[kv]);
+    const uint32_t bits = __float_as_uint(s);       // a power of two, unless `before` was not
+    const float inv = bits & 0x7fffff ? 1.f / s : __uint_as_float(0x7f000000u - bits);
     const auto store = [&](int c, const uint4& v) {
       const uint32_t* u = (const uint32_t*)&v;
       float2 f[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) f[e] = pair_to_float2<BF16>(u[e]);
-      uint2 q;
-      q.x = float4_to_e4m3x4(f[0].x * inv, f[0].y * inv, f[1].x * inv, f[1].y * inv);
-      q.y = float4_to_e4m3x4(f[2].x * inv, f[2].y * inv, f[3].x * inv, f[3].y * inv);
-      *(uint2*)(codes[kv] + off * D + c * 8) = q;
+      for (int e = 0; e < 4; e++) f[e] = mul2(pair_to_float2<BF16>(u[e]), make_float2(inv, inv));
+      *(uint2*)(codes[kv] + off * D + c * 8) = make_uint2(float4_to_e4m3x4(f[0].x, f[0].y, f[1].x, f[1].y),
+                                                          float4_to_e4m3x4(f[2].x, f[2].y, f[3].x, f[3].y));
     };
 #pragma unroll
     for (int i = 0; i < KEEP; i++) {
@@ -304,6 +319,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
   pdl_trigger();
   __shared__ float red[2][kAppendThreads / 32];
   __shared__ int sl[3 * 128];        // slots of the window and one block's tokens to either side
+  __shared__ int4 job[128];
   __shared__ uint32_t follows[12];   // bit i: row lo + i is the next token of row lo + i - 1's run
   const int T = a.c.tokens, heads = a.c.heads;
   const int w0 = blockIdx.x * a.window, w1 = min(a.x.rows, w0 + a.window);
@@ -319,11 +335,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
     if ((i & 31) == 0) follows[i >> 5] = bits;
   }
   __syncthreads();
-  const int warp = threadIdx.x >> 5;
-  for (int i = w0 - lo; i < w1 - lo; i++) {
-    const int s = sl[i];
-    if (s < 0) continue;
-    // rows of the run before and after row i (the same for every thread)
+  // each row of the window by a thread: rows of its run before it, rows of the run, its heads
+  const int rows = w1 - w0;
+  for (int j0 = threadIdx.x; j0 < rows; j0 += blockDim.x) {
+    const int i = w0 - lo + j0;
     int back = 0, ahead = 0;
     for (int j = i; j >= 0;) {         // consecutive set bits from i down
       const int ones = __clz(~(follows[j >> 5] << (31 - (j & 31))));
@@ -339,13 +354,21 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
       if (got < 32 - (j & 31)) break;
       j += got;
     }
-    const int n = back + ahead + 1, first = lo + i - back;
-    const int h0 = back * heads / n, h1 = (back + 1) * heads / n;
-    if (n * (a.c.dim / 8) <= 64) {
-      for (int h = h0 + warp; h < h1; h += kAppendThreads / 32)
-        append_head<BF16, false, 2>(a, h, first, n, s - back, threadIdx.x & 31, red);
+    const int n = back + ahead + 1;
+    const bool there = sl[i] >= 0;
+    job[j0] = make_int4(back, n, there ? back * heads / n : 0, there ? (back + 1) * heads / n : 0);
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5;
+  for (int j = 0; j < rows; j++) {
+    const int4 w = job[j];             // the same for every thread
+    if (w.z >= w.w) continue;
+    const int first = w0 + j - w.x, slot = sl[w0 - lo + j] - w.x;
+    if (w.y * (a.c.dim / 8) <= 64) {
+      for (int h = w.z + warp; h < w.w; h += kAppendThreads / 32)
+        append_head<BF16, false, 2>(a, h, first, w.y, slot, threadIdx.x & 31, red);
     } else {
-      for (int h = h0; h < h1; h++) append_head<BF16, true, 4>(a, h, first, n, s - back, threadIdx.x, red);
+      for (int h = w.z; h < w.w; h++) append_head<BF16, true, 4>(a, h, first, w.y, slot, threadIdx.x, red);
     }
   }
 }

@@ -11,7 +11,7 @@ namespace yk {
 // maximum takes shuffles only; one scale a row takes one block reduction.  ROWS rows share a block
 // (a warp each) when a row is short.
 template <bool BF16, int V, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 512) rmsnorm8_vec_kernel(const __grid_constant__ YkRmsNorm8 p, int lanes) {
+__global__ void __launch_bounds__(WARP ? 128 : 512) rmsnorm8_vec_kernel(const __grid_constant__ YkRmsNorm8 p, int lanes, int shift) {
   __shared__ float part[2][16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = WARP ? 1 : blockDim.x >> 5;
   const int id = WARP ? lane : threadIdx.x, size = WARP ? 32 : blockDim.x;
@@ -32,31 +32,24 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) rmsnorm8_vec_kernel(const __
   uint4 wv[V];
 #pragma unroll
   for (int i = 0; i < V; i++) wv[i] = id + i * size < chunks ? ((const uint4*)p.weight)[id + i * size] : make_uint4(0, 0, 0, 0);
-  float h[V][8];
+  float2 h[V][4];
   const float over_c = 1.f / (float)p.cols;
-  float ss = 0.f;
+  float2 ss2 = make_float2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const uint32_t *xu = (const uint32_t*)&xv[i], *au = (const uint32_t*)&av[i];
-    uint4 o;
-    uint32_t* ou = (uint32_t*)&o;
+    uint32_t o[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      float2 f = pair_to_float2<BF16>(xu[e]);
-      if (add) {
-        const float2 g = pair_to_float2<BF16>(au[e]);
-        f.x += g.x;
-        f.y += g.y;
-      }
-      h[i][2 * e] = f.x;
-      h[i][2 * e + 1] = f.y;
-      ou[e] = float2_to_pair<BF16>(f.x, f.y);
-      ss = fmaf(f.x, f.x * over_c, ss);   // the mean itself: the sum would overflow sooner
-      ss = fmaf(f.y, f.y * over_c, ss);
+      h[i][e] = pair_to_float2<BF16>(xu[e]);
+      if (add) h[i][e] = add2(h[i][e], pair_to_float2<BF16>(au[e]));
+      o[e] = float2_to_pair<BF16>(h[i][e].x, h[i][e].y);
+      ss2 = ffma2(h[i][e], mul2(h[i][e], make_float2(over_c, over_c)), ss2);   // the mean itself: the sum would overflow sooner
     }
-    if (p.sum && id + i * size < chunks) ((uint4*)((uint16_t*)p.sum + r * p.sum_row))[id + i * size] = o;
+    if (p.sum && id + i * size < chunks)
+      ((uint4*)((uint16_t*)p.sum + r * p.sum_row))[id + i * size] = make_uint4(o[0], o[1], o[2], o[3]);
   }
-  ss = warp_sum(ss);
+  float ss = warp_sum(ss2.x + ss2.y);
   if (!WARP) {
     if (lane == 0) part[0][warp] = ss;
     __syncthreads();
@@ -65,22 +58,23 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) rmsnorm8_vec_kernel(const __
   }
   const float inv = rsqrtf(ss + p.eps);
   float amax[V], row_max = 0.f;
+  const auto amax8 = [&](int i, auto abs_of) {      // of chunk i; fmaxf leaves NaN out
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) m = fmaxf(m, fmaxf(abs_of(h[i][e].x), abs_of(h[i][e].y)));
+    return id + i * size < chunks ? m : 0.f;
+  };
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const uint32_t* wu = (const uint32_t*)&wv[i];
-    uint4 o;
-    uint32_t* ou = (uint32_t*)&o;
-    amax[i] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float2 w = pair_to_float2<BF16>(wu[e]);
-      h[i][2 * e] *= inv * w.x;
-      h[i][2 * e + 1] *= inv * w.y;
-      ou[e] = float2_to_pair<BF16>(h[i][2 * e], h[i][2 * e + 1]);
-      amax[i] = fmaxf(amax[i], fmaxf(finite_abs(h[i][2 * e]), finite_abs(h[i][2 * e + 1])));
-    }
-    if (id + i * size >= chunks) amax[i] = 0.f;
-    else if (p.out) ((uint4*)((uint16_t*)p.out + r * p.out_row))[id + i * size] = o;
+    for (int e = 0; e < 4; e++) h[i][e] = mul2(h[i][e], mul2(make_float2(inv, inv), pair_to_float2<BF16>(wu[e])));
+    if (p.out && id + i * size < chunks)
+      ((uint4*)((uint16_t*)p.out + r * p.out_row))[id + i * size] =
+          make_uint4(float2_to_pair<BF16>(h[i][0].x, h[i][0].y), float2_to_pair<BF16>(h[i][1].x, h[i][1].y),
+                     float2_to_pair<BF16>(h[i][2].x, h[i][2].y), float2_to_pair<BF16>(h[i][3].x, h[i][3].y));
+    amax[i] = amax8(i, [](float v) { return fabsf(v); });
+    if (amax[i] == INFINITY) amax[i] = amax8(i, finite_abs);
     row_max = fmaxf(row_max, amax[i]);
   }
   if (!p.codes) return;
@@ -97,13 +91,17 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) rmsnorm8_vec_kernel(const __
   for (int i = 0; i < V; i++) {
     const int c = id + i * size;
     float m = lanes ? amax[i] : row_max;
-    for (int o = lanes >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    const float s = fmaxf(m / kE4m3Max, kMinScale), up = 1.f / s;
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      if (lanes > o) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const float s = fmaxf(m * (1.f / kE4m3Max), kMinScale), up = rcp_fast(s);
     if (c >= chunks) continue;
-    if (lanes ? c % lanes == 0 : c == 0) p.scales[r * p.scales_row + (lanes ? c / lanes : 0)] = s;
+    if (lanes ? (c & (lanes - 1)) == 0 : c == 0) p.scales[r * p.scales_row + (c >> shift)] = s;
+    float2 q[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) q[e] = mul2(h[i][e], make_float2(up, up));
     ((uint2*)((uint8_t*)p.codes + r * p.codes_row))[c] =
-        make_uint2(float4_to_e4m3x4(h[i][0] * up, h[i][1] * up, h[i][2] * up, h[i][3] * up),
-                   float4_to_e4m3x4(h[i][4] * up, h[i][5] * up, h[i][6] * up, h[i][7] * up));
+        make_uint2(float4_to_e4m3x4(q[0].x, q[0].y, q[1].x, q[1].y), float4_to_e4m3x4(q[2].x, q[2].y, q[3].x, q[3].y));
   }
 }
 
@@ -189,15 +187,16 @@ extern "C" int yk_rmsnorm8(const YkRmsNorm8* p, yk_stream_t st) {
     fits = fits && group % 8 == 0 && lanes <= 32 && !(lanes & (lanes - 1));
   }
   if (fits) {
+    const int shift = lanes ? __builtin_ctz(lanes) : 0;
     // a warp a row while its chunks are at most two a lane; else four chunks a thread (eight from
     // 16384 columns on): fewer threads leave more rows in flight on an SM
     const int chunks = p->cols / 8;
     if (chunks <= 64)
-      launch_k(bf ? rmsnorm8_vec_kernel<true, 2, true> : rmsnorm8_vec_kernel<false, 2, true>, (unsigned)((p->rows + 3ll) / 4), 128, 0, s, *p, lanes);
+      launch_k(bf ? rmsnorm8_vec_kernel<true, 2, true> : rmsnorm8_vec_kernel<false, 2, true>, (unsigned)((p->rows + 3ll) / 4), 128, 0, s, *p, lanes, shift);
     else if (chunks <= 2048)
-      launch_k(bf ? rmsnorm8_vec_kernel<true, 4, false> : rmsnorm8_vec_kernel<false, 4, false>, p->rows, (chunks + 127) / 128 * 32, 0, s, *p, lanes);
+      launch_k(bf ? rmsnorm8_vec_kernel<true, 4, false> : rmsnorm8_vec_kernel<false, 4, false>, p->rows, (chunks + 127) / 128 * 32, 0, s, *p, lanes, shift);
     else
-      launch_k(bf ? rmsnorm8_vec_kernel<true, 8, false> : rmsnorm8_vec_kernel<false, 8, false>, p->rows, 512, 0, s, *p, lanes);
+      launch_k(bf ? rmsnorm8_vec_kernel<true, 8, false> : rmsnorm8_vec_kernel<false, 8, false>, p->rows, 512, 0, s, *p, lanes, shift);
     note_launch();
     return check_launch("rmsnorm8");
   }

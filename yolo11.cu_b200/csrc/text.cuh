@@ -74,6 +74,24 @@ __device__ __forceinline__ float finite_abs(float v) {
   return a <= 3.402823466e38f ? a : 0.f;
 }
 
+// 1 / v to within one unit in the last place, for normal v with a normal inverse.
+__device__ __forceinline__ float rcp_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return ffma2(a, b, make_float2(0.f, 0.f)); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return ffma2(a, make_float2(1.f, 1.f), b); }
+// Packed 16-bit maximum of m and |v|; a NaN in v is left out.
+template <bool BF16>
+__device__ __forceinline__ uint32_t amax_pair(uint32_t m, uint32_t v) {
+  v &= 0x7fff7fffu;
+  uint32_t r;
+  if (BF16) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(v));
+  else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(v));
+  return r;
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
