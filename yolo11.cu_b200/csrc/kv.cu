@@ -261,7 +261,7 @@ __device__ __forceinline__ void append_head(const AppendArgs& a, int h, int firs
   };
   meet();
   if (m[0] == INFINITY || m[1] == INFINITY) {       // again, without the infinities
-#pragma unroll 1
+#pragma unroll
     for (int kv = 0; kv < 2; kv++) {
       float top = 0.f;
       for (int c = id; c < chunks; c += size) {
@@ -314,7 +314,7 @@ __device__ __forceinline__ void append_head(const AppendArgs& a, int h, int firs
 }
 
 template <bool BF16>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_wait();
   pdl_trigger();
   __shared__ float red[2][kAppendThreads / 32];
