@@ -41,6 +41,7 @@ constexpr int kDecGran = 16 * kDecSub;     // tokens of a granule
 // 431 keys: least share 3, 6 give 10.0, 8.5 us).
 constexpr int kDecLead = 2, kDecMin = 6;
 constexpr int kDecCtas = 148 * 2;
+constexpr int kProRows = 64;               // rows a request and key head, on average, from which on tcgen05 tiles are used
 constexpr int kAtOnce = 8;                 // parts that a join reads at a time
 
 template <int D>
@@ -728,6 +729,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
   }
 }
 
+#include "attn8_prompt.cuh"
+
 }  // namespace yk
 
 using namespace yk;
@@ -768,6 +771,13 @@ extern "C" int yk_attn_kv8(const YkKvCache* c, const YkAttnKv8* a, yk_stream_t s
   p.scale_log2 = p.a.scale * 1.4426950408889634f;
   const bool bf = a->dtype == YK_BF16;
   cudaStream_t s = (cudaStream_t)st;
+  if ((long long)a->rows * (a->heads / c->heads) >= kProRows * (long long)a->requests) {
+    switch (c->dim) {
+      case 64: return bf ? launch_attn8_prompt<true, 64>(p, s) : launch_attn8_prompt<false, 64>(p, s);
+      case 128: return bf ? launch_attn8_prompt<true, 128>(p, s) : launch_attn8_prompt<false, 128>(p, s);
+      default: return bf ? launch_attn8_prompt<true, 256>(p, s) : launch_attn8_prompt<false, 256>(p, s);
+    }
+  }
   switch (c->dim) {
     case 64: return bf ? launch_attn8_split<true, 64>(p, s) : launch_attn8_split<false, 64>(p, s);
     case 128: return bf ? launch_attn8_split<true, 128>(p, s) : launch_attn8_split<false, 128>(p, s);

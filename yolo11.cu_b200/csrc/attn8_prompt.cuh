@@ -1,0 +1,467 @@
+// Attention over the paged 8-bit cache, many rows: the rows of a request that share a key head
+// fill 128-row tiles of tcgen05 MMAs (included by attn8.cu).
+//
+// Tensor bound.  One CTA a (128-row tile, key head); per 128 keys S = Q K^T (fp32 in TMEM), softmax,
+// O += P V (O in TMEM, fp16 operands).  Roles:
+//  * warps 0-3, softmax: a thread owns a row (a TMEM lane), so maxima and sums need no shuffles.  It
+//    reads S twice, for the maximum and for the weights, and writes P as fp16 over the S columns that
+//    it has read: P is the A operand straight from TMEM.  O is rescaled only when a row's maximum
+//    passed its reference by 2^6, which is seldom.
+//  * warps 4-7 read the codes of the next tile into registers while this one's MMAs run, convert them
+//    (exactly) to fp16 and write them into the 128-byte-swizzled K-major tiles that the MMA reads: keys
+//    as they are, values transposed, 8 tokens a 16-byte store, by interleaving the bytes of token
+//    pairs.
+//  * one thread of warp 8 issues the MMAs: PV of tile j, then, once that is done, QK of tile j + 1
+//    into the same TMEM columns.
+// One set of buffers a CTA and two CTAs an SM (up to 128 channels): one's softmax runs beside the
+// other's MMAs.
+constexpr int kProThreads = 288;
+
+template <int D>
+struct Pro {
+  static constexpr int kTile = 128 * D * 2;             // fp16 bytes of 128 rows
+  static constexpr int kSmem = 3 * kTile + 1024;        // q, keys, values; alignment
+  static constexpr int kCols = D == 256 ? 512 : 256;    // TMEM columns: S 128, O D
+  static constexpr int kK = 4 * (D / 64);               // 16-byte code chunks of a converting thread
+  static constexpr int kV = D == 256 ? 2 : 1;           // its 8-token x 16-channel pieces
+};
+
+// D[tmem] (+)= A[tmem] * B[smem desc]^T, fp16 inputs, fp32 accumulate.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t dtmem, uint32_t atmem, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(dtmem),
+      "r"(atmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+      "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// 16-byte chunk `ch` (of 64 columns: 8 a row) of row `row` of a swizzled slab of 128-byte rows
+__device__ __forceinline__ uint32_t swz_at(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_kernel(const __grid_constant__ Attn8Args p) {
+  using L = Pro<D>;
+  extern __shared__ uint8_t pro_raw[];
+  __shared__ __align__(8) uint64_t bars[5];
+  __shared__ uint32_t tslot;
+  __shared__ volatile int abort_flag;
+  __shared__ int nan_lo, nan_hi;                  // tiles of keys where a NaN value was taken out
+  __shared__ float ks_sm[2][8], vs_sm[2][8];      // scales of the tile's 16-token groups; ks < 0: not there
+  const YkAttnKv8& a = p.a;
+  const YkKvCache& c = p.c;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = a.heads / c.heads, T = c.tokens;
+  pdl_wait();
+  pdl_trigger();
+
+  // Request r owns the tile numbers from rows_before * G / 128 + r on: at least as many as it has
+  // tiles.  Later tiles of a request see more keys, so high numbers go first.
+  const int kh = blockIdx.x % c.heads;
+  const long long number = gridDim.x / c.heads - 1 - blockIdx.x / c.heads;
+  const auto first_number = [&](int r) { return (long long)min(max(a.cu[r], 0), a.rows) * G / 128 + r; };
+  int r = 0;
+  for (int hi = a.requests; hi - r > 1;) {
+    const int m = (r + hi) >> 1;
+    if (first_number(m) <= number) r = m; else hi = m;
+  }
+  const Req rq = attn_req(c, a, r);
+  const long long tile = number - first_number(r);
+  if (tile < 0 || tile * 128 >= (long long)rq.q * G) return;
+  const int row0 = (int)tile * 128, row_n = min(128, rq.q * G - row0);
+  const int t0 = row0 / G, t1 = (row0 + row_n - 1) / G;              // the tile's tokens
+  const int hi_key = a.causal ? max(0, rq.kv - rq.q + t1 + 1) : rq.kv;   // keys that some row sees: [lo_key, hi_key)
+  const int lo_key = a.causal ? first_key(rq.kv - rq.q + t0, a.window) : 0;
+  const int all_hi = a.causal ? rq.kv - rq.q + t0 + 1 : rq.kv;          // that every row sees: [all_lo, all_hi)
+  const int all_lo = a.causal ? first_key(rq.kv - rq.q + t1, a.window) : 0;
+  const int j0 = lo_key / 128, j1 = (hi_key + 127) / 128;             // tiles of 128 keys
+
+  // this thread's row (softmax warps; rows past row_n follow the last one and are not written)
+  const int rr = row0 + min(tid & 127, row_n - 1), tok = rr / G, head = kh * G + rr - tok * G;
+  const long long out_row = rq.q0 + tok;
+  if (j1 <= j0) {                       // no keys at all
+    if (tid < row_n) {
+      for (int d = 0; d < D; d += 8) *(uint4*)((uint16_t*)a.out + out_row * a.out_row + (long long)head * D + d) = make_uint4(0, 0, 0, 0);
+      if (a.lse) a.lse[out_row * a.heads + head] = -INFINITY;
+    }
+    return;
+  }
+
+  const uint32_t base = (smem_u32(pro_raw) + 1023) & ~1023u;
+  const uint32_t q_sm = base, k_sm = base + L::kTile, v_sm = base + 2 * L::kTile;
+  const uint32_t k_full = smem_u32(&bars[0]), v_full = smem_u32(&bars[1]), s_full = smem_u32(&bars[2]),
+                 p_full = smem_u32(&bars[3]), o_done = smem_u32(&bars[4]);
+  if (tid == 0) {
+    mbar_init(k_full, 128);
+    mbar_init(v_full, 128);
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 128);
+    mbar_init(o_done, 1);
+    mbar_fence_init();
+    abort_flag = 0;
+    nan_lo = 0x7fffffff;
+    nan_hi = -1;
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(&tslot), L::kCols);
+    tmem_relinquish();
+  }
+  // q: a thread its row, bf16 scaled by a power of two to fp16
+  float fac = p.scale_log2;             // score factor of the row: scale * log2 e * the power of two taken out of q
+  if (warp < 4) {
+    const uint4* qp = (const uint4*)((const uint16_t*)a.q + out_row * a.q_row + (long long)head * D);
+    float up = 1.f;
+    if (BF16) {
+      uint32_t m2 = 0;
+#pragma unroll 4
+      for (int i = 0; i < D / 8; i++) {
+        const uint4 v = qp[i];
+        m2 = amax_pair<true>(amax_pair<true>(m2, v.x), v.y);
+        m2 = amax_pair<true>(amax_pair<true>(m2, v.z), v.w);
+      }
+      const float2 f = pair_to_float2<true>(m2);
+      const float m = fmaxf(f.x, f.y);
+      int e = (int)((__float_as_uint(m) >> 23) & 255) - 127;   // m in [2^e, 2^(e+1))
+      e = m > 0.f ? max(-110, min(e, 120)) : 13;
+      up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);     // the largest becomes 2^13 .. 2^14
+      fac = p.scale_log2 * __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+    }
+#pragma unroll 4
+    for (int i = 0; i < D / 8; i++) {
+      uint4 v = qp[i];
+      if (BF16) {
+        uint32_t* u = (uint32_t*)&v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float2 x = pair_to_float2<true>(u[e]);
+          u[e] = pack_half2(x.x * up, x.y * up);
+        }
+      }
+      sts128(q_sm + (i >> 3) * 16384 + swz_at(tid, i & 7), v.x, v.y, v.z, v.w);
+    }
+    fence_proxy_async();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tslot, s_tm = tmem, o_tm = tmem + 128;
+  const int tiles = j1 - j0;
+
+  if (warp < 4) {
+    // ---------------- softmax ----------------
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const int pos = rq.kv - rq.q + tok;
+    const int last = a.causal ? min(rq.kv - 1, pos) : rq.kv - 1, first = a.causal ? first_key(pos, a.window) : 0;
+    constexpr float kNone = -1e30f, kSlack = 6.f;      // as in the split kernel
+    float m = kNone, M = kNone, gain = 1.f, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < tiles; j++) {
+      if (!mbar_wait(s_full, j & 1, 0x503)) { abort_flag = 1; ok = false; break; }
+      tc_fence_after();
+      const int key0 = (j0 + j) * 128;
+      float kk[8], vs[8];
+      bool gone = false;
+#pragma unroll
+      for (int g = 0; g < 8; g++) {
+        const float k = ks_sm[j & 1][g];
+        gone |= k < 0.f;
+        kk[g] = fmaxf(k * fac, 1e-38f);      // above 0: masked scores stay -inf
+        vs[g] = vs_sm[j & 1][g];
+      }
+      const bool edge = gone || key0 < all_lo || key0 + 128 > all_hi;
+      const auto hide = [&](uint32_t (&s)[32], int c0) {   // scores that this row does not see
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+          const int key = key0 + c0 + i;
+          if (key < first || key > last || ks_sm[j & 1][(c0 + i) >> 4] < 0.f) s[i] = 0xff800000u;
+        }
+      };
+      float top = -INFINITY, top_v = -INFINITY;
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        uint32_t s[32];
+        tmem_ld16p(s_tm + lanes + c0, s);
+        tmem_ld16p(s_tm + lanes + c0 + 16, s + 16);
+        tmem_ld_wait();
+        if (edge) hide(s, c0);
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          float x = __uint_as_float(s[16 * g]);
+#pragma unroll
+          for (int i = 1; i < 16; i++) x = fmaxf(x, __uint_as_float(s[16 * g + i]));
+          x *= kk[c0 / 16 + g];
+          top = fmaxf(top, x);
+          top_v = fmaxf(top_v, x + __log2f(vs[c0 / 16 + g]));
+        }
+      }
+      if (__any_sync(~0u, top > m + kSlack || top_v > M + kSlack)) {
+        const float mn = fmaxf(m, top), Mn = fmaxf(M, top_v);
+        l *= ex2(m - mn);
+        const float corr = ex2(M - Mn);
+        m = mn;
+        M = Mn;
+        gain = ex2(mn - Mn);
+        if (j > 0) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            tmem_ld16p(o_tm + lanes + c0, o);
+            tmem_ld16p(o_tm + lanes + c0 + 16, o + 16);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st16(o_tm + lanes + c0, o);
+            tmem_st16(o_tm + lanes + c0 + 16, o + 16);
+          }
+          tmem_st_wait();
+        }
+      }
+      float2 sum = make_float2(0.f, 0.f);
+      const float2 neg = make_float2(-m, -m);
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        uint32_t s[32];
+        tmem_ld16p(s_tm + lanes + c0, s);
+        tmem_ld16p(s_tm + lanes + c0 + 16, s + 16);
+        tmem_ld_wait();
+        if (edge) hide(s, c0);
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int g = c0 / 16 + i / 8;
+          const float f = vs[g] * gain;
+          float2 x = ffma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), make_float2(kk[g], kk[g]), neg);
+          x.x = ex2(x.x);
+          x.y = ex2(x.y);
+          sum = add2(sum, x);
+          x = mul2(x, make_float2(f, f));
+          w[i] = pack_half2(x.x, x.y);
+        }
+        tmem_st16(s_tm + lanes + c0 / 2, w);      // over columns that were read
+      }
+      l += sum.x + sum.y;
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_full);
+    }
+    if (ok && mbar_wait(o_done, (tiles - 1) & 1, 0x505)) {
+      tc_fence_after();
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      uint16_t* op = (uint16_t*)a.out + out_row * a.out_row + (long long)head * D;
+      // o is relative to M, l to m
+      const float k = (m == kNone ? 0.f : ex2(M - m)) * inv;
+      const int n_lo = nan_lo, n_hi = nan_hi;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld16p(o_tm + lanes + c0, o);
+        tmem_ld16p(o_tm + lanes + c0 + 16, o + 16);
+        tmem_ld_wait();
+        if (n_hi >= 0) {
+          // a NaN that was taken out of the edge tiles' values reaches the rows that see its token
+          for (int key = max(first, n_lo * 128); key <= min(last, n_hi * 128 + 127); key++) {
+            const int b = a.table[r * a.table_stride + key / T];
+            if ((unsigned)b >= (unsigned)c.blocks) continue;
+            const uint8_t* v = (const uint8_t*)c.v + b * c.block_stride + ((long long)kh * T + (key & (T - 1))) * D + c0;
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+              if ((v[i] & 0x7f) == 0x7f) o[i] = 0x7fffffffu;
+          }
+        }
+        if (tid < row_n) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              u[e] = float2_to_pair<BF16>(__uint_as_float(o[i + 2 * e]) * k, __uint_as_float(o[i + 2 * e + 1]) * k);
+            *(uint4*)(op + c0 + i) = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        }
+      }
+      if (a.lse && tid < row_n)
+        a.lse[out_row * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    }
+  } else if (warp < 8) {
+    // ---------------- codes to fp16 tiles ----------------
+    const int w = warp - 4, u0 = tid - 128;
+    const int* table = a.table + r * a.table_stride;
+    const auto block_at = [&](int j) -> int {            // of 16-token group `lane` (< 8) of tile j; -1: none
+      const int key = (j0 + j) * 128 + lane * 16;
+      if (lane >= 8 || j >= tiles || key >= hi_key) return -1;
+      const int b = table[key / T];
+      return (unsigned)b < (unsigned)c.blocks ? b : -1;
+    };
+    const auto token_at = [&](const void* codes, int id, int key) {
+      return (const uint8_t*)codes + id * c.block_stride + ((long long)kh * T + (key & (T - 1))) * D;
+    };
+    // keys: pieces (slab of 64 channels, 8 rows); lane: row lane / 4, 16 channels (lane % 4) of the slab
+    uint4 kv[L::kK];
+    const auto load_k = [&](int j, int ids) {
+#pragma unroll
+      for (int i = 0; i < L::kK; i++) {
+        const int piece = w + 4 * i, slab = piece % (D / 64), row = piece / (D / 64) * 8 + lane / 4;
+        const int id = __shfl_sync(~0u, ids, row >> 4), key = (j0 + j) * 128 + row;
+        kv[i] = make_uint4(0, 0, 0, 0);
+        if (id >= 0 && key < hi_key) kv[i] = *(const uint4*)(token_at(c.k, id, key) + slab * 64 + (lane & 3) * 16);
+      }
+    };
+    const auto store_k = [&] {
+#pragma unroll
+      for (int i = 0; i < L::kK; i++) {
+        const int piece = w + 4 * i, slab = piece % (D / 64), row = piece / (D / 64) * 8 + lane / 4;
+        uint32_t h[8];
+        e4m3x4_to_half2x2(kv[i].x, h[0], h[1]);
+        e4m3x4_to_half2x2(kv[i].y, h[2], h[3]);
+        e4m3x4_to_half2x2(kv[i].z, h[4], h[5]);
+        e4m3x4_to_half2x2(kv[i].w, h[6], h[7]);
+        const uint32_t at = k_sm + slab * 16384;
+        sts128(at + swz_at(row, (lane & 3) * 2), h[0], h[1], h[2], h[3]);
+        sts128(at + swz_at(row, (lane & 3) * 2 + 1), h[4], h[5], h[6], h[7]);
+      }
+    };
+    // values: piece u: 8 tokens (octet) x 16 channels
+    uint4 vv[L::kV][8];
+    const auto octet_of = [&](int u) { return (u & 7) | ((u >> 2) & 8); };
+    const auto chunk_of = [&](int u) { return ((u >> 3) & 3) | ((u >> 6) << 2); };
+    const auto load_v = [&](int j, int ids) {
+#pragma unroll
+      for (int x = 0; x < L::kV; x++) {
+        const int u = u0 + 128 * x, octet = octet_of(u), id = __shfl_sync(~0u, ids, octet >> 1);
+        const int key = (j0 + j) * 128 + octet * 8;
+        const uint8_t* v = token_at(c.v, max(id, 0), key) + chunk_of(u) * 16;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          vv[x][i] = make_uint4(0, 0, 0, 0);
+          if (id >= 0 && key + i < hi_key && u < D) vv[x][i] = *(const uint4*)(v + i * D);
+        }
+      }
+    };
+    const auto store_v = [&](int j) {
+      const int key0 = (j0 + j) * 128;
+      const bool edge = key0 < all_lo || key0 + 128 > all_hi;
+#pragma unroll
+      for (int x = 0; x < L::kV; x++) {
+        const int u = u0 + 128 * x, octet = octet_of(u), ch = chunk_of(u);
+        if (u >= D) break;
+        if (edge) {       // 0 * NaN: a NaN that some row does not see is taken out here, see the end
+          uint32_t any = 0;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            uint32_t* v = (uint32_t*)&vv[x][i];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t nan = ((v[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+              any |= nan;
+              v[e] &= ~((nan >> 7) * 0xffu);
+            }
+          }
+          if (any) {
+            atomicMin(&nan_lo, j0 + j);
+            atomicMax(&nan_hi, j0 + j);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t lo[4][2], hi[4][2];      // token pairs of channels 4 e + 0, 1 and 2, 3
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t x0 = ((const uint32_t*)&vv[x][2 * i])[e], x1 = ((const uint32_t*)&vv[x][2 * i + 1])[e];
+            e4m3x4_to_half2x2(__byte_perm(x0, x1, 0x5140), lo[i][0], lo[i][1]);
+            e4m3x4_to_half2x2(__byte_perm(x0, x1, 0x7362), hi[i][0], hi[i][1]);
+          }
+          const uint32_t at = v_sm + (octet >> 3) * (D * 128);
+          const int d = ch * 16 + e * 4;
+          sts128(at + swz_at(d, octet & 7), lo[0][0], lo[1][0], lo[2][0], lo[3][0]);
+          sts128(at + swz_at(d + 1, octet & 7), lo[0][1], lo[1][1], lo[2][1], lo[3][1]);
+          sts128(at + swz_at(d + 2, octet & 7), hi[0][0], hi[1][0], hi[2][0], hi[3][0]);
+          sts128(at + swz_at(d + 3, octet & 7), hi[0][1], hi[1][1], hi[2][1], hi[3][1]);
+        }
+      }
+    };
+    int ids = block_at(0), ids_next = block_at(1);
+    load_k(0, ids);
+    load_v(0, ids);
+    for (int j = 0; j < tiles; j++) {
+      const float ks = ids >= 0 ? c.kscale[ids * c.scale_stride + kh] : -1.f;
+      const float vs = ids >= 0 ? c.vscale[ids * c.scale_stride + kh] : 0.f;
+      const int ids_after = block_at(j + 2);
+      if (j > 0 && !mbar_wait(s_full, (j - 1) & 1, 0x501)) { abort_flag = 1; break; }   // QK j - 1 has read its keys
+      store_k();
+      if (w == 0 && lane < 8) {
+        ks_sm[j & 1][lane] = ks;
+        vs_sm[j & 1][lane] = vs;
+      }
+      fence_proxy_async();
+      mbar_arrive(k_full);
+      load_k(j + 1, ids_next);
+      if (j > 0 && !mbar_wait(o_done, (j - 1) & 1, 0x502)) { abort_flag = 1; break; }   // PV j - 1 its values
+      store_v(j);
+      fence_proxy_async();
+      mbar_arrive(v_full);
+      load_v(j + 1, ids_next);
+      ids = ids_next;
+      ids_next = ids_after;
+    }
+  } else if (lane == 0) {
+    // ---------------- MMA ----------------
+    const auto qk = [&] {
+#pragma unroll
+      for (int s = 0; s < D / 16; s++)
+        tc_mma_f16(s_tm, sw128_desc(q_sm + (s >> 2) * 16384 + (s & 3) * 32), sw128_desc(k_sm + (s >> 2) * 16384 + (s & 3) * 32),
+                   idesc_f16_m128(128), s != 0);
+      tc_commit(s_full);
+    };
+    bool ok = mbar_wait(k_full, 0, 0x504);
+    if (ok) {
+      tc_fence_after();
+      qk();
+    }
+    for (int j = 0; j < tiles && ok; j++) {
+      ok = mbar_wait(p_full, j & 1, 0x506) && mbar_wait(v_full, j & 1, 0x507);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int s = 0; s < 8; s++)
+        tc_mma_f16_ts(o_tm, s_tm + s * 8, sw128_desc(v_sm + (s >> 2) * (D * 128) + (s & 3) * 32), idesc_f16_m128(D), (j | s) != 0);
+      tc_commit(o_done);
+      if (j + 1 < tiles) {
+        // S and P share columns: the order of MMAs with different accumulators is not promised
+        ok = mbar_wait(o_done, j & 1, 0x508) && mbar_wait(k_full, (j + 1) & 1, 0x504);
+        if (!ok) break;
+        tc_fence_after();
+        qk();
+      }
+    }
+    if (!ok) abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kCols);
+  }
+}
+
+template <bool BF16, int D>
+static int launch_attn8_prompt(const Attn8Args& p, cudaStream_t st) {
+  const auto kern = attn8_prompt_kernel<BF16, D>;
+  if (smem_attr(kern, Pro<D>::kSmem) != cudaSuccess) return check_launch("attn_kv8 attr");
+  const long long tiles = (long long)p.a.rows * (p.a.heads / p.c.heads) / 128 + p.a.requests;
+  if (tiles * p.c.heads > 0x7fffffffll) return refuse(YK_EUNSUP, "attn_kv8: too many rows");
+  launch_k(kern, (unsigned)(tiles * p.c.heads), kProThreads, Pro<D>::kSmem, st, p);
+  note_launch();
+  return check_launch("attn_kv8");
+}
