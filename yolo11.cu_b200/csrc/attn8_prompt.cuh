@@ -1,29 +1,30 @@
 // Attention over the paged 8-bit cache, many rows: the rows of a request that share a key head
 // fill 128-row tiles of tcgen05 MMAs (included by attn8.cu).
 //
-// Tensor bound.  One CTA a (128-row tile, key head); per 128 keys S = Q K^T (fp32 in TMEM), softmax,
-// O += P V (O in TMEM, fp16 operands).  Roles:
-//  * warps 0-3, softmax: a thread owns a row (a TMEM lane), so maxima and sums need no shuffles.  It
-//    reads S twice, for the maximum and for the weights, and writes P as fp16 over the S columns that
-//    it has read: P is the A operand straight from TMEM.  O is rescaled only when a row's maximum
-//    passed its reference by 2^6, which is seldom.
-//  * warps 4-7 read the codes of the next tile into registers while this one's MMAs run, convert them
+// Tensor and exponential bound.  One CTA a (128-row tile, key head); per 64 keys S = Q K^T (fp32 in
+// TMEM), softmax, O += P V (O in TMEM, fp16 operands).  Roles:
+//  * warps 0-3, softmax: a thread owns a row (a TMEM lane), so maxima and sums need no shuffles.
+//    Weights are taken relative to a reference that follows the row's maximum only when that passes
+//    it by 2^6, so a tile is read once: if its maximum stays below, the weights stand; else (seldom)
+//    the reference moves, O is rescaled, and the tile is done again.  P goes as fp16 over the columns of
+//    its S: it is the A operand straight from TMEM.
+//  * warps 4-7 read the codes of the next tile into registers while this one's are in use, convert them
 //    (exactly) to fp16 and write them into the 128-byte-swizzled K-major tiles that the MMA reads: keys
 //    as they are, values transposed, 8 tokens a 16-byte store, by interleaving the bytes of token
 //    pairs.
-//  * one thread of warp 8 issues the MMAs: PV of tile j, then, once that is done, QK of tile j + 1
-//    into the same TMEM columns.
-// One set of buffers a CTA and two CTAs an SM (up to 128 channels): one's softmax runs beside the
-// other's MMAs.
+//  * one thread of warp 8 issues the MMAs.  Everything comes twice (S and P, keys, values), so QK of
+//    tile j + 1 is done before the softmax of tile j is, and PV of tile j runs beside the softmax of
+//    tile j + 1.
+// Two CTAs an SM up to 128 channels.
 constexpr int kProThreads = 288;
 
 template <int D>
 struct Pro {
-  static constexpr int kTile = 128 * D * 2;             // fp16 bytes of 128 rows
-  static constexpr int kSmem = 3 * kTile + 1024;        // q, keys, values; alignment
-  static constexpr int kCols = D == 256 ? 512 : 256;    // TMEM columns: S 128, O D
-  static constexpr int kK = 4 * (D / 64);               // 16-byte code chunks of a converting thread
-  static constexpr int kV = D == 256 ? 2 : 1;           // its 8-token x 16-channel pieces
+  static constexpr int kTile = 64 * D * 2;              // fp16 bytes of 64 keys
+  static constexpr int kSmem = 6 * kTile + 1024;        // q (128 rows), two of keys, two of values; alignment
+  static constexpr int kCols = D == 256 ? 512 : 256;    // TMEM columns: S twice 64, O D
+  static constexpr int kK = 2 * (D / 64);               // 16-byte code chunks of a converting thread
+  static constexpr int kV = D == 256 ? 2 : 1;           // its 8-token x 8-channel pieces
 };
 
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, fp16 inputs, fp32 accumulate.
@@ -54,11 +55,12 @@ template <bool BF16, int D>
 __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_kernel(const __grid_constant__ Attn8Args p) {
   using L = Pro<D>;
   extern __shared__ uint8_t pro_raw[];
-  __shared__ __align__(8) uint64_t bars[5];
+  __shared__ __align__(8) uint64_t bars[10];
   __shared__ uint32_t tslot;
   __shared__ volatile int abort_flag;
   __shared__ int nan_lo, nan_hi;                  // tiles of keys where a NaN value was taken out
-  __shared__ float ks_sm[2][8], vs_sm[2][8];      // scales of the tile's 16-token groups; ks < 0: not there
+  // scales of the 16-token groups of tile j at j % 4, with the logarithm of the value scale; ks < 0: not there
+  __shared__ float ks_sm[4][4], vs_sm[4][4], lv_sm[4][4];
   const YkAttnKv8& a = p.a;
   const YkKvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -85,7 +87,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
   const int lo_key = a.causal ? first_key(rq.kv - rq.q + t0, a.window) : 0;
   const int all_hi = a.causal ? rq.kv - rq.q + t0 + 1 : rq.kv;          // that every row sees: [all_lo, all_hi)
   const int all_lo = a.causal ? first_key(rq.kv - rq.q + t1, a.window) : 0;
-  const int j0 = lo_key / 128, j1 = (hi_key + 127) / 128;             // tiles of 128 keys
+  const int j0 = lo_key / 64, j1 = (hi_key + 63) / 64;                // tiles of 64 keys
 
   // this thread's row (softmax warps; rows past row_n follow the last one and are not written)
   const int rr = row0 + min(tid & 127, row_n - 1), tok = rr / G, head = kh * G + rr - tok * G;
@@ -99,15 +101,18 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
   }
 
   const uint32_t base = (smem_u32(pro_raw) + 1023) & ~1023u;
-  const uint32_t q_sm = base, k_sm = base + L::kTile, v_sm = base + 2 * L::kTile;
-  const uint32_t k_full = smem_u32(&bars[0]), v_full = smem_u32(&bars[1]), s_full = smem_u32(&bars[2]),
-                 p_full = smem_u32(&bars[3]), o_done = smem_u32(&bars[4]);
+  const uint32_t q_sm = base, k_sm = base + 2 * L::kTile, v_sm = base + 4 * L::kTile;
+  // two of each, for even and odd tiles
+  const uint32_t k_full = smem_u32(&bars[0]), v_full = smem_u32(&bars[2]), s_full = smem_u32(&bars[4]),
+                 p_full = smem_u32(&bars[6]), o_done = smem_u32(&bars[8]);
   if (tid == 0) {
-    mbar_init(k_full, 128);
-    mbar_init(v_full, 128);
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 128);
-    mbar_init(o_done, 1);
+    for (int i = 0; i < 16; i += 8) {
+      mbar_init(k_full + i, 128);
+      mbar_init(v_full + i, 128);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 128);
+      mbar_init(o_done + i, 1);
+    }
     mbar_fence_init();
     abort_flag = 0;
     nan_lo = 0x7fffffff;
@@ -167,95 +172,119 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     float m = kNone, M = kNone, gain = 1.f, l = 0.f;
     bool ok = true;
     for (int j = 0; j < tiles; j++) {
-      if (!mbar_wait(s_full, j & 1, 0x503)) { abort_flag = 1; ok = false; break; }
+      const int buf = j & 1, turn = (j >> 1) & 1;
+      const uint32_t s_at = s_tm + lanes + buf * 64;
+      if (!mbar_wait(s_full + buf * 8, turn, 0x503)) { abort_flag = 1; ok = false; break; }
       tc_fence_after();
-      const int key0 = (j0 + j) * 128;
-      float kk[8], vs[8];
+      const int key0 = (j0 + j) * 64;
+      float kk[4], vs[4], lv[4];
       bool gone = false;
 #pragma unroll
-      for (int g = 0; g < 8; g++) {
-        const float k = ks_sm[j & 1][g];
+      for (int g = 0; g < 4; g++) {
+        const float k = ks_sm[j & 3][g];
         gone |= k < 0.f;
         kk[g] = fmaxf(k * fac, 1e-38f);      // above 0: masked scores stay -inf
-        vs[g] = vs_sm[j & 1][g];
+        vs[g] = vs_sm[j & 3][g];
+        lv[g] = lv_sm[j & 3][g];
       }
-      const bool edge = gone || key0 < all_lo || key0 + 128 > all_hi;
-      const auto hide = [&](uint32_t (&s)[32], int c0) {   // scores that this row does not see
+      const bool edge = gone || key0 < all_lo || key0 + 64 > all_hi;
+      const int c_lo = first - key0, c_hi = last - key0;       // columns that this row sees
+      const auto load_s = [&](uint32_t (&s)[32], int c0) {
+        tmem_ld16p(s_at + c0, s);
+        tmem_ld16p(s_at + c0 + 16, s + 16);
+        tmem_ld_wait();
+        if (edge) {
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-          const int key = key0 + c0 + i;
-          if (key < first || key > last || ks_sm[j & 1][(c0 + i) >> 4] < 0.f) s[i] = 0xff800000u;
+          for (int i = 0; i < 32; i++)
+            if (c0 + i < c_lo || c0 + i > c_hi) s[i] = 0xff800000u;
+          if (gone) {
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+              if (ks_sm[j & 3][c0 / 16 + g] < 0.f) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[16 * g + i] = 0xff800000u;
+              }
+          }
         }
       };
-      float top = -INFINITY, top_v = -INFINITY;
-#pragma unroll
-      for (int c0 = 0; c0 < 128; c0 += 32) {
-        uint32_t s[32];
-        tmem_ld16p(s_tm + lanes + c0, s);
-        tmem_ld16p(s_tm + lanes + c0 + 16, s + 16);
-        tmem_ld_wait();
-        if (edge) hide(s, c0);
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-          float x = __uint_as_float(s[16 * g]);
-#pragma unroll
-          for (int i = 1; i < 16; i++) x = fmaxf(x, __uint_as_float(s[16 * g + i]));
-          x *= kk[c0 / 16 + g];
-          top = fmaxf(top, x);
-          top_v = fmaxf(top_v, x + __log2f(vs[c0 / 16 + g]));
-        }
-      }
-      if (__any_sync(~0u, top > m + kSlack || top_v > M + kSlack)) {
-        const float mn = fmaxf(m, top), Mn = fmaxf(M, top_v);
-        l *= ex2(m - mn);
-        const float corr = ex2(M - Mn);
-        m = mn;
-        M = Mn;
-        gain = ex2(mn - Mn);
-        if (j > 0) {
+      uint32_t w[32];
+      float2 sum;
+      bool move = j == 0;
+      while (true) {
+        if (move) {              // the reference moves up to this tile's maximum
+          float top = -INFINITY, top_v = -INFINITY;
 #pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t o[32];
-            tmem_ld16p(o_tm + lanes + c0, o);
-            tmem_ld16p(o_tm + lanes + c0 + 16, o + 16);
-            tmem_ld_wait();
+          for (int c0 = 0; c0 < 64; c0 += 32) {
+            uint32_t s[32];
+            load_s(s, c0);
 #pragma unroll
-            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            tmem_st16(o_tm + lanes + c0, o);
-            tmem_st16(o_tm + lanes + c0 + 16, o + 16);
+            for (int g = 0; g < 2; g++) {
+              float x = __uint_as_float(s[16 * g]);
+#pragma unroll
+              for (int i = 1; i < 16; i++) x = fmaxf(x, __uint_as_float(s[16 * g + i]));
+              x *= c0 ? kk[2 + g] : kk[g];
+              top = fmaxf(top, x);
+              top_v = fmaxf(top_v, x + (c0 ? lv[2 + g] : lv[g]));
+            }
           }
-          tmem_st_wait();
-        }
-      }
-      float2 sum = make_float2(0.f, 0.f);
-      const float2 neg = make_float2(-m, -m);
+          const float mn = fmaxf(m, top), Mn = fmaxf(M, top_v);
+          l *= ex2(m - mn);
+          const float corr = ex2(M - Mn);
+          m = mn;
+          M = Mn;
+          gain = ex2(mn - Mn);
+          if (j > 0) {
+            if (!mbar_wait(o_done + (buf ^ 1) * 8, ((j - 1) >> 1) & 1, 0x509)) { abort_flag = 1; ok = false; break; }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 16) {
+              uint32_t o[16];
+              tmem_ld16p(o_tm + lanes + c0, o);
+              tmem_ld_wait();
 #pragma unroll
-      for (int c0 = 0; c0 < 128; c0 += 32) {
-        uint32_t s[32];
-        tmem_ld16p(s_tm + lanes + c0, s);
-        tmem_ld16p(s_tm + lanes + c0 + 16, s + 16);
-        tmem_ld_wait();
-        if (edge) hide(s, c0);
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int g = c0 / 16 + i / 8;
-          const float f = vs[g] * gain;
-          float2 x = ffma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), make_float2(kk[g], kk[g]), neg);
-          x.x = ex2(x.x);
-          x.y = ex2(x.y);
-          sum = add2(sum, x);
-          x = mul2(x, make_float2(f, f));
-          w[i] = pack_half2(x.x, x.y);
+              for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st16(o_tm + lanes + c0, o);
+            }
+            tmem_st_wait();
+          }
         }
-        tmem_st16(s_tm + lanes + c0 / 2, w);      // over columns that were read
+        sum = make_float2(0.f, 0.f);
+        float over = -INFINITY;          // how far the tile passes the references
+        const float2 neg = make_float2(-m, -m);
+        const float to_v = m - M;
+#pragma unroll
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          uint32_t s[32];
+          load_s(s, c0);
+#pragma unroll
+          for (int g = 0; g < 2; g++) {
+            const float k = kk[c0 / 16 + g], f = vs[c0 / 16 + g] * gain;
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 8 * g; i < 8 * g + 8; i++) {
+              float2 x = ffma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), make_float2(k, k), neg);
+              top = fmaxf(top, fmaxf(x.x, x.y));
+              x.x = ex2(x.x);
+              x.y = ex2(x.y);
+              sum = add2(sum, x);
+              x = mul2(x, make_float2(f, f));
+              w[c0 / 2 + i] = pack_half2(x.x, x.y);
+            }
+            over = fmaxf(over, fmaxf(top, top + (lv[c0 / 16 + g] + to_v)));
+          }
+        }
+        if (move || !__any_sync(~0u, over > kSlack)) break;
+        move = true;
       }
+      if (!ok) break;
       l += sum.x + sum.y;
+      tmem_st16(s_at, w);                // over columns that were read
+      tmem_st16(s_at + 16, w + 16);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(p_full);
+      mbar_arrive(p_full + buf * 8);
     }
-    if (ok && mbar_wait(o_done, (tiles - 1) & 1, 0x505)) {
+    if (ok && mbar_wait(o_done + ((tiles - 1) & 1) * 8, ((tiles - 1) >> 1) & 1, 0x505)) {
       tc_fence_after();
       const float inv = l > 0.f ? 1.f / l : 0.f;
       uint16_t* op = (uint16_t*)a.out + out_row * a.out_row + (long long)head * D;
@@ -270,7 +299,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
         tmem_ld_wait();
         if (n_hi >= 0) {
           // a NaN that was taken out of the edge tiles' values reaches the rows that see its token
-          for (int key = max(first, n_lo * 128); key <= min(last, n_hi * 128 + 127); key++) {
+          for (int key = max(first, n_lo * 64); key <= min(last, n_hi * 64 + 63); key++) {
             const int b = a.table[r * a.table_stride + key / T];
             if ((unsigned)b >= (unsigned)c.blocks) continue;
             const uint8_t* v = (const uint8_t*)c.v + b * c.block_stride + ((long long)kh * T + (key & (T - 1))) * D + c0;
@@ -297,9 +326,9 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     // ---------------- codes to fp16 tiles ----------------
     const int w = warp - 4, u0 = tid - 128;
     const int* table = a.table + r * a.table_stride;
-    const auto block_at = [&](int j) -> int {            // of 16-token group `lane` (< 8) of tile j; -1: none
-      const int key = (j0 + j) * 128 + lane * 16;
-      if (lane >= 8 || j >= tiles || key >= hi_key) return -1;
+    const auto block_at = [&](int j) -> int {            // of 16-token group `lane` (< 4) of tile j; -1: none
+      const int key = (j0 + j) * 64 + lane * 16;
+      if (lane >= 4 || j >= tiles || key >= hi_key) return -1;
       const int b = table[key / T];
       return (unsigned)b < (unsigned)c.blocks ? b : -1;
     };
@@ -312,12 +341,12 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
 #pragma unroll
       for (int i = 0; i < L::kK; i++) {
         const int piece = w + 4 * i, slab = piece % (D / 64), row = piece / (D / 64) * 8 + lane / 4;
-        const int id = __shfl_sync(~0u, ids, row >> 4), key = (j0 + j) * 128 + row;
+        const int id = __shfl_sync(~0u, ids, row >> 4), key = (j0 + j) * 64 + row;
         kv[i] = make_uint4(0, 0, 0, 0);
         if (id >= 0 && key < hi_key) kv[i] = *(const uint4*)(token_at(c.k, id, key) + slab * 64 + (lane & 3) * 16);
       }
     };
-    const auto store_k = [&] {
+    const auto store_k = [&](uint32_t tile_at) {
 #pragma unroll
       for (int i = 0; i < L::kK; i++) {
         const int piece = w + 4 * i, slab = piece % (D / 64), row = piece / (D / 64) * 8 + lane / 4;
@@ -326,34 +355,32 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
         e4m3x4_to_half2x2(kv[i].y, h[2], h[3]);
         e4m3x4_to_half2x2(kv[i].z, h[4], h[5]);
         e4m3x4_to_half2x2(kv[i].w, h[6], h[7]);
-        const uint32_t at = k_sm + slab * 16384;
+        const uint32_t at = tile_at + slab * 8192;
         sts128(at + swz_at(row, (lane & 3) * 2), h[0], h[1], h[2], h[3]);
         sts128(at + swz_at(row, (lane & 3) * 2 + 1), h[4], h[5], h[6], h[7]);
       }
     };
-    // values: piece u: 8 tokens (octet) x 16 channels
-    uint4 vv[L::kV][8];
-    const auto octet_of = [&](int u) { return (u & 7) | ((u >> 2) & 8); };
-    const auto chunk_of = [&](int u) { return ((u >> 3) & 3) | ((u >> 6) << 2); };
+    // values: piece u: tokens 8 * (u % 8) .., channels 8 * (u / 8) ..
+    uint2 vv[L::kV][8];
     const auto load_v = [&](int j, int ids) {
 #pragma unroll
       for (int x = 0; x < L::kV; x++) {
-        const int u = u0 + 128 * x, octet = octet_of(u), id = __shfl_sync(~0u, ids, octet >> 1);
-        const int key = (j0 + j) * 128 + octet * 8;
-        const uint8_t* v = token_at(c.v, max(id, 0), key) + chunk_of(u) * 16;
+        const int u = u0 + 128 * x, id = __shfl_sync(~0u, ids, (u & 7) >> 1);
+        const int key = (j0 + j) * 64 + (u & 7) * 8;
+        const uint8_t* v = token_at(c.v, max(id, 0), key) + (u >> 3) * 8;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          vv[x][i] = make_uint4(0, 0, 0, 0);
-          if (id >= 0 && key + i < hi_key && u < D) vv[x][i] = *(const uint4*)(v + i * D);
+          vv[x][i] = make_uint2(0, 0);
+          if (id >= 0 && key + i < hi_key && u < D) vv[x][i] = *(const uint2*)(v + i * D);
         }
       }
     };
-    const auto store_v = [&](int j) {
-      const int key0 = (j0 + j) * 128;
-      const bool edge = key0 < all_lo || key0 + 128 > all_hi;
+    const auto store_v = [&](int j, uint32_t tile_at) {
+      const int key0 = (j0 + j) * 64;
+      const bool edge = key0 < all_lo || key0 + 64 > all_hi;
 #pragma unroll
       for (int x = 0; x < L::kV; x++) {
-        const int u = u0 + 128 * x, octet = octet_of(u), ch = chunk_of(u);
+        const int u = u0 + 128 * x;
         if (u >= D) break;
         if (edge) {       // 0 * NaN: a NaN that some row does not see is taken out here, see the end
           uint32_t any = 0;
@@ -361,7 +388,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
           for (int i = 0; i < 8; i++) {
             uint32_t* v = (uint32_t*)&vv[x][i];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
+            for (int e = 0; e < 2; e++) {
               const uint32_t nan = ((v[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
               any |= nan;
               v[e] &= ~((nan >> 7) * 0xffu);
@@ -373,7 +400,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
           }
         }
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; e < 2; e++) {
           uint32_t lo[4][2], hi[4][2];      // token pairs of channels 4 e + 0, 1 and 2, 3
 #pragma unroll
           for (int i = 0; i < 4; i++) {
@@ -381,12 +408,11 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
             e4m3x4_to_half2x2(__byte_perm(x0, x1, 0x5140), lo[i][0], lo[i][1]);
             e4m3x4_to_half2x2(__byte_perm(x0, x1, 0x7362), hi[i][0], hi[i][1]);
           }
-          const uint32_t at = v_sm + (octet >> 3) * (D * 128);
-          const int d = ch * 16 + e * 4;
-          sts128(at + swz_at(d, octet & 7), lo[0][0], lo[1][0], lo[2][0], lo[3][0]);
-          sts128(at + swz_at(d + 1, octet & 7), lo[0][1], lo[1][1], lo[2][1], lo[3][1]);
-          sts128(at + swz_at(d + 2, octet & 7), hi[0][0], hi[1][0], hi[2][0], hi[3][0]);
-          sts128(at + swz_at(d + 3, octet & 7), hi[0][1], hi[1][1], hi[2][1], hi[3][1]);
+          const int d = (u >> 3) * 8 + e * 4;
+          sts128(tile_at + swz_at(d, u & 7), lo[0][0], lo[1][0], lo[2][0], lo[3][0]);
+          sts128(tile_at + swz_at(d + 1, u & 7), lo[0][1], lo[1][1], lo[2][1], lo[3][1]);
+          sts128(tile_at + swz_at(d + 2, u & 7), hi[0][0], hi[1][0], hi[2][0], hi[3][0]);
+          sts128(tile_at + swz_at(d + 3, u & 7), hi[0][1], hi[1][1], hi[2][1], hi[3][1]);
         }
       }
     };
@@ -394,55 +420,54 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     load_k(0, ids);
     load_v(0, ids);
     for (int j = 0; j < tiles; j++) {
+      const int buf = j & 1, before = ((j >> 1) - 1) & 1;      // turn of tile j - 2 in the same buffers
       const float ks = ids >= 0 ? c.kscale[ids * c.scale_stride + kh] : -1.f;
       const float vs = ids >= 0 ? c.vscale[ids * c.scale_stride + kh] : 0.f;
       const int ids_after = block_at(j + 2);
-      if (j > 0 && !mbar_wait(s_full, (j - 1) & 1, 0x501)) { abort_flag = 1; break; }   // QK j - 1 has read its keys
-      store_k();
-      if (w == 0 && lane < 8) {
-        ks_sm[j & 1][lane] = ks;
-        vs_sm[j & 1][lane] = vs;
+      if (j > 1 && !mbar_wait(s_full + buf * 8, before, 0x501)) { abort_flag = 1; break; }   // QK j - 2 has read its keys
+      store_k(k_sm + buf * L::kTile);
+      if (w == 0 && lane < 4) {
+        ks_sm[j & 3][lane] = ks;
+        vs_sm[j & 3][lane] = vs;
+        lv_sm[j & 3][lane] = __log2f(vs);
       }
       fence_proxy_async();
-      mbar_arrive(k_full);
+      mbar_arrive(k_full + buf * 8);
       load_k(j + 1, ids_next);
-      if (j > 0 && !mbar_wait(o_done, (j - 1) & 1, 0x502)) { abort_flag = 1; break; }   // PV j - 1 its values
-      store_v(j);
+      if (j > 1 && !mbar_wait(o_done + buf * 8, before, 0x502)) { abort_flag = 1; break; }   // PV j - 2 its values
+      store_v(j, v_sm + buf * L::kTile);
       fence_proxy_async();
-      mbar_arrive(v_full);
+      mbar_arrive(v_full + buf * 8);
       load_v(j + 1, ids_next);
       ids = ids_next;
       ids_next = ids_after;
     }
   } else if (lane == 0) {
     // ---------------- MMA ----------------
-    const auto qk = [&] {
+    const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(k_sm), v_desc = sw128_desc(v_sm);   // addresses count 16 bytes
+    const auto qk = [&](int j) {
+      const int buf = j & 1;
+      if (!mbar_wait(k_full + buf * 8, (j >> 1) & 1, 0x504)) return false;
+      tc_fence_after();
 #pragma unroll
       for (int s = 0; s < D / 16; s++)
-        tc_mma_f16(s_tm, sw128_desc(q_sm + (s >> 2) * 16384 + (s & 3) * 32), sw128_desc(k_sm + (s >> 2) * 16384 + (s & 3) * 32),
-                   idesc_f16_m128(128), s != 0);
-      tc_commit(s_full);
+        tc_mma_f16(s_tm + buf * 64, q_desc + (s >> 2) * 1024 + (s & 3) * 2, k_desc + buf * (L::kTile / 16) + (s >> 2) * 512 + (s & 3) * 2,
+                   idesc_f16_m128(64), s != 0);
+      tc_commit(s_full + buf * 8);
+      return true;
     };
-    bool ok = mbar_wait(k_full, 0, 0x504);
-    if (ok) {
-      tc_fence_after();
-      qk();
-    }
+    bool ok = qk(0) && (tiles < 2 || qk(1));
     for (int j = 0; j < tiles && ok; j++) {
-      ok = mbar_wait(p_full, j & 1, 0x506) && mbar_wait(v_full, j & 1, 0x507);
+      const int buf = j & 1, turn = (j >> 1) & 1;
+      ok = mbar_wait(v_full + buf * 8, turn, 0x507) && mbar_wait(p_full + buf * 8, turn, 0x506);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
-      for (int s = 0; s < 8; s++)
-        tc_mma_f16_ts(o_tm, s_tm + s * 8, sw128_desc(v_sm + (s >> 2) * (D * 128) + (s & 3) * 32), idesc_f16_m128(D), (j | s) != 0);
-      tc_commit(o_done);
-      if (j + 1 < tiles) {
-        // S and P share columns: the order of MMAs with different accumulators is not promised
-        ok = mbar_wait(o_done, j & 1, 0x508) && mbar_wait(k_full, (j + 1) & 1, 0x504);
-        if (!ok) break;
-        tc_fence_after();
-        qk();
-      }
+      for (int s = 0; s < 4; s++)
+        tc_mma_f16_ts(o_tm, s_tm + buf * 64 + s * 8, v_desc + buf * (L::kTile / 16) + s * 2, idesc_f16_m128(D), (j | s) != 0);
+      tc_commit(o_done + buf * 8);
+      // QK j + 2 takes the columns of P j: the order of MMAs with different accumulators is not promised
+      if (j + 2 < tiles) ok = mbar_wait(o_done + buf * 8, turn, 0x508) && qk(j + 2);
     }
     if (!ok) abort_flag = 1;
   }
