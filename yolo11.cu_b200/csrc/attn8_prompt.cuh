@@ -326,30 +326,30 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     // ---------------- codes to fp16 tiles ----------------
     const int w = warp - 4, u0 = tid - 128;
     const int* table = a.table + r * a.table_stride;
-    const auto block_at = [&](int j) -> int {            // of 16-token group `lane` (< 4) of tile j; -1: none
+    // table entry of 16-token group `lane` (< 4) of tile j, as it is; -1: none
+    const auto entry = [&](int j) -> int {
       const int key = (j0 + j) * 64 + lane * 16;
-      if (lane >= 4 || j >= tiles || key >= hi_key) return -1;
-      const int b = table[key / T];
-      return (unsigned)b < (unsigned)c.blocks ? b : -1;
+      return lane < 4 && j < tiles && key < hi_key ? table[key / T] : -1;
     };
-    const auto token_at = [&](const void* codes, int id, int key) {
-      return (const uint8_t*)codes + id * c.block_stride + ((long long)kh * T + (key & (T - 1))) * D;
-    };
-    // keys: pieces (slab of 64 channels, 8 rows); lane: row lane / 4, 16 channels (lane % 4) of the slab
+    const auto in_pool = [&](int b) { return (unsigned)b < (unsigned)c.blocks ? b : -1; };
+    const int wrap = min(T, 64) - 1;      // tokens of a block that a tile's groups repeat after
+    // keys: warp w takes group w, 16 rows: lane row lane / 4 (and 8 more), 16 channels (lane % 4) of each slab
+    const uint8_t* kbase = (const uint8_t*)c.k + ((long long)kh * T + ((w * 16 + lane / 4) & wrap)) * D + (lane & 3) * 16;
     uint4 kv[L::kK];
     const auto load_k = [&](int j, int ids) {
+      const int id = __shfl_sync(~0u, ids, w), key0 = (j0 + j) * 64, left = id < 0 ? 0 : hi_key - key0 - w * 16;
+      const uint8_t* at = kbase + max(id, 0) * c.block_stride + (key0 & (T - 1)) * D;
 #pragma unroll
       for (int i = 0; i < L::kK; i++) {
-        const int piece = w + 4 * i, slab = piece % (D / 64), row = piece / (D / 64) * 8 + lane / 4;
-        const int id = __shfl_sync(~0u, ids, row >> 4), key = (j0 + j) * 64 + row;
+        const int slab = i % (D / 64), more = i / (D / 64) * 8;
         kv[i] = make_uint4(0, 0, 0, 0);
-        if (id >= 0 && key < hi_key) kv[i] = *(const uint4*)(token_at(c.k, id, key) + slab * 64 + (lane & 3) * 16);
+        if (lane / 4 + more < left) kv[i] = *(const uint4*)(at + more * D + slab * 64);
       }
     };
     const auto store_k = [&](uint32_t tile_at) {
 #pragma unroll
       for (int i = 0; i < L::kK; i++) {
-        const int piece = w + 4 * i, slab = piece % (D / 64), row = piece / (D / 64) * 8 + lane / 4;
+        const int slab = i % (D / 64), row = w * 16 + lane / 4 + i / (D / 64) * 8;
         uint32_t h[8];
         e4m3x4_to_half2x2(kv[i].x, h[0], h[1]);
         e4m3x4_to_half2x2(kv[i].y, h[2], h[3]);
@@ -361,19 +361,18 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       }
     };
     // values: piece u: tokens 8 * (u % 8) .., channels 8 * (u / 8) ..
+    const uint8_t* vbase = (const uint8_t*)c.v + ((long long)kh * T + (((u0 & 7) * 8) & wrap)) * D + (u0 >> 3) * 8;
     uint2 vv[L::kV][8];
     const auto load_v = [&](int j, int ids) {
+      const int id = __shfl_sync(~0u, ids, (u0 & 7) >> 1), key0 = (j0 + j) * 64, left = id < 0 ? 0 : hi_key - key0 - (u0 & 7) * 8;
+      const uint8_t* at = vbase + max(id, 0) * c.block_stride + (key0 & (T - 1)) * D;
 #pragma unroll
-      for (int x = 0; x < L::kV; x++) {
-        const int u = u0 + 128 * x, id = __shfl_sync(~0u, ids, (u & 7) >> 1);
-        const int key = (j0 + j) * 64 + (u & 7) * 8;
-        const uint8_t* v = token_at(c.v, max(id, 0), key) + (u >> 3) * 8;
+      for (int x = 0; x < L::kV; x++)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           vv[x][i] = make_uint2(0, 0);
-          if (id >= 0 && key + i < hi_key && u < D) vv[x][i] = *(const uint2*)(v + i * D);
+          if (i < left && u0 + 128 * x < D) vv[x][i] = *(const uint2*)(at + i * D + x * 128);
         }
-      }
     };
     const auto store_v = [&](int j, uint32_t tile_at) {
       const int key0 = (j0 + j) * 64;
@@ -416,31 +415,34 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
         }
       }
     };
-    int ids = block_at(0), ids_next = block_at(1);
+    // one tile ahead: codes and scales; two tiles ahead: table entries
+    int ids = in_pool(entry(0)), ahead = entry(1);
+    const auto scale_of = [&](const float* scales, int id) { return scales[max(id, 0) * c.scale_stride + kh]; };
     load_k(0, ids);
     load_v(0, ids);
+    float ks = scale_of(c.kscale, ids), vs = scale_of(c.vscale, ids);
     for (int j = 0; j < tiles; j++) {
       const int buf = j & 1, before = ((j >> 1) - 1) & 1;      // turn of tile j - 2 in the same buffers
-      const float ks = ids >= 0 ? c.kscale[ids * c.scale_stride + kh] : -1.f;
-      const float vs = ids >= 0 ? c.vscale[ids * c.scale_stride + kh] : 0.f;
-      const int ids_after = block_at(j + 2);
+      const int ids_next = in_pool(ahead);
+      ahead = entry(j + 2);
       if (j > 1 && !mbar_wait(s_full + buf * 8, before, 0x501)) { abort_flag = 1; break; }   // QK j - 2 has read its keys
       store_k(k_sm + buf * L::kTile);
       if (w == 0 && lane < 4) {
-        ks_sm[j & 3][lane] = ks;
-        vs_sm[j & 3][lane] = vs;
-        lv_sm[j & 3][lane] = __log2f(vs);
+        ks_sm[j & 3][lane] = ids < 0 ? -1.f : ks;
+        vs_sm[j & 3][lane] = ids < 0 ? 0.f : vs;
+        lv_sm[j & 3][lane] = ids < 0 ? -INFINITY : __log2f(vs);
       }
       fence_proxy_async();
       mbar_arrive(k_full + buf * 8);
       load_k(j + 1, ids_next);
+      ks = scale_of(c.kscale, ids_next);
+      vs = scale_of(c.vscale, ids_next);
       if (j > 1 && !mbar_wait(o_done + buf * 8, before, 0x502)) { abort_flag = 1; break; }   // PV j - 2 its values
       store_v(j, v_sm + buf * L::kTile);
       fence_proxy_async();
       mbar_arrive(v_full + buf * 8);
       load_v(j + 1, ids_next);
       ids = ids_next;
-      ids_next = ids_after;
     }
   } else if (lane == 0) {
     // ---------------- MMA ----------------
