@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
   __shared__ volatile int abort_flag;
   __shared__ int nan_lo, nan_hi;                  // tiles of keys where a NaN value was taken out
   // scales of the 16-token groups of tile j at j % 4, with the logarithm of the value scale; ks < 0: not there
-  __shared__ float ks_sm[4][4], vs_sm[4][4], lv_sm[4][4];
+  __shared__ __align__(16) float ks_sm[4][4], vs_sm[4][4], lv_sm[4][4];
   const YkAttnKv8& a = p.a;
   const YkKvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -177,15 +177,15 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       if (!mbar_wait(s_full + buf * 8, turn, 0x503)) { abort_flag = 1; ok = false; break; }
       tc_fence_after();
       const int key0 = (j0 + j) * 64;
-      float kk[4], vs[4], lv[4];
+      __align__(16) float kk[4], vs[4], lv[4];
       bool gone = false;
+      *(float4*)kk = *(const float4*)ks_sm[j & 3];
+      *(float4*)vs = *(const float4*)vs_sm[j & 3];
+      *(float4*)lv = *(const float4*)lv_sm[j & 3];
 #pragma unroll
       for (int g = 0; g < 4; g++) {
-        const float k = ks_sm[j & 3][g];
-        gone |= k < 0.f;
-        kk[g] = fmaxf(k * fac, 1e-38f);      // above 0: masked scores stay -inf
-        vs[g] = vs_sm[j & 3][g];
-        lv[g] = lv_sm[j & 3][g];
+        gone |= kk[g] < 0.f;
+        kk[g] = fmaxf(kk[g] * fac, 1e-38f);      // above 0: masked scores stay -inf
       }
       const bool edge = gone || key0 < all_lo || key0 + 64 > all_hi;
       const int c_lo = first - key0, c_hi = last - key0;       // columns that this row sees
@@ -287,7 +287,8 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     if (ok && mbar_wait(o_done + ((tiles - 1) & 1) * 8, ((tiles - 1) >> 1) & 1, 0x505)) {
       tc_fence_after();
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      uint16_t* op = (uint16_t*)a.out + out_row * a.out_row + (long long)head * D;
+      // rows leave through shared memory (the key tiles, no longer in use) so that they are stored whole
+      const uint32_t stage = k_sm + warp * (64 * D);
       // o is relative to M, l to m
       const float k = (m == kNone ? 0.f : ex2(M - m)) * inv;
       const int n_lo = nan_lo, n_hi = nan_hi;
@@ -308,16 +309,27 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
               if ((v[i] & 0x7f) == 0x7f) o[i] = 0x7fffffffu;
           }
         }
-        if (tid < row_n) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint32_t u[4];
+        for (int i = 0; i < 32; i += 8) {
+          uint32_t u[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              u[e] = float2_to_pair<BF16>(__uint_as_float(o[i + 2 * e]) * k, __uint_as_float(o[i + 2 * e + 1]) * k);
-            *(uint4*)(op + c0 + i) = make_uint4(u[0], u[1], u[2], u[3]);
-          }
+          for (int e = 0; e < 4; e++)
+            u[e] = float2_to_pair<BF16>(__uint_as_float(o[i + 2 * e]) * k, __uint_as_float(o[i + 2 * e + 1]) * k);
+          const int ch = (c0 + i) / 8;
+          sts128(stage + lane * (2 * D) + ((ch ^ (lane & 7)) << 4), u[0], u[1], u[2], u[3]);
         }
+      }
+      __syncwarp();
+      constexpr int kChunks = D / 8, kRows = 32 / kChunks > 1 ? 32 / kChunks : 1;   // 16-byte chunks of a row; rows an instruction stores
+      const long long mine = out_row * a.out_row + (long long)head * D;
+#pragma unroll 4
+      for (int i = 0; i < 32; i += kRows) {
+        const int row = i + lane / kChunks % kRows, ch = lane % kChunks;
+        const long long to = __shfl_sync(~0u, mine, row);
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(stage + row * (2 * D) + ((ch ^ (row & 7)) << 4)));
+        if (warp * 32 + row < row_n) *(uint4*)((uint16_t*)a.out + to + ch * 8) = v;
       }
       if (a.lse && tid < row_n)
         a.lse[out_row * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
@@ -415,6 +427,25 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
         }
       }
     };
+    // kAhead tiles ahead the codes are called into L2, a line (128 bytes) a lane: half of the lanes
+    // the keys, half the values of group w; its block id is read one tile before that
+    constexpr int kAhead = 4, kLines = 16 * D / 128;
+    const auto far_entry = [&](int j) -> int {
+      const int key = (j0 + j) * 64 + w * 16;
+      return j < tiles && key < hi_key ? table[key / T] : -1;
+    };
+    const auto call = [&](int j, int raw) {
+      const int id = in_pool(raw), key0 = (j0 + j) * 64;
+      const uint8_t* at = (const uint8_t*)(lane < 16 ? c.k : c.v) + id * c.block_stride +
+                          ((long long)kh * T + ((key0 + w * 16) & (T - 1))) * D;
+      if (id >= 0)
+        for (int line = lane & 15; line < kLines; line += 16) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + line * 128));
+    };
+    int far = far_entry(1);
+    for (int j = 1; j <= kAhead; j++) {
+      call(j, far);
+      far = far_entry(j + 1);
+    }
     // one tile ahead: codes and scales; two tiles ahead: table entries
     int ids = in_pool(entry(0)), ahead = entry(1);
     const auto scale_of = [&](const float* scales, int id) { return scales[max(id, 0) * c.scale_stride + kh]; };
@@ -425,6 +456,8 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       const int buf = j & 1, before = ((j >> 1) - 1) & 1;      // turn of tile j - 2 in the same buffers
       const int ids_next = in_pool(ahead);
       ahead = entry(j + 2);
+      call(j + kAhead + 1, far);
+      far = far_entry(j + kAhead + 2);
       if (j > 1 && !mbar_wait(s_full + buf * 8, before, 0x501)) { abort_flag = 1; break; }   // QK j - 2 has read its keys
       store_k(k_sm + buf * L::kTile);
       if (w == 0 && lane < 4) {
