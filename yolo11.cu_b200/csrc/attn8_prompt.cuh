@@ -9,9 +9,8 @@
 //    the reference moves, O is rescaled, and the tile is done again.  P goes as fp16 over the columns of
 //    its S: it is the A operand straight from TMEM.
 //  * warps 4-7 read the codes of the next tile into registers while this one's are in use, convert them
-//    (exactly) to fp16 and write them into the 128-byte-swizzled K-major tiles that the MMA reads: keys
-//    as they are, values transposed, 8 tokens a 16-byte store, by interleaving the bytes of token
-//    pairs.
+//    (exactly) to fp16 and write them into 128-byte-swizzled tiles [slab of 64 channels][token][64], which
+//    the MMA reads as a K-major operand for the keys and as an MN-major one for the values.
 //  * one thread of warp 8 issues the MMAs.  Everything comes twice (S and P, keys, values), so QK of
 //    tile j + 1 is done before the softmax of tile j is, and PV of tile j runs beside the softmax of
 //    tile j + 1.
@@ -24,7 +23,6 @@ struct Pro {
   static constexpr int kSmem = 6 * kTile + 1024;        // q (128 rows), two of keys, two of values; alignment
   static constexpr int kCols = D == 256 ? 512 : 256;    // TMEM columns: S twice 64, O D
   static constexpr int kK = 2 * (D / 64);               // 16-byte code chunks of a converting thread
-  static constexpr int kV = D == 256 ? 2 : 1;           // its 8-token x 8-channel pieces
 };
 
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, fp16 inputs, fp32 accumulate.
@@ -36,6 +34,12 @@ __device__ __forceinline__ void tc_mma_f16_ts(uint32_t dtmem, uint32_t atmem, ui
       "r"(atmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// Shared-memory descriptor of an MN-major operand in the 128-byte swizzle layout: slabs of 64 elements
+// (128-byte rows, one for each k) `slab` bytes apart, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t slab) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(slab >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+constexpr uint32_t kBMnMajor = 1u << 16;       // instruction descriptor: B is MN-major
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
@@ -336,7 +340,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     }
   } else if (warp < 8) {
     // ---------------- codes to fp16 tiles ----------------
-    const int w = warp - 4, u0 = tid - 128;
+    const int w = warp - 4;
     const int* table = a.table + r * a.table_stride;
     // table entry of 16-token group `lane` (< 4) of tile j, as it is; -1: none
     const auto entry = [&](int j) -> int {
@@ -345,86 +349,50 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     };
     const auto in_pool = [&](int b) { return (unsigned)b < (unsigned)c.blocks ? b : -1; };
     const int wrap = min(T, 64) - 1;      // tokens of a block that a tile's groups repeat after
-    // keys: warp w takes group w, 16 rows: lane row lane / 4 (and 8 more), 16 channels (lane % 4) of each slab
-    const uint8_t* kbase = (const uint8_t*)c.k + ((long long)kh * T + ((w * 16 + lane / 4) & wrap)) * D + (lane & 3) * 16;
-    uint4 kv[L::kK];
-    const auto load_k = [&](int j, int ids) {
+    // warp w takes group w, 16 rows: lane row lane / 4 (and 8 more), 16 channels (lane % 4) of each slab
+    const long long mine = ((long long)kh * T + ((w * 16 + lane / 4) & wrap)) * D + (lane & 3) * 16;
+    uint4 kv[L::kK], vv[L::kK];
+    const auto load = [&](uint4 (&x)[L::kK], const void* codes, int j, int ids) {
       const int id = __shfl_sync(~0u, ids, w), key0 = (j0 + j) * 64, left = id < 0 ? 0 : hi_key - key0 - w * 16;
-      const uint8_t* at = kbase + max(id, 0) * c.block_stride + (key0 & (T - 1)) * D;
+      const uint8_t* at = (const uint8_t*)codes + mine + max(id, 0) * c.block_stride + (key0 & (T - 1)) * D;
 #pragma unroll
       for (int i = 0; i < L::kK; i++) {
         const int slab = i % (D / 64), more = i / (D / 64) * 8;
-        kv[i] = make_uint4(0, 0, 0, 0);
-        if (lane / 4 + more < left) kv[i] = *(const uint4*)(at + more * D + slab * 64);
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (lane / 4 + more < left) x[i] = *(const uint4*)(at + more * D + slab * 64);
       }
     };
-    const auto store_k = [&](uint32_t tile_at) {
+    // chunk pairs (lane % 4) * 2, + 1 of row lane / 4 of the group: the same place in the swizzle 8 rows on
+    const uint32_t to0 = swz_at(w * 16 + lane / 4, (lane & 3) * 2), to1 = swz_at(w * 16 + lane / 4, (lane & 3) * 2 + 1);
+    const auto store = [&](const uint4 (&x)[L::kK], uint32_t tile_at) {
 #pragma unroll
       for (int i = 0; i < L::kK; i++) {
-        const int slab = i % (D / 64), row = w * 16 + lane / 4 + i / (D / 64) * 8;
+        const uint32_t at = tile_at + i % (D / 64) * 8192 + i / (D / 64) * 1024;
         uint32_t h[8];
-        e4m3x4_to_half2x2(kv[i].x, h[0], h[1]);
-        e4m3x4_to_half2x2(kv[i].y, h[2], h[3]);
-        e4m3x4_to_half2x2(kv[i].z, h[4], h[5]);
-        e4m3x4_to_half2x2(kv[i].w, h[6], h[7]);
-        const uint32_t at = tile_at + slab * 8192;
-        sts128(at + swz_at(row, (lane & 3) * 2), h[0], h[1], h[2], h[3]);
-        sts128(at + swz_at(row, (lane & 3) * 2 + 1), h[4], h[5], h[6], h[7]);
+        e4m3x4_to_half2x2(x[i].x, h[0], h[1]);
+        e4m3x4_to_half2x2(x[i].y, h[2], h[3]);
+        e4m3x4_to_half2x2(x[i].z, h[4], h[5]);
+        e4m3x4_to_half2x2(x[i].w, h[6], h[7]);
+        sts128(at + to0, h[0], h[1], h[2], h[3]);
+        sts128(at + to1, h[4], h[5], h[6], h[7]);
       }
     };
-    // values: piece u: tokens 8 * (u % 8) .., channels 8 * (u / 8) ..
-    const uint8_t* vbase = (const uint8_t*)c.v + ((long long)kh * T + (((u0 & 7) * 8) & wrap)) * D + (u0 >> 3) * 8;
-    uint2 vv[L::kV][8];
-    const auto load_v = [&](int j, int ids) {
-      const int id = __shfl_sync(~0u, ids, (u0 & 7) >> 1), key0 = (j0 + j) * 64, left = id < 0 ? 0 : hi_key - key0 - (u0 & 7) * 8;
-      const uint8_t* at = vbase + max(id, 0) * c.block_stride + (key0 & (T - 1)) * D;
+    // 0 * NaN: a NaN value that some row does not see is taken out here, see the end
+    const auto take_out = [&](int j) {
+      uint32_t any = 0;
 #pragma unroll
-      for (int x = 0; x < L::kV; x++)
+      for (int i = 0; i < L::kK; i++) {
+        uint32_t* v = (uint32_t*)&vv[i];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          vv[x][i] = make_uint2(0, 0);
-          if (i < left && u0 + 128 * x < D) vv[x][i] = *(const uint2*)(at + i * D + x * 128);
+        for (int e = 0; e < 4; e++) {
+          const uint32_t nan = ((v[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+          any |= nan;
+          v[e] &= ~((nan >> 7) * 0xffu);
         }
-    };
-    const auto store_v = [&](int j, uint32_t tile_at) {
-      const int key0 = (j0 + j) * 64;
-      const bool edge = key0 < all_lo || key0 + 64 > all_hi;
-#pragma unroll
-      for (int x = 0; x < L::kV; x++) {
-        const int u = u0 + 128 * x;
-        if (u >= D) break;
-        if (edge) {       // 0 * NaN: a NaN that some row does not see is taken out here, see the end
-          uint32_t any = 0;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            uint32_t* v = (uint32_t*)&vv[x][i];
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              const uint32_t nan = ((v[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-              any |= nan;
-              v[e] &= ~((nan >> 7) * 0xffu);
-            }
-          }
-          if (any) {
-            atomicMin(&nan_lo, j0 + j);
-            atomicMax(&nan_hi, j0 + j);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          uint32_t lo[4][2], hi[4][2];      // token pairs of channels 4 e + 0, 1 and 2, 3
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t x0 = ((const uint32_t*)&vv[x][2 * i])[e], x1 = ((const uint32_t*)&vv[x][2 * i + 1])[e];
-            e4m3x4_to_half2x2(__byte_perm(x0, x1, 0x5140), lo[i][0], lo[i][1]);
-            e4m3x4_to_half2x2(__byte_perm(x0, x1, 0x7362), hi[i][0], hi[i][1]);
-          }
-          const int d = (u >> 3) * 8 + e * 4;
-          sts128(tile_at + swz_at(d, u & 7), lo[0][0], lo[1][0], lo[2][0], lo[3][0]);
-          sts128(tile_at + swz_at(d + 1, u & 7), lo[0][1], lo[1][1], lo[2][1], lo[3][1]);
-          sts128(tile_at + swz_at(d + 2, u & 7), hi[0][0], hi[1][0], hi[2][0], hi[3][0]);
-          sts128(tile_at + swz_at(d + 3, u & 7), hi[0][1], hi[1][1], hi[2][1], hi[3][1]);
-        }
+      }
+      if (any) {
+        atomicMin(&nan_lo, j0 + j);
+        atomicMax(&nan_hi, j0 + j);
       }
     };
     // kAhead tiles ahead the codes are called into L2, a line (128 bytes) a lane: half of the lanes
@@ -449,8 +417,8 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     // one tile ahead: codes and scales; two tiles ahead: table entries
     int ids = in_pool(entry(0)), ahead = entry(1);
     const auto scale_of = [&](const float* scales, int id) { return scales[max(id, 0) * c.scale_stride + kh]; };
-    load_k(0, ids);
-    load_v(0, ids);
+    load(kv, c.k, 0, ids);
+    load(vv, c.v, 0, ids);
     float ks = scale_of(c.kscale, ids), vs = scale_of(c.vscale, ids);
     for (int j = 0; j < tiles; j++) {
       const int buf = j & 1, before = ((j >> 1) - 1) & 1;      // turn of tile j - 2 in the same buffers
@@ -459,7 +427,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       call(j + kAhead + 1, far);
       far = far_entry(j + kAhead + 2);
       if (j > 1 && !mbar_wait(s_full + buf * 8, before, 0x501)) { abort_flag = 1; break; }   // QK j - 2 has read its keys
-      store_k(k_sm + buf * L::kTile);
+      store(kv, k_sm + buf * L::kTile);
       if (w == 0 && lane < 4) {
         ks_sm[j & 3][lane] = ids < 0 ? -1.f : ks;
         vs_sm[j & 3][lane] = ids < 0 ? 0.f : vs;
@@ -467,19 +435,21 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       }
       fence_proxy_async();
       mbar_arrive(k_full + buf * 8);
-      load_k(j + 1, ids_next);
+      load(kv, c.k, j + 1, ids_next);
       ks = scale_of(c.kscale, ids_next);
       vs = scale_of(c.vscale, ids_next);
       if (j > 1 && !mbar_wait(o_done + buf * 8, before, 0x502)) { abort_flag = 1; break; }   // PV j - 2 its values
-      store_v(j, v_sm + buf * L::kTile);
+      const int key0 = (j0 + j) * 64;
+      if (key0 < all_lo || key0 + 64 > all_hi) take_out(j);
+      store(vv, v_sm + buf * L::kTile);
       fence_proxy_async();
       mbar_arrive(v_full + buf * 8);
-      load_v(j + 1, ids_next);
+      load(vv, c.v, j + 1, ids_next);
       ids = ids_next;
     }
   } else if (lane == 0) {
     // ---------------- MMA ----------------
-    const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(k_sm), v_desc = sw128_desc(v_sm);   // addresses count 16 bytes
+    const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(k_sm), v_desc = sw128_mn_desc(v_sm, 8192);   // addresses count 16 bytes
     const auto qk = [&](int j) {
       const int buf = j & 1;
       if (!mbar_wait(k_full + buf * 8, (j >> 1) & 1, 0x504)) return false;
@@ -499,7 +469,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       tc_fence_after();
 #pragma unroll
       for (int s = 0; s < 4; s++)
-        tc_mma_f16_ts(o_tm, s_tm + buf * 64 + s * 8, v_desc + buf * (L::kTile / 16) + s * 2, idesc_f16_m128(D), (j | s) != 0);
+        tc_mma_f16_ts(o_tm, s_tm + buf * 64 + s * 8, v_desc + buf * (L::kTile / 16) + s * 128, idesc_f16_m128(D) | kBMnMajor, (j | s) != 0);
       tc_commit(o_done + buf * 8);
       // QK j + 2 takes the columns of P j: the order of MMAs with different accumulators is not promised
       if (j + 2 < tiles) ok = mbar_wait(o_done + buf * 8, turn, 0x508) && qk(j + 2);
