@@ -16,6 +16,7 @@
 //    tile j + 1.
 // Two CTAs an SM up to 128 channels.
 constexpr int kProThreads = 288;
+constexpr int kProSort = 128;          // requests up to which tiles are ordered by their length
 
 template <int D>
 struct Pro {
@@ -72,19 +73,76 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
   pdl_wait();
   pdl_trigger();
 
-  // Request r owns the tile numbers from rows_before * G / 128 + r on: at least as many as it has
-  // tiles.  Later tiles of a request see more keys, so high numbers go first.
-  const int kh = blockIdx.x % c.heads;
-  const long long number = gridDim.x / c.heads - 1 - blockIdx.x / c.heads;
-  const auto first_number = [&](int r) { return (long long)min(max(a.cu[r], 0), a.rows) * G / 128 + r; };
+  const int kh = blockIdx.x % c.heads, index = blockIdx.x / c.heads;
   int r = 0;
-  for (int hi = a.requests; hi - r > 1;) {
-    const int m = (r + hi) >> 1;
-    if (first_number(m) <= number) r = m; else hi = m;
+  long long tile;
+  Req rq;
+  if (a.requests <= kProSort) {
+    // Tiles in descending order of the keys they see, in tiles of 64 (then of request and tile), so
+    // that the longest start first.  A request's tiles see more and more: those of length >= n start
+    // at tile `from`.  Every warp finds tile `index` by itself, its lanes sharing the requests out.
+    const auto all_tiles = [&](const Req& q) { return (int)(((long long)q.q * G + 127) / 128); };
+    const auto from = [&](const Req& q, int n) {
+      const long long key = (n - 1) * 64ll;                    // the first key past n - 1 tiles is seen
+      if (n <= 0) return 0;
+      if (!a.causal) return q.kv > key ? 0 : all_tiles(q);
+      const long long t = key - q.kv + q.q;                    // from this token on
+      return t >= q.q ? all_tiles(q) : t <= 0 ? 0 : (int)(t * G / 128);
+    };
+    const auto longer = [&](int n) {                           // tiles of length >= n, over all requests
+      int sum = 0;
+      for (int i = lane; i < a.requests; i += 32) {
+        const Req q = attn_req(c, a, i);
+        sum += all_tiles(q) - from(q, n);
+      }
+      return (int)__reduce_add_sync(~0u, (unsigned)sum);
+    };
+    if (index >= longer(0)) return;
+    int n = 0, most = 0;
+    for (int i = lane; i < a.requests; i += 32) most = max(most, attn_req(c, a, i).kv);
+    for (int hi = __reduce_max_sync(~0u, most) / 64 + 2; hi - n > 1;) {     // longer(n) > index >= longer(hi)
+      const int m = (n + hi) >> 1;
+      if (longer(m) > index) n = m; else hi = m;
+    }
+    int rank = index - longer(n + 1);                          // among the tiles of length n
+    tile = -1;
+    for (int i0 = 0; i0 < a.requests && tile < 0; i0 += 32) {
+      int mine = 0, first = 0;
+      if (i0 + lane < a.requests) {
+        const Req q = attn_req(c, a, i0 + lane);
+        first = from(q, n);
+        mine = from(q, n + 1) - first;
+      }
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned past = __ballot_sync(~0u, upto > rank);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        r = i0 + l;
+        tile = __shfl_sync(~0u, first + rank - (upto - mine), l);
+      }
+      rank -= __shfl_sync(~0u, upto, 31);
+    }
+    if (tile < 0) return;
+    rq = attn_req(c, a, r);
+  } else {
+    // Request r owns the tile numbers from rows_before * G / 128 + r on: at least as many as it has
+    // tiles.  High numbers go first.
+    const long long number = gridDim.x / c.heads - 1 - index;
+    const auto first_number = [&](int r) { return (long long)min(max(a.cu[r], 0), a.rows) * G / 128 + r; };
+    for (int hi = a.requests; hi - r > 1;) {
+      const int m = (r + hi) >> 1;
+      if (first_number(m) <= number) r = m; else hi = m;
+    }
+    rq = attn_req(c, a, r);
+    tile = number - first_number(r);
+    if (tile < 0) return;
   }
-  const Req rq = attn_req(c, a, r);
-  const long long tile = number - first_number(r);
-  if (tile < 0 || tile * 128 >= (long long)rq.q * G) return;
+  if (tile * 128 >= (long long)rq.q * G) return;
   const int row0 = (int)tile * 128, row_n = min(128, rq.q * G - row0);
   const int t0 = row0 / G, t1 = (row0 + row_n - 1) / G;              // the tile's tokens
   const int hi_key = a.causal ? max(0, rq.kv - rq.q + t1 + 1) : rq.kv;   // keys that some row sees: [lo_key, hi_key)
