@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
   extern __shared__ uint8_t pro_raw[];
   __shared__ __align__(8) uint64_t bars[10];
   __shared__ uint32_t tslot;
+  __shared__ int found_r, found_tile;
   __shared__ volatile int abort_flag;
   __shared__ int nan_lo, nan_hi;                  // tiles of keys where a NaN value was taken out
   // scales of the 16-token groups of tile j at j % 4, with the logarithm of the value scale; ks < 0: not there
@@ -75,12 +76,11 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
 
   const int kh = blockIdx.x % c.heads, index = blockIdx.x / c.heads;
   int r = 0;
-  long long tile;
-  Req rq;
-  if (a.requests <= kProSort) {
+  long long tile = -1;
+  if (a.requests <= kProSort && warp == 0) {
     // Tiles in descending order of the keys they see, in tiles of 64 (then of request and tile), so
     // that the longest start first.  A request's tiles see more and more: those of length >= n start
-    // at tile `from`.  Every warp finds tile `index` by itself, its lanes sharing the requests out.
+    // at tile `from`.  One warp finds tile `index`, its lanes sharing the requests out.
     const auto all_tiles = [&](const Req& q) { return (int)(((long long)q.q * G + 127) / 128); };
     const auto from = [&](const Req& q, int n) {
       const long long key = (n - 1) * 64ll;                    // the first key past n - 1 tiles is seen
@@ -97,7 +97,6 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       }
       return (int)__reduce_add_sync(~0u, (unsigned)sum);
     };
-    if (index >= longer(0)) return;
     int n = 0, most = 0;
     for (int i = lane; i < a.requests; i += 32) most = max(most, attn_req(c, a, i).kv);
     for (int hi = __reduce_max_sync(~0u, most) / 64 + 2; hi - n > 1;) {     // longer(n) > index >= longer(hi)
@@ -105,8 +104,8 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       if (longer(m) > index) n = m; else hi = m;
     }
     int rank = index - longer(n + 1);                          // among the tiles of length n
-    tile = -1;
-    for (int i0 = 0; i0 < a.requests && tile < 0; i0 += 32) {
+    const int end = index < longer(0) ? a.requests : 0;
+    for (int i0 = 0; i0 < end && tile < 0; i0 += 32) {
       int mine = 0, first = 0;
       if (i0 + lane < a.requests) {
         const Req q = attn_req(c, a, i0 + lane);
@@ -127,8 +126,15 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       }
       rank -= __shfl_sync(~0u, upto, 31);
     }
-    if (tile < 0) return;
-    rq = attn_req(c, a, r);
+    if (lane == 0) {
+      found_r = r;
+      found_tile = (int)tile;
+    }
+  }
+  if (a.requests <= kProSort) {
+    __syncthreads();
+    r = found_r;
+    tile = found_tile;
   } else {
     // Request r owns the tile numbers from rows_before * G / 128 + r on: at least as many as it has
     // tiles.  High numbers go first.
@@ -138,10 +144,10 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       const int m = (r + hi) >> 1;
       if (first_number(m) <= number) r = m; else hi = m;
     }
-    rq = attn_req(c, a, r);
     tile = number - first_number(r);
-    if (tile < 0) return;
   }
+  if (tile < 0) return;
+  const Req rq = attn_req(c, a, r);
   if (tile * 128 >= (long long)rq.q * G) return;
   const int row0 = (int)tile * 128, row_n = min(128, rq.q * G - row0);
   const int t0 = row0 / G, t1 = (row0 + row_n - 1) / G;              // the tile's tokens
