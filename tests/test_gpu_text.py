@@ -590,6 +590,20 @@ def test_gemv(lib, cuda, kind, rows, n, k, group):
     run_gemv(lib, rt, kind, rows, n, k, group, shift=1)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,n,k,group", [
+    (1, 9472, 128, 128), (5, 9500, 1024, 64), (16, 9473, 672, 32), (17, 9600, 1280, 128), (33, 9472, 576, 64),
+    (64, 9489, 288, 32), (64, 9475, 640, 128), (40, 9472, 1152, 64), (2, 9472, 32, 32), (9, 9601, 4224, 128)])
+def test_gemv_many_outputs(lib, cuda, kind, rows, n, k, group):
+    from yolo11_cu_b200 import runtime as rt
+    run_gemv(lib, rt, kind, rows, n, k, group)
+    run_gemv(lib, rt, kind, rows, n, k, group, zero=True, bias=True, extra=1)
+    run_gemv(lib, rt, kind, rows, n, k, group, xgroup=0, bias=True, shift=1)
+    run_gemv(lib, rt, kind, rows, n, k, group, xgroup=128, zero=True, extra=8)
+    run_gemv(lib, rt, kind, rows, n, k, group, xgroup=384, shift=8)
+    run_gemv(lib, rt, kind, rows, n, k, group, xgroup=3 * group, shift=3)
+
+
 def test_gemv_large_values(lib, cuda):
     """fp16 x near its largest value: sums stay in 32 bits; x of infinities gives no finite sum."""
     from yolo11_cu_b200 import runtime as rt
