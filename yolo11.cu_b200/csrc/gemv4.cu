@@ -72,19 +72,24 @@ __device__ __forceinline__ Zero zero_of(uint32_t z) {
   if (F16) return {0x64006400u + z * 0x10001u, 0xd400d400u + z * 0x100010u};   // 1024 + z, -(64 + z)
   return {0x43004300u + z * 0x10001u, 0};                                      // 128 + z
 }
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {   // (a & b) | c
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
 // The 8 codes of a word minus the zero point: pairs (0, 4), (1, 5), (2, 6), (3, 7).
 // fp16: 1024 + q in the low nibble's place; 1024 + 16 q a nibble higher, times 1/16.
 template <bool F16>
 __device__ __forceinline__ void codes8(uint32_t w, const Zero& z, uint32_t (&o)[4]) {
   if (F16) {
-    o[0] = hsub2((w & 0x000f000fu) | 0x64006400u, z.a);
-    o[1] = hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z.b);
+    o[0] = hsub2(and_or(w, 0x000f000fu, 0x64006400u), z.a);
+    o[1] = hfma2(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, z.b);
     w >>= 8;
-    o[2] = hsub2((w & 0x000f000fu) | 0x64006400u, z.a);
-    o[3] = hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z.b);
+    o[2] = hsub2(and_or(w, 0x000f000fu, 0x64006400u), z.a);
+    o[3] = hfma2(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, z.b);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = bsub2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u, z.a);
+    for (int i = 0; i < 4; i++) o[i] = bsub2(and_or(w >> (4 * i), 0x000f000fu, 0x43004300u), z.a);
   }
 }
 template <int NT, int R>

@@ -13,7 +13,9 @@
 //  * One thread of the last warp issues the MMAs.
 template <int XT, int GB, int N>
 struct GemvTc {
-  static constexpr int kStageWarps = N == 16 ? 2 : 4;
+  static constexpr int kTeam = N / 16;                             // warps that stage a chunk of x together
+  static constexpr int kTeams = N == 16 ? 4 : 2;                   // chunks in the making: a load's latency each
+  static constexpr int kStageWarps = kTeam * kTeams;
   static constexpr int kThreads = (8 + kStageWarps + 1) * 32;
   static constexpr int kStages = 4, kXStages = 4;
   static constexpr int kUnits = GB == 1 ? 2 : 1;                   // accumulators of a half
@@ -24,7 +26,7 @@ struct GemvTc {
   static constexpr int kRing = 2 * kStages * 128 * 64;             // codes
   static constexpr int kX = N * 256;                               // x of a chunk
   static constexpr int kSmem = kRing + kXStages * kX + 1024;
-  static constexpr int kPieces = N * 16 / (kStageWarps * 32);      // 8-column pieces of x a staging thread
+  static constexpr int kPieces = 8;                                // 8-column pieces of x a staging thread and chunk
 };
 
 template <int XT, int GB, int N>
@@ -52,7 +54,7 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
       mbar_init(done + i * 8, 1);
     }
     for (int i = 0; i < S::kXStages; i++) {
-      mbar_init(x_full + i * 8, S::kStageWarps * 32);
+      mbar_init(x_full + i * 8, S::kTeam * 32);
       mbar_init(x_free + i * 8, 1);
     }
     mbar_fence_init();
@@ -179,15 +181,20 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
     cp_async_wait<0>();
   } else if (warp < kMmaWarp) {
     // ---------------- x ----------------
-    const int st = tid - 256;
+    // team t takes chunks t, t + kTeams, ..; a lane 8 columns of every other row of its warp's 16
+    const int team = (warp - 8) / S::kTeam, row0 = (warp - 8) % S::kTeam * 16 + (lane >> 4), ch = lane & 15;
     constexpr int kSize = X8 ? 1 : 2;
+    const uint8_t* const x0 = (const uint8_t*)p.x + ((long long)row0 * p.x_row + ch * 8) * kSize;
+    const long long step = 2 * p.x_row * kSize;
+    const int m_xs = (warp - 8) % S::kTeam * 32 + lane;             // (lanes below N in all) reads a row's scale
     uint32_t raw[S::kPieces][2 * kSize];
+    float xs = 1.f;
     const auto load = [&](int c) {
+      const bool in_k = c * 128 + ch * 8 < K;
 #pragma unroll
       for (int i = 0; i < S::kPieces; i++) {
-        const int piece = st + i * (S::kStageWarps * 32), m = piece / 16, k = c * 128 + piece % 16 * 8;
-        const uint8_t* x = (const uint8_t*)p.x + ((long long)m * p.x_row + k) * kSize;
-        const bool ok = m < p.rows && k < K;
+        const uint8_t* x = x0 + i * step + c * 128 * kSize;
+        const bool ok = in_k && row0 + 2 * i < p.rows;
         if (ga.x_vec) {
           if (X8) {
             const uint2 u = ok ? *(const uint2*)x : make_uint2(0, 0);
@@ -206,16 +213,16 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
           }
         }
       }
+      if (X8 && ga.xgroup && m_xs < N && c < chunks)
+        xs = p.xscale[min(m_xs, p.rows - 1) * p.xscale_row + (ga.x_shift >= 0 ? c * 128 >> ga.x_shift : c * 128 / ga.xgroup)];
     };
-    load(0);
-    for (int c = 0; c < chunks; c++) {
+    load(team);
+    for (int c = team; c < chunks; c += S::kTeams) {
       const int stage = c % S::kXStages;
-      float xs = 1.f;
-      if (X8 && ga.xgroup && st < N) xs = p.xscale[min(st, p.rows - 1) * p.xscale_row + (ga.x_shift >= 0 ? c * 128 >> ga.x_shift : c * 128 / ga.xgroup)];
       if (c >= S::kXStages && !mbar_wait(x_free + stage * 8, (c / S::kXStages - 1) & 1, 0x602)) { abort_flag = 1; break; }
 #pragma unroll
       for (int i = 0; i < S::kPieces; i++) {
-        const int piece = st + i * (S::kStageWarps * 32), m = piece / 16, ch = piece % 16;
+        const int m = row0 + 2 * i;
         uint32_t o[4];
         if (X8) {
           e4m3x4_to_half2x2(__byte_perm(raw[i][0], raw[i][1], 0x5140), o[0], o[1]);
@@ -230,10 +237,10 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
                          x_sm + stage * S::kX + (ch >> 3) * (N * 128) + m * 128 + (((ch & 7) ^ (m & 7)) << 4)),
                      "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
       }
-      if (st < N) xs_sm[c & 7][st] = xs;
+      if (m_xs < N) xs_sm[c & 7][m_xs] = xs;
       fence_proxy_async();
       mbar_arrive(x_full + stage * 8);
-      load(c + 1);
+      load(c + S::kTeams);
     }
   } else if (lane == 0) {
     // ---------------- MMA ----------------
