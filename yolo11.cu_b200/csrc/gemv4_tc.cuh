@@ -5,8 +5,8 @@
 // (a TMEM lane): it turns its row's codes into 16-bit integers in registers (about one instruction a
 // code), stores them into TMEM as the A operand, and scales its own sums: one scale and zero point a
 // group, no shuffles.  x is the B operand in shared memory, staged once for all 128 outputs.
-//  * A chunk is 128 columns of 128 outputs; warps 0-3 take even chunks, warps 4-7 odd ones (each
-//    thread its output's 64 bytes, by cp.async into its own ring slots), as two halves of 64 columns.
+//  * A chunk is 128 columns of 128 outputs; warps 0-3 take even chunks, warps 4-7 odd ones (a warp its
+//    32 outputs' 64 bytes each, by cp.async), as two halves of 64 columns.
 //    Half h goes to A buffer h % 2 and its sums (one accumulator for each group, or half a group) to D
 //    buffer h % 2; a half's sums are read after the next half is stored, so the MMA runs behind.
 //  * The next warps stage x: 8 columns in the order (0, 4, 1, 5, 2, 6, 3, 7) that the codes come out in.
@@ -23,7 +23,8 @@ struct GemvTc {
   static constexpr bool kOneD = 4 * kUnits * N > 384;              // (or 2 x kUnits x N: one D buffer each)
   static constexpr int kNeed = kD0 + (kOneD ? 2 : 4) * kUnits * N;
   static constexpr int kCols = kNeed <= 256 ? 256 : 512;
-  static constexpr int kRing = 2 * kStages * 128 * 64;             // codes
+  static constexpr int kPlane = 128 * 16 + 32, kStage = 4 * kPlane;  // a 16-byte piece of 128 rows (banks apart), a chunk's four
+  static constexpr int kRing = 2 * kStages * kStage;               // codes
   static constexpr int kX = N * 256;                               // x of a chunk
   static constexpr int kSmem = kRing + kXStages * kX + 1024;
   static constexpr int kPieces = 8;                                // 8-column pieces of x a staging thread and chunk
@@ -84,18 +85,23 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
     const int set = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const long long n = min(n0 + row, p.n - 1);
-    const uint8_t* w = (const uint8_t*)p.w + n * p.w_row;
     const uint16_t* scales = (const uint16_t*)p.wscale + n * p.group_row;
     const uint8_t* zeros = (const uint8_t*)p.wzero + n * p.group_row;
     const bool zero = ga.zero;
     const int mine = chunks > set ? (chunks - set + 1) / 2 : 0, groups = K / (32 * GB);
-    const uint32_t slot = ring + set * (S::kStages * 8192) + row * 16;
+    const uint32_t slots = ring + set * (S::kStages * S::kStage), slot = slots + row * 16;
+    // a warp copies its own 32 rows, four lanes a row's 64 bytes: 8 lines an instruction, not 32
+    const int q_in = lane & 3, row_in = (warp & 3) * 32 + (lane >> 2);
+    const uint8_t* w_in[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w_in[i] = (const uint8_t*)p.w + min((long long)n0 + row_in + 8 * i, p.n - 1ll) * p.w_row + q_in * 16;
     const auto issue = [&](int i) {
       if (i < mine) {
         const int k = (set + 2 * i) * 128;
-        const uint32_t to = slot + (i % S::kStages) * 8192;
+        const uint32_t to = slots + (i % S::kStages) * S::kStage + q_in * S::kPlane + row_in * 16;
+        const bool ok = k + q_in * 32 < K;
 #pragma unroll
-        for (int q = 0; q < 4; q++) cp_async_at<16>(to + q * 2048, w + (k + q * 32 < K ? k / 2 + q * 16 : 0), k + q * 32 < K);
+        for (int x = 0; x < 4; x++) cp_async_at<16>(to + x * 128, w_in[x] + (ok ? k / 2 : 0), ok);
       }
       cp_async_commit();
     };
@@ -143,8 +149,10 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
     for (int h = 0; h < 2 * mine && ok; h++) {
       const int i = h >> 1, buf = h & 1;
       if (buf == 0) {
+        __syncwarp();                          // the stage that is filled next has been read
         issue(i + S::kStages - 1);
-        cp_async_wait<S::kStages - 1>();       // a thread reads only what it copied
+        cp_async_wait<S::kStages - 1>();
+        __syncwarp();                          // every lane's pieces are there
       }
       if (S::kOneD && h > 0 && !add_sums(h - 1)) { ok = false; break; }
       float s_now[S::kUnits];
@@ -155,11 +163,11 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
         z[u] = zero_of<F16>(z_next[u]);
       }
       load_scales(h + 1);
-      const uint32_t from = slot + (i % S::kStages) * 8192 + buf * 4096;
+      const uint32_t from = slot + (i % S::kStages) * S::kStage + buf * 2 * S::kPlane;
 #pragma unroll
       for (int q = 0; q < 2; q++) {            // 32 columns: 16 TMEM columns
         uint32_t v[4], a[16];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(from + q * 2048));
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(from + q * S::kPlane));
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           uint32_t o[4];
