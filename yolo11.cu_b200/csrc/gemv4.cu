@@ -22,6 +22,7 @@ struct Gemv4Args {
   YkGemv4 p;
   int x_vec;       // x rows allow 16-byte (e4m3: 8-byte) loads
   int zero;        // there are zero points
+  int s_vec;       // scales and zero points allow loads of 8 groups
   int bf16;        // type of scales and y
   int xgroup;      // columns of a scale of e4m3 x; 0: one a row, or none
   int x_shift;     // its logarithm, -1: not a power of two
@@ -396,6 +397,7 @@ extern "C" int yk_gemv4(const YkGemv4* p, yk_stream_t st) {
   Gemv4Args a{*p};
   a.x_vec = at % (x8 ? 8 : 16) == 0;
   a.zero = p->wzero != nullptr;
+  a.s_vec = aligned16(p->wscale) && p->group_row % 8 == 0 && p->k / p->group % 8 == 0 && (uintptr_t)p->wzero % 8 == 0;
   a.bf16 = p->dtype == YK_BF16;
   a.xgroup = x8 ? p->xgroup : 0;
   a.x_shift = a.xgroup && !(a.xgroup & (a.xgroup - 1)) ? __builtin_ctz(a.xgroup) : -1;

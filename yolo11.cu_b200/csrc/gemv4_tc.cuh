@@ -5,18 +5,20 @@
 // (a TMEM lane): it turns its row's codes into 16-bit integers in registers (about one instruction a
 // code), stores them into TMEM as the A operand, and scales its own sums: one scale and zero point a
 // group, no shuffles.  x is the B operand in shared memory, staged once for all 128 outputs.
-//  * A chunk is 128 columns of 128 outputs; warps 0-3 take even chunks, warps 4-7 odd ones (a warp its
+//  * A chunk is 128 columns of 128 outputs; warps 0-3 take the first half of them, warps 4-7 the rest (a warp its
 //    32 outputs' 64 bytes each, by cp.async), as two halves of 64 columns.
 //    Half h goes to A buffer h % 2 and its sums (one accumulator for each group, or half a group) to D
 //    buffer h % 2; a half's sums are read after the next half is stored, so the MMA runs behind.
 //  * The next warps stage x: 8 columns in the order (0, 4, 1, 5, 2, 6, 3, 7) that the codes come out in.
-//  * One thread of the last warp issues the MMAs.
+//  * One thread of each of the last two warps issues one set's MMAs.
+//  * Scales and zero points come 8 groups at a time where their rows allow it: a thread a row means a
+//    line a lane, so each load costs the warp 32 lines.
 template <int XT, int GB, int N>
 struct GemvTc {
   static constexpr int kTeam = N / 16;                             // warps that stage a chunk of x together
   static constexpr int kTeams = N == 16 ? 4 : 2;                   // chunks in the making: a load's latency each
   static constexpr int kStageWarps = kTeam * kTeams;
-  static constexpr int kThreads = (8 + kStageWarps + 1) * 32;
+  static constexpr int kThreads = (8 + kStageWarps + 2) * 32;
   static constexpr int kStages = 4, kXStages = 4;
   static constexpr int kUnits = GB == 1 ? 2 : 1;                   // accumulators of a half
   static constexpr int kD0 = 128;                                  // TMEM columns: A 2 x 2 x 32, then D 2 x 2 x kUnits x N
@@ -38,12 +40,14 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
   __shared__ __align__(8) uint64_t bars[4 + 4 + 2 * S::kXStages];
   __shared__ uint32_t tslot;
   __shared__ volatile int abort_flag;
-  // scales of e4m3 x of chunk c at c % 8 (1 where there are none): x stages are free before the sums are read
+  // scales of e4m3 x of a chunk at its number in turn % 8 (1 where there are none): x stages are free before the sums are read
   __shared__ __align__(16) float xs_sm[8][N];
   const YkGemv4& p = ga.p;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int K = p.k, chunks = (K + 127) / 128;
   const int n0 = blockIdx.x * 128;
+  // set 0 has chunks 0 .. split - 1; split * 128 columns are a multiple of 8 groups
+  const int split = min(chunks, ((chunks + 1) / 2 + 2 * GB - 1) / (2 * GB) * (2 * GB));
   const uint32_t base = (smem_u32(gemv_tc_raw) + 1023) & ~1023u;
   const uint32_t x_sm = base, ring = base + S::kXStages * S::kX;
   // A of (set of warps, buffer) is full; its MMA is done; x stage is full; is free
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
     const uint16_t* scales = (const uint16_t*)p.wscale + n * p.group_row;
     const uint8_t* zeros = (const uint8_t*)p.wzero + n * p.group_row;
     const bool zero = ga.zero;
-    const int mine = chunks > set ? (chunks - set + 1) / 2 : 0, groups = K / (32 * GB);
+    const int c_first = set ? split : 0, mine = set ? chunks - split : split, groups = K / (32 * GB);
     const uint32_t slots = ring + set * (S::kStages * S::kStage), slot = slots + row * 16;
     // a warp copies its own 32 rows, four lanes a row's 64 bytes: 8 lines an instruction, not 32
     const int q_in = lane & 3, row_in = (warp & 3) * 32 + (lane >> 2);
@@ -97,7 +101,7 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
     for (int i = 0; i < 4; i++) w_in[i] = (const uint8_t*)p.w + min((long long)n0 + row_in + 8 * i, p.n - 1ll) * p.w_row + q_in * 16;
     const auto issue = [&](int i) {
       if (i < mine) {
-        const int k = (set + 2 * i) * 128;
+        const int k = (c_first + i) * 128;
         const uint32_t to = slots + (i % S::kStages) * S::kStage + q_in * S::kPlane + row_in * 16;
         const bool ok = k + q_in * 32 < K;
 #pragma unroll
@@ -107,24 +111,44 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
     };
 #pragma unroll
     for (int i = 0; i < S::kStages - 1; i++) issue(i);
-    // scales and zero points of a half's units, as they are in memory, one half ahead
+    // scales and zero points of a half's units, as they are in memory, one half ahead; in eights
+    // (s8, z8), the next eight on their way
     uint32_t s_next[S::kUnits], z_next[S::kUnits];
+    uint4 s8, s8_next = make_uint4(0, 0, 0, 0);
+    uint2 z8, z8_next = make_uint2(0x08080808u, 0x08080808u);
+    const auto load8 = [&](int at) {
+      if (at >= groups || !mine) return;
+      s8_next = *(const uint4*)(scales + at);
+      if (zero) z8_next = *(const uint2*)(zeros + at);
+    };
     const auto load_scales = [&](int h) {
-      const int k = (set + 2 * (h >> 1)) * 128 + (h & 1) * 64;
+      const int k = (c_first + (h >> 1)) * 128 + (h & 1) * 64;
 #pragma unroll
       for (int u = 0; u < S::kUnits; u++) {
         const int at = k / (32 * GB) + u;
-        const bool ok = h < 2 * mine && at < groups;
-        s_next[u] = ok ? scales[at] : 0;
-        z_next[u] = zero && ok ? zeros[at] : 8;
+        if (ga.s_vec) {
+          if (at % 8 == 0 && (GB < 4 || (h & 1) == 0)) {
+            s8 = s8_next;
+            z8 = z8_next;
+            load8(at + 8);
+          }
+          const uint32_t w = at & 4 ? (at & 2 ? s8.w : s8.z) : (at & 2 ? s8.y : s8.x);
+          s_next[u] = at & 1 ? w >> 16 : w & 0xffffu;
+          z_next[u] = (at & 4 ? z8.y : z8.x) >> (8 * (at & 3)) & 0xffu;
+        } else {
+          const bool ok = h < 2 * mine && at < groups;
+          s_next[u] = ok ? scales[at] : 0;
+          z_next[u] = zero && ok ? zeros[at] : 8;
+        }
       }
     };
+    if (ga.s_vec) load8(c_first * 4 / GB);
     load_scales(0);
     bool ok = true;
     float s_last[S::kUnits];
     // sums of half h (its scales in s_last), once its MMA is done
     const auto add_sums = [&](int h) {
-      const int buf = h & 1, c = set + 2 * (h >> 1);
+      const int buf = h & 1, seq = (h & ~1) + set;           // of the chunk, among both sets' in turn
       if (!mbar_wait(done + (set * 2 + buf) * 8, (h >> 1) & 1, 0x601)) return false;
       tc_fence_after();
 #pragma unroll
@@ -137,7 +161,7 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
 #pragma unroll
           for (int m = 0; m < 8; m++) {
             float2 f = make_float2(s_last[u], s_last[u]);
-            if (X8) f = mul2(f, *(const float2*)&xs_sm[c & 7][m0 + 2 * m]);
+            if (X8) f = mul2(f, *(const float2*)&xs_sm[seq & 7][m0 + 2 * m]);
             float2& t = tot[m0 / 2 + m];
             t = ffma2(make_float2(__uint_as_float(d[2 * m]), __uint_as_float(d[2 * m + 1])), f, t);
           }
@@ -189,7 +213,7 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
     cp_async_wait<0>();
   } else if (warp < kMmaWarp) {
     // ---------------- x ----------------
-    // team t takes chunks t, t + kTeams, ..; a lane 8 columns of every other row of its warp's 16
+    // chunks in turn, one of each set: team t takes numbers t, t + kTeams, ..; a lane 8 columns of every other row of its warp's 16
     const int team = (warp - 8) / S::kTeam, row0 = (warp - 8) % S::kTeam * 16 + (lane >> 4), ch = lane & 15;
     constexpr int kSize = X8 ? 1 : 2;
     const uint8_t* const x0 = (const uint8_t*)p.x + ((long long)row0 * p.x_row + ch * 8) * kSize;
@@ -197,7 +221,10 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
     const int m_xs = (warp - 8) % S::kTeam * 32 + lane;             // (lanes below N in all) reads a row's scale
     uint32_t raw[S::kPieces][2 * kSize];
     float xs = 1.f;
-    const auto load = [&](int c) {
+    const int turns = 2 * split;
+    const auto chunk_at = [&](int seq) { return seq & 1 ? split + (seq >> 1) : seq >> 1; };   // (chunks on: none)
+    const auto load = [&](int seq) {
+      const int c = seq < turns ? chunk_at(seq) : chunks;
       const bool in_k = c * 128 + ch * 8 < K;
 #pragma unroll
       for (int i = 0; i < S::kPieces; i++) {
@@ -225,9 +252,10 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
         xs = p.xscale[min(m_xs, p.rows - 1) * p.xscale_row + (ga.x_shift >= 0 ? c * 128 >> ga.x_shift : c * 128 / ga.xgroup)];
     };
     load(team);
-    for (int c = team; c < chunks; c += S::kTeams) {
-      const int stage = c % S::kXStages;
-      if (c >= S::kXStages && !mbar_wait(x_free + stage * 8, (c / S::kXStages - 1) & 1, 0x602)) { abort_flag = 1; break; }
+    for (int seq = team; seq < turns; seq += S::kTeams) {
+      if (chunk_at(seq) >= chunks) continue;
+      const int stage = seq % S::kXStages;
+      if (seq >= S::kXStages && !mbar_wait(x_free + stage * 8, (seq / S::kXStages - 1) & 1, 0x602)) { abort_flag = 1; break; }
 #pragma unroll
       for (int i = 0; i < S::kPieces; i++) {
         const int m = row0 + 2 * i;
@@ -245,31 +273,34 @@ __global__ void __launch_bounds__(GemvTc<XT, GB, N>::kThreads, N == 16 ? 2 : 1) 
                          x_sm + stage * S::kX + (ch >> 3) * (N * 128) + m * 128 + (((ch & 7) ^ (m & 7)) << 4)),
                      "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
       }
-      if (m_xs < N) xs_sm[c & 7][m_xs] = xs;
+      if (m_xs < N) xs_sm[seq & 7][m_xs] = xs;
       fence_proxy_async();
       mbar_arrive(x_full + stage * 8);
-      load(c + S::kTeams);
+      load(seq + S::kTeams);
     }
   } else if (lane == 0) {
     // ---------------- MMA ----------------
     constexpr uint32_t idesc = idesc_f16_m128(N) | (F16 ? 0u : (1u << 7) | (1u << 10));     // bf16 A and B
     const uint64_t x_desc = sw128_desc(x_sm);
+    const int set = warp - kMmaWarp;
     bool ok = true;
-    for (int c0 = 0; c0 < chunks && ok; c0 += 2)
-      for (int t = 0; t < 4 && ok; t++) {          // halves of chunks c0, c0 + 1 in turn
-        const int set = t & 1, half = t >> 1, c = c0 + set, buf = half, stage = c % S::kXStages;
-        if (c >= chunks) continue;
-        if (half == 0) ok = mbar_wait(x_full + stage * 8, (c / S::kXStages) & 1, 0x603);
-        ok = ok && mbar_wait(a_full + (set * 2 + buf) * 8, (c >> 1) & 1, 0x604);
+    const int mine = set ? chunks - split : split;
+    for (int i = 0; i < mine && ok; i++) {
+      const int stage = (2 * i + set) % S::kXStages;
+      ok = mbar_wait(x_full + stage * 8, ((2 * i + set) / S::kXStages) & 1, 0x603);
+#pragma unroll
+      for (int half = 0; half < 2 && ok; half++) {
+        ok = mbar_wait(a_full + (set * 2 + half) * 8, i & 1, 0x604);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int s = 0; s < 4; s++)
-          tc_mma_f16_ts(d_at(set, buf) + (S::kUnits == 2 ? (s >> 1) * N : 0), a_at(set, buf) + s * 8,
+          tc_mma_f16_ts(d_at(set, half) + (S::kUnits == 2 ? (s >> 1) * N : 0), a_at(set, half) + s * 8,
                         x_desc + (stage * S::kX + half * (N * 128)) / 16 + s * 2, idesc, S::kUnits == 2 ? s & 1 : s);
-        tc_commit(done + (set * 2 + buf) * 8);
+        tc_commit(done + (set * 2 + half) * 8);
         if (half == 1) tc_commit(x_free + stage * 8);
       }
+    }
     if (!ok) abort_flag = 1;
   }
   // the two sets' sums meet: odd chunks' through shared memory (the ring, no longer in use)
