@@ -114,7 +114,8 @@ template <bool BF16, int D>
 __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_kernel(const __grid_constant__ Attn8Args p) {
   using L = Dec<D>;
   extern __shared__ __align__(128) uint8_t dec_sm[];    // rings, then q rows (two), then meeting rows
-  __shared__ long long part[32], pre[32 * kDecWarps];
+  __shared__ Sums part[32];
+  __shared__ long long pre[32 * kDecWarps];
   __shared__ float wm[kDecWarps][16], wl[kDecWarps][16], row_m[16], row_l[16];
   __shared__ uint4 qsm[D == 256 ? D / 16 : 1][32];   // q fragments (registers below 256 channels)
   __shared__ int arrived;
@@ -130,9 +131,10 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
   const auto row_tiles = [&](const Req& q) { return (int)(((long long)q.q * G + 15) / 16); };
   const auto req_cost = [&](const Req& q) { return q.q ? (long long)(item_gran(q) + lead) * row_tiles(q) * c.heads : 0ll; };
   const int per_thread = (a.requests + 32 * kDecWarps - 1) / (32 * kDecWarps);
-  long long sum = 0, total;
-  for (int r = tid * per_thread; r < min(a.requests, (tid + 1) * per_thread); r++) sum += req_cost(attn_req(c, a, r));
-  pre[tid] = block_exclusive(sum, part, &total);
+  Sums sum = {0, 0}, total2;
+  for (int r = tid * per_thread; r < min(a.requests, (tid + 1) * per_thread); r++) sum.a += req_cost(attn_req(c, a, r));
+  pre[tid] = block_exclusive2(sum, part, &total2).a;
+  const long long total = total2.a;
   __syncthreads();
   const long long per = max((total + gridDim.x - 1) / gridDim.x, (long long)p.min_part);
   long long f = blockIdx.x * per;

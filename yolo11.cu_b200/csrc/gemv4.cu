@@ -28,11 +28,11 @@ struct Gemv4Args {
   int x_shift;     // its logarithm, -1: not a power of two
   int x_inside;    // it may change inside a chunk of 128 columns
 };
-#ifndef TCN
-#define TCN 64 * 148
-#endif
 constexpr int kGemvWarps = 8;
-constexpr int kGemvTcOutputs = TCN;      // outputs from which on tcgen05 is used
+// tcgen05 (gemv4_tc.cuh) from this many outputs on, for more than 8 rows.  28672 x 8192, 1, 8, 16, 32, 64
+// rows: 58, 67, 72, 154, 425 us on warp MMAs, 70, 70, 71, 92, 149 us there; with fewer outputs its CTAs
+// (128 outputs each) leave most SMs without work.
+constexpr int kGemvTcOutputs = 64 * 148;
 
 // d = a * b + (first ? 0 : d)
 template <bool F16>
@@ -352,13 +352,13 @@ static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
 template <int XT, int GB>
 static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
   const int m = a.p.rows, n = a.p.n;
-  if (n >= kGemvTcOutputs && (!a.xgroup || !a.x_inside)) {
+  if (m > 8 && n >= kGemvTcOutputs && (!a.xgroup || !a.x_inside)) {
     if (m <= 16) return launch_gemv4_tc<XT, GB, 16>(a, st);
     if (m <= 32) return launch_gemv4_tc<XT, GB, 32>(a, st);
     return launch_gemv4_tc<XT, GB, 64>(a, st);
   }
   if (m <= 8) return launch_gemv4<XT, GB, 1, 1, 1>(a, st);
-  if (m <= 16) return n >= 64 * 148 ? launch_gemv4<XT, GB, 2, 2, 4>(a, st) : launch_gemv4<XT, GB, 2, 1, 1>(a, st);
+  if (m <= 16) return launch_gemv4<XT, GB, 2, 1, 1>(a, st);
   if (m <= 32) return launch_gemv4<XT, GB, 4, 1, 2>(a, st);
   return launch_gemv4<XT, GB, 8, 1, 2>(a, st);
 }

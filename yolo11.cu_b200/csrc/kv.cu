@@ -26,38 +26,40 @@ __device__ __forceinline__ int plan_last_le(const int* a, int n, int v) {
   return lo;
 }
 
-// Exclusive sum of one value a thread over the block; *total: the whole sum.
-__device__ __forceinline__ long long block_exclusive(long long v, long long* part, long long* total) {
+// Exclusive sums of two values a thread over the block, in one go; totals: the whole sums.
+struct Sums {
+  long long a, b;
+};
+__device__ __forceinline__ Sums block_exclusive2(Sums v, Sums* part, Sums* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  long long s = v;
+  Sums s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(~0u, s, o);
-    if (lane >= o) s += u;
+    const long long a = __shfl_up_sync(~0u, s.a, o), b = __shfl_up_sync(~0u, s.b, o);
+    if (lane >= o) { s.a += a; s.b += b; }
   }
   if (lane == 31) part[warp] = s;
   __syncthreads();
   if (warp == 0) {
-    long long w = lane < warps ? part[lane] : 0;
+    Sums w = lane < warps ? part[lane] : Sums{0, 0};
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(~0u, w, o);
-      if (lane >= o) w += u;
+      const long long a = __shfl_up_sync(~0u, w.a, o), b = __shfl_up_sync(~0u, w.b, o);
+      if (lane >= o) { w.a += a; w.b += b; }
     }
     part[lane] = w;
   }
   __syncthreads();
-  const long long before = (warp ? part[warp - 1] : 0) + s - v;
+  const Sums before = warp ? part[warp - 1] : Sums{0, 0};
   *total = part[warps - 1];
-  __syncthreads();   // part is used again
-  return before;
+  return {before.a + s.a - v.a, before.b + s.b - v.b};
 }
 
 __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ PlanArgs a) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ int plan_sm[];
-  __shared__ long long part[32];
+  __shared__ Sums part[32];
   __shared__ int stat[3];
   const YkKvPlan& p = a.p;
   const int R = p.requests, T = p.tokens, shift = 31 - __clz(T);
@@ -70,40 +72,34 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
   const int avail = p.free_count - head;
   if (threadIdx.x < 3) stat[threadIdx.x] = 0;
 
-  long long sum = 0, total;
-  for (int r = r0; r < r1; r++) sum += max(0, p.fresh[r]);
-  long long at = block_exclusive(sum, part, &total);
-  // blocks needed by request r, whose rows start at `from`; -1: refused whatever is free
-  const auto need_of = [&](int past, int fresh, long long from) -> int {
-    if (past < 0 || fresh < 0 || (fresh && from + fresh > p.rows)) return -1;
-    const long long end = (long long)past + fresh;
-    if (end > (long long)p.max_blocks * T || end > 0x7fffffffll) return -1;
-    return (int)((end + T - 1) / T - ((long long)past + T - 1) / T);
-  };
-  long long blocks = 0;
-  const long long from0 = at;
+  // Both sums at once: a request past the row limit takes no block, but every later one that needs
+  // any is past it too, so that what it counts here moves no accepted request.
+  Sums sum = {0, 0}, total;
   for (int r = r0; r < r1; r++) {
     const int f = p.fresh[r], past = p.past[r];
-    cu[r] = (int)min(at, (long long)p.rows);
-    past_sm[r] = past;
-    const int need = need_of(past, f, at);
+    const long long end = (long long)past + f;
+    const bool fits = past >= 0 && f >= 0 && end <= (long long)p.max_blocks * T && end <= 0x7fffffffll;
+    const int need = fits ? (int)(((end + T - 1) >> shift) - (((long long)past + T - 1) >> shift)) : -1;
+    cu[r] = max(0, f);
     boff[r] = need;
-    blocks += max(0, need);
-    at += max(0, f);
+    past_sm[r] = past;
+    sum.a += max(0, f);
+    sum.b += max(0, need);
   }
-  if (threadIdx.x == 0) cu[R] = (int)min(total, (long long)p.rows);
-  const long long all_rows = total;
-  long long boffs = block_exclusive(blocks, part, &total);
+  Sums at = block_exclusive2(sum, part, &total);
+  if (threadIdx.x == 0) cu[R] = (int)min(total.a, (long long)p.rows);
+  const long long all_rows = total.a;
   int taken = 0, placed = 0, refused = 0;
-  at = from0;
   for (int r = r0; r < r1; r++) {
-    const int need = boff[r];
-    const bool ok = need == 0 || (need > 0 && boffs + need <= avail);
-    const int before = (int)min(boffs, 0x7fffffffll);
+    const int f = cu[r], need = boff[r];
+    const bool ok = need >= 0 && !(f && at.a + f > p.rows) && (need == 0 || at.b + need <= avail);
+    const int before = (int)min(at.b, 0x7fffffffll);
+    cu[r] = (int)min(at.a, (long long)p.rows);
     boff[r] = ok ? before : ~before;
-    if (ok && need > 0) taken = (int)(boffs + need);
-    if (ok) placed += p.fresh[r]; else refused++;
-    boffs += max(0, need);
+    if (ok && need > 0) taken = (int)(at.b + need);
+    if (ok) placed += f; else refused++;
+    at.a += f;
+    at.b += max(0, need);
   }
   if (taken) atomicMax(&stat[0], taken);      // whole numbers: any order gives the same
   if (placed) atomicAdd(&stat[1], placed);
@@ -162,8 +158,7 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
   if (!a.finish || blockIdx.x) return;
   // kv_lens may be past: each request's length is read before, by this thread
   for (int r = r0; r < r1; r++) {
-    const int f = p.fresh[r];
-    p.kv_lens[r] = boff[r] >= 0 ? past_sm[r] + f : past_sm[r];
+    p.kv_lens[r] = boff[r] >= 0 ? past_sm[r] + cu[r + 1] - cu[r] : past_sm[r];
     p.cu[r] = cu[r];
   }
   if (threadIdx.x == 0) {
