@@ -603,15 +603,14 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
       row_sum[x] = row_l[e / (D / 4)];
     }
     // ---- a whole item is written out; a part goes to the workspace ----
-    // Parts join in two steps, groups of about the square root of their number first, so that no
-    // CTA has many to read; the last to arrive does it, in the order of the parts.
+    // Parts join in two steps, groups of 8 (16 from 129 parts on) first, so that no CTA has many to
+    // read; the last to arrive does it, in the order of the parts.
     bool write = true;
     if (cur.g0 > 0 || cur.g1 < cur.n) {
       const long long f0 = f + cur.cost - cur.g1;       // the item's first granule
       const int ca = (int)(f0 / per), cb = (int)((f0 + cur.n - 1) / per);   // the CTAs of this item
       const int parts = cb - ca + 1;
-      int size = kAtOnce;
-      while (size * size < parts) size++;
+      const int size = parts <= 16 * kAtOnce ? kAtOnce : 2 * kAtOnce;
       const int me = (int)blockIdx.x - ca, head_g = me - me % size, count_g = min(size, parts - head_g);
       // counters and parts of CTA b: 1 where an item begins that goes on, 0 where one continues
       const auto at_of = [&](int i) { return (ca + i) * 2 + (i == 0 ? 1 : 0); };
