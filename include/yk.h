@@ -273,7 +273,7 @@ typedef struct {
   long long table_stride;
   int max_blocks;          // table entries of a request
   int requests;            // 1 .. 16384
-  int rows;
+  int rows;                // rows * heads below 2^31
   int heads;               // query heads, a multiple of c->heads
   int dtype;               // YK_F16 or YK_BF16 (q and out)
   int causal;

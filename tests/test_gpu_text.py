@@ -373,6 +373,26 @@ def test_attention_many_requests(lib, cuda):
     run_attention(lib, rt, "bf16", 2, 1, 64, 16, lens, lse=False)
 
 
+def test_attention_many_prompts(lib, cuda):
+    """More requests than are ordered by their length."""
+    from yolo11_cu_b200 import runtime as rt
+    rng = random.Random(4)
+    lens = []
+    for _ in range(150):
+        q = rng.choice([0, 1, 20, 66, 130])
+        lens.append((q + rng.randrange(0, 70), q))
+    assert sum(q for _, q in lens) * 2 >= 64 * len(lens)
+    run_attention(lib, rt, "bf16", 2, 1, 64, 32, lens)
+
+
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_prompt_among_decodes(lib, cuda, window):
+    """A long prompt in a batch whose average is a few rows: many row tiles share the split list."""
+    from yolo11_cu_b200 import runtime as rt
+    run_attention(lib, rt, "f16", 6, 2, 128, 16, [(50, 1)] * 20 + [(300, 200)] + [(33, 1), (0, 0), (700, 2)] * 9,
+                  window=window)
+
+
 @pytest.mark.parametrize("qscale,scale,vspread", [(30.0, 0.0, 0.5), (1.0, 3.0, 0.5), (1.0, 0.0, 9.0),
                                                   (1e-4, 0.0, 0.5), (8.0, 0.5, 9.0)])
 @pytest.mark.parametrize("q", [1, 70])

@@ -52,7 +52,7 @@ ROWS = [(dict(k=None), EINVAL), (dict(slots=None), EINVAL), (dict(rows=-1), EINV
         (dict(k=PTR + 2), EINVAL), (dict(k_row=12), EINVAL), (dict(v_head=4), EINVAL)]
 ATTN = [(dict(cu=None), EINVAL), (dict(ws=None), EINVAL), (dict(ws_bytes=100), EINVAL), (dict(ws=PTR + 4), EINVAL),
         (dict(heads=3), EINVAL), (dict(heads=0), EINVAL), (dict(dtype=2), EUNSUP), (dict(requests=0), EINVAL),
-        (dict(requests=20000), EUNSUP), (dict(q=None), EINVAL), (dict(out=PTR + 2), EINVAL), (dict(q_row=513), EINVAL),
+        (dict(requests=20000), EUNSUP), (dict(rows=1 << 30), EUNSUP), (dict(q=None), EINVAL), (dict(out=PTR + 2), EINVAL), (dict(q_row=513), EINVAL),
         (dict(out_row=256), EINVAL), (dict(window=5, causal=0), EINVAL), (dict(window=-1), EINVAL),
         (dict(scale=-1.0), EINVAL), (dict(scale=float("nan")), EINVAL), (dict(table_stride=3), EINVAL)]
 NORM = [(dict(x=None), EINVAL), (dict(codes=None), EINVAL), (dict(scales=None), EINVAL), (dict(dtype=2), EUNSUP),

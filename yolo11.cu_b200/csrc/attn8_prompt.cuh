@@ -15,6 +15,10 @@
 //    tile j + 1 is done before the softmax of tile j is, and PV of tile j runs beside the softmax of
 //    tile j + 1.
 // Two CTAs an SM up to 128 channels.
+// Measured: 8 ragged requests, 5616 rows of 16 heads over up to 3832 keys (67.6 GFLOP) 139 us, 0.49 PFLOP/s, 29 %
+// of the measured burst rate (the warp-MMA tiles of the split kernel: 650 us).  A CTA spends about 2700
+// cycles a tile: 1100 in the weights (64 exponentials a row, shared with the other CTA), the rest in
+// waits for S and in the chain P -> PV -> QK; longest tiles first leave an SM within 10 % of the mean.
 constexpr int kProThreads = 288;
 constexpr int kProSort = 128;          // requests up to which tiles are ordered by their length
 

