@@ -339,6 +339,9 @@ int yk_test_inject(int withhold, unsigned long long wait_ns);
 // restores the default, the largest power of two up to 8 with batch x size <= the SM count).
 // Results do not depend on it; tests compare every size bit for bit.
 int yk_test_nms_cluster(int size);
+// Test hook: the kernel behind yk_attn_kv8 (1: keys split over all CTAs, 2: 128-row tiles, 0: the
+// library's rule); tests compare both with the definition.
+int yk_test_attn_kv8(int kernel);
 const char* yk_last_cuda_error(void);
 // Number of kernels this library launched since load (all devices) — a host-side counter.
 long long yk_launch_count(void);

@@ -19,6 +19,12 @@ pytestmark = pytest.mark.gpu
 TYPES = {"f16": (torch.float16, 0, 2.0 ** -11), "bf16": (torch.bfloat16, 1, 2.0 ** -8)}
 
 
+@pytest.fixture(autouse=True)
+def the_librarys_rule(lib):
+    yield
+    lib.yk_test_attn_kv8(0)
+
+
 def within(got, want, bound, dt):
     """|got - want| <= bound, where a result that the type does not hold is an infinity."""
     top = 65520.0 if dt == torch.float16 else 3.3961775e38     # rounds up to infinity from here on
@@ -309,32 +315,38 @@ def run_attention(lib, rt, kind, heads, kv_heads, D, T, lens, causal=1, window=0
                      kv_lens=kvd.data_ptr(), table=t.data_ptr(), table_stride=cols, max_blocks=cols,
                      requests=len(lens), rows=n, heads=heads, dtype=code, causal=causal,
                      window=window, scale=scale, ws=ws.data_ptr(), ws_bytes=size)
-    first = None
-    for _ in range(repeat):        # the workspace is left as it was found: the same bits again
-        out.fill_(9.0)
-        ok(lib, lib.yk_attn_kv8(C.byref(c), C.byref(a), stream()))
-        torch.cuda.synchronize()
-        if first is None:
-            first = out.clone()
-        assert torch.equal(first.view(torch.int16), out.view(torch.int16))
+    results = []
+    for kernel in (1, 2, 0):           # both kernels, and the one that the rule takes
+        assert lib.yk_test_attn_kv8(kernel) == 0
+        first = None
+        for _ in range(repeat):        # the workspace is left as it was found: the same bits again
+            out.fill_(9.0)
+            ls.fill_(9.0)
+            ok(lib, lib.yk_attn_kv8(C.byref(c), C.byref(a), stream()))
+            torch.cuda.synchronize()
+            if first is None:
+                first = out.clone()
+            assert torch.equal(first.view(torch.int16), out.view(torch.int16))
+        assert lib.yk_fetch_device_error() == 0
+        results.append((out.clone(), ls.clone()))
     o, l, mag, big = ref.attention(f64(q), view[:, 0].cpu().numpy(), f64(sc[0])[:, :kv_heads],
                                    view[:, 1].cpu().numpy(), f64(sc[1])[:, :kv_heads], table,
                                    [kv for kv, _ in lens], cu, T, causal, window,
                                    scale or D ** -0.5)
     ds = ((D + 8) * 2.0 ** -24 * big + 2.0 ** -21)[..., None]    # error of a score
-    got = f64(out[:, :heads])[:cu[-1]]
-    bound = u * np.abs(o) + (2.0 ** -10 + 2 * ds) * mag + 2.0 ** -24
-    fine = within(got, o[:cu[-1]], bound[:cu[-1]], dt)
-    assert fine.all(), (np.argwhere(~fine)[:3], (np.abs(got - o[:cu[-1]]) / bound[:cu[-1]]).max())
-    assert (f64(out[cu[-1]:]) == 9).all() and (f64(out[:, heads]) == 9).all()
-    if lse:
-        gl, l = f64(ls)[:cu[-1]], l[:cu[-1]]
-        assert np.array_equal(np.isnan(gl), np.isnan(l))
-        empty = np.isinf(l) | np.isnan(l)
-        assert (gl[np.isinf(l)] == -np.inf).all()
-        lb = ds[:cu[-1], :, 0] + 2.0 ** -20 * (1 + np.abs(np.where(empty, 0, l)))
-        assert (np.abs(gl[~empty] - l[~empty]) <= lb[~empty]).all()
-    return got
+    for out, ls in results:
+        got = f64(out[:, :heads])[:cu[-1]]
+        bound = u * np.abs(o) + (2.0 ** -10 + 2 * ds) * mag + 2.0 ** -24
+        fine = within(got, o[:cu[-1]], bound[:cu[-1]], dt)
+        assert fine.all(), (np.argwhere(~fine)[:3], (np.abs(got - o[:cu[-1]]) / bound[:cu[-1]]).max())
+        assert (f64(out[cu[-1]:]) == 9).all() and (f64(out[:, heads]) == 9).all()
+        if lse:
+            gl, l = f64(ls)[:cu[-1]], l[:cu[-1]]
+            assert np.array_equal(np.isnan(gl), np.isnan(l))
+            empty = np.isinf(l) | np.isnan(l)
+            assert (gl[np.isinf(l)] == -np.inf).all()
+            lb = ds[:cu[-1], :, 0] + 2.0 ** -20 * (1 + np.abs(np.where(empty, 0, l)))
+            assert (np.abs(gl[~empty] - l[~empty]) <= lb[~empty]).all()
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
@@ -448,7 +460,8 @@ def test_attention_offsets_past_32_bits(lib, cuda):
                            np.zeros_like(mine), np.ones((3, heads)), T)
     same_values(mine, val)
     assert int((pool != 0).any(-1).any(-1).any(-1).sum()) == 3
-    for q in (1, 65):
+    for q, kernel in ((1, 1), (65, 1), (65, 2)):
+        lib.yk_test_attn_kv8(kernel)
         qs = torch.randn(q, heads, D, device="cuda").half()
         out = torch.zeros_like(qs)
         size = lib.yk_attn_kv8_workspace_bytes(1, q, heads, heads, D)

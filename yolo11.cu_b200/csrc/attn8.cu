@@ -45,7 +45,17 @@ constexpr int kDecGran = 16 * kDecSub;     // tokens of a granule
 // 431 keys: least share 3, 6 give 10.0, 8.5 us).
 constexpr int kDecLead = 2, kDecMin = 6;
 constexpr int kDecCtas = 148 * 2;
-constexpr int kProRows = 64;               // rows a request and key head, on average, from which on tcgen05 tiles are used
+// Which kernel: the tcgen05 tiles take whole rows of keys, so they need enough tiles to fill the SMs; the
+// split list fills them with anything but does 16 rows at a time.  Measured, 16 / 4 heads, rows a request and
+// key head -> us on the split list | on tiles: 8 requests of 2000 keys, 128 channels: 16: 24 | 50, 64: 26 | 50,
+// 128: 38 | 51, 256: 60 | 52; 64 requests of 500 keys: 16: 17 | 32, 32: 37 | 33, 64: 54 | 33; 1 request of 8000
+// keys: 256: 44 | 162; 256 channels, 8 of 2000: 16: 32 | 64, 64: 66 | 66, 128: 94 | 69.  So tiles from kProTiles
+// 16-row tiles on, or that many for every round of CTAs; and only for several new tokens a request, since a
+// decode batch's lengths may differ by any factor, which only the split evens out.
+constexpr int kProTokens = 8;              // new tokens a request, on average
+template <int D>
+constexpr int kProTiles = D == 256 ? 150 : 430;
+static std::atomic<int> g_attn_kernel{0};  // test hook: 1 split list, 2 tiles, 0 the rule
 constexpr int kAtOnce = 8;                 // parts that a join reads at a time
 
 template <int D>
@@ -741,6 +751,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
 
 using namespace yk;
 
+extern "C" int yk_test_attn_kv8(int kernel) {
+  if (kernel < 0 || kernel > 2) return refuse(YK_EINVAL, "test_attn_kv8: 0, 1 or 2");
+  g_attn_kernel = kernel;
+  return YK_OK;
+}
+
 extern "C" size_t yk_attn_kv8_workspace_bytes(int requests, int rows, int heads, int kv_heads, int dim) {
   // three counters and two parts (o, m, l of 16 rows) for each CTA, whatever the lengths
   (void)requests; (void)rows; (void)heads; (void)kv_heads;
@@ -778,7 +794,11 @@ extern "C" int yk_attn_kv8(const YkKvCache* c, const YkAttnKv8* a, yk_stream_t s
   p.scale_log2 = p.a.scale * 1.4426950408889634f;
   const bool bf = a->dtype == YK_BF16;
   cudaStream_t s = (cudaStream_t)st;
-  if ((long long)a->rows * (a->heads / c->heads) >= kProRows * (long long)a->requests) {
+  const long long G = a->heads / c->heads, tiles16 = (long long)a->rows * a->heads / 16;
+  const long long ctas = (a->rows * G / 128 + a->requests) * c->heads, slots = c->dim == 256 ? 148 : 296;
+  const int least = c->dim == 256 ? kProTiles<256> : kProTiles<128>, force = g_attn_kernel.load();
+  if (force ? force == 2
+            : a->rows >= (long long)kProTokens * a->requests && tiles16 * slots >= least * std::max(slots, ctas)) {
     switch (c->dim) {
       case 64: return bf ? launch_attn8_prompt<true, 64>(p, s) : launch_attn8_prompt<false, 64>(p, s);
       case 128: return bf ? launch_attn8_prompt<true, 128>(p, s) : launch_attn8_prompt<false, 128>(p, s);

@@ -146,6 +146,7 @@ _SIGS = {
     "yk_fetch_device_error": (C.c_int, []),
     "yk_test_inject": (C.c_int, [C.c_int, C.c_ulonglong]),
     "yk_test_nms_cluster": (C.c_int, [C.c_int]),
+    "yk_test_attn_kv8": (C.c_int, [C.c_int]),
     "yk_last_cuda_error": (C.c_char_p, []),
     "yk_launch_count": (C.c_longlong, []),
     # engine ABI (include/yolo.h)
