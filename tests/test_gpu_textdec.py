@@ -142,3 +142,21 @@ def test_example_runs(lib, cuda, pkg, capsys):
     from yolo11_cu_b200 import textdec
     textdec.main(["--frames", "2", "--steps", "4"])
     assert "400 image tokens" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_full_requests_stop(lib, cuda, pkg, graph):
+    """A request that holds all the blocks of its table is refused from then on and keeps its length;
+    the others go on.  max_tokens is no multiple of the block: the last block is used to its end."""
+    from yolo11_cu_b200 import textdec
+    dec = textdec.TextDecoder(2, rows=300, max_tokens=100, pool=16, seed=3)
+    rows = torch.randn(300, dec.width, generator=torch.Generator().manual_seed(2)).cuda().half()
+    dec.prompt(rows[:216], [90, 126])
+    dec.decode(2, graph=graph)
+    assert dec.lens.tolist() == [92, 128] and int(dec.counts[2]) == 0
+    for step in range(1, 4):
+        dec.decode(1, graph=graph)
+        assert dec.lens.tolist() == [92 + step, 128] and int(dec.counts[2]) == 1
+    dec.prompt(rows[:200], [200, 0])            # a prompt past the table's end
+    assert dec.lens.tolist() == [95, 128] and int(dec.counts[2]) == 1
+    torch.cuda.synchronize()

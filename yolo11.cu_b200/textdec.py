@@ -64,7 +64,7 @@ class TextDecoder:
         self.norms = [(1 + 0.1 * rand(2 * layers + 1, width)).half()[i] for i in range(2 * layers + 1)]
         self.head = quantize_w4(rand(vocab, width) * width ** -0.5, group)
         self.embed = rand(vocab, width).half()
-        self.place = (0.3 * rand(max_tokens, width)).half()
+        self.place = (0.3 * rand(self.max_blocks * block, width)).half()
         new = lambda *s, dtype=torch.half: torch.zeros(*s, dtype=dtype, device=device)  # noqa: E731
         i32 = torch.int32
         n = self.rows
@@ -143,10 +143,15 @@ class TextDecoder:
                          ws_bytes=self.ws.numel())
         self._ok(self.lib.yk_attn_kv8(C.byref(c), C.byref(b), self._stream))
 
+    def _places(self, n):
+        """The position rows of a step.  The plan writes the positions of refused rows too (past the last
+        block) and -1 for rows of no request; both take the nearest row, which nothing reads."""
+        return self.place[self.pos[:n].long().clamp(0, self.place.shape[0] - 1)]
+
     def _layers(self, n):
         """The residual rows self.res[:n] through every layer; leaves the last rows' logits."""
         self._plan(n)
-        self.res[:n] += self.place[self.pos[:n].clamp(min=0).long()]
+        self.res[:n] += self._places(n)
         self.delta[:n].zero_()
         for i, w in enumerate(self.w):
             self._norm(self.delta, self.res, self.norms[2 * i], n)
