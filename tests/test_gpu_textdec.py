@@ -160,3 +160,42 @@ def test_full_requests_stop(lib, cuda, pkg, graph):
     dec.prompt(rows[:200], [200, 0])            # a prompt past the table's end
     assert dec.lens.tolist() == [95, 128] and int(dec.counts[2]) == 1
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_admission_leaves_other_requests_alone(lib, cuda, pkg, graph):
+    """Prompts of other requests in the middle of a request's generation: its pending token stays, and
+    its tokens are those of a run without them."""
+    from yolo11_cu_b200 import textdec
+    rows = torch.randn(71, 512, generator=torch.Generator().manual_seed(2)).cuda().half()
+    runs = []
+    for admit in (False, True):
+        dec = textdec.TextDecoder(3, rows=64, max_tokens=256, pool=30, seed=3)
+        dec.prompt(rows[:30], [0, 30, 0])
+        ids = [dec.decode(3, graph=graph)]
+        pending = int(dec.next[1])
+        if admit:
+            dec.prompt(rows[30:], [20, 0, 21])
+            assert int(dec.next[1]) == pending
+            dec.prompt(rows[:0], [0, 0, 0])
+            assert int(dec.next[1]) == pending
+        ids.append(dec.decode(5, graph=graph))
+        runs.append(torch.cat(ids)[:, 1].tolist())
+    assert runs[0] == runs[1]
+
+
+@pytest.mark.parametrize("lens,last", [([5, 0, 7], [4, None, 11]), ([0, 3, 0], [None, 2, None]), ([0, 0, 1], [None, None, 0])])
+def test_a_prompt_picks_from_its_own_last_row(lib, cuda, pkg, lens, last):
+    from yolo11_cu_b200 import textdec
+    dec = textdec.TextDecoder(3, rows=64, max_tokens=256, pool=30, seed=3)
+    dec.next.copy_(torch.tensor([11, 22, 33]))
+    rows = torch.randn(sum(lens), dec.width, generator=torch.Generator().manual_seed(2)).cuda().half()
+    dec.prompt(rows, lens)
+    for r, row in enumerate(last):
+        if row is None:
+            assert int(dec.next[r]) == [11, 22, 33][r]
+            continue
+        x = dec.x8[row].view(F8).float() * dec.xs[row]
+        want = dequant(dec.head, dec.group) @ x
+        # fp16 scores: the picked one is the largest but for two roundings
+        assert want[dec.next[r]] >= want.max() - 2 * 2.0 ** -11 * want.abs().max()

@@ -149,7 +149,9 @@ class TextDecoder:
         return self.place[self.pos[:n].long().clamp(0, self.place.shape[0] - 1)]
 
     def _layers(self, n):
-        """The residual rows self.res[:n] through every layer; leaves the last rows' logits."""
+        """The residual rows self.res[:n] through every layer, then the scores of each request's last row and
+        the next token.  A request without a row in the step keeps the token that it has (its row of
+        `logits` is then none of its own)."""
         self._plan(n)
         self.res[:n] += self._places(n)
         self.delta[:n].zero_()
@@ -167,12 +169,13 @@ class TextDecoder:
         self.last8.copy_(self.x8[last])
         self.lasts.copy_(self.xs[last])
         self._matmul(self.last8, self.head, self.logits, self.requests, self.lasts)
-        torch.argmax(self.logits, 1, out=self.next)
+        self.next.copy_(torch.where(self.cu[1:] > self.cu[:-1], self.logits.argmax(1), self.next))
 
     # ---- what a caller uses ----
     def prompt(self, rows, lens):
         """rows [sum(lens), width]: each request's new rows one after another (embeddings of prompt
-        tokens, image tokens); lens[r] may be 0.  Fills the cache and picks every request's next token."""
+        tokens, image tokens); lens[r] may be 0.  Fills the cache and picks the next token of each request
+        that has rows; the others keep theirs."""
         n = sum(lens)
         if n > self.rows or n != rows.shape[0] or len(lens) != self.requests:
             raise ValueError(f"{n} rows in {len(lens)} requests, {rows.shape[0]} given: at most {self.rows} "
