@@ -199,3 +199,33 @@ def test_a_prompt_picks_from_its_own_last_row(lib, cuda, pkg, lens, last):
         want = dequant(dec.head, dec.group) @ x
         # fp16 scores: the picked one is the largest but for two roundings
         assert want[dec.next[r]] >= want.max() - 2 * 2.0 ** -11 * want.abs().max()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_refused_requests_keep_their_token(lib, cuda, pkg, graph):
+    """A step that the pool refuses a request gives it no token (-1) and keeps the one that waits; once there
+    are blocks again, that one goes in."""
+    from yolo11_cu_b200 import textdec
+    rows = torch.randn(95, 512, generator=torch.Generator().manual_seed(2)).cuda().half()
+    free, dec = (textdec.TextDecoder(3, rows=128, max_tokens=256, pool=p, seed=3) for p in (30, 4))
+    for d in (free, dec):
+        d.prompt(rows, [32, 31, 32])
+        assert d.placed.tolist() == [True] * 3
+    start = dec.next.tolist()
+    want = free.decode(3, graph=graph).tolist()
+    assert want[0] == start
+    assert dec.decode(1, graph=graph).tolist() == [[start[0], start[1], -1]]      # the last block goes to request 0
+    assert dec.placed.tolist() == [True, True, False] and dec.lens.tolist() == [33, 32, 32]
+    assert int(dec.next[2]) == start[2]
+    waits = int(dec.next[1])
+    assert dec.decode(2, graph=graph).tolist() == [[want[1][0], -1, -1], [want[2][0], -1, -1]]
+    assert dec.next.tolist()[1:] == [waits, start[2]] and dec.lens.tolist() == [35, 32, 32]
+    # request 0 leaves; its two blocks are free again
+    dec.lens[0] = 0
+    dec.free[2:4] = dec.table[0, :2]
+    dec.taken.fill_(2)
+    got = dec.decode(1, graph=graph).tolist()
+    assert got[0][1:] == [waits, -1] and dec.lens.tolist() == [1, 33, 32]
+    # a prompt that does not fit changes nothing either
+    dec.prompt(rows[:60], [0, 0, 60])
+    assert dec.placed.tolist() == [False] * 3 and int(dec.next[2]) == start[2] and int(dec.lens[2]) == 32

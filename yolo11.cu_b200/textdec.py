@@ -88,7 +88,9 @@ class TextDecoder:
         self.up, self.act = new(n, 2 * hidden), new(n, hidden)
         self.last8, self.lasts = new(requests, width, dtype=torch.uint8), new(requests, 1, dtype=torch.float32)
         self.logits = new(requests, vocab)
-        self.next = new(requests, dtype=torch.long)
+        # next: the token that goes in with the next step; given: the one that went in with the last (-1: refused)
+        self.next, self.given = new(requests, dtype=torch.long), new(requests, dtype=torch.long)
+        self.held, self.placed = new(requests, dtype=i32), new(requests, dtype=torch.bool)
         size = self.lib.yk_attn_kv8_workspace_bytes(requests, n, heads, kv_heads, dim)
         self.ws = new(size, dtype=torch.uint8)
         self.graph = None
@@ -150,9 +152,11 @@ class TextDecoder:
 
     def _layers(self, n):
         """The residual rows self.res[:n] through every layer, then the scores of each request's last row and
-        the next token.  A request without a row in the step keeps the token that it has (its row of
-        `logits` is then none of its own)."""
+        the next token.  A request whose rows the plan refused, or that has none in the step, keeps the token
+        that it has (its row of `logits` is then none of its own); `placed` says which have theirs in the cache."""
+        self.held.copy_(self.lens)
         self._plan(n)
+        torch.gt(self.lens, self.held, out=self.placed)
         self.res[:n] += self._places(n)
         self.delta[:n].zero_()
         for i, w in enumerate(self.w):
@@ -169,13 +173,13 @@ class TextDecoder:
         self.last8.copy_(self.x8[last])
         self.lasts.copy_(self.xs[last])
         self._matmul(self.last8, self.head, self.logits, self.requests, self.lasts)
-        self.next.copy_(torch.where(self.cu[1:] > self.cu[:-1], self.logits.argmax(1), self.next))
+        self.next.copy_(torch.where(self.placed, self.logits.argmax(1), self.next))
 
     # ---- what a caller uses ----
     def prompt(self, rows, lens):
         """rows [sum(lens), width]: each request's new rows one after another (embeddings of prompt
         tokens, image tokens); lens[r] may be 0.  Fills the cache and picks the next token of each request
-        that has rows; the others keep theirs."""
+        whose rows went in (`placed`); the others, without rows or refused, keep theirs."""
         n = sum(lens)
         if n > self.rows or n != rows.shape[0] or len(lens) != self.requests:
             raise ValueError(f"{n} rows in {len(lens)} requests, {rows.shape[0]} given: at most {self.rows} "
@@ -186,15 +190,18 @@ class TextDecoder:
         return self.next
 
     def _step(self):
+        self.given.copy_(self.next)
         self.res[:self.requests].copy_(self.embed[self.next])
         self._layers(self.requests)
+        self.given.masked_fill_(~self.placed, -1)
 
     def decode(self, steps: int, graph: bool = True):
-        """`steps` tokens for every request, greedily; [steps, requests].  The first call captures the step."""
+        """`steps` tokens for every request, greedily; [steps, requests].  Where the plan refuses a request
+        a step (no free block, or its table is full) it gives -1, and its token waits for the next step.
+        The first call captures the step."""
         out = torch.empty(steps, self.requests, dtype=torch.long, device=self.device)
         self.fresh.fill_(1)
         for i in range(steps):
-            out[i] = self.next
             if not graph:
                 self._step()
             elif self.graph is None:
@@ -206,6 +213,7 @@ class TextDecoder:
                     self._step()
             else:
                 self.graph.replay()
+            out[i] = self.given
         return out
 
 
