@@ -212,9 +212,11 @@ typedef struct {
 // takes the blocks it needs more from free_blocks (from entry *free_head on, when given) and
 // appends them to its table row.  Row n of the step is token past + j of its request r, with
 // n = cu[r] + j: pos[n] is that position and slots[n] its place in the pool.
-// A request is refused, and takes no block, when the free blocks that earlier requests left do
-// not suffice (one that needs none still goes on), when its tokens pass max_blocks blocks, when
-// its rows pass `rows`, or when a length is negative (a negative fresh counts as no rows).  Its
+// A request is refused, and takes no block, when its needs and those of all requests before it pass
+// the free blocks (one that needs none still goes on): after the first that does not fit, each later
+// one that needs a block is refused too, so that none is overtaken, even where enough are left for it.
+// It is also refused when its tokens pass max_blocks blocks or a length is negative (a negative fresh
+// counts as no rows), which does not hold up the ones after it, and when its rows pass `rows`.  Its
 // kv_lens stays past and its rows' slots are -1; so are the slots of rows past the last
 // request's (their pos too), and of tokens whose table entry lies outside the pool.
 typedef struct {

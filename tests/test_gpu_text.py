@@ -144,6 +144,29 @@ def test_plan_table_entry_outside_pool(lib, cuda):
     run_plan(lib, rt, [5, 20], [3, 20], [1, 99, 2], 16, 23, 4, 8, table=[[8, -1, -1, -1], [0, -3, -1, -1]])
 
 
+@pytest.mark.parametrize("past,fresh,free,want", [
+    # one free block: the first request needs three, so the second, which needs one, waits behind it
+    ([0, 0], [33, 1], [7], dict(kv=[0, 0], counts=[0, 0, 2, 34], head=0, slots=[-1] * 34, tables=[[-1] * 4, [-1] * 4])),
+    # a request that needs none goes on; whoever needs one after the shortage does not
+    ([16, 3, 16], [40, 2, 1], [7, 9], dict(kv=[16, 5, 16], counts=[0, 2, 2, 43], head=0,
+                                           slots=[-1] * 40 + [4 * 16 + 3, 4 * 16 + 4, -1],
+                                           tables=[[4, -1, -1, -1], [4, -1, -1, -1], [4, -1, -1, -1]])),
+    # the shortage comes second: what the first took stays its own
+    ([0, 0, 0], [5, 20, 1], [7, 9], dict(kv=[5, 0, 0], counts=[1, 5, 2, 26], head=1,
+                                         slots=[7 * 16 + i for i in range(5)] + [-1] * 21,
+                                         tables=[[7, -1, -1, -1], [-1] * 4, [-1] * 4])),
+    # past the table's end or negative: refused for itself, the ones after it find the blocks untouched
+    ([0, -1, 0], [65, 4, 1], [7], dict(kv=[0, -1, 1], counts=[1, 1, 2, 70], head=1,
+                                       slots=[-1] * 69 + [7 * 16], tables=[[-1] * 4, [-1] * 4, [7, -1, -1, -1]]))])
+def test_plan_does_not_overtake(lib, cuda, past, fresh, free, want):
+    """Results written out by hand: no request goes past one before it that waits for blocks."""
+    from yolo11_cu_b200 import runtime as rt
+    table = [[4 if p > 0 else -1, -1, -1, -1] for p in past]
+    got = run_plan(lib, rt, past, fresh, free, 16, sum(max(f, 0) for f in fresh), 4, 20, head=0, table=table)
+    assert (got[0], got[1], got[3], got[5], got[6]) == (want["tables"], want["kv"], want["slots"], want["counts"],
+                                                         want["head"])
+
+
 # ---------------------------------------------------------------- cache
 
 def make_cache(rt, blocks, heads, T, D, seed=0, joint=False, spread=0.5, vspread=0.5):

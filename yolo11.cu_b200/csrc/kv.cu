@@ -74,8 +74,8 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
   const int avail = p.free_count - head;
   if (threadIdx.x < 3) stat[threadIdx.x] = 0;
 
-  // Both sums at once: a request past the row limit takes no block, but every later one that needs
-  // any is past it too, so that what it counts here moves no accepted request.
+  // Both sums at once.  A refused request's need stays in the sum, so that none is overtaken.  A request
+  // past the row limit counts too, but every later one that needs a block is past that limit itself.
   Sums sum = {0, 0}, total;
   for (int r = r0; r < r1; r++) {
     const int f = p.fresh[r], past = p.past[r];
