@@ -460,6 +460,57 @@ def test_attention_nan_is_seen_only_where_visible(lib, cuda, D, window, lens):
                   nan=[(0, 37, 0, 3), (0, 26, 1, 9), (1, 30, 1, 0)])
 
 
+def attend_one(lib, rt, kind, q, k, v, ks, vs, T, scale):
+    """One request of one key head: q [rows, heads, dim] as its last tokens over codes k, v [blocks, T, dim]
+    with scales ks, vs [blocks], both kernels against the definition."""
+    dt, code, u = TYPES[kind]
+    n, heads, D = q.shape
+    blocks = k.shape[0]
+    q = q.to(dt).cuda()
+    k, v = k.to(ref.F8).view(torch.uint8).cuda().contiguous(), v.to(ref.F8).view(torch.uint8).cuda().contiguous()
+    ks, vs = ks.float().cuda(), vs.float().cuda()
+    c = rt.YkKvCache(k=k.data_ptr(), v=v.data_ptr(), kscale=ks.data_ptr(), vscale=vs.data_ptr(),
+                     block_stride=T * D, scale_stride=1, blocks=blocks, heads=1, tokens=T, dim=D)
+    out, lse = torch.zeros_like(q), torch.zeros(n, heads, device="cuda")
+    size = lib.yk_attn_kv8_workspace_bytes(1, n, heads, 1, D)
+    ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    cu, kv, t = i32([0, n]), i32([blocks * T]), i32([list(range(blocks))])
+    a = rt.YkAttnKv8(q=q.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(), q_row=heads * D, out_row=heads * D,
+                     cu=cu.data_ptr(), kv_lens=kv.data_ptr(), table=t.data_ptr(), table_stride=blocks,
+                     max_blocks=blocks, requests=1, rows=n, heads=heads, dtype=code, causal=1, scale=scale,
+                     ws=ws.data_ptr(), ws_bytes=size)
+    o, l, mag, big = ref.attention(f64(q), k[:, None].cpu().numpy(), f64(ks)[:, None], v[:, None].cpu().numpy(),
+                                   f64(vs)[:, None], [list(range(blocks))], [blocks * T], [0, n], T, 1, 0, scale)
+    ds = ((D + 8) * 2.0 ** -24 * big + 2.0 ** -21)[..., None]
+    bound = u * np.abs(o) + (2.0 ** -10 + 2 * ds) * mag + 2.0 ** -24
+    for kernel in (1, 2):
+        assert lib.yk_test_attn_kv8(kernel) == 0
+        out.fill_(9.0)
+        ok(lib, lib.yk_attn_kv8(C.byref(c), C.byref(a), stream()))
+        fine = within(f64(out), o, bound, dt)
+        assert fine.all(), (kernel, np.argwhere(~fine)[:3], np.nanmax(np.abs(f64(out) - o) / bound))
+        assert (np.abs(f64(lse) - l) <= ds[..., 0] + 2.0 ** -20 * (1 + np.abs(l))).all()
+
+
+@pytest.mark.parametrize("rows", [1, 66])
+@pytest.mark.parametrize("gap,spread", [(16.0, 1.5), (17.0, 0.5), (18.0, 1.0)])
+def test_attention_flat_tail_behind_a_loud_key(lib, cuda, rows, gap, spread):
+    """One key far above thousands of others, with a value of zero: the output is the others' alone, though
+    each weight is 2^-22 .. 2^-27 of the largest."""
+    from yolo11_cu_b200 import runtime as rt
+    T, D, blocks = 16, 64, 375
+    g = torch.Generator().manual_seed(int(gap * 2))
+    k, v = (torch.randn(blocks, T, D, generator=g) * 20 for _ in range(2))
+    k[..., 0] = 0
+    k[0, 0] = 0
+    k[0, 0, 0] = 16
+    v[0, 0] = 0
+    q = torch.randn(rows, 2, D, generator=g) * (spread / (20 * (D - 1) ** 0.5))    # scores of this spread
+    q[..., 0] = gap / 16
+    for kind in ("f16", "bf16"):
+        attend_one(lib, rt, kind, q, k, v, torch.ones(blocks), torch.ones(blocks), T, 1.0)
+
+
 def test_attention_offsets_past_32_bits(lib, cuda):
     """A pool whose code offsets pass 2^31 and 2^32."""
     from yolo11_cu_b200 import runtime as rt

@@ -33,6 +33,10 @@ struct Attn8Args {
 //  * One scale a (block, head): the key scale multiplies the scores; the value scale multiplies
 //    the weights, whose 16-bit form is taken relative to the largest weight * scale so far (M
 //    below, kept beside the softmax's m), so blocks of very different loudness keep their bits.
+//  * Weights enter the second product as fp16 (one rounding, 2^-11 of a weight: bf16 has 8 bits, and a
+//    second fp16 part would double the MMAs); their sum l stays in fp32.  The largest lies at 2^9 .. 2^15
+//    (kLift, kSlack), so a weight keeps its bits down to 2^-23 of the largest, times scale, and is lost below
+//    2^-34: a long flat tail behind one loud key still counts.
 // Measured: 2 requests over 393,000 keys (8 query heads a key head, 128 channels, 145 MB) 50 us, 2.9 TB/s:
 // the keys themselves pass at 5.6 TB/s (26 us), 5 us go before the first of them (lengths, table, block,
 // codes: four loads in a row), the rest into meeting and joining 74 parts an item; 64 requests of 64 to
@@ -45,6 +49,14 @@ constexpr int kDecGran = 16 * kDecSub;     // tokens of a granule
 // 431 keys: least share 3, 6 give 10.0, 8.5 us).
 constexpr int kDecLead = 2, kDecMin = 6;
 constexpr int kDecCtas = 148 * 2;
+// References of the weights, both kernels: m of 2^(score - m), M of the 16-bit weight * value scale.  Both
+// follow the running maximum only when it passes them by more than 2^kSlack, so the sums are rescaled a
+// few times a segment; M lies 2^kLift below its maximum, so the 16-bit weights stay below 2^(kLift + kSlack)
+// (fp16 holds 2^15), and no more than 2^126 below m, so that 2^(m - M) is finite.
+constexpr float kNone = -1e30f, kSlack = 6.f, kLift = 9.f;
+__device__ __forceinline__ float lifted(float M, float top_v, float m) {
+  return fmaxf(M, fmaxf(top_v - kLift, m - 126.f));
+}
 // Which kernel: the tcgen05 tiles take whole rows of keys, so they need enough tiles to fill the SMs; the
 // split list fills them with anything but does 16 rows at a time.  Measured, 16 / 4 heads, rows a request and
 // key head -> us on the split list | on tiles: 8 requests of 2000 keys, 128 channels: 16: 24 | 50, 64: 26 | 50,
@@ -378,10 +390,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
     float o[D / 8][4];
 #pragma unroll
     for (int j = 0; j < D / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    // m: reference of the weights (2^(score - m)), M: of weight * value scale; both follow the
-    // running maximum only when it passes them by more than 2^kSlack, so the sums are rescaled
-    // a few times a segment, and weights stay below 2^kSlack (fp16 holds 2^15)
-    constexpr float kNone = -1e30f, kSlack = 6.f;
+    // references and sums of rows g, g + 8; gain = 2^(m - M)
     float m[2] = {kNone, kNone}, M[2] = {kNone, kNone}, gain[2] = {1.f, 1.f}, l[2] = {0.f, 0.f};
     int tok0 = s_first * 16, id_c = -1;
     float ks_c = 0.f, vs_c = 0.f;
@@ -451,7 +460,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
         }
       }
       const bool grew = top[0] > m[0] + kSlack || top[1] > m[1] + kSlack ||
-                        top_v[0] > M[0] + kSlack || top_v[1] > M[1] + kSlack;
+                        top_v[0] > M[0] + (kSlack + kLift) || top_v[1] > M[1] + (kSlack + kLift);
       if (__any_sync(~0u, grew)) {
 #pragma unroll
         for (int r2 = 0; r2 < 2; r2++) {
@@ -460,7 +469,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
           x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
           y = fmaxf(y, __shfl_xor_sync(~0u, y, 1));
           y = fmaxf(y, __shfl_xor_sync(~0u, y, 2));
-          const float mn = fmaxf(m[r2], x), Mn = fmaxf(M[r2], y);
+          const float mn = fmaxf(m[r2], x), Mn = lifted(M[r2], y, mn);
           l[r2] *= ex2(m[r2] - mn);
           const float corr = ex2(M[r2] - Mn);
           m[r2] = mn;

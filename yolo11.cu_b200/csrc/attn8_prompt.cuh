@@ -240,7 +240,6 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const int pos = rq.kv - rq.q + tok;
     const int last = a.causal ? min(rq.kv - 1, pos) : rq.kv - 1, first = a.causal ? first_key(pos, a.window) : 0;
-    constexpr float kNone = -1e30f, kSlack = 6.f;      // as in the split kernel
     float m = kNone, M = kNone, gain = 1.f, l = 0.f;
     bool ok = true;
     for (int j = 0; j < tiles; j++) {
@@ -299,7 +298,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
               top_v = fmaxf(top_v, x + (c0 ? lv[2 + g] : lv[g]));
             }
           }
-          const float mn = fmaxf(m, top), Mn = fmaxf(M, top_v);
+          const float mn = fmaxf(m, top), Mn = lifted(M, top_v, mn);
           l *= ex2(m - mn);
           const float corr = ex2(M - Mn);
           m = mn;
@@ -323,7 +322,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
         sum = make_float2(0.f, 0.f);
         float over = -INFINITY;          // how far the tile passes the references
         const float2 neg = make_float2(-m, -m);
-        const float to_v = m - M;
+        const float to_v = m - M - kLift;
 #pragma unroll
         for (int c0 = 0; c0 < 64; c0 += 32) {
           uint32_t s[32];
