@@ -511,6 +511,29 @@ def test_attention_flat_tail_behind_a_loud_key(lib, cuda, rows, gap, spread):
         attend_one(lib, rt, kind, q, k, v, torch.ones(blocks), torch.ones(blocks), T, 1.0)
 
 
+@pytest.mark.parametrize("rows", [1, 66])
+@pytest.mark.parametrize("order", [1, -1])
+@pytest.mark.parametrize("gap,loud", [(84.0, 11), (95.0, 11), (90.0, 90), (110.0, 110), (70.0, 110), (0.0, 110)])
+def test_attention_value_scales_far_apart(lib, cuda, rows, order, gap, loud):
+    """A block of zero values has the smallest scale (2^-126); with the highest scores and a block of a large
+    scale beside it, the factor between weights and their 16-bit form stays finite."""
+    from yolo11_cu_b200 import runtime as rt
+    T, D, blocks = 16, 64, 13
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(blocks, T, D, generator=g) * 20 for _ in range(2))
+    vs = torch.ones(blocks)
+    for b, e in ((0, -126), (1, loud), (2, -20)):
+        vs[b] = 2.0 ** e
+    k[..., 0] = 0
+    k[0, :, 0] = 16
+    v[0] = 0
+    q = torch.randn(rows, 2, D, generator=g) * (1 / 160)
+    q[..., 0] = gap / 16
+    if order < 0:
+        k, v, vs = k.flip(0), v.flip(0), vs.flip(0)
+    attend_one(lib, rt, "bf16", q, k, v, torch.ones(blocks), vs, T, 1.0)
+
+
 def test_attention_offsets_past_32_bits(lib, cuda):
     """A pool whose code offsets pass 2^31 and 2^32."""
     from yolo11_cu_b200 import runtime as rt

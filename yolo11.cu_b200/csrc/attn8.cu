@@ -57,6 +57,10 @@ constexpr float kNone = -1e30f, kSlack = 6.f, kLift = 9.f;
 __device__ __forceinline__ float lifted(float M, float top_v, float m) {
   return fmaxf(M, fmaxf(top_v - kLift, m - 126.f));
 }
+// Value scale * 2^(m - M), by which weights become their 16-bit form.  It passes 2^128 only for a block whose
+// scores lie 2^113 and more below the row's (a block of zero values has scale 2^-126, so M can lie that far
+// below m); its weights 0 .. 2^-113 then count for less, but not as 0 * inf.
+__device__ __forceinline__ float weight_factor(float scale, float gain) { return fminf(scale * gain, 3.402823466e38f); }
 // Which kernel: the tcgen05 tiles take whole rows of keys, so they need enough tiles to fill the SMs; the
 // split list fills them with anything but does 16 rows at a time.  Measured, 16 / 4 heads, rows a request and
 // key head -> us on the split list | on tiles: 8 requests of 2000 keys, 128 channels: 16: 24 | 50, 64: 26 | 50,
@@ -487,7 +491,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
       for (int u = 0; u < 2; u++) {
 #pragma unroll
         for (int r2 = 0; r2 < 2; r2++) {
-          const float f_v = vs[u] * gain[r2];
+          const float f_v = weight_factor(vs[u], gain[r2]);
 #pragma unroll
           for (int j = 0; j < 2; j++) {
             const float x0 = ex2(fmaf(s[u][j][2 * r2], k[u][r2], -m[r2]));

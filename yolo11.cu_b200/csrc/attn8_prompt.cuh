@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
           load_s(s, c0);
 #pragma unroll
           for (int g = 0; g < 2; g++) {
-            const float k = kk[c0 / 16 + g], f = vs[c0 / 16 + g] * gain;
+            const float k = kk[c0 / 16 + g], f = weight_factor(vs[c0 / 16 + g], gain);
             float top = -INFINITY;
 #pragma unroll
             for (int i = 8 * g; i < 8 * g + 8; i++) {
