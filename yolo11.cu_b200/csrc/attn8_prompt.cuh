@@ -67,7 +67,6 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
   __shared__ __align__(8) uint64_t bars[10];
   __shared__ uint32_t tslot;
   __shared__ int found_r, found_tile;
-  __shared__ volatile int abort_flag;
   __shared__ int nan_lo, nan_hi;                  // tiles of keys where a NaN value was taken out
   // scales of the 16-token groups of tile j at j % 4, with the logarithm of the value scale; ks < 0: not there
   __shared__ __align__(16) float ks_sm[4][4], vs_sm[4][4], lv_sm[4][4];
@@ -186,7 +185,6 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       mbar_init(o_done + i, 1);
     }
     mbar_fence_init();
-    abort_flag = 0;
     nan_lo = 0x7fffffff;
     nan_hi = -1;
   }
@@ -245,7 +243,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
     for (int j = 0; j < tiles; j++) {
       const int buf = j & 1, turn = (j >> 1) & 1;
       const uint32_t s_at = s_tm + lanes + buf * 64;
-      if (!mbar_wait(s_full + buf * 8, turn, 0x503)) { abort_flag = 1; ok = false; break; }
+      if (!mbar_wait(s_full + buf * 8, turn, 0x503)) { ok = false; break; }
       tc_fence_after();
       const int key0 = (j0 + j) * 64;
       __align__(16) float kk[4], vs[4], lv[4];
@@ -305,7 +303,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
           M = Mn;
           gain = ex2(mn - Mn);
           if (j > 0) {
-            if (!mbar_wait(o_done + (buf ^ 1) * 8, ((j - 1) >> 1) & 1, 0x509)) { abort_flag = 1; ok = false; break; }
+            if (!mbar_wait(o_done + (buf ^ 1) * 8, ((j - 1) >> 1) & 1, 0x509)) { ok = false; break; }
             tc_fence_after();
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 16) {
@@ -493,7 +491,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       ahead = entry(j + 2);
       call(j + kAhead + 1, far);
       far = far_entry(j + kAhead + 2);
-      if (j > 1 && !mbar_wait(s_full + buf * 8, before, 0x501)) { abort_flag = 1; break; }   // QK j - 2 has read its keys
+      if (j > 1 && !mbar_wait(s_full + buf * 8, before, 0x501)) break;   // QK j - 2 has read its keys
       store(kv, k_sm + buf * L::kTile);
       if (w == 0 && lane < 4) {
         ks_sm[j & 3][lane] = ids < 0 ? -1.f : ks;
@@ -505,7 +503,7 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       load(kv, c.k, j + 1, ids_next);
       ks = scale_of(c.kscale, ids_next);
       vs = scale_of(c.vscale, ids_next);
-      if (j > 1 && !mbar_wait(o_done + buf * 8, before, 0x502)) { abort_flag = 1; break; }   // PV j - 2 its values
+      if (j > 1 && !mbar_wait(o_done + buf * 8, before, 0x502)) break;   // PV j - 2 its values
       const int key0 = (j0 + j) * 64;
       if (key0 < all_lo || key0 + 64 > all_hi) take_out(j);
       store(vv, v_sm + buf * L::kTile);
@@ -541,7 +539,6 @@ __global__ void __launch_bounds__(kProThreads, D == 256 ? 1 : 2) attn8_prompt_ke
       // QK j + 2 takes the columns of P j: the order of MMAs with different accumulators is not promised
       if (j + 2 < tiles) ok = mbar_wait(o_done + buf * 8, turn, 0x508) && qk(j + 2);
     }
-    if (!ok) abort_flag = 1;
   }
   tc_fence_before();
   __syncthreads();
