@@ -16,12 +16,12 @@ namespace yk {
 //  * Lane (g, t) reads the scales and zero points of block t of its outputs one chunk ahead; they
 //    reach the other lanes by shuffles.  (In the ring, by aligned words, they cost as many L2
 //    sectors as the codes.)
-//  * The CTA's 8 warps are WN along the outputs times WK along the columns; each warp takes R
-//    output tiles, which share the x operand.  The WK partial sums meet in shared memory.
+//  * The CTA's 8 warps are WN along the outputs times WK along the columns.  The WK partial sums meet
+//    in shared memory.
 // Measured (fp16 x, groups of 128): 1 x 4096 x 4096 6.7 us (of which a launch is about 2.5), 1 x 28672 x 8192 58 us,
-// 2.0 TB/s: bound by the instructions around the MMAs (about 300 a KB of codes).  With one row 1 or 2 tiles
-// a warp (R) and 1 or 2 warps along the outputs (WN) are within 5 % there; small products want R = WN = 1
-// (512 outputs: 4.6 us, else 6.5 and more).
+// 2.0 TB/s: bound by the instructions around the MMAs (about 300 a KB of codes).  With one row 1 or 2 warps
+// along the outputs (WN) are within 5 % there; small products want WN = 1 (512 outputs: 4.6 us, else 6.5 and
+// more).
 struct Gemv4Args {
   YkGemv4 p;
   int x_vec;       // x rows allow 16-byte (e4m3: 8-byte) loads
@@ -97,48 +97,45 @@ __device__ __forceinline__ void codes8(uint32_t w, const Zero& z, uint32_t (&o)[
     for (int i = 0; i < 4; i++) o[i] = bsub2(and_or(w >> (4 * i), 0x000f000fu, 0x43004300u), z.a);
   }
 }
-template <int NT, int R>
+template <int NT>
 struct Gemv {
-  static constexpr int kStages = R == 1 ? 5 : 4;
+  static constexpr int kStages = 5;
   // codes of 16 outputs: four blocks, 32 bytes more than 256 apart so that the pieces a warp
   // writes at once fall into different banks
   static constexpr int kBlock = 256 + 32, kTile = 4 * kBlock;
-  static constexpr int kStage = R * kTile;
-  static constexpr int kRing = kGemvWarps * kStages * kStage, kMeet = kGemvWarps * R * NT * 512;
+  static constexpr int kRing = kGemvWarps * kStages * kTile, kMeet = kGemvWarps * NT * 512;
   static constexpr int kSmem = kRing > kMeet ? kRing : kMeet;
 };
 
 // XT: type of x; the MMA is bf16 for bf16 rows and fp16 otherwise (e4m3 converts exactly).
 // GB: blocks (32 columns) of a group of w.
-template <int XT, int GB, int NT, int R, int WN>
+template <int XT, int GB, int NT, int WN>
 __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel(const __grid_constant__ Gemv4Args ga) {
-  using S = Gemv<NT, R>;
+  using S = Gemv<NT>;
   constexpr bool X8 = XT == YK_E4M3, F16 = XT != YK_BF16;
-  constexpr int WK = kGemvWarps / WN, kStages = S::kStages, kStage = S::kStage, kTile = S::kTile;
+  constexpr int WK = kGemvWarps / WN, kStages = S::kStages, kTile = S::kTile;
   extern __shared__ __align__(16) uint8_t gemv_sm[];
   uint8_t* const sm = gemv_sm;
   const YkGemv4& p = ga.p;
   const bool zero = ga.zero;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int wn = warp % WN, wk = warp / WN;
-  const int n0 = (blockIdx.x * WN + wn) * R * 16;   // this warp's first output
+  const int n0 = (blockIdx.x * WN + wn) * 16;   // this warp's first output
   const int K = p.k, chunks = (K + 127) / 128;
   const int count = n0 < p.n && chunks > wk ? (chunks - wk + WK - 1) / WK : 0;
-  const uint32_t ring = smem_u32(sm) + warp * kStages * kStage;
-  const uint8_t* const ring_p = sm + warp * kStages * kStage;
+  const uint32_t ring = smem_u32(sm) + warp * kStages * kTile;
+  const uint8_t* const ring_p = sm + warp * kStages * kTile;
 
-  // first codes, scales and zero points of this lane's outputs g, g + 8 of each tile
-  const uint8_t *wrow[R][2], *zrow[R][2];
-  const uint16_t* srow[R][2];
+  // first codes, scales and zero points of this lane's outputs g, g + 8
+  const uint8_t *wrow[2], *zrow[2];
+  const uint16_t* srow[2];
 #pragma unroll
-  for (int r = 0; r < R; r++)
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const long long n = min(n0 + r * 16 + g + 8 * h, p.n - 1);
-      wrow[r][h] = (const uint8_t*)p.w + n * p.w_row + t * 16;
-      srow[r][h] = (const uint16_t*)p.wscale + n * p.group_row + t / GB;
-      zrow[r][h] = (const uint8_t*)p.wzero + n * p.group_row + t / GB;
-    }
+  for (int h = 0; h < 2; h++) {
+    const long long n = min(n0 + g + 8 * h, p.n - 1);
+    wrow[h] = (const uint8_t*)p.w + n * p.w_row + t * 16;
+    srow[h] = (const uint16_t*)p.wscale + n * p.group_row + t / GB;
+    zrow[h] = (const uint8_t*)p.wzero + n * p.group_row + t / GB;
+  }
   constexpr int kPer = 4 / GB;       // groups of a chunk
   const auto x_group = [&](int k) { return ga.x_shift >= 0 ? k >> ga.x_shift : k / ga.xgroup; };
   uint32_t fill = ring;
@@ -148,10 +145,8 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
       const int c = wk + i * WK;
       const bool ok = c * 128 + t * 32 < K;
 #pragma unroll
-      for (int r = 0; r < R; r++)
-#pragma unroll
-        for (int h = 0; h < 2; h++) cp_async_at<16>(fill + piece + r * kTile + h * 128, wrow[r][h] + c * 64, ok);
-      fill = fill + kStage == ring + kStages * kStage ? ring : fill + kStage;
+      for (int h = 0; h < 2; h++) cp_async_at<16>(fill + piece + h * 128, wrow[h] + c * 64, ok);
+      fill = fill + kTile == ring + kStages * kTile ? ring : fill + kTile;
     }
     cp_async_commit();
   };
@@ -160,11 +155,9 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
 #pragma unroll
   for (int i = 0; i < kStages - 1; i++) issue(i);
 
-  float tot[R][NT][4];
+  float tot[NT][4];
 #pragma unroll
-  for (int r = 0; r < R; r++)
-#pragma unroll
-    for (int j = 0; j < NT; j++) tot[r][j][0] = tot[r][j][1] = tot[r][j][2] = tot[r][j][3] = 0.f;
+  for (int j = 0; j < NT; j++) tot[j][0] = tot[j][1] = tot[j][2] = tot[j][3] = 0.f;
 
   // x of rows j * 8 + g (past the last row that row again: its sums are not written): this lane's
   // 8 columns of a block
@@ -216,17 +209,15 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
       xs_row[j][e] = X8 ? p.xscale + min(j * 8 + 2 * t + e, p.rows - 1) * p.xscale_row : nullptr;
 
   // scales and zero points of the next chunk's block t
-  uint32_t s_next[R][2], z_next[R][2];
+  uint32_t s_next[2], z_next[2];
   const auto load_scales = [&](int i) {
     const int c = wk + i * WK;
     const bool ok = i < count && c * 128 + t * 32 < K;
 #pragma unroll
-    for (int r = 0; r < R; r++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        s_next[r][h] = ok ? srow[r][h][c * kPer] : 0;
-        z_next[r][h] = zero && ok ? zrow[r][h][c * kPer] : 8;
-      }
+    for (int h = 0; h < 2; h++) {
+      s_next[h] = ok ? srow[h][c * kPer] : 0;
+      z_next[h] = zero && ok ? zrow[h][c * kPer] : 8;
+    }
   };
   load_scales(0);
 
@@ -248,21 +239,19 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
     for (int j = 0; j < NT; j++)
 #pragma unroll
       for (int e = 0; e < 2; e++) xs[j][e] = X8 && ga.xgroup ? xs_row[j][e][xg] : 1.f;
-    float sw[R][2];               // of block t
-    uint32_t zw[R][2];
+    float sw[2];                  // of block t
+    uint32_t zw[2];
 #pragma unroll
-    for (int r = 0; r < R; r++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        sw[r][h] = XT == YK_BF16 || (X8 && ga.bf16) ? elem_to_float<true>(s_next[r][h]) : elem_to_float<false>(s_next[r][h]);
-        zw[r][h] = z_next[r][h];
-      }
+    for (int h = 0; h < 2; h++) {
+      sw[h] = XT == YK_BF16 || (X8 && ga.bf16) ? elem_to_float<true>(s_next[h]) : elem_to_float<false>(s_next[h]);
+      zw[h] = z_next[h];
+    }
     issue(i + kStages - 1);
     load_scales(i + 1);
     cp_async_wait<kStages - 1>();
     __syncwarp();                 // every lane's pieces of this stage are there
-    float acc[R][NT][4];
-    Zero zp[R][2];
+    float acc[NT][4];
+    Zero zp[2];
 #pragma unroll
     for (int b = 0; b < 4; b++) {
       uint32_t x[NT][4];
@@ -278,64 +267,59 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
 #pragma unroll
           for (int e = 0; e < 2; e++) xs[j][e] = xs_row[j][e][xb];
       }
+      const uint8_t* at = src + b * S::kBlock;
+      if (b % GB == 0) {
 #pragma unroll
-      for (int r = 0; r < R; r++) {
-        const uint8_t* at = src + r * kTile + b * S::kBlock;
-        if (b % GB == 0) {
+        for (int h = 0; h < 2; h++)
+          zp[h] = zero_of<F16>(zero ? __shfl_sync(~0u, zw[h], (lane & ~3) + b) : 8);
+      }
+      uint32_t q[2][4];
 #pragma unroll
-          for (int h = 0; h < 2; h++)
-            zp[r][h] = zero_of<F16>(zero ? __shfl_sync(~0u, zw[r][h], (lane & ~3) + b) : 8);
-        }
-        uint32_t q[2][4];
+      for (int h = 0; h < 2; h++) codes8<F16>(*(const uint32_t*)(at + 128 * h), zp[h], q[h]);
 #pragma unroll
-        for (int h = 0; h < 2; h++) codes8<F16>(*(const uint32_t*)(at + 128 * h), zp[r][h], q[h]);
+      for (int e = 0; e < 2; e++) {
+        const uint32_t a[4] = {q[0][2 * e], q[1][2 * e], q[0][2 * e + 1], q[1][2 * e + 1]};
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const uint32_t a[4] = {q[0][2 * e], q[1][2 * e], q[0][2 * e + 1], q[1][2 * e + 1]};
+        for (int j = 0; j < NT; j++) mma_gemv<F16>(acc[j], a, x[j][2 * e], x[j][2 * e + 1], b % GB == 0 && e == 0);
+      }
+      if (b % GB == GB - 1) {
 #pragma unroll
-          for (int j = 0; j < NT; j++) mma_gemv<F16>(acc[r][j], a, x[j][2 * e], x[j][2 * e + 1], b % GB == 0 && e == 0);
-        }
-        if (b % GB == GB - 1) {
+        for (int h = 0; h < 2; h++) {
+          const float f = GB == 4 ? sw[h] : __shfl_sync(~0u, sw[h], (lane & ~3) + b);
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const float f = GB == 4 ? sw[r][h] : __shfl_sync(~0u, sw[r][h], (lane & ~3) + b);
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-              const float2 both = X8 ? ffma2(make_float2(f, f), make_float2(xs[j][0], xs[j][1]), make_float2(0.f, 0.f))
-                                     : make_float2(f, f);
-              const float2 v = ffma2(make_float2(acc[r][j][2 * h], acc[r][j][2 * h + 1]), both,
-                                     make_float2(tot[r][j][2 * h], tot[r][j][2 * h + 1]));
-              tot[r][j][2 * h] = v.x;
-              tot[r][j][2 * h + 1] = v.y;
-            }
+          for (int j = 0; j < NT; j++) {
+            const float2 both = X8 ? ffma2(make_float2(f, f), make_float2(xs[j][0], xs[j][1]), make_float2(0.f, 0.f))
+                                   : make_float2(f, f);
+            const float2 v = ffma2(make_float2(acc[j][2 * h], acc[j][2 * h + 1]), both,
+                                   make_float2(tot[j][2 * h], tot[j][2 * h + 1]));
+            tot[j][2 * h] = v.x;
+            tot[j][2 * h + 1] = v.y;
           }
         }
       }
     }
     __syncwarp();                 // every lane has read the stage
-    src += kStage;
-    if (src >= ring_p + kStages * kStage) src -= kStages * kStage;
+    src += kTile;
+    if (src >= ring_p + kStages * kTile) src -= kStages * kTile;
   }
   cp_async_wait<0>();
   __syncthreads();
-  // sums of the WK warps along the columns: [warp][tile][row of x][output]
+  // sums of the WK warps along the columns: [warp][row of x][output]
   float* meet = (float*)sm;
 #pragma unroll
-  for (int r = 0; r < R; r++)
+  for (int j = 0; j < NT; j++)
 #pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        meet[((warp * R + r) * NT * 8 + j * 8 + 2 * t + (e & 1)) * 16 + g + (e >> 1) * 8] = tot[r][j][e];
+    for (int e = 0; e < 4; e++)
+      meet[(warp * NT * 8 + j * 8 + 2 * t + (e & 1)) * 16 + g + (e >> 1) * 8] = tot[j][e];
   __syncthreads();
-  constexpr int kOut = WN * R * 16;
+  constexpr int kOut = WN * 16;
   for (int i = tid; i < kOut * p.rows; i += 32 * kGemvWarps) {
     const int m = i / kOut, j = i % kOut, n = blockIdx.x * kOut + j;
     if (n >= p.n) continue;
-    const int w = j / (R * 16), r = j / 16 % R;
+    const int w = j / 16;
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < WK; k++) v += meet[(((k * WN + w) * R + r) * NT * 8 + m) * 16 + j % 16];
+    for (int k = 0; k < WK; k++) v += meet[((k * WN + w) * NT * 8 + m) * 16 + j % 16];
     if (X8 && !ga.xgroup) v *= p.xscale[m * p.xscale_row];
     if (p.bias) v += p.bias[n];
     ((uint16_t*)p.y)[m * p.y_row + n] = ga.bf16 ? float_to_elem<true>(v) : float_to_elem<false>(v);
@@ -344,12 +328,12 @@ __global__ void __launch_bounds__(32 * kGemvWarps, NT == 8 ? 1 : 2) gemv4_kernel
 
 #include "gemv4_tc.cuh"
 
-template <int XT, int GB, int NT, int R, int WN>
+template <int XT, int GB, int NT, int WN>
 static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
-  const auto kern = gemv4_kernel<XT, GB, NT, R, WN>;
-  if (smem_attr(kern, Gemv<NT, R>::kSmem) != cudaSuccess) return check_launch("gemv4 attr");
-  constexpr int outputs = WN * R * 16;
-  launch_k(kern, (a.p.n + outputs - 1) / outputs, 32 * kGemvWarps, Gemv<NT, R>::kSmem, st, a);
+  const auto kern = gemv4_kernel<XT, GB, NT, WN>;
+  if (smem_attr(kern, Gemv<NT>::kSmem) != cudaSuccess) return check_launch("gemv4 attr");
+  constexpr int outputs = WN * 16;
+  launch_k(kern, (a.p.n + outputs - 1) / outputs, 32 * kGemvWarps, Gemv<NT>::kSmem, st, a);
   note_launch();
   return check_launch("gemv4");
 }
@@ -361,10 +345,10 @@ static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
     if (m <= 32) return launch_gemv4_tc<XT, GB, 32>(a, st);
     return launch_gemv4_tc<XT, GB, 64>(a, st);
   }
-  if (m <= 8) return launch_gemv4<XT, GB, 1, 1, 1>(a, st);
-  if (m <= 16) return launch_gemv4<XT, GB, 2, 1, 1>(a, st);
-  if (m <= 32) return launch_gemv4<XT, GB, 4, 1, 2>(a, st);
-  return launch_gemv4<XT, GB, 8, 1, 2>(a, st);
+  if (m <= 8) return launch_gemv4<XT, GB, 1, 1>(a, st);
+  if (m <= 16) return launch_gemv4<XT, GB, 2, 1>(a, st);
+  if (m <= 32) return launch_gemv4<XT, GB, 4, 2>(a, st);
+  return launch_gemv4<XT, GB, 8, 2>(a, st);
 }
 template <int XT>
 static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
