@@ -734,6 +734,21 @@ def test_gemv_many_outputs(lib, cuda, kind, rows, n, k, group):
     run_gemv(lib, rt, kind, rows, n, k, group, xgroup=3 * group, shift=3)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,n,k,group", [
+    (8, 4737, 128, 128), (9, 14209, 128, 32), (16, 14208, 320, 64), (16, 14300, 672, 32), (12, 18950, 256, 128),
+    (17, 9473, 96, 32), (32, 9472, 384, 128), (33, 4737, 576, 64), (64, 4736, 288, 32), (64, 4750, 640, 128),
+    (64, 48, 2048, 64), (33, 100, 2176, 128), (64, 130, 2048, 32), (40, 333, 1984, 64)])
+def test_gemv_either_side_of_the_rule(lib, cuda, kind, rows, n, k, group):
+    from yolo11_cu_b200 import runtime as rt
+    run_gemv(lib, rt, kind, rows, n, k, group)
+    run_gemv(lib, rt, kind, rows, n, k, group, zero=True, bias=True, extra=1)
+    run_gemv(lib, rt, kind, rows, n, k, group, xgroup=0, bias=True, shift=1)
+    run_gemv(lib, rt, kind, rows, n, k, group, xgroup=128, zero=True, extra=8)
+    run_gemv(lib, rt, kind, rows, n, k, group, xgroup=384, shift=8)
+    run_gemv(lib, rt, kind, rows, n, k, group, xgroup=group, shift=3)
+
+
 def test_gemv_large_values(lib, cuda):
     """fp16 x near its largest value: sums stay in 32 bits; x of infinities gives no finite sum."""
     from yolo11_cu_b200 import runtime as rt

@@ -33,10 +33,17 @@ struct Gemv4Args {
   int x_inside;    // it may change inside a chunk of 128 columns
 };
 constexpr int kGemvWarps = 8;
-// tcgen05 (gemv4_tc.cuh) from this many outputs on, for more than 8 rows.  28672 x 8192, 1, 8, 16, 32, 64
-// rows: 58, 67, 72, 154, 425 us on warp MMAs, 70, 70, 71, 92, 149 us there; with fewer outputs its CTAs
-// (128 outputs each) leave most SMs without work.
-constexpr int kGemvTcOutputs = 64 * 148;
+// Which kernel, for more than 8 rows.  A round of this one's CTAs (two an SM of 16 or of 32 outputs, or one of
+// 32) covers 1, 2, 1 times kGemvRound outputs for 9 - 16, 17 - 32, 33 - 64 rows.  The tcgen05 kernel
+// (gemv4_tc.cuh) has 128 outputs a CTA, so one of its rounds covers four times that, at a higher price: it is
+// taken where this one would need a fourth, a second, a second round.  Measured, us here | there, fp16 rows, 4096
+// columns in groups of 64: 16 rows: 9472 outputs 18.5 | 26.3, 14208: 26.4 | 26.8, 18944: 34.1 | 27.6; 32 rows:
+// 9472: 24.8 | 26.0, 9600: 41.3 | 26.0; 64 rows: 4096: 36.3 | 40.4, 4800: 66.2 | 40.4, 28672: 221 | 80 (512
+// columns: 4800: 11.9 | 12.7).  1 and 8 rows of 28672 x 8192: 58 | 70, 67 | 70.
+// e4m3 rows cost this kernel twice as much at 33 - 64 rows: 4096 x 4096, 64 rows 81 | 53, 33 rows 59 | 50 (512
+// columns: 13.6 | 17.6, 9.6 | 15.1; groups of 32: 82 | 77, 61 | 73).  So there tcgen05 takes any number of outputs
+// from kGemvLong columns on, except in groups of 32.
+constexpr int kGemvRound = 32 * 148, kGemvLong = 2048;
 
 // d = a * b + (first ? 0 : d)
 template <bool F16>
@@ -340,7 +347,9 @@ static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
 template <int XT, int GB>
 static int launch_gemv4(const Gemv4Args& a, cudaStream_t st) {
   const int m = a.p.rows, n = a.p.n;
-  if (m > 8 && n >= kGemvTcOutputs && (!a.xgroup || !a.x_inside)) {
+  const bool many = n > kGemvRound * (m <= 16 ? 3 : m <= 32 ? 2 : 1);
+  const bool dear = XT == YK_E4M3 && GB > 1 && m > 32 && a.p.k >= kGemvLong;
+  if (m > 8 && (many || dear) && (!a.xgroup || !a.x_inside)) {
     if (m <= 16) return launch_gemv4_tc<XT, GB, 16>(a, st);
     if (m <= 32) return launch_gemv4_tc<XT, GB, 32>(a, st);
     return launch_gemv4_tc<XT, GB, 64>(a, st);

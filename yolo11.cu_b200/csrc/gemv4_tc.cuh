@@ -1,4 +1,4 @@
-// Products with a 4-bit weight matrix of many outputs, on tcgen05 (included by gemv4.cu).
+// Products with a 4-bit weight matrix, many outputs or rows, on tcgen05 (included by gemv4.cu).
 //
 // The warp-MMA kernel spends most of its instructions around the products: x fragments, scales and zero
 // points that every lane of a quad needs, sums of eight columns a lane.  Here a thread owns an output
