@@ -214,10 +214,13 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
   const uint32_t ring = smem_u32(dec_sm) + warp * L::kWarpBytes;
   uint8_t* const q_sm = dec_sm + kDecWarps * L::kWarpBytes;
   float* const meet = (float*)(q_sm + 2 * L::kQBytes);
+  // Twin tiles: with at most 8 rows, rows 8 .. 15 of an fp16 tile are the same rows again, and hold what the
+  // 16-bit rounding of the weights leaves (bf16 outputs are too coarse to show it).
+  const auto twins = [&](const Seg& s) { return !BF16 && s.row_n <= 8; };
   // rows of a segment's q into buffer b (each thread its own 16-byte chunks)
   const auto load_q = [&](const Seg& s, int b) {
     for (int i = tid; i < 16 * D / 8; i += 32 * kDecWarps) {
-      const int rr = s.tile * 16 + min(i / (D / 8), s.row_n - 1), tok = rr / G;
+      const int rr = s.tile * 16 + min(i / (D / 8) & (twins(s) ? 7 : 15), s.row_n - 1), tok = rr / G;
       cp_async_at<16>(smem_u32(q_sm) + b * L::kQBytes + i / (D / 8) * L::kQRow + i % (D / 8) * 16,
                         (const uint16_t*)a.q + (long long)(s.q0 + tok) * a.q_row + (long long)(s.kh * G + rr - tok * G) * D + i % (D / 8) * 8);
     }
@@ -310,11 +313,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
   for (int turn = 0;; turn ^= 1) {
     const long long f_next = f + cur.cost;
 
+    const bool twin = twins(cur);
     // rows g and g + 8 of this lane: the keys they see, [first, last]
     int first[2], last[2], all_lo = 0, all_hi = cur.kv;    // [all_lo, all_hi): keys that every row sees
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const int pos = cur.kv - cur.q + (cur.tile * 16 + min(g + 8 * i, cur.row_n - 1)) / G;
+      const int pos = cur.kv - cur.q + (cur.tile * 16 + min(g + (twin ? 0 : 8 * i), cur.row_n - 1)) / G;
       last[i] = a.causal ? min(cur.kv - 1, pos) : cur.kv - 1;
       first[i] = a.causal ? first_key(pos, a.window) : 0;
     }
@@ -463,6 +467,10 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
           top_v[r2] = fmaxf(top_v[r2], x + lv[u]);
         }
       }
+      if (twin) {                // one reference for both
+        top[1] = top[0];
+        top_v[1] = top_v[0];
+      }
       const bool grew = top[0] > m[0] + kSlack || top[1] > m[1] + kSlack ||
                         top_v[0] > M[0] + (kSlack + kLift) || top_v[1] > M[1] + (kSlack + kLift);
       if (__any_sync(~0u, grew)) {
@@ -489,16 +497,29 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
       uint32_t pa[2][4];
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-#pragma unroll
-        for (int r2 = 0; r2 < 2; r2++) {
+        const auto weights = [&](int r2, int j) {
+          const float x0 = ex2(fmaf(s[u][j][2 * r2], k[u][r2], -m[r2]));
+          const float x1 = ex2(fmaf(s[u][j][2 * r2 + 1], k[u][r2], -m[r2]));
+          l[r2] += x0 + x1;
           const float f_v = weight_factor(vs[u], gain[r2]);
+          return make_float2(x0 * f_v, x1 * f_v);
+        };
+        if (twin) {
 #pragma unroll
           for (int j = 0; j < 2; j++) {
-            const float x0 = ex2(fmaf(s[u][j][2 * r2], k[u][r2], -m[r2]));
-            const float x1 = ex2(fmaf(s[u][j][2 * r2 + 1], k[u][r2], -m[r2]));
-            l[r2] += x0 + x1;
-            pa[u][2 * j + r2] = pack_half2(x0 * f_v, x1 * f_v);
+            const float2 x = weights(0, j);
+            pa[u][2 * j] = pack_half2(x.x, x.y);
+            const float2 is = pair_to_float2<false>(pa[u][2 * j]);
+            pa[u][2 * j + 1] = pack_half2(x.x - is.x, x.y - is.y);
           }
+        } else {
+#pragma unroll
+          for (int r2 = 0; r2 < 2; r2++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              const float2 x = weights(r2, j);
+              pa[u][2 * j + r2] = pack_half2(x.x, x.y);
+            }
         }
       }
 #pragma unroll
@@ -558,6 +579,14 @@ __global__ void __launch_bounds__(32 * kDecWarps, D == 256 ? 1 : 2) attn8_split_
                 if (g == (r16 & 7) && (e >> 1) == (r16 >> 3)) o[h * 16 + j][e] += one[j][e];
           }
         }
+      }
+    }
+
+    if (twin) {
+#pragma unroll
+      for (int j = 0; j < D / 8; j++) {
+        o[j][0] += o[j][2];
+        o[j][1] += o[j][3];
       }
     }
 
