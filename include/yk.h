@@ -261,7 +261,9 @@ int yk_kv_append(const YkKvCache* c, const YkKvRows* x, yk_stream_t st);
 // tokens, query head h reads key/value head h / (heads / c->heads).  causal: row i of a request
 // of q rows sees keys j <= kv_lens[r] - q + i, with a window w > 0 only j > kv_lens[r] - q + i
 // - w; else every key.  A row that sees no key gives zeros (lse -inf); keys in blocks outside
-// the pool are not seen.  What the cache holds past kv_lens is never used.
+// the pool are not seen.  What the cache holds past kv_lens is never used.  Scores, their maximum and
+// the weights' sum are in 32 bits.  The weights meet the values as fp16, rounded once; for fp16 rows of a
+// request with at most 8 rows a key head, in a call of few rows, as two parts of fp16 (22 bits).
 typedef struct {
   const void* q;           // head h of row n at n*q_row + h*dim; fp16 or bf16, 16-byte aligned
   void* out;               // likewise, with out_row

@@ -33,14 +33,17 @@ struct Attn8Args {
 //  * One scale a (block, head): the key scale multiplies the scores; the value scale multiplies
 //    the weights, whose 16-bit form is taken relative to the largest weight * scale so far (M
 //    below, kept beside the softmax's m), so blocks of very different loudness keep their bits.
-//  * Weights enter the second product as fp16 (one rounding, 2^-11 of a weight: bf16 has 8 bits, and a
-//    second fp16 part would double the MMAs); their sum l stays in fp32.  The largest lies at 2^9 .. 2^15
-//    (kLift, kSlack), so a weight keeps its bits down to 2^-23 of the largest, times scale, and is lost below
-//    2^-34: a long flat tail behind one loud key still counts.
-// Measured: 2 requests over 393,000 keys (8 query heads a key head, 128 channels, 145 MB) 50 us, 2.9 TB/s:
-// the keys themselves pass at 5.6 TB/s (26 us), 5 us go before the first of them (lengths, table, block,
+//  * Weights enter the second product as fp16 (11 bits, where bf16 has 8); their sum l stays in fp32.  The
+//    largest lies at 2^9 .. 2^15 (kLift, kSlack), so a weight keeps its bits down to 2^-23 of the largest, times
+//    scale, and is lost below 2^-34: a long flat tail behind one loud key still counts.  One rounding makes
+//    an fp16 output 1.27 - 1.42 times as far from 64 bits as its own rounding alone; up to 8 rows a tile, the other 8
+//    rows carry the rest of the weights for nothing (1.00 times).  For more rows the rest would need MMAs of
+//    its own (64 requests of 4 rows 68.8 -> 74.0 us), so they round once, like bf16 outputs, where it does not show.
+//  * References that move only when the maximum passes them by a slack are a known variant of the one-pass softmax.
+// Measured: 2 requests over 283,000 keys (8 query heads a key head, 128 channels, 145 MB) 50 us, 2.9 TB/s:
+// the keys themselves pass at 5.3 TB/s (28 us), 5 us go before the first of them (lengths, table, block,
 // codes: four loads in a row), the rest into meeting and joining 74 parts an item; 64 requests of 64 to
-// 8192 keys (221 MB) 63 us, 3.5 TB/s; one request of 431 keys 8.2 us.
+// 8192 keys (221 MB) 64 us, 3.5 TB/s; one request of 431 keys 8.4 us.
 constexpr int kDecWarps = 4;
 constexpr int kDecSub = 2 * kDecWarps;     // 16-token subtiles of a granule: two for each warp
 constexpr int kDecGran = 16 * kDecSub;     // tokens of a granule

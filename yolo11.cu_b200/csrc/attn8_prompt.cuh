@@ -7,7 +7,8 @@
 //    Weights are taken relative to a reference that follows the row's maximum only when that passes
 //    it by 2^6, so a tile is read once: if its maximum stays below, the weights stand; else (seldom)
 //    the reference moves, O is rescaled, and the tile is done again.  P goes as fp16 over the columns of
-//    its S: it is the A operand straight from TMEM.
+//    its S: it is the A operand straight from TMEM.  (One rounding: fp16 outputs 1.39 - 1.42 times as far from 64 bits as
+//    their own rounding alone; a second part would double the PV products and half of the weights' work again.)
 //  * warps 4-7 read the codes of the next tile into registers while this one's are in use, convert them
 //    (exactly) to fp16 and write them into 128-byte-swizzled tiles [slab of 64 channels][token][64], which
 //    the MMA reads as a K-major operand for the keys and as an MN-major one for the values.
@@ -16,8 +17,8 @@
 //    tile j + 1.
 // Two CTAs an SM up to 128 channels.
 // Measured: 8 ragged requests, 5616 rows of 16 heads over up to 3832 keys (67.6 GFLOP) 139 us, 0.49 PFLOP/s, 29 %
-// of the measured burst rate (the warp-MMA tiles of the split kernel: 650 us).  A CTA spends about 2700
-// cycles a tile: 1100 in the weights (64 exponentials a row, shared with the other CTA), the rest in
+// of the measured burst rate (the warp-MMA tiles of the split kernel: 650 us).  A CTA spends about 2800
+// cycles a tile: 1200 in the weights (64 exponentials a row, shared with the other CTA), the rest in
 // waits for S and in the chain P -> PV -> QK; longest tiles first leave an SM within 10 % of the mean.
 constexpr int kProThreads = 288;
 constexpr int kProSort = 128;          // requests up to which tiles are ordered by their length

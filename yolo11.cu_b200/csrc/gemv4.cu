@@ -19,7 +19,7 @@ namespace yk {
 //  * The CTA's 8 warps are WN along the outputs times WK along the columns.  The WK partial sums meet
 //    in shared memory.
 // Measured (fp16 x, groups of 128): 1 x 4096 x 4096 6.7 us (of which a launch is about 2.5), 1 x 28672 x 8192 58 us,
-// 2.0 TB/s: bound by the instructions around the MMAs (about 300 a KB of codes).  With one row 1 or 2 warps
+// 2.0 TB/s: bound by the instructions around the MMAs (275 a KB of codes).  With one row 1 or 2 warps
 // along the outputs (WN) are within 5 % there; small products want WN = 1 (512 outputs: 4.6 us, else 6.5 and
 // more).
 struct Gemv4Args {
@@ -89,7 +89,8 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-// The 8 codes of a word minus the zero point: pairs (0, 4), (1, 5), (2, 6), (3, 7).
+// The 8 codes of a word minus the zero point: pairs (0, 4), (1, 5), (2, 6), (3, 7).  A known conversion: small
+// integers put into the low mantissa bits of a power of two are that power plus the integer.
 // fp16: 1024 + q in the low nibble's place; 1024 + 16 q a nibble higher, times 1/16.
 template <bool F16>
 __device__ __forceinline__ void codes8(uint32_t w, const Zero& z, uint32_t (&o)[4]) {

@@ -14,7 +14,7 @@
 //  * Scales and zero points come 8 groups at a time where their rows allow it: a thread a row means a
 //    line a lane, so each load costs the warp 32 lines.
 // Measured: 16 e4m3 rows x 28672 outputs x 8192 columns, groups of 64 with zero points (129 MB) 81 us, 1.6 TB/s (warp
-// MMAs: 96 us).  Two CTAs an SM take twice as long as one: an MMA of 16 columns of x ends only every 160
+// MMAs: 102 us).  Two CTAs an SM take twice as long as one: an MMA of 16 columns of x ends only every 160
 // cycles, whoever issues it; with the operand in shared memory instead the chain store -> MMA -> sums
 // got longer (109 us).
 template <int XT, int GB, int N>
