@@ -189,6 +189,7 @@ int yk_decode_nms_static(const YkLevel* levels, int nlevels, int batch, int nc, 
 #define YK_F16 0
 #define YK_BF16 1
 #define YK_E4M3 2
+#define YK_F32 3
 
 // Key/value cache in 8 bits: a pool of blocks of `tokens` tokens, one scale for each (block,
 // head).  Channel d of token t of head h in block b is code b*block_stride + (h*tokens + t)*dim
@@ -330,6 +331,112 @@ typedef struct {
 } YkGemv4;
 int yk_gemv4(const YkGemv4* p, yk_stream_t st);
 
+// Norm of each query and key head, and its rotary position, in one pass: h = a head's row (dim channels),
+// y = h / sqrt(mean(h^2) + eps) * weight in 32 bits (without a weight: y = h), then pair i < rot/2 turns by
+// the angle pos[axis of i][n] * freqs[i]: (a, b) -> (a cos - b sin, b cos + a sin), rounded once to dtype.
+// The pair is channels (i, i + rot/2), or (2i, 2i + 1) if interleaved; channels from rot on do not turn.
+// The first sections[0] pairs follow axis 0, the next sections[1] axis 1, and so on (time, row, column of
+// an image's tokens).  Angles are products in 64 bits, so far positions lose nothing.  Rows whose pos on
+// axis 0 is negative are left as they are.  Outputs may be the inputs themselves.
+typedef struct {
+  const void* q;           // head h of row n at n*q_row + h*dim; fp16 or bf16, 16-byte aligned
+  const void* k;           // likewise with k_row; NULL with kv_heads 0
+  void* q_out;             // likewise with q_out_row; q itself, or apart from it
+  void* k_out;
+  const void* q_weight;    // [dim] of dtype, or NULL: no norm
+  const void* k_weight;
+  const int* pos;          // axis a of row n at a*pos_axis + n
+  const float* freqs;      // [rot / 2] radians a position
+  long long q_row, k_row, q_out_row, k_out_row;   // elements, multiples of 8
+  long long pos_axis;
+  int rows;
+  int heads;               // query heads
+  int kv_heads;            // key heads (0: queries only); heads + kv_heads at most 1024
+  int dim;                 // 32, 64, 128 or 256
+  int rot;                 // channels that turn: a multiple of 16, at most dim
+  int axes;                // 1 .. 4
+  int sections[4];         // pairs of each axis, rot / 2 in all; with one axis all zeros serve too
+  int interleaved;
+  int dtype;               // YK_F16 or YK_BF16
+  float eps;
+} YkQkRotate;
+int yk_qk_rotate(const YkQkRotate* p, yk_stream_t st);
+
+// Matrices of 4-bit floats (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with a scale for each group
+// of columns of a row: YK_NVFP4 has groups of 16 with e4m3 scales, YK_MXFP4 groups of 32 with powers of two
+// (one byte e: 2^(e - 127), 255: NaN).  A value is code * scale of its group * scale of the whole matrix.
+// Byte i of a row holds column 2i in its low and 2i + 1 in its high half.  Scales lie in blocks of 128
+// rows x 4 groups, 512 bytes each, along the groups first: with B = ceil(groups / 4), the scale of row r
+// and group g is byte ((r / 128) * B + g / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + g % 4.
+#define YK_NVFP4 0
+#define YK_MXFP4 1
+// Bytes of the scales of rows x cols: whole blocks.  0 if an argument is out of range.
+size_t yk_fp4_scale_bytes(int rows, int cols, int format);
+// Rounds rows to 4 bits.  t = largest finite |x| of the group / (6 scale); the group's scale is t rounded to
+// e4m3, between 2^-9 and 448 (YK_NVFP4), or the smallest power of two >= t between 2^-96 and 2^96 (YK_MXFP4);
+// codes are x / (group's scale * scale) rounded to nearest, ties to even, at most 6 (infinities too).  A group
+// with a NaN has a NaN scale and codes 0.  Codes of columns past the last up to a multiple of 8, scales of groups past
+// the last up to a multiple of 4 and of rows past the last up to a multiple of 128 are 0.
+typedef struct {
+  const void* x;           // [rows][x_row] of dtype
+  void* codes;             // [rows][codes_row bytes], 16-byte aligned
+  void* scales;            // yk_fp4_scale_bytes, 16-byte aligned
+  void* values;            // [rows][values_row]: what the codes stand for, rounded to dtype; or NULL
+  long long x_row, values_row;   // elements
+  long long codes_row;     // bytes, a multiple of 16
+  int rows, cols;
+  int format;              // YK_NVFP4 or YK_MXFP4
+  int dtype;               // YK_F16 or YK_BF16
+  float scale;             // of the whole matrix, 2^-30 .. 2^30; 0: 1
+} YkQuantFp4;
+int yk_quant_fp4(const YkQuantFp4* p, yk_stream_t st);
+
+// y[m][j] = alpha * sum_k x[m][k] w[j][k] + bias[j] of two such matrices of one format, or, with w2, a gated
+// pair: g = alpha * x w^T, y = g / (1 + exp(-g)) * (alpha2 * x w2^T).  alpha takes the scales of the whole
+// matrices.  Sums in 32 bits, one rounding to dtype.  Any rows, n and k; with an odd k the last byte's high half
+// has to be 0 in x or w, and scales of groups past the last up to a multiple of 4 no NaN (yk_quant_fp4 writes both so).
+typedef struct {
+  const void* x;           // [rows][x_row bytes], 16-byte aligned
+  const void* xscale;      // yk_fp4_scale_bytes(rows, k, format), 16-byte aligned
+  const void* w;           // [n][w_row bytes]
+  const void* wscale;      // yk_fp4_scale_bytes(n, k, format)
+  const void* w2;          // as w, or NULL: not gated
+  const void* w2scale;
+  const float* bias;       // [n] or NULL; not with w2
+  void* y;                 // [rows][y_row]
+  long long x_row, w_row;  // bytes, multiples of 16
+  long long y_row;         // elements
+  int rows, n, k;
+  int format;              // YK_NVFP4 or YK_MXFP4
+  int dtype;               // YK_F16 or YK_BF16: y
+  float alpha, alpha2;     // 0: 1
+} YkGemmFp4;
+int yk_gemm_fp4(const YkGemmFp4* p, yk_stream_t st);
+
+// The next token of each row of scores.  weight_i = exp((l_i - max) / temperature) (a score of NaN or -infinity has
+// none; if the largest is +infinity, those that are have weight 1 and the others none).  In the order of falling scores,
+// equal ones by index, stay the first top_k; of these the shortest beginning whose weight reaches top_p
+// of theirs; and of these the ones of at least min_p times the largest weight.  The token is the first, by index, at which
+// the sum of the weights that stay passes u times their total.  Weights and sums are exact to 2^-44 of the
+// largest weight, whatever the launch.  A temperature that is not positive takes the largest score, the
+// lowest index among equal ones.  A row without any weight gives token -1, log probability -infinity, 0 kept.
+typedef struct {
+  const void* logits;      // [rows][row]: fp16, bf16 or fp32
+  const float* temperature;// [rows], or NULL: 1
+  const int* top_k;        // [rows]: 0 or less: all; or NULL
+  const float* top_p;      // [rows]: 1 or more, or NaN: all; 0 or less: one; or NULL
+  const float* min_p;      // [rows]: 0 or less, or NaN: all; or NULL
+  const float* u;          // [rows] in [0, 1) (a smaller one or NaN counts as 0, a larger as the last token); NULL: largest score
+  int* token;              // out [rows]
+  float* logprob;          // out [rows]: log of the token's weight over the total of those that stay; or NULL
+  int* kept;               // out [rows]: how many stay (of a weight that is not 0); or NULL
+  long long row;           // elements, >= n
+  int rows;
+  int n;                   // scores of a row, 1 .. 262144
+  int dtype;               // YK_F16, YK_BF16 or YK_F32
+} YkSample;
+int yk_sample(const YkSample* p, yk_stream_t st);
+
 // Device error word (bounded-wait timeouts) of the current device; cleared by the call.
 int yk_fetch_device_error(void);
 // Test hook for the bounded-wait failure path (no counterpart in the reference, which has no
@@ -346,6 +453,12 @@ int yk_test_nms_cluster(int size);
 // Test hook: the kernel behind yk_attn_kv8 (1: keys split over all CTAs, 2: 128-row tiles, 0: the
 // library's rule); tests compare both with the definition.
 int yk_test_attn_kv8(int kernel);
+// Test hook: the kernel behind yk_gemm_fp4 (1: whole tiles, 2: columns split over `split` = 1, 2, 4 or 8
+// CTAs; 0: the library's rules, each for itself); tests compare all with the definition.
+int yk_test_gemm_fp4(int kernel, int split);
+// Test hook: CTAs of a row in yk_sample (1, 2, 4 or 8; 0: the library's rule, as where a row needs more).
+// Results do not depend on it; tests compare all bit for bit.
+int yk_test_sample(int split);
 const char* yk_last_cuda_error(void);
 // Number of kernels this library launched since load (all devices) — a host-side counter.
 long long yk_launch_count(void);

@@ -1,0 +1,69 @@
+// Helpers of the 4-bit float operators (quant_fp4.cu, gemm_fp4.cu): conversion, scale places, scaled MMAs.
+#pragma once
+#include "text.cuh"
+
+namespace yk {
+
+constexpr int kFp4Block = 512;       // bytes of 128 rows x 4 groups of scales
+static inline int fp4_group(int format) { return format == YK_NVFP4 ? 16 : 32; }
+// Scale blocks along a row of `cols` columns.
+static inline int fp4_blocks(int cols, int format) { return (int)(((long long)cols + 4 * fp4_group(format) - 1) / (4 * fp4_group(format))); }
+static inline bool fp4_format(int f) { return f == YK_NVFP4 || f == YK_MXFP4; }
+
+// Eight floats to e2m1 codes, the first in the lowest 4 bits; round to nearest even, saturating at +-6.
+__device__ __forceinline__ uint32_t floats_to_e2m1x8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+// Eight codes as half2 pairs of 2^-14 times their values; exact (a code's three low bits are the low end of fp16's
+// exponent and the first bit of its fraction).
+__device__ __forceinline__ void e2m1x8_to_half2x4(uint32_t codes, uint32_t (&h)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const uint32_t c = codes >> (8 * e);
+    h[e] = (c & 7u) << 9 | (c & 8u) << 12 | (c & 0x70u) << 21 | (c & 0x80u) << 24;
+  }
+}
+
+// Scales from shared memory (a 512-byte block, as it lies in memory) into four TMEM columns: row r's four
+// scales go to lane r % 32 (and the three lanes 32 apart), column r / 32.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// The block's descriptor: four groups of 8 rows x 16 bytes, 128 bytes apart.
+__device__ __forceinline__ uint64_t scales_desc(uint32_t saddr) { return nosw_desc(saddr, 16, 128); }
+// D[tmem] (+)= A[smem] * B[smem]^T over 64 columns of e2m1 codes with scales in TMEM, fp32 sums.
+template <bool NV>
+__device__ __forceinline__ void tc_mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                           uint32_t accumulate) {
+  if (NV)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+}
+// Instruction descriptor: e2m1 A and B, both K-major, M = 128, N = n; the scales are e4m3 or powers of two.  The
+// latter come two a step: `half` says which two of the four in a TMEM word.
+template <bool NV>
+__host__ __device__ constexpr uint32_t idesc_fp4_m128(int n, int half = 0) {
+  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (NV ? 0u : 1u << 23) | (1u << 27) |
+         (uint32_t)(2 * half) << 4 | (uint32_t)(2 * half) << 29;
+}
+
+// Bytes from global to shared memory, completing on the mbarrier; 16-byte aligned, a multiple of 16 bytes.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+}  // namespace yk

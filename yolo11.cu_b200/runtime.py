@@ -50,7 +50,8 @@ class YoloOptions(C.Structure):
                 ("max_det", C.c_int), ("autotune", C.c_int), ("fuse", C.c_int)]
 
 
-YK_F16, YK_BF16, YK_E4M3 = 0, 1, 2
+YK_F16, YK_BF16, YK_E4M3, YK_F32 = 0, 1, 2, 3
+YK_NVFP4, YK_MXFP4 = 0, 1
 
 
 class YkKvCache(C.Structure):
@@ -102,6 +103,40 @@ class YkGemv4(C.Structure):
                 ("xgroup", C.c_int), ("xtype", C.c_int), ("dtype", C.c_int)]
 
 
+class YkQkRotate(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("pos", C.c_void_p),
+                ("freqs", C.c_void_p), ("q_row", C.c_longlong), ("k_row", C.c_longlong),
+                ("q_out_row", C.c_longlong), ("k_out_row", C.c_longlong),
+                ("pos_axis", C.c_longlong), ("rows", C.c_int), ("heads", C.c_int),
+                ("kv_heads", C.c_int), ("dim", C.c_int), ("rot", C.c_int), ("axes", C.c_int),
+                ("sections", C.c_int * 4), ("interleaved", C.c_int), ("dtype", C.c_int),
+                ("eps", C.c_float)]
+
+
+class YkQuantFp4(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("codes", C.c_void_p), ("scales", C.c_void_p),
+                ("values", C.c_void_p), ("x_row", C.c_longlong), ("values_row", C.c_longlong),
+                ("codes_row", C.c_longlong), ("rows", C.c_int), ("cols", C.c_int),
+                ("format", C.c_int), ("dtype", C.c_int), ("scale", C.c_float)]
+
+
+class YkGemmFp4(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("xscale", C.c_void_p), ("w", C.c_void_p),
+                ("wscale", C.c_void_p), ("w2", C.c_void_p), ("w2scale", C.c_void_p),
+                ("bias", C.c_void_p), ("y", C.c_void_p), ("x_row", C.c_longlong),
+                ("w_row", C.c_longlong), ("y_row", C.c_longlong), ("rows", C.c_int),
+                ("n", C.c_int), ("k", C.c_int), ("format", C.c_int), ("dtype", C.c_int),
+                ("alpha", C.c_float), ("alpha2", C.c_float)]
+
+
+class YkSample(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+                ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("u", C.c_void_p),
+                ("token", C.c_void_p), ("logprob", C.c_void_p), ("kept", C.c_void_p),
+                ("row", C.c_longlong), ("rows", C.c_int), ("n", C.c_int), ("dtype", C.c_int)]
+
+
 _P = C.POINTER
 _SIGS = {
     # kernel ABI (include/yk.h)
@@ -143,10 +178,17 @@ _SIGS = {
     "yk_attn_kv8": (C.c_int, [_P(YkKvCache), _P(YkAttnKv8), C.c_void_p]),
     "yk_rmsnorm8": (C.c_int, [_P(YkRmsNorm8), C.c_void_p]),
     "yk_gemv4": (C.c_int, [_P(YkGemv4), C.c_void_p]),
+    "yk_qk_rotate": (C.c_int, [_P(YkQkRotate), C.c_void_p]),
+    "yk_fp4_scale_bytes": (C.c_size_t, [C.c_int] * 3),
+    "yk_quant_fp4": (C.c_int, [_P(YkQuantFp4), C.c_void_p]),
+    "yk_gemm_fp4": (C.c_int, [_P(YkGemmFp4), C.c_void_p]),
+    "yk_sample": (C.c_int, [_P(YkSample), C.c_void_p]),
     "yk_fetch_device_error": (C.c_int, []),
     "yk_test_inject": (C.c_int, [C.c_int, C.c_ulonglong]),
     "yk_test_nms_cluster": (C.c_int, [C.c_int]),
     "yk_test_attn_kv8": (C.c_int, [C.c_int]),
+    "yk_test_gemm_fp4": (C.c_int, [C.c_int, C.c_int]),
+    "yk_test_sample": (C.c_int, [C.c_int]),
     "yk_last_cuda_error": (C.c_char_p, []),
     "yk_launch_count": (C.c_longlong, []),
     # engine ABI (include/yolo.h)
