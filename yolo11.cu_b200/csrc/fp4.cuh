@@ -30,13 +30,6 @@ __device__ __forceinline__ void e2m1x8_to_half2x4(uint32_t codes, uint32_t (&h)[
   }
 }
 
-// Scales from shared memory (a 512-byte block, as it lies in memory) into four TMEM columns: row r's four
-// scales go to lane r % 32 (and the three lanes 32 apart), column r / 32.
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-// The block's descriptor: four groups of 8 rows x 16 bytes, 128 bytes apart.
-__device__ __forceinline__ uint64_t scales_desc(uint32_t saddr) { return nosw_desc(saddr, 16, 128); }
 // D[tmem] (+)= A[smem] * B[smem]^T over 64 columns of e2m1 codes with scales in TMEM, fp32 sums.
 template <bool NV>
 __device__ __forceinline__ void tc_mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
@@ -52,12 +45,49 @@ __device__ __forceinline__ void tc_mma_fp4(uint32_t d, uint64_t a, uint64_t b, u
         "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
 }
-// Instruction descriptor: e2m1 A and B, both K-major, M = 128, N = n; the scales are e4m3 or powers of two.  The
-// latter come two a step: `half` says which two of the four in a TMEM word.
+// The same over the shared memory of a CTA pair, M = 256.
 template <bool NV>
-__host__ __device__ constexpr uint32_t idesc_fp4_m128(int n, int half = 0) {
-  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (NV ? 0u : 1u << 23) | (1u << 27) |
+__device__ __forceinline__ void tc_mma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                                uint32_t accumulate) {
+  if (NV)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+}
+// Instruction descriptor: e2m1 A and B, both K-major, M = m (128, a pair 256), N = n; the scales are e4m3 or powers of
+// two.  The latter come two a step: `half` says which two of the four in a TMEM word.
+template <bool NV>
+__host__ __device__ constexpr uint32_t idesc_fp4(int m, int n, int half = 0) {
+  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (NV ? 0u : 1u << 23) | ((uint32_t)(m >> 7) << 27) |
          (uint32_t)(2 * half) << 4 | (uint32_t)(2 * half) << 29;
+}
+
+// One lane of the warp, the same at each call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Arrive on another CTA's barrier, for accesses to TMEM that tcgen05.wait and tcgen05.fence have ordered.  A release at
+// cluster scope would wait for the thread's own stores too (1200 cycles beside the loads of a product).
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// mbar_wait for a phase that is due: tries a while before it reads the clock and the limit of the wait, as the load of the
+// limit from memory alone takes longer than four MMAs.
+__device__ __forceinline__ bool mbar_wait_due(uint32_t bar, uint32_t parity, int code) {
+#pragma unroll 1
+  for (int i = 0; i < 256; i++)
+    if (mbar_try(bar, parity)) return true;
+  return mbar_wait(bar, parity, code);
 }
 
 // Bytes from global to shared memory, completing on the mbarrier; 16-byte aligned, a multiple of 16 bytes.

@@ -7,7 +7,7 @@ struct GemmFp4Args {
   YkGemmFp4 p;
   int blocks;              // scale blocks along a row
   int chunks;              // of 256 columns
-  int tiles_m, tiles_n;    // of the tile kernel
+  int tiles_m, tiles_n;    // of the pair kernel
   int y_vec;               // y allows 16-byte stores
   int y_pair;              // y allows 4-byte stores
 };
@@ -18,216 +18,301 @@ constexpr int kFp4Threads = 192;           // loads, MMAs, four warps of sums
 template <bool NV>
 constexpr int kFp4Bpc = NV ? 4 : 2;        // scale blocks of 256 columns
 
-// ---------------- many rows: 128 x 256 tiles ----------------
-// y tiles of 128 rows x 256 outputs (gated: 128 of g and the 128 of the other factor), persistent CTAs, one an SM.
-//  * warp 0: codes by tensor copies (128-byte swizzle, zeros past the edges), scales by plain bulk copies of
-//    whole blocks, one ring of stages of 256 columns.
-//  * warp 1: copies a stage's scales into TMEM, issues its four MMAs.  Scales have two places there, by
-//    turns, so that a stage's copies do not wait for the last stage's MMAs.
-//  * warps 2-5: sums out of TMEM, factor, bias or gate, rounding, through shared memory to rows of 64 bytes.
-// TMEM: two accumulators of 256 columns and two scale places of 48 are 96 columns too many.  So the
+// v / (1 + exp(-v)), within 2^-20 + |v| 2^-23 of itself
+__device__ __forceinline__ float fp4_silu(float v) { return __fdividef(v, 1.f + __expf(-v)); }
+
+// Scales go from shared memory to TMEM through registers: row r's four scales of a 512-byte block belong in lane r % 32,
+// column r / 32, so a lane's 16 bytes of the block are four columns.  All four warps of a group do the same for their
+// lanes, as the MMA wants them.  Copies by the tensor pipe itself (tcgen05.cp) take 45 of its cycles each, beside 128 for an MMA.
+__device__ __forceinline__ void fp4_get_scales(uint32_t* v, uint32_t sm, int lane) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(sm + lane * 16) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  tmem_ld16p(taddr, r);
+  tmem_ld16p(taddr + 16, r + 16);
+}
+template <int N>
+__device__ __forceinline__ void fp4_put_scales(uint32_t taddr, const uint32_t* v) {
+#pragma unroll
+  for (int i = 0; i < N; i += 8)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr + i), "r"(v[i]), "r"(v[i + 1]),
+                 "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7]) : "memory");
+}
+
+// ---------------- many rows: 256 x 256 tiles of CTA pairs ----------------
+// One MMA of 256 rows x 256 outputs (gated: 128 of g and the 128 of the other factor) over the shared memory of two SMs: each
+// CTA holds 128 rows of x and 128 of w, so that it takes in 64 bytes a cycle at the full rate, where an SM by itself would
+// need 96.  An MMA of 64 columns takes 128 cycles whatever its outputs, so only full tiles reach the rate.
+//  * warp 0: codes by tensor copies (128-byte swizzle, zeros past the edges) onto the leader's barrier, scales by plain
+//    bulk copies of whole blocks onto the CTA's own; one ring of stages of 256 columns.
+//  * warps 2-5 and 6-9: scales from shared memory to TMEM (x's of the CTA's own rows, w's of all) for every other stage,
+//    each four warps with a place of their own there.
+//  * warp 1 of the leader: the MMAs.
+//  * warps 10-13: sums out of TMEM, factor, bias or gate, rounding, through shared memory to rows of 64 bytes.
+// TMEM: two accumulators of 256 columns and two places of 48 for scales are 96 columns too many.  So the
 // accumulators share 96 columns (0-255 and 160-415): a tile's shared ones are drained first, and the next tile
 // may begin.
+constexpr int kFp4PairThreads = 448;
 template <bool NV>
-struct Fp4Tile {
-  static constexpr int kStages = 4;
-  static constexpr int kSa = kFp4Bpc<NV> * kFp4Block;
-  static constexpr int kStage = 3 * kFp4Codes + 3 * 2048;
+struct Fp4Pair {
+  static constexpr int kStages = 5;
+  static constexpr int kStage = 2 * kFp4Codes + 3 * 2048;
   static constexpr int kStaging = 4 * 32 * 64;
   static constexpr int kSmem = kStages * kStage + kStaging + 1024;
   static constexpr int kD1 = 160, kSf = 416, kSfSet = 48;
 };
 
 __device__ __forceinline__ void fp4_tile_at(const GemmFp4Args& a, int t, int& tm, int& tn) {
-  // bands of 16 row tiles, so that a band's rows and the outputs in work stay in L2
-  const int band = t / (16 * a.tiles_n), in = t - band * 16 * a.tiles_n, high = min(16, a.tiles_m - band * 16);
+  // bands of 8 row tiles, so that a band's rows and the outputs in work stay in L2
+  const int band = t / (8 * a.tiles_n), in = t - band * 8 * a.tiles_n, high = min(8, a.tiles_m - band * 8);
   tn = in / high;
-  tm = band * 16 + in - tn * high;
+  tm = band * 8 + in - tn * high;
 }
 
 template <bool NV, bool GATED, bool BF16>
-__global__ void __launch_bounds__(kFp4Threads, 1)
-gemm_fp4_tile_kernel(const __grid_constant__ GemmFp4Args a, const __grid_constant__ CUtensorMap tx,
+__global__ void __launch_bounds__(kFp4PairThreads, 1)
+gemm_fp4_pair_kernel(const __grid_constant__ GemmFp4Args a, const __grid_constant__ CUtensorMap tx,
                      const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tw2) {
-  using S = Fp4Tile<NV>;
+  using S = Fp4Pair<NV>;
   extern __shared__ uint8_t fp4_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * S::kStages + 2];
+  __shared__ __align__(8) uint64_t bars[3 * S::kStages + 4];
   __shared__ uint32_t tslot;
-  __shared__ volatile int abort_flag;
   const YkGemmFp4& p = a.p;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
   const uint32_t base = (smem_u32(fp4_raw) + 1023) & ~1023u;
-  const uint32_t full = smem_u32(&bars[0]), empty = smem_u32(&bars[S::kStages]),
-                 done = smem_u32(&bars[2 * S::kStages]), shared_free = done + 8;
+  // codes of both CTAs (leader's), the CTA's scales; a stage is free; scales in TMEM of both CTAs (leader's); a tile's
+  // sums are complete; the shared columns are drained in both CTAs (leader's)
+  const uint32_t full = smem_u32(&bars[0]), sfull = full + 8 * S::kStages, empty = sfull + 8 * S::kStages,
+                 sready = empty + 8 * S::kStages, done = sready + 16, shared_free = done + 8;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (tid == 0) {
     for (int i = 0; i < S::kStages; i++) {
       mbar_init(full + i * 8, 1);
+      mbar_init(sfull + i * 8, 1);
       mbar_init(empty + i * 8, 1);
     }
+    mbar_init(sready, 8);
+    mbar_init(sready + 8, 8);
     mbar_init(done, 1);
-    mbar_init(shared_free, 4);
-    abort_flag = 0;
+    mbar_init(shared_free, 8);
     mbar_fence_init();
   }
   pdl_wait();
   pdl_trigger();
   if (warp == 1) {
-    tmem_alloc(smem_u32(&tslot), 512);
-    tmem_relinquish();
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tslot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  cluster_barrier();                 // barriers and TMEM of both CTAs
   tc_fence_after();
-  const uint32_t tmem = tslot;
+  const uint32_t tmem = __shfl_sync(~0u, tslot, 0);
   const int tiles = a.tiles_m * a.tiles_n;
   constexpr int kBpc = kFp4Bpc<NV>, kOut = GATED ? 128 : 256;   // outputs of a tile
+  bool ok = true;                    // a wait that ran out ends the warp's part (the others' waits run out then too)
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t g = 0;
-      for (int t = blockIdx.x; t < tiles && !abort_flag; t += gridDim.x) {
-        int tm, tn;
-        fp4_tile_at(a, t, tm, tn);
-        const int m0 = tm * 128, n0 = tn * kOut;
-        const bool second = GATED || n0 + 128 < p.n;
-        const uint8_t* sx = (const uint8_t*)p.xscale + (long long)tm * a.blocks * kFp4Block;
-        const uint8_t* sw = (const uint8_t*)p.wscale + (long long)(n0 / 128) * a.blocks * kFp4Block;
-        const uint8_t* sw2 = GATED ? (const uint8_t*)p.w2scale + (long long)(n0 / 128) * a.blocks * kFp4Block
-                                   : sw + (long long)a.blocks * kFp4Block;
-        for (int c = 0; c < a.chunks; c++, g++) {
-          const int s = g % S::kStages;
-          if (g >= S::kStages && !mbar_wait(empty + s * 8, (g / S::kStages - 1) & 1, 0x611)) { abort_flag = 1; break; }
-          const uint32_t at = base + s * S::kStage, sc = at + 3 * kFp4Codes, bar = full + s * 8;
+    // (the whole warp takes part and one lane issues, here and below: operands then stay in uniform registers)
+    const bool issuer = elect_one();
+    const uint32_t lead_full = cluster_map(full, 0);
+    uint32_t g = 0, s = 0, phase = 1;                // of the stage's last use
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      int tm, tn;
+      fp4_tile_at(a, t, tm, tn);
+      const int m0 = tm * 256 + (int)rank * 128, n0 = tn * kOut, w0 = n0 + (int)rank * (GATED ? 64 : 128);
+      const bool rows_there = m0 < p.rows, second = GATED || n0 + 128 < p.n;
+      const uint8_t* sx = (const uint8_t*)p.xscale + (long long)(m0 / 128) * a.blocks * kFp4Block;
+      const uint8_t* sw = (const uint8_t*)p.wscale + (long long)(n0 / 128) * a.blocks * kFp4Block;
+      const uint8_t* sw2 = GATED ? (const uint8_t*)p.w2scale + (long long)(n0 / 128) * a.blocks * kFp4Block
+                                 : sw + (long long)a.blocks * kFp4Block;
+      for (int c = 0; c < a.chunks; c++) {
+        if (g >= S::kStages && !__all_sync(~0u, mbar_wait_due(empty + s * 8, phase, 0x611))) { ok = false; break; }
+        if (issuer) {
+          const uint32_t at = base + s * S::kStage, sc = at + 2 * kFp4Codes, bar = sfull + s * 8, lead_bar = lead_full + s * 8;
           const uint32_t bytes = min(kBpc, a.blocks - c * kBpc) * kFp4Block;
-          mbar_expect_tx(bar, 2 * (kFp4Codes + bytes) + (second ? kFp4Codes + bytes : 0));
-          tma_load_2d(at, &tx, bar, c * 128, m0);
-          tma_load_2d(at + kFp4Codes, &tw, bar, c * 128, n0);
-          bulk_load(sc, sx + c * (kBpc * kFp4Block), bytes, bar);
-          bulk_load(sc + 2048, sw + c * (kBpc * kFp4Block), bytes, bar);
-          if (second) {
-            tma_load_2d(at + 2 * kFp4Codes, GATED ? &tw2 : &tw, bar, c * 128, GATED ? n0 : n0 + 128);
-            bulk_load(sc + 4096, sw2 + c * (kBpc * kFp4Block), bytes, bar);
-          }
+          const long long off = (long long)c * (kBpc * kFp4Block);
+          if (rank == 0) mbar_expect_tx(full + s * 8, 4 * kFp4Codes);
+          tma_pair_2d(at, &tx, lead_bar, c * 128, m0);
+          tma_pair_2d(at + kFp4Codes, &tw, lead_bar, c * 128, w0);
+          if (GATED) tma_pair_2d(at + kFp4Codes + kFp4Codes / 2, &tw2, lead_bar, c * 128, w0);   // (64 rows of each)
+          mbar_expect_tx(bar, bytes * (1 + rows_there + second));
+          if (rows_there) bulk_load(sc, sx + off, bytes, bar);
+          bulk_load(sc + 2048, sw + off, bytes, bar);
+          if (second) bulk_load(sc + 4096, sw2 + off, bytes, bar);
         }
+        __syncwarp();
+        g++;
+        if (++s == S::kStages) { s = 0; phase ^= 1; }
       }
-      if (abort_flag)                // copies in flight land before the CTA ends
-        for (uint32_t i = g > S::kStages ? g - S::kStages : 0; i < g; i++) mbar_wait(full + i % S::kStages * 8, (i / S::kStages) & 1, 0x612);
     }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t g = 0, li = 0;
-      const uint64_t x_desc = sw128_desc(base), w_desc = sw128_desc(base + kFp4Codes), s_desc = scales_desc(base + 3 * kFp4Codes);
-      for (int t = blockIdx.x; t < tiles && !abort_flag; t += gridDim.x, li++) {
-        if (li && !mbar_wait(shared_free, (li - 1) & 1, 0x613)) { abort_flag = 1; break; }
-        tc_fence_after();
-        const uint32_t d = tmem + (li & 1) * S::kD1;
-        for (int c = 0; c < a.chunks; c++, g++) {
-          const int s = g % S::kStages;
-          if (!mbar_wait(full + s * 8, (g / S::kStages) & 1, 0x614)) { abort_flag = 1; break; }
-          // the MMAs that read this place of the scales are those of two stages ago
-          if (g >= 2 && !mbar_wait(empty + (g - 2) % S::kStages * 8, ((g - 2) / S::kStages) & 1, 0x615)) { abort_flag = 1; break; }
-          tc_fence_after();
-          const uint32_t sf = tmem + S::kSf + (g & 1) * S::kSfSet;
-          const uint64_t step = (uint64_t)(s * S::kStage) >> 4;
-          const int blocks = min(kBpc, a.blocks - c * kBpc);
-#pragma unroll
-          for (int b = 0; b < kBpc; b++) {
-            if (b >= blocks) break;
-            tmem_cp_scales(sf + b * 4, s_desc + step + b * (kFp4Block >> 4));
-            tmem_cp_scales(sf + 16 + b * 8, s_desc + step + ((2048 + b * kFp4Block) >> 4));
-            tmem_cp_scales(sf + 20 + b * 8, s_desc + step + ((4096 + b * kFp4Block) >> 4));
-          }
-          const int steps = min(4, (p.k - c * kFp4Cols + 63) / 64);
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            if (k >= steps) break;
-            const int b = NV ? k : k >> 1;
-            tc_mma_fp4<NV>(d, x_desc + step + k * 2, w_desc + step + k * 2, idesc_fp4_m128<NV>(256, NV ? 0 : k & 1),
-                           sf + b * 4, sf + 16 + b * 8, (c | k) != 0);
-          }
-          tc_commit(empty + s * 8);
-        }
-        if (!abort_flag) tc_commit(done);
+    if (!ok)                  // copies in flight land before the CTA ends
+      for (uint32_t i = g > S::kStages ? g - S::kStages : 0; i < g; i++) {
+        mbar_wait(sfull + i % S::kStages * 8, (i / S::kStages) & 1, 0x612);
+        if (rank == 0) mbar_wait(full + i % S::kStages * 8, (i / S::kStages) & 1, 0x612);
       }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool issuer = elect_one();
+      const uint32_t peer_empty = cluster_map(empty, 1), peer_done = cluster_map(done, 1);
+      uint32_t s = 0, phase = 0, set = 0, set_phase = 0, li = 0;
+      for (int t = pair; t < tiles && ok; t += pairs, li++) {
+        if (li && !__all_sync(~0u, mbar_wait_due(shared_free, (li - 1) & 1, 0x613))) { ok = false; break; }
+        const uint32_t d = tmem + (li & 1) * S::kD1;
+        int c = 0;
+        for (; c < a.chunks; c++) {
+          if (!__all_sync(~0u, mbar_wait_due(full + s * 8, phase, 0x614) && mbar_wait_due(sready + set * 8, set_phase, 0x615))) { ok = false; break; }
+          tc_fence_after();
+          if (issuer) {
+            const uint32_t sf = tmem + S::kSf + set * S::kSfSet, at = base + s * S::kStage;
+            const uint64_t x_desc = sw128_desc(at), w_desc = sw128_desc(at + kFp4Codes);
+            const int steps = (p.k - c * kFp4Cols + 63) / 64;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const int b = NV ? k : k >> 1;
+              if (k == 0 || k < steps)
+                tc_mma_fp4_pair<NV>(d, x_desc + k * 2, w_desc + k * 2, idesc_fp4<NV>(256, 256, NV ? 0 : k & 1),
+                                    sf + b * 4, sf + 4 * kBpc + b * 8, (c | k) != 0);
+            }
+            tc_commit_pair(empty + s * 8);
+            tc_commit_pair(peer_empty + s * 8);
+          }
+          __syncwarp();
+          if (++s == S::kStages) { s = 0; phase ^= 1; }
+          set ^= 1;
+          set_phase ^= set == 0;
+        }
+        if (issuer && c == a.chunks) {
+          tc_commit_pair(done);
+          tc_commit_pair(peer_done);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < 10) {
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, lead_ready = cluster_map(sready, 0);
+    const uint32_t sc0 = base + 2 * kFp4Codes;
+    constexpr int kWords = 12 * kBpc;                // x's 4 a block, then w's 8 a block
+    const uint32_t total = (uint32_t)((tiles - pair + pairs - 1) / pairs) * a.chunks;   // (the launch has no pair without a tile)
+    const uint32_t set = warp >= 6, place = tmem + lanes + S::kSf + set * S::kSfSet;
+    for (uint32_t g = set; g < total; g += 2) {
+      const uint32_t s = g % S::kStages;
+      uint32_t v[kWords];
+      if (!__all_sync(~0u, mbar_wait_due(sfull + s * 8, (g / S::kStages) & 1, 0x616))) { ok = false; break; }
+#pragma unroll
+      for (int b = 0; b < kBpc; b++) {
+        const uint32_t sc = sc0 + s * S::kStage + b * kFp4Block;
+        fp4_get_scales(v + 4 * b, sc, lane);
+        uint32_t w[8];
+        fp4_get_scales(w, sc + 2048, lane);
+        fp4_get_scales(w + 4, sc + 4096, lane);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[4 * kBpc + 8 * b + i] = GATED ? w[(i & 2) * 2 + (i >> 2) * 2 + (i & 1)] : w[i];
+      }
+      // the MMAs that read this place are those of two stages ago
+      if (g >= 2 && !__all_sync(~0u, mbar_wait_due(empty + (g - 2) % S::kStages * 8, ((g - 2) / S::kStages) & 1, 0x617))) { ok = false; break; }
+      tc_fence_after();
+      fp4_put_scales<kWords>(place, v);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster_relaxed(lead_ready + set * 8);
     }
   } else {
     const int sub = warp & 3;
-    const uint32_t lanes = (uint32_t)(sub * 32) << 16;
+    const uint32_t lanes = (uint32_t)(sub * 32) << 16, lead_free = cluster_map(shared_free, 0);
     const uint32_t stage = base + S::kStages * S::kStage + sub * 2048;
     const uint8_t* stage_p = fp4_raw + (stage - smem_u32(fp4_raw));
     const float alpha = p.alpha, alpha2 = p.alpha2;
+    // 32 outputs of the warp's 32 rows, from column c0 on: rounded ..
+    const auto finish = [&](const uint32_t* r, const uint32_t* r2, int c0, uint32_t (&o)[16]) {
+      float v[32];
+      if (GATED) {
+#pragma unroll
+        for (int e = 0; e < 32; e++) v[e] = fp4_silu(__uint_as_float(r[e]) * alpha) * (__uint_as_float(r2[e]) * alpha2);
+      } else {
+        const float bias = p.bias && c0 + lane < p.n ? p.bias[c0 + lane] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; e++) v[e] = fmaf(__uint_as_float(r[e]), alpha, p.bias ? __shfl_sync(~0u, bias, e) : 0.f);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++) o[e] = float2_to_pair<BF16>(v[2 * e], v[2 * e + 1]);
+    };
+    // .. and stored
+    const auto emit = [&](const uint32_t (&o)[16], int m0, int c0) {
+      if (c0 >= p.n || m0 >= p.rows) return;
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < 4; h++)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((h ^ ((lane >> 1) & 3)) << 4)),
+                     "r"(o[4 * h]), "r"(o[4 * h + 1]), "r"(o[4 * h + 2]), "r"(o[4 * h + 3]) : "memory");
+      __syncwarp();
+      uint4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int row = j * 8 + (lane >> 2), h = lane & 3;
+        v[j] = *(const uint4*)(stage_p + row * 64 + ((h ^ ((row >> 1) & 3)) << 4));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int row = j * 8 + (lane >> 2), c = c0 + (lane & 3) * 8;
+        if (m0 + row >= p.rows || c >= p.n) continue;
+        uint16_t* y = (uint16_t*)p.y + (long long)(m0 + row) * p.y_row + c;
+        if (a.y_vec && c + 8 <= p.n) {
+          *(uint4*)y = v[j];
+        } else {
+          const uint32_t* w = (const uint32_t*)&v[j];
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (c + e < p.n) y[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        }
+      }
+    };
     uint32_t li = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, li++) {
-      if (!mbar_wait(done, li & 1, 0x616)) { abort_flag = 1; break; }
+    for (int t = pair; t < tiles && ok; t += pairs, li++) {
+      if (!__all_sync(~0u, mbar_wait_due(done, li & 1, 0x618))) { ok = false; break; }
       tc_fence_after();
       int tm, tn;
       fp4_tile_at(a, t, tm, tn);
-      const int m0 = tm * 128 + sub * 32, n0 = tn * kOut;
+      const int m0 = tm * 256 + (int)rank * 128 + sub * 32, n0 = tn * kOut;
       const uint32_t d = tmem + (li & 1) * S::kD1 + lanes;
-      constexpr int kUnits = kOut / 32, kFirst = 3;   // units that hold the shared columns
-#pragma unroll 1
-      for (int i = 0; i < kUnits; i++) {
-        const int u = (li & 1) ? i : (i + kUnits - kFirst) % kUnits;
-        uint32_t r[32], o[16];
-        tmem_ld16p(d + u * 32, r);
-        tmem_ld16p(d + u * 32 + 16, r + 16);
-        if (GATED) {
-          uint32_t r2[32];
-          tmem_ld16p(d + 128 + u * 32, r2);
-          tmem_ld16p(d + 128 + u * 32 + 16, r2 + 16);
-          tmem_ld_wait();
+      // 32 outputs are a unit of 32 columns (gated: and as many 64 further on, for the other factor).  The ones that hold shared columns
+      // first and together (a load takes 600 cycles beside the MMAs, however much it brings); then the next tile may begin
+      constexpr int kUnits = kOut / 32, kCols = GATED ? 64 : 32, kFirst = GATED ? 2 : 3;
+      const auto unit = [&](int i) { return (li & 1) ? i : (i + kUnits - kFirst) % kUnits; };
+      uint32_t o[16];
 #pragma unroll
-          for (int e = 0; e < 32; e++) {
-            const float v = __uint_as_float(r[e]) * alpha;
-            r[e] = __float_as_uint(v / (1.f + __expf(-v)) * (__uint_as_float(r2[e]) * alpha2));
-          }
-        } else {
-          tmem_ld_wait();
+      for (int i0 = 0; i0 < kUnits; i0 += kFirst) {
+        uint32_t r[kFirst][kCols];
+#pragma unroll
+        for (int i = 0; i < kFirst; i++) {
+          if (i0 + i >= kUnits) break;
+          const int u = unit(i0 + i), at = GATED ? (u >> 1) * 128 + (u & 1) * 32 : u * 32;
+          tmem_ld32(d + at, r[i]);
+          if (GATED) tmem_ld32(d + at + 64, r[i] + 32);
         }
-        if (i == kFirst - 1) {
+        tmem_ld_wait();
+        if (i0 == 0) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(shared_free);
-        }
-        const int c0 = n0 + u * 32;
-        if (c0 >= p.n) continue;
-        if (!GATED) {
-          const float bias = p.bias && c0 + lane < p.n ? p.bias[c0 + lane] : 0.f;
-#pragma unroll
-          for (int e = 0; e < 32; e++)
-            r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), alpha, p.bias ? __shfl_sync(~0u, bias, e) : 0.f));
+          if (lane == 0) mbar_arrive_cluster_relaxed(lead_free);
         }
 #pragma unroll
-        for (int e = 0; e < 16; e++) o[e] = float2_to_pair<BF16>(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
-        __syncwarp();
-#pragma unroll
-        for (int h = 0; h < 4; h++)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((h ^ ((lane >> 1) & 3)) << 4)),
-                       "r"(o[4 * h]), "r"(o[4 * h + 1]), "r"(o[4 * h + 2]), "r"(o[4 * h + 3]) : "memory");
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int row = j * 8 + (lane >> 2), h = lane & 3, c = c0 + h * 8;
-          if (m0 + row >= p.rows || c >= p.n) continue;
-          const uint4 v = *(const uint4*)(stage_p + row * 64 + ((h ^ ((row >> 1) & 3)) << 4));
-          uint16_t* y = (uint16_t*)p.y + (long long)(m0 + row) * p.y_row + c;
-          if (a.y_vec && c + 8 <= p.n) {
-            *(uint4*)y = v;
-          } else {
-            const uint32_t* w = (const uint32_t*)&v;
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-              if (c + e < p.n) y[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-          }
+        for (int i = 0; i < kFirst; i++) {
+          if (i0 + i >= kUnits) break;
+          finish(r[i], r[i] + (GATED ? 32 : 0), n0 + unit(i0 + i) * 32, o);
+          emit(o, m0, n0 + unit(i0 + i) * 32);
         }
       }
     }
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  cluster_barrier();                 // no remote arrivals or MMAs into the other CTA remain
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
 }
 
@@ -256,13 +341,13 @@ gemm_fp4_split_kernel(const __grid_constant__ GemmFp4Args a, const __grid_consta
                       const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tw2, int split) {
   using S = Fp4Split<NV, GATED, NT>;
   extern __shared__ uint8_t fp4_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * S::kStages + 1];
+  __shared__ __align__(8) uint64_t bars[2 * S::kStages + 3];
   __shared__ uint32_t tslot;
-  __shared__ volatile int abort_flag;
   const YkGemmFp4& p = a.p;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
   const uint32_t base = (smem_u32(fp4_raw) + 1023) & ~1023u;
-  const uint32_t full = smem_u32(&bars[0]), empty = smem_u32(&bars[S::kStages]), done = smem_u32(&bars[2 * S::kStages]);
+  const uint32_t full = smem_u32(&bars[0]), empty = smem_u32(&bars[S::kStages]), done = smem_u32(&bars[2 * S::kStages]),
+                 sready = done + 8;
   const int rank = split > 1 ? (int)cluster_rank() : 0;
   const int n0 = blockIdx.x / split * 128, m0 = blockIdx.y * NT;
   const int c_first = (int)((long long)a.chunks * rank / split), c_end = (int)((long long)a.chunks * (rank + 1) / split);
@@ -272,7 +357,8 @@ gemm_fp4_split_kernel(const __grid_constant__ GemmFp4Args a, const __grid_consta
       mbar_init(empty + i * 8, 1);
     }
     mbar_init(done, 1);
-    abort_flag = 0;
+    mbar_init(sready, 4);
+    mbar_init(sready + 8, 4);
     mbar_fence_init();
   }
   pdl_wait();
@@ -284,17 +370,18 @@ gemm_fp4_split_kernel(const __grid_constant__ GemmFp4Args a, const __grid_consta
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tslot;
+  const uint32_t tmem = __shfl_sync(~0u, tslot, 0);
   constexpr int kBpc = kFp4Bpc<NV>;
   constexpr int kScales = S::kA * kFp4Codes + S::kX;            // of a stage: weights', second weights', x's
+  bool ok = true;                    // a wait that ran out ends the warp's part (the others' waits run out then too)
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t g = 0;
-      const long long wb = (long long)(n0 / 128) * a.blocks * kFp4Block, xb = (long long)(m0 / 128) * a.blocks * kFp4Block;
-      for (int c = c_first; c < c_end; c++, g++) {
-        const int s = g % S::kStages;
-        if (g >= S::kStages && !mbar_wait(empty + s * 8, (g / S::kStages - 1) & 1, 0x621)) { abort_flag = 1; break; }
+    const bool issuer = elect_one();
+    const long long wb = (long long)(n0 / 128) * a.blocks * kFp4Block, xb = (long long)(m0 / 128) * a.blocks * kFp4Block;
+    uint32_t g = 0, s = 0, phase = 1;                // of the stage's last use
+    for (int c = c_first; c < c_end; c++) {
+      if (g >= S::kStages && !__all_sync(~0u, mbar_wait_due(empty + s * 8, phase, 0x621))) { ok = false; break; }
+      if (issuer) {
         const uint32_t at = base + s * S::kStage, sc = at + kScales, bar = full + s * 8;
         const uint32_t bytes = min(kBpc, a.blocks - c * kBpc) * kFp4Block;
         const long long off = (long long)c * (kBpc * kFp4Block);
@@ -306,61 +393,80 @@ gemm_fp4_split_kernel(const __grid_constant__ GemmFp4Args a, const __grid_consta
         if (GATED) bulk_load(sc + 2048, (const uint8_t*)p.w2scale + wb + off, bytes, bar);
         bulk_load(sc + S::kA * 2048, (const uint8_t*)p.xscale + xb + off, bytes, bar);
       }
-      if (abort_flag)
-        for (uint32_t i = g > S::kStages ? g - S::kStages : 0; i < g; i++) mbar_wait(full + i % S::kStages * 8, (i / S::kStages) & 1, 0x622);
+      __syncwarp();
+      g++;
+      if (++s == S::kStages) { s = 0; phase ^= 1; }
     }
+    if (!ok)
+      for (uint32_t i = g > S::kStages ? g - S::kStages : 0; i < g; i++) mbar_wait(full + i % S::kStages * 8, (i / S::kStages) & 1, 0x622);
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint64_t w_desc = sw128_desc(base), x_desc = sw128_desc(base + S::kA * kFp4Codes), s_desc = scales_desc(base + kScales);
-      uint32_t g = 0;
-      for (int c = c_first; c < c_end; c++, g++) {
-        const int s = g % S::kStages;
-        if (!mbar_wait(full + s * 8, (g / S::kStages) & 1, 0x623)) { abort_flag = 1; break; }
-        if (g >= 2 && !mbar_wait(empty + (g - 2) % S::kStages * 8, ((g - 2) / S::kStages) & 1, 0x624)) { abort_flag = 1; break; }
-        tc_fence_after();
-        const uint32_t sf = tmem + S::kSf + (g & 1) * S::kSfSet;
-        const uint64_t step = (uint64_t)(s * S::kStage) >> 4;
-        const int blocks = min(kBpc, a.blocks - c * kBpc);
-#pragma unroll
-        for (int b = 0; b < kBpc; b++) {
-          if (b >= blocks) break;
-#pragma unroll
-          for (int x = 0; x <= S::kA; x++) tmem_cp_scales(sf + x * 16 + b * 4, s_desc + step + ((x * 2048 + b * kFp4Block) >> 4));
-        }
-        const int steps = min(4, (p.k - c * kFp4Cols + 63) / 64);
+    const bool issuer = elect_one();
+    uint32_t s = 0, phase = 0, set = 0, set_phase = 0;
+    int c = c_first;
+    for (; c < c_end; c++) {
+      if (!__all_sync(~0u, mbar_wait_due(full + s * 8, phase, 0x623) && mbar_wait_due(sready + set * 8, set_phase, 0x624))) { ok = false; break; }
+      tc_fence_after();
+      if (issuer) {
+        const uint32_t sf = tmem + S::kSf + set * S::kSfSet, at = base + s * S::kStage;
+        const uint64_t w_desc = sw128_desc(at), x_desc = sw128_desc(at + S::kA * kFp4Codes);
+        const int steps = (p.k - c * kFp4Cols + 63) / 64;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          if (k >= steps) break;
           const int b = NV ? k : k >> 1;
 #pragma unroll
           for (int x = 0; x < S::kA; x++)
-            tc_mma_fp4<NV>(tmem + x * NT, w_desc + step + x * (kFp4Codes >> 4) + k * 2, x_desc + step + k * 2,
-                           idesc_fp4_m128<NV>(NT, NV ? 0 : k & 1), sf + x * 16 + b * 4, sf + S::kA * 16 + b * 4, (c - c_first) | k);
+            if (k == 0 || k < steps)
+              tc_mma_fp4<NV>(tmem + x * NT, w_desc + x * (kFp4Codes >> 4) + k * 2, x_desc + k * 2, idesc_fp4<NV>(128, NT, NV ? 0 : k & 1),
+                             sf + (x * kBpc + b) * 4, sf + (S::kA * kBpc + b) * 4, (c - c_first) | k);
         }
         tc_commit(empty + s * 8);
       }
-      if (!abort_flag) tc_commit(done);
+      __syncwarp();
+      if (++s == S::kStages) { s = 0; phase ^= 1; }
+      set ^= 1;
+      set_phase ^= set == 0;
     }
+    if (issuer && c == c_end) tc_commit(done);
+    __syncwarp();
   }
   const int rows = min(NT, p.rows - m0);
   float* const part = (float*)(fp4_raw + (base - smem_u32(fp4_raw)));     // [matrix][row][128 outputs], in the ring
   if (warp >= 2) {
     const int sub = warp & 3;
-    if (mbar_wait(done, 0, 0x625)) {
+    const uint32_t lanes = (uint32_t)(sub * 32) << 16;
+    constexpr int kWords = 4 * kBpc * (S::kA + 1);   // weights', second weights', x's
+    uint32_t g = 0;
+    for (int c = c_first; c < c_end; c++, g++) {
+      const int s = g % S::kStages;
+      uint32_t v[kWords];
+      if (!__all_sync(~0u, mbar_wait_due(full + s * 8, (g / S::kStages) & 1, 0x626))) { ok = false; break; }
+#pragma unroll
+      for (int x = 0; x <= S::kA; x++)
+#pragma unroll
+        for (int b = 0; b < kBpc; b++)
+          fp4_get_scales(v + (x * kBpc + b) * 4, base + s * S::kStage + kScales + x * 2048 + b * kFp4Block, lane);
+      // the MMAs that read this place of the scales are those of two stages ago
+      if (g >= 2 && !__all_sync(~0u, mbar_wait_due(empty + (g - 2) % S::kStages * 8, ((g - 2) / S::kStages) & 1, 0x627))) { ok = false; break; }
+      tc_fence_after();
+      fp4_put_scales<kWords>(tmem + lanes + S::kSf + (g & 1) * S::kSfSet, v);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sready + (g & 1) * 8);
+    }
+    if (ok && __all_sync(~0u, mbar_wait_due(done, 0, 0x625))) {
       tc_fence_after();
 #pragma unroll 1
       for (int x = 0; x < S::kA; x++) {
 #pragma unroll 1
         for (int m = 0; m < rows; m += 16) {
           uint32_t r[16];
-          tmem_ld16p(tmem + ((uint32_t)(sub * 32) << 16) + x * NT + m, r);
+          tmem_ld16p(tmem + lanes + x * NT + m, r);
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 16; e++) part[(x * NT + m + e) * 128 + sub * 32 + lane] = __uint_as_float(r[e]);
         }
       }
-    } else {
-      abort_flag = 1;
     }
   }
   tc_fence_before();
@@ -391,7 +497,7 @@ gemm_fp4_split_kernel(const __grid_constant__ GemmFp4Args a, const __grid_consta
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       o[e] = v[0][e] * p.alpha;
-      if (GATED) o[e] = o[e] / (1.f + __expf(-o[e])) * (v[S::kA - 1][e] * p.alpha2);
+      if (GATED) o[e] = fp4_silu(o[e]) * (v[S::kA - 1][e] * p.alpha2);
       else if (p.bias && n0 + j + e < p.n) o[e] = fmaf(v[0][e], p.alpha, p.bias[n0 + j + e]);
     }
     uint16_t* y = (uint16_t*)p.y + (long long)(m0 + m) * p.y_row + n0 + j;
@@ -441,17 +547,17 @@ static int fp4_sms() {
 }
 
 template <bool NV, bool GATED, bool BF16>
-static int launch_fp4_tile(const GemmFp4Args& a, cudaStream_t st) {
-  using S = Fp4Tile<NV>;
-  const auto kern = gemm_fp4_tile_kernel<NV, GATED, BF16>;
+static int launch_fp4_pair(const GemmFp4Args& a, cudaStream_t st) {
+  using S = Fp4Pair<NV>;
+  const auto kern = gemm_fp4_pair_kernel<NV, GATED, BF16>;
   const YkGemmFp4& p = a.p;
   CUtensorMap tx, tw, tw2;
-  if (!encode_fp4(&tx, p.x, p.rows, p.k, p.x_row, 128) || !encode_fp4(&tw, p.w, p.n, p.k, p.w_row, 128) ||
-      !encode_fp4(&tw2, GATED ? p.w2 : p.w, p.n, p.k, p.w_row, 128))
+  if (!encode_fp4(&tx, p.x, p.rows, p.k, p.x_row, 128) || !encode_fp4(&tw, p.w, p.n, p.k, p.w_row, GATED ? 64 : 128) ||
+      !encode_fp4(&tw2, GATED ? p.w2 : p.w, p.n, p.k, p.w_row, GATED ? 64 : 128))
     return refuse(YK_EUNSUP, "gemm_fp4: no tensor map for these sizes");
   if (smem_attr(kern, S::kSmem) != cudaSuccess) return check_launch("gemm_fp4 attr");
-  const int tiles = a.tiles_m * a.tiles_n, sms = fp4_sms();
-  launch_k(kern, tiles < sms ? tiles : sms, kFp4Threads, S::kSmem, st, a, tx, tw, tw2);
+  const int tiles = a.tiles_m * a.tiles_n, pairs = fp4_sms() / 2;
+  launch_kc(kern, 2 * (tiles < pairs ? tiles : pairs), kFp4PairThreads, S::kSmem, 2, st, a, tx, tw, tw2);
   note_launch();
   return check_launch("gemm_fp4");
 }
@@ -478,7 +584,7 @@ template <bool NV, bool GATED>
 static int launch_fp4(GemmFp4Args& a, cudaStream_t st) {
   const YkGemmFp4& p = a.p;
   const int sms = fp4_sms();
-  a.tiles_m = (p.rows + 127) / 128;
+  a.tiles_m = (p.rows + 255) / 256;
   a.tiles_n = (p.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
   const long long tiles = (long long)a.tiles_m * a.tiles_n;
   if (tiles > 0x7fffffffll) return refuse(YK_EUNSUP, "gemm_fp4: rows * n too large");
@@ -487,8 +593,8 @@ static int launch_fp4(GemmFp4Args& a, cudaStream_t st) {
   int split = 1;
   while (split < 8 && small * split * 2 <= sms * (GATED ? 1 : 2) && a.chunks >= 2 * split) split *= 2;
   if (g_fp4_split && g_fp4_split <= a.chunks) split = g_fp4_split;
-  if (g_fp4_kernel ? g_fp4_kernel == 1 : p.rows > 128 && tiles * 2 >= sms)
-    return p.dtype == YK_BF16 ? launch_fp4_tile<NV, GATED, true>(a, st) : launch_fp4_tile<NV, GATED, false>(a, st);
+  if (g_fp4_kernel ? g_fp4_kernel == 1 : p.rows > 128 && tiles * 4 >= sms)
+    return p.dtype == YK_BF16 ? launch_fp4_pair<NV, GATED, true>(a, st) : launch_fp4_pair<NV, GATED, false>(a, st);
   if ((p.rows + nt - 1) / nt > 65535 || small * split > 0x7fffffffll) return refuse(YK_EUNSUP, "gemm_fp4: rows * n too large");
   return nt == 32 ? launch_fp4_split<NV, GATED, 32>(a, split, st) : launch_fp4_split<NV, GATED, 128>(a, split, st);
 }

@@ -12,18 +12,28 @@ struct SampleArgs {
 
 // A row's scores are read once, into the shared memory of a cluster, as keys whose order is that of the
 // scores.  What stays (top-k, top-p, min-p) is always a beginning of one order, falling scores and equal ones by index, so
-// it is described by a key and how many of the scores with that key stay.  Both borders are found
-// digit by digit: counts (for top-p: weights) of the keys that share the digits so far, by digit, summed over the cluster.
+// it is described by a key and how many of the scores with that key stay.
 // Weights are whole numbers, 2^44 for the largest, so that their sums do not depend on any order: the
 // result is the same for every split.  They come from 64-bit exponentials: with 32 bits a sum over 10^5
 // scores is off by about 10^-7 of the total, which would decide the token of one row in 10^2 to 10^4.
-constexpr int kSampThreads = 1024, kSampWarps = kSampThreads / 32;
+// The borders:
+//  * Scores are counted by bins of 1/64 octave of weight, together with the sum of where in its bin each lies: two 32-bit
+//    additions in shared memory a score (64-bit ones take 6 to 150 times as long, and the counts need no weight).  A cluster's
+//    CTAs sum a share of the bins each.  That gives the bin of the k-th score, and the weight up to each bin
+//    within 10^-4: the bins in which the sum may reach top_p.
+//  * One pass adds up the exact weights of all others, and lists the scores of those bins (some hundreds).
+//  * Every CTA sorts the list and finds both borders in it.
+//  * Where the list would be too long (thousands of equal scores, temperature infinity) the borders are
+//    found digit by digit of the key instead: sums by digit of the keys that share the digits so far, two or
+//    three turns a border.
 constexpr int kSampSlice = 32768;          // scores of a CTA at most
-constexpr int kSampBins = 2048;
+constexpr int kSampBins = 46 * 64;         // weights below 2^-46 count nothing
+constexpr int kSampDigits = 2048;
+constexpr int kSampThreads = 512;
 constexpr double kSampOne = 17592186044416.0;   // 2^44
 
 struct SampPart {                          // what the CTAs of a row tell each other
-  unsigned long long mass;
+  unsigned long long mass, rest;
   unsigned int count, ties;
 };
 
@@ -31,14 +41,15 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t a, unsigned long long v)
   asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
 
-// Keys: 0 for NaN and -infinity, else rising with the score; both zeros are equal.
+// Keys rise with the score; NaN has the least one, that of -infinity (kNone), and both zeros are equal.
 template <int DT>
 struct SampKey {
   using type = uint16_t;
-  static constexpr int kBits = 16, kLevels = 2;
+  static constexpr int kLevels = 2;
+  static constexpr uint32_t kInf = DT == YK_F16 ? 0x7c00u : 0x7f80u, kNone = 0x7fffu - kInf;
   __device__ static uint32_t of(uint16_t b) {
-    const uint32_t inf = DT == YK_F16 ? 0x7c00u : 0x7f80u, m = b & 0x7fffu;
-    if (m > inf || b == (0x8000u | inf)) return 0;
+    const uint32_t m = b & 0x7fffu;
+    if (m > kInf) return kNone;
     if (m == 0) return 0x8000u;
     return b & 0x8000u ? (uint16_t)~b : b | 0x8000u;
   }
@@ -52,10 +63,11 @@ struct SampKey {
 template <>
 struct SampKey<YK_F32> {
   using type = uint32_t;
-  static constexpr int kBits = 32, kLevels = 3;
+  static constexpr int kLevels = 3;
+  static constexpr uint32_t kNone = 0x007fffffu;
   __device__ static uint32_t of(uint32_t b) {
     const uint32_t m = b & 0x7fffffffu;
-    if (m > 0x7f800000u || b == 0xff800000u) return 0;
+    if (m > 0x7f800000u) return kNone;
     if (m == 0) return 0x80000000u;
     return b & 0x80000000u ? ~b : b | 0x80000000u;
   }
@@ -64,26 +76,65 @@ struct SampKey<YK_F32> {
   __device__ static constexpr int bits(int level) { return level == 2 ? 10 : 11; }
 };
 
-// 2^44 exp((l - top) / temperature), rounded; c = log2(e) / temperature.
-__device__ __forceinline__ unsigned long long samp_weight(float l, float top, double c) {
-  if (l == top) return 1ull << 44;
-  const double z = ((double)l - (double)top) * c;
-  return z > -46.0 ? (unsigned long long)__double2ll_rn(exp2(z) * kSampOne) : 0ull;
-}
+// Weights 2^44 exp((l - top) / temperature), rounded.  A power of two by a table and a short series (Tang, 1989):
+// z = (l - top) log2(e) / temperature = n / 32 + r, 2^z = 2^(n / 32) (1 + r ln 2 + ..), within 2^-47.  A sum with a large constant
+// rounds to a whole number, and a float becomes a double by its bits, for conversions are slow.  No branch parts a warp, so
+// that several are in work at once.  The table is there 16 times, side by side: a lane reads its own banks.
+struct SampWeights {
+  float top;
+  double c, at_top;                        // log2(e) / temperature, -top c
+  int mode;                                // 0 as above; 1: l - top first, for a far top or a tiny temperature; 2: top is infinite
+  __device__ void set(float top_, float temperature) {
+    top = top_;
+    c = 1.4426950408889634074 / (double)temperature;
+    at_top = -(double)top * c;
+    mode = top == INFINITY ? 2 : fabs(at_top) < 512. && c < 1e20 ? 0 : 1;
+  }
+  __device__ __forceinline__ static unsigned long long power(double z, const double* table) {
+    const double t = z + 211106232532992.0;          // 1.5 * 2^52 / 32
+    const int n = __double2loint(t);
+    const double r = z - (t - 211106232532992.0);
+    const double p = r * fma(r, fma(r, fma(r, fma(r, 0.0013333558146428443423, 0.0096181291076284771619), 0.055504108664821579953),
+                                    0.24022650695910071233), 0.69314718055994530942);
+    const double w = table[(n & 31) * 16 + (threadIdx.x & 15)];
+    const double s = __hiloint2double(__double2hiint(w) + ((n >> 5) + 44) * 0x100000, __double2loint(w));
+    const unsigned long long v = (unsigned long long)__double_as_longlong(fma(s, p, s) + 4503599627370496.0) & 0xfffffffffffffull;
+    return (uint32_t)__double2hiint(z) < 0xc0470000u ? v : 0ull;     // z > -46
+  }
+  // mode 0 (of 0 and subnormal numbers 10^-38 off; a NaN gives anything)
+  __device__ __forceinline__ unsigned long long of_near(float l, const double* table) const {
+    const uint32_t b = __float_as_uint(l);
+    const double d = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+    return power(fma(d, c, at_top), table);
+  }
+  __device__ __forceinline__ unsigned long long of(float l, const double* table) const {
+    if (mode == 0) return of_near(l, table);
+    if (mode == 2) return l == top ? 1ull << 44 : 0ull;
+    return power(((double)l - (double)top) * c, table);
+  }
+};
 
 template <int DT>
-__global__ void __launch_bounds__(kSampThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
   using K = SampKey<DT>;
   using key_t = typename K::type;
-  constexpr int kVec = 16 / sizeof(key_t);
+  using u64 = unsigned long long;
+  constexpr int T = kSampThreads, kVec = 16 / sizeof(key_t), kWarps = T / 32;
+  constexpr int kList = 2 * T;                       // of listed scores
+  constexpr int kPer = (kSampBins + T - 1) / T;      // bins of a thread
   extern __shared__ __align__(16) uint8_t samp_raw[];
   key_t* const keys = (key_t*)samp_raw;
-  __shared__ uint32_t lo[kSampBins], hi[kSampBins];
-  __shared__ SampPart part[2][8];                    // of the row's CTAs
-  __shared__ unsigned long long warp_mass[kSampWarps];
-  __shared__ uint32_t warp_a[kSampWarps], warp_b[kSampWarps];
-  __shared__ unsigned long long found_mass;
-  __shared__ uint32_t found_bin;
+  __shared__ uint32_t hist[2 * kSampBins];           // counts, places; then the row's list; or two sums by digit
+  __shared__ uint32_t own[kList];
+  __shared__ uint8_t own_warp[kList];                // whose they are
+  __shared__ double table[512];
+  __shared__ SampPart part[3][8];                    // of the row's CTAs
+  __shared__ u64 warp_mass[kWarps], warp_rest[kWarps];
+  __shared__ uint32_t warp_a[kWarps], warp_b[kWarps];
+  __shared__ float warp_lo[kWarps], warp_hi[kWarps];
+  __shared__ u64 found_mass;
+  __shared__ uint32_t border_key[5];
+  __shared__ uint32_t found_bin, found_above, found_first, found_last, own_n;
   const YkSample& p = a.p;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, split = a.split;
   const int row = blockIdx.x / split, rank = split > 1 ? (int)cluster_rank() : 0;
@@ -94,36 +145,49 @@ __global__ void __launch_bounds__(kSampThreads) sample_kernel(const __grid_const
     if (tid < split) {
       const uint32_t to = smem_u32(&part[which][rank]), at = split > 1 ? cluster_map(to, tid) : to;
       st_cluster_u64(at, v.mass);
-      st_cluster_u32(at + 8, v.count);
-      st_cluster_u32(at + 12, v.ties);
+      st_cluster_u64(at + 8, v.rest);
+      st_cluster_u32(at + 16, v.count);
+      st_cluster_u32(at + 20, v.ties);
     }
     meet();
   };
+  for (int i = tid; i < 512; i += T) table[i] = exp2((double)(i / 16) / 32);
+  if (tid == 0) own_n = 0;
+  for (int i = tid; i < 2 * kSampBins; i += T) hist[i] = 0;
   pdl_wait();
   pdl_trigger();
 
   // ---- scores into shared memory, the largest
-  uint32_t top_key = 0;
+  uint32_t top_key = K::kNone;
   {
     const key_t* from = (const key_t*)p.logits + row * p.row + first;
     if (a.vec) {
-      for (int i = tid * kVec; i < size; i += kSampThreads * kVec) {
-        key_t k[kVec];
-        if (i + kVec <= size) {
-          *(uint4*)k = *(const uint4*)(from + i);
-        } else {
-          for (int e = 0; e < kVec; e++) k[e] = i + e < size ? from[i + e] : 0;
+      constexpr int kAhead = 4;                      // loads on their way
+      for (int i0 = tid * kVec; i0 < a.slice; i0 += T * kVec * kAhead) {
+        uint4 raw[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+          const int i = i0 + j * T * kVec;
+          if (i + kVec <= size) raw[j] = __ldcs((const uint4*)(from + i));
         }
 #pragma unroll
-        for (int e = 0; e < kVec; e++) {
-          k[e] = (key_t)(i + e < size ? K::of(k[e]) : 0);
-          top_key = max(top_key, (uint32_t)k[e]);
+        for (int j = 0; j < kAhead; j++) {
+          const int i = i0 + j * T * kVec;
+          if (i >= a.slice) break;
+          key_t* k = (key_t*)&raw[j];
+          if (i + kVec > size)
+            for (int e = 0; e < kVec; e++) k[e] = i + e < size ? from[i + e] : (key_t)~0u;   // (NaN)
+#pragma unroll
+          for (int e = 0; e < kVec; e++) {
+            k[e] = (key_t)K::of(k[e]);
+            top_key = max(top_key, (uint32_t)k[e]);
+          }
+          *(uint4*)(keys + i) = raw[j];
         }
-        *(uint4*)(keys + i) = *(const uint4*)k;
       }
     } else {
-      for (int i = tid; i < (size + kVec - 1) / kVec * kVec; i += kSampThreads) {
-        const key_t k = (key_t)(i < size ? K::of(from[i]) : 0);
+      for (int i = tid; i < a.slice; i += T) {
+        const key_t k = (key_t)(i < size ? K::of(from[i]) : K::kNone);
         top_key = max(top_key, (uint32_t)k);
         keys[i] = k;
       }
@@ -134,143 +198,573 @@ __global__ void __launch_bounds__(kSampThreads) sample_kernel(const __grid_const
     __syncthreads();
     if (lane == 0) warp_a[warp] = v;
     __syncthreads();
-    return __reduce_max_sync(~0u, warp_a[lane]);
+    return __reduce_max_sync(~0u, lane < kWarps ? warp_a[lane] : 0);
   };
-  tell(0, {0, block_max(top_key), 0});
+  tell(0, {0, 0, block_max(top_key), 0});
   for (int i = 0; i < split; i++) top_key = max(top_key, part[0][i].count);
   const float temperature = p.temperature ? p.temperature[row] : 1.f;
   const bool greedy = !(temperature > 0.f) || !p.u;
-  if (top_key == 0 || greedy) {
+  const bool any = top_key > K::kNone;
+  if (!any || greedy) {
     // the lowest index of the largest score
     uint32_t at = 0xffffffffu;
-    if (top_key)
-      for (int i = tid; i < size; i += kSampThreads)
+    if (any)
+      for (int i = tid; i < size; i += T)
         if (keys[i] == top_key) at = min(at, (uint32_t)(first + i));
     at = ~block_max(~at);
-    tell(1, {0, at, 0});
+    tell(1, {0, 0, at, 0});
     for (int i = 0; i < split; i++) at = min(at, part[1][i].count);
     if (rank == 0 && tid == 0) {
-      p.token[row] = top_key ? (int)at : -1;
-      if (p.logprob) p.logprob[row] = top_key ? 0.f : -INFINITY;
-      if (p.kept) p.kept[row] = top_key ? 1 : 0;
+      p.token[row] = any ? (int)at : -1;
+      if (p.logprob) p.logprob[row] = any ? 0.f : -INFINITY;
+      if (p.kept) p.kept[row] = any ? 1 : 0;
     }
     return;
   }
   const float top = K::value(top_key);
-  const double c = 1.4426950408889634074 / (double)temperature;
+  SampWeights weights;
+  weights.set(top, temperature);
+  const auto weight = [&](uint32_t k) { return weights.of(K::value(k), table); };
+  const u64 least = p.min_p && p.min_p[row] > 0.f ? min((u64)ceil(fmin((double)p.min_p[row], 1.0) * kSampOne), weight(top_key)) : 1ull;
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
-  const int top_k = p.top_k ? p.top_k[row] : 0;
+  const bool by_p = top_p < 1.f;
+  int top_k = p.top_k ? p.top_k[row] : 0;
+  if (top_k <= 0 || top_k >= p.n) top_k = 0;
 
   // Keys above `cut` stay, and of those that equal it the first `take`.
-  uint32_t cut = 0, take = 0;
+  uint32_t cut = K::kNone, take = 0;
   bool limited = false;                              // by the cut
-  // One digit of a border.  The keys that stay so far and agree with `prefix` above this digit are summed by
-  // digit over the row (their number, or their weights); from the largest digit down, the sums reach `want` (top_p of
-  // the first level's total) in the digit that is returned.  `before` is what lies above it; returns -1 if the total stays below.
-  const auto digit_of = [&](int level, uint32_t prefix, bool by_mass, unsigned long long& want, unsigned long long& before) {
-    const int shift = K::shift(level), bits = K::bits(level), bins = 1 << bits;
-    const auto agrees = [&](uint32_t k) { return level == 0 || k >> (shift + bits) == prefix; };
-    for (int i = tid; i < bins; i += kSampThreads) lo[i] = hi[i] = 0;
-    if (tid == 0) found_bin = 0xffffffffu;
-    __syncthreads();
-    const auto add = [&](uint32_t k, unsigned long long w) {
-      const uint32_t bin = (k >> shift) & (bins - 1), l = (uint32_t)w, old = atomicAdd(&lo[bin], l);
-      atomicAdd(&hi[bin], (uint32_t)(w >> 32) + (old + l < old));
-    };
-    for (int i = tid; i < size; i += kSampThreads) {
-      const uint32_t k = keys[i];
-      if (k <= cut || !agrees(k)) continue;          // (those equal to the cut: below, as many as stay)
-      if (by_mass) {
-        const unsigned long long w = samp_weight(K::value(k), top, c);
-        if (w) add(k, w);
-      } else {
-        atomicAdd(&lo[(k >> shift) & (bins - 1)], 1u);
+  bool by_list = false;                              // `mass` and `count` hold what of this warp's run stays, but for the list
+  u64 mass = 0;
+  uint32_t count = 0;
+  const int run = a.slice / kWarps, from = warp * run, to = min(size, from + run);
+
+  // 1/256 bins below the top, rounded (by the sum with 2^23); rises with falling scores
+  const float c256 = (float)fmin(16384.0 * weights.c, 1e38);   // (times 0 is 0)
+  const auto place = [&](uint32_t k) {
+    return __float_as_uint(fminf(fmaf(top - K::value(k), c256, 8388608.f), 8388608.f + 256.f * kSampBins)) - 0x4b000000u;
+  };
+  const auto bin_of = [&](uint32_t k) { return (int)(place(k) >> 8); };
+  bool open = top_k || by_p;                         // borders to find
+  if (open && top < INFINITY) {
+    // ---- counts by bin
+    for (int i = tid * kVec; i < a.slice; i += T * kVec) {     // (keys behind the last score are kNone: beyond the bins)
+      const uint4 raw = *(const uint4*)(keys + i);
+      const key_t* k = (const key_t*)&raw;
+      uint32_t q[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; e++) q[e] = place(k[e]);
+#pragma unroll
+      for (int e = 0; e < kVec; e++) {
+        if (q[e] >= kSampBins * 256) continue;
+        atomicAdd(&hist[q[e] >> 8], 1u);
+        if (by_p) atomicAdd(&hist[kSampBins + (q[e] >> 8)], q[e] & 255u);
       }
     }
-    if (limited && by_mass && rank == 0 && tid == 0 && agrees(cut)) add(cut, samp_weight(K::value(cut), top, c) * take);
     meet();
-    // thread t: the t-th two digits from the top
-    unsigned long long v[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int bin = bins - 1 - 2 * tid - e;
-      if (bin < 0) continue;
-      const uint32_t l = smem_u32(&lo[bin]), h = smem_u32(&hi[bin]);
-      if (split == 1) {
-        v[e] = lo[bin] + ((unsigned long long)hi[bin] << 32);
-      } else {
-        for (int q = 0; q < split; q++)
-          v[e] += ld_cluster_u32(cluster_map(l, q)) + (by_mass ? (unsigned long long)ld_cluster_u32(cluster_map(h, q)) << 32 : 0ull);
+    if (split > 1) {
+      // this CTA's share of the bins: the row's sums to all
+      const int share = kSampBins / split;           // (46 * 64 is a multiple of 8)
+      for (int i = tid; i < (by_p ? 2 : 1) * share; i += T) {
+        const int b = i < share ? rank * share + i : kSampBins + rank * share + i - share;
+        const uint32_t at = smem_u32(&hist[b]);
+        uint32_t v = 0;
+        for (int q = 0; q < split; q++) v += ld_cluster_u32(cluster_map(at, q));
+        for (int q = 0; q < split; q++) st_cluster_u32(cluster_map(at, q), v);
       }
+      meet();
     }
-    unsigned long long sum = v[0] + v[1];
+    // ---- thread t: kPer bins behind one another
+    uint32_t n[kPer], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; e++) {
+      const int b = tid * kPer + e;
+      n[e] = b < kSampBins ? hist[b] : 0;
+      sum += n[e];
+    }
+    uint32_t above = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long b = __shfl_up_sync(~0u, sum, o);
-      if (lane >= o) sum += b;
+      const uint32_t v = __shfl_up_sync(~0u, above, o);
+      if (lane >= o) above += v;
     }
-    if (lane == 31) warp_mass[warp] = sum;
+    if (lane == 31) warp_a[warp] = above;
+    if (tid == 0) {
+      found_bin = found_first = kSampBins;
+      found_last = kSampBins - 1;
+      found_above = 0;
+    }
     __syncthreads();
-    unsigned long long warps = warp_mass[lane];
+    above += __reduce_add_sync(~0u, lane < warp ? warp_a[lane] : 0) - sum;
+    if (top_k) {
+      uint32_t at = above;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long b = __shfl_up_sync(~0u, warps, o);
-      if (lane >= o) warps += b;
-    }
-    const unsigned long long total = __shfl_sync(~0u, warps, 31), above = __shfl_sync(~0u, warps, max(warp - 1, 0));
-    if (level == 0 && by_mass) want = max(1ull, (unsigned long long)ceil((double)top_p * (double)total));
-    unsigned long long at = (warp ? above : 0) + sum - v[0] - v[1];
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      if (at < want && at + v[e] >= want) {
-        found_bin = bins - 1 - 2 * tid - e;
-        found_mass = at;
+      for (int e = 0; e < kPer; e++) {
+        if (at < (uint32_t)top_k && at + n[e] >= (uint32_t)top_k) {
+          found_bin = tid * kPer + e;
+          found_above = at;
+        }
+        at += n[e];
       }
-      at += v[e];
+      __syncthreads();
     }
-    meet();                                          // found, and every CTA has read the sums
-    before = found_mass;
-    const int bin = (int)found_bin;
+    const int bin_k = (int)found_bin;                // kSampBins: no score of a weight is left out by top-k
+    const uint32_t above_k = found_above;
+    int bin1 = bin_k, bin2 = bin_k;                  // bins below bin1 stay whole, those up to bin2 (and bin_k) are listed
+    if (by_p) {
+      // weights up to each bin, from below and from above: a bin's n scores at places f (in units of 1 / 256, half
+      // a unit off at most and a tenth by the product's rounding) weigh 2^(-b / 64) (n - s sum f / 256 + at most n s^2 / 2),
+      // s = ln 2 / 64
+      constexpr float kS = 0.010830424696249145f, kOff = 2e-5f;
+      float lo[kPer], hi[kPer], lo_sum = 0, hi_sum = 0;
+#pragma unroll
+      for (int e = 0; e < kPer; e++) {
+        const int b = tid * kPer + e;
+        lo[e] = hi[e] = 0;
+        if (b <= bin_k && n[e]) {
+          const float w = exp2f((float)b * -0.015625f), m = (float)n[e], f = (float)hist[kSampBins + b];
+          lo[e] = w * (m - (kS / 256) * (f + 0.6f * m)) * (1 - kOff);
+          hi[e] = w * (m - (kS / 256) * (f - 0.6f * m) + m * (kS * kS / 2)) * (1 + kOff);
+          if (b == bin_k) {
+            hi[e] = w * (float)(top_k - above_k) * (1 + kS / 256 + kOff);
+            lo[e] = w * (float)(top_k - above_k) * (1 - kS * 1.01f - kOff);
+          }
+        }
+        lo_sum += lo[e];
+        hi_sum += hi[e];
+      }
+      float lo_at = lo_sum, hi_at = hi_sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float u = __shfl_up_sync(~0u, lo_at, o), v = __shfl_up_sync(~0u, hi_at, o);
+        if (lane >= o) {
+          lo_at += u;
+          hi_at += v;
+        }
+      }
+      if (lane == 31) {
+        warp_lo[warp] = lo_at;
+        warp_hi[warp] = hi_at;
+      }
+      __syncthreads();
+      float lo_all = lane < kWarps ? warp_lo[lane] : 0, hi_all = lane < kWarps ? warp_hi[lane] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float u = __shfl_up_sync(~0u, lo_all, o), v = __shfl_up_sync(~0u, hi_all, o);
+        if (lane >= o) {
+          lo_all += u;
+          hi_all += v;
+        }
+      }
+      const float lo_before = __shfl_sync(~0u, lo_all, max(warp - 1, 0)), hi_before = __shfl_sync(~0u, hi_all, max(warp - 1, 0));
+      lo_at += (warp ? lo_before : 0) - lo_sum;
+      hi_at += (warp ? hi_before : 0) - hi_sum;
+      lo_all = __shfl_sync(~0u, lo_all, 31);
+      hi_all = __shfl_sync(~0u, hi_all, 31);
+      const float want_lo = fmaxf(top_p * lo_all * (1 - kOff), 1e-30f), want_hi = top_p * hi_all * (1 + kOff);
+      // (bounds that miss a bin by these sums' own rounding are found out below)
+      uint32_t at_hi = kSampBins, at_lo = kSampBins - 1;
+#pragma unroll
+      for (int e = kPer - 1; e >= 0; e--) {          // from the last bin down, so that the first one stays
+        if (hi[e] > 0 && hi_at + hi_sum >= want_lo) at_hi = tid * kPer + e;
+        if (lo[e] > 0 && lo_at + lo_sum >= want_hi) at_lo = tid * kPer + e;
+        hi_sum -= hi[e];
+        lo_sum -= lo[e];
+      }
+      at_hi = __reduce_min_sync(~0u, at_hi);
+      at_lo = __reduce_min_sync(~0u, at_lo);
+      if (lane == 0) {
+        atomicMin(&found_first, at_hi);
+        atomicMin(&found_last, at_lo);
+      }
+      __syncthreads();
+      bin1 = (int)found_first;
+      bin2 = max(bin1, min((int)found_last, bin_k));
+    }
+    // ---- exact weights of the bins that stay whole and (for top-p) of those that do not, and the list of the others
+    u64 all = 0, rest = 0;
+    // the smallest keys of bins below these five, a warp each, 33 parts a turn: bins fall as keys rise
+    if (warp < 5) {
+      const int b = warp == 0 ? bin1 : warp == 1 ? bin2 + 1 : warp == 2 ? bin_k : warp == 3 ? bin_k + 1 : kSampBins;
+      uint32_t lo = 0, hi = top_key + 1u;            // (bins of lo and below are not, those of hi and above are)
+      while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 32) / 33, m = lo + step * (lane + 1);
+        const uint32_t yes = __ballot_sync(~0u, m >= hi || m < lo || bin_of(m) < b);
+        const int i = yes ? __ffs(yes) - 1 : 32;     // the first that is
+        const uint32_t next = lo + step * (i + 1);
+        if (i < 32 && next < hi && next > lo) hi = next;
+        lo += step * i;
+      }
+      if (lane == 0) border_key[warp] = hi;
+    }
     __syncthreads();
-    return bin;
-  };
-  const auto border = [&](bool by_mass, unsigned long long want) {
-    uint32_t prefix = 0;
-    for (int level = 0; level < K::kLevels; level++) {
-      unsigned long long before;
-      const int bin = digit_of(level, prefix, by_mass, want, before);
-      if (bin < 0) return;                           // all of them stay
-      want -= before;
-      prefix = prefix << K::bits(level) | bin;
+    // keys from `whole` on stay, from `low` on are listed; so are those from k_low below k_high (bin_k may be bin2)
+    const bool by_k = bin_k < kSampBins;
+    const uint32_t whole = border_key[0], low = bin1 < kSampBins ? border_key[1] : whole;
+    const uint32_t k_high = by_k ? border_key[2] : 0, k_low = by_k ? border_key[3] : 0;
+    const uint32_t least_key = by_k ? min(k_low, low) : by_p ? border_key[4] : low;
+    const auto note = [&](key_t k) {
+      const uint32_t at = atomicAdd(&own_n, 1u);
+      if (at < kList) {
+        own[at] = k;
+        own_warp[at] = (uint8_t)warp;
+      }
+    };
+    for (int i = from + lane * kVec; i < from + run; i += 32 * kVec) {
+      const uint4 raw = *(const uint4*)(keys + i);
+      const key_t* k = (const key_t*)&raw;
+      if (by_p && !by_k && least == 1 && weights.mode == 0) {
+        // all weights count: no branch, but for the few that are listed
+        u64 w[kVec];
+        bool some = false;
+#pragma unroll
+        for (int e = 0; e < kVec; e++) w[e] = weights.of_near(K::value(k[e]), table);
+#pragma unroll
+        for (int e = 0; e < kVec; e++) {
+          rest += w[e];
+          if (k[e] >= whole) {
+            all += w[e];
+            count++;
+          }
+          some |= k[e] >= low && k[e] < whole;
+        }
+        if (some) {
+#pragma unroll
+          for (int e = 0; e < kVec; e++)
+            if (k[e] >= low && k[e] < whole) {
+              note(k[e]);
+              rest -= w[e];
+            }
+        }
+      } else {                                       // few do
+#pragma unroll
+        for (int e = 0; e < kVec; e++) {
+          if (k[e] < least_key) continue;
+          if ((k[e] < whole && k[e] >= low) || (k[e] < k_high && k[e] >= k_low)) {
+            note(k[e]);
+            continue;
+          }
+          const u64 w = weight(k[e]);
+          rest += w;
+          if (k[e] < whole) continue;
+          all += w;
+          if (w < least) continue;
+          mass += w;
+          count++;
+        }
+      }
     }
-    cut = prefix;
-    const unsigned long long w = by_mass ? samp_weight(K::value(cut), top, c) : 1;
-    take = (uint32_t)((want + w - 1) / w);
-    limited = true;
-  };
-  if (top_k > 0 && top_k < p.n) border(false, top_k);
-  if (top_p < 1.f) border(true, 0);
+    rest -= all;
+    if (by_p && !by_k && least == 1 && weights.mode == 0) mass = all;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      mass += __shfl_xor_sync(~0u, mass, o);
+      all += __shfl_xor_sync(~0u, all, o);
+      rest += __shfl_xor_sync(~0u, rest, o);
+    }
+    count = __reduce_add_sync(~0u, count);
+    if (lane == 0) {
+      warp_mass[warp] = all;
+      warp_rest[warp] = rest;
+    }
+    __syncthreads();
+    all = lane < kWarps ? warp_mass[lane] : 0;
+    rest = lane < kWarps ? warp_rest[lane] : 0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      all += __shfl_xor_sync(~0u, all, o);
+      rest += __shfl_xor_sync(~0u, rest, o);
+    }
+    tell(2, {all, rest, own_n, 0});
+    u64 before = 0, total = 0;                       // weight of the bins below bin1; of all but the list
+    uint32_t m = 0;
+    for (int q = 0; q < split; q++) {
+      before += part[2][q].mass;
+      total += part[2][q].mass + part[2][q].rest;
+      m += min(part[2][q].count, kList + 1u);
+    }
+    by_list = true;
+    if (m == 0 && !by_p) {
+      open = false;                                  // top-k alone, and it leaves all that count
+    } else if (m && m <= 32) {
+      // ---- the row's list, sorted, by each warp for itself: lane i has place i
+      uint32_t v = 0;
+      if (lane < m) {
+        uint32_t i = lane;
+        int q = 0;
+        while (i >= part[2][q].count) i -= part[2][q++].count;
+        v = split > 1 ? ld_cluster_u32(cluster_map(smem_u32(own + i), q)) : own[i];
+      }
+#pragma unroll
+      for (int k = 2; k <= 32; k *= 2) {
+#pragma unroll
+        for (int j = k / 2; j; j /= 2) {
+          const uint32_t o = __shfl_xor_sync(~0u, v, j);
+          v = ((lane & j) == 0) == ((lane & k) == 0) ? max(v, o) : min(v, o);
+        }
+      }
+      open = false;
+      uint32_t stay = m;                             // of the list, by top-k
+      if (by_k) {
+        stay = __popc(__ballot_sync(~0u, lane < m && bin_of(v) < bin_k)) + top_k - above_k;
+        cut = __shfl_sync(~0u, v, stay - 1);
+        take = stay - __popc(__ballot_sync(~0u, v > cut));
+        limited = true;
+      }
+      if (by_p) {
+        const u64 w = lane < stay ? weight(v) : 0;
+        u64 in = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 u = __shfl_up_sync(~0u, in, o);
+          if (lane >= o) in += u;
+        }
+        total += __shfl_sync(~0u, in, 31);
+        const u64 want = max(1ull, (u64)ceil(fmax((double)top_p, 0.0) * (double)total));
+        in += before;
+        const uint32_t hit = __ballot_sync(~0u, in >= want && in - w < want && bin_of(v) <= bin2);
+        if (hit == 0) {
+          open = true;                               // (as below)
+        } else {
+          const int i = __ffs(hit) - 1;
+          cut = __shfl_sync(~0u, v, i);
+          take = i + 1 - __popc(__ballot_sync(~0u, v > cut));
+          limited = true;
+        }
+      }
+    } else if (m && m <= kList) {
+      // ---- the row's list, sorted: thread t has places t and t + T
+      uint32_t* const list = hist;
+      for (uint32_t i = tid; i < m; i += T) {
+        uint32_t at = i;
+        int q = 0;
+        while (at >= part[2][q].count) at -= part[2][q++].count;
+        const uint32_t l = smem_u32(own + at);
+        list[i] = split > 1 ? ld_cluster_u32(cluster_map(l, q)) : own[at];
+      }
+      uint32_t len = 32;
+      while (len < m) len *= 2;
+      for (uint32_t i = m + tid; i < len; i += T) list[i] = 0;
+      __syncthreads();
+      if (tid < len) {                               // whole warps
+        uint32_t v[2];
+        const uint32_t i1 = tid + T;
+        const bool two = len > T;
+        v[0] = list[tid];
+        v[1] = two ? list[i1] : 0;
+        const auto sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(min(len, (uint32_t)T)) : "memory"); };
+        for (uint32_t k = 2; k <= len; k *= 2) {
+          for (uint32_t j = k / 2; j; j /= 2) {
+            if (j == T) {                            // both are this thread's
+              const uint32_t x = max(v[0], v[1]), y = min(v[0], v[1]);
+              v[0] = x;
+              v[1] = y;
+              continue;
+            }
+            uint32_t o[2] = {0, 0};
+            if (j >= 32) {
+              sync();
+              list[tid] = v[0];
+              if (two) list[i1] = v[1];
+              sync();
+              o[0] = list[tid ^ j];
+              if (two) o[1] = list[i1 ^ j];
+            } else {
+              o[0] = __shfl_xor_sync(~0u, v[0], j);
+              if (two) o[1] = __shfl_xor_sync(~0u, v[1], j);
+            }
+            // falling: of a pair the lower place has the larger one where bit k of the place is 0
+            v[0] = ((tid & j) == 0) == ((tid & k) == 0) ? max(v[0], o[0]) : min(v[0], o[0]);
+            if (two) v[1] = ((i1 & j) == 0) == ((i1 & k) == 0) ? max(v[1], o[1]) : min(v[1], o[1]);
+          }
+        }
+        sync();
+        list[tid] = v[0];
+        if (two) list[i1] = v[1];
+      }
+      __syncthreads();
+      // the first place of the list with a key of at most v
+      const auto first_of = [&](uint32_t v) {
+        uint32_t lo = 0, hi = m;
+        while (lo < hi) {
+          const uint32_t i = (lo + hi) / 2;
+          if (list[i] > v) lo = i + 1; else hi = i;
+        }
+        return lo;
+      };
+      uint32_t stay = m;                             // of the list, by top-k
+      if (by_k) {
+        uint32_t lo = 0, hi = m;
+        while (lo < hi) {
+          const uint32_t i = (lo + hi) / 2;
+          if (bin_of(list[i]) < bin_k) lo = i + 1; else hi = i;
+        }
+        stay = lo + (top_k - above_k);
+        cut = list[stay - 1];
+        take = stay - first_of(cut);
+        limited = true;
+      }
+      open = false;
+      if (by_p) {
+        u64 w[2], sum = 0;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          w[e] = 2 * tid + e < (int)stay ? weight(list[2 * tid + e]) : 0;
+          sum += w[e];
+        }
+        u64 in = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 v = __shfl_up_sync(~0u, in, o);
+          if (lane >= o) in += v;
+        }
+        if (lane == 31) warp_mass[warp] = in;
+        if (tid == 0) found_bin = 0xffffffffu;
+        __syncthreads();
+        u64 sums = lane < kWarps ? warp_mass[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 v = __shfl_up_sync(~0u, sums, o);
+          if (lane >= o) sums += v;
+        }
+        total += __shfl_sync(~0u, sums, 31);
+        const u64 ahead = __shfl_sync(~0u, sums, max(warp - 1, 0));
+        const u64 want = max(1ull, (u64)ceil(fmax((double)top_p, 0.0) * (double)total));
+        u64 at = before + (warp ? ahead : 0) + in - sum;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          if (at < want && at + w[e] >= want && bin_of(list[2 * tid + e]) <= bin2) found_bin = 2 * tid + e;
+          at += w[e];
+        }
+        __syncthreads();
+        if (found_bin == 0xffffffffu) {
+          open = true;                               // (the bounds above leave this out; all CTAs agree on it)
+        } else {
+          cut = list[found_bin];
+          take = found_bin + 1 - first_of(cut);
+          limited = true;
+        }
+      }
+    }
+  }
+  if (open) {
+    // ---- digit by digit
+    cut = K::kNone;
+    take = count = 0;
+    limited = by_list = false;
+    mass = 0;
+    meet();                                          // the list has been read
+    uint32_t* const lo = hist;
+    uint32_t* const hi = hist + kSampDigits;
+    // One digit of a border.  The keys that stay so far and agree with `prefix` above this digit are summed by
+    // digit over the row (their number, or their weights); from the largest digit down, the sums reach `want` (top_p of
+    // the first level's total) in the digit that is returned.  `before` is what lies above it; returns -1 if the total stays below.
+    const auto digit_of = [&](int level, uint32_t prefix, bool by_mass, u64& want, u64& before) {
+      const int shift = K::shift(level), bits = K::bits(level), bins = 1 << bits;
+      constexpr int kEach = kSampDigits / T;         // digits of a thread, from the top
+      const auto agrees = [&](uint32_t k) { return level == 0 || k >> (shift + bits) == prefix; };
+      for (int i = tid; i < bins; i += T) lo[i] = hi[i] = 0;
+      if (tid == 0) found_bin = 0xffffffffu;
+      __syncthreads();
+      const auto add = [&](uint32_t k, u64 w) {
+        const uint32_t bin = (k >> shift) & (bins - 1), l = (uint32_t)w, old = atomicAdd(&lo[bin], l);
+        atomicAdd(&hi[bin], (uint32_t)(w >> 32) + (old + l < old));
+      };
+      for (int i = tid; i < size; i += T) {
+        const uint32_t k = keys[i];
+        if (k <= cut || !agrees(k)) continue;        // (those equal to the cut: below, as many as stay)
+        if (by_mass) {
+          const u64 w = weight(k);
+          if (w) add(k, w);
+        } else {
+          atomicAdd(&lo[(k >> shift) & (bins - 1)], 1u);
+        }
+      }
+      if (limited && by_mass && rank == 0 && tid == 0 && agrees(cut)) add(cut, weight(cut) * take);
+      meet();
+      u64 v[kEach], in = 0;
+#pragma unroll
+      for (int e = 0; e < kEach; e++) {
+        const int bin = bins - 1 - kEach * tid - e;
+        v[e] = 0;
+        if (bin < 0) continue;
+        const uint32_t l = smem_u32(&lo[bin]), h = smem_u32(&hi[bin]);
+        if (split == 1) {
+          v[e] = lo[bin] + ((u64)hi[bin] << 32);
+        } else {
+          for (int q = 0; q < split; q++)
+            v[e] += ld_cluster_u32(cluster_map(l, q)) + (by_mass ? (u64)ld_cluster_u32(cluster_map(h, q)) << 32 : 0ull);
+        }
+        in += v[e];
+      }
+      u64 sum = in;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 b = __shfl_up_sync(~0u, sum, o);
+        if (lane >= o) sum += b;
+      }
+      if (lane == 31) warp_mass[warp] = sum;
+      __syncthreads();
+      u64 warps = lane < kWarps ? warp_mass[lane] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 b = __shfl_up_sync(~0u, warps, o);
+        if (lane >= o) warps += b;
+      }
+      const u64 total = __shfl_sync(~0u, warps, 31), ahead = __shfl_sync(~0u, warps, max(warp - 1, 0));
+      if (level == 0 && by_mass) want = max(1ull, (u64)ceil(fmax((double)top_p, 0.0) * (double)total));
+      u64 at = (warp ? ahead : 0) + sum - in;
+#pragma unroll
+      for (int e = 0; e < kEach; e++) {
+        if (at < want && at + v[e] >= want) {
+          found_bin = bins - 1 - kEach * tid - e;
+          found_mass = at;
+        }
+        at += v[e];
+      }
+      meet();                                        // found, and every CTA has read the sums
+      before = found_mass;
+      const int bin = (int)found_bin;
+      __syncthreads();
+      return bin;
+    };
+    const auto border = [&](bool by_mass, u64 want) {
+      uint32_t prefix = 0;
+      for (int level = 0; level < K::kLevels; level++) {
+        u64 before;
+        const int bin = digit_of(level, prefix, by_mass, want, before);
+        if (bin < 0) return;                         // all of them stay
+        want -= before;
+        prefix = prefix << K::bits(level) | bin;
+      }
+      cut = prefix;
+      const u64 w = by_mass ? weight(cut) : 1;
+      take = (uint32_t)((want + w - 1) / w);
+      limited = true;
+    };
+    if (top_k) border(false, top_k);
+    if (by_p) border(true, 0);
+  }
 
   // ---- what stays, by warp: a warp has a run of consecutive scores
-  const unsigned long long least = p.min_p && p.min_p[row] > 0.f ? (unsigned long long)ceil(fmin((double)p.min_p[row], 1.0) * kSampOne) : 1ull;
-  const unsigned long long cut_w = limited ? samp_weight(K::value(cut), top, c) : 0;
+  const u64 cut_w = limited ? weight(cut) : 0;
   if (cut_w < least) take = 0;
-  const int run = a.slice / kSampWarps, from = warp * run, to = min(size, from + run);
-  unsigned long long mass = 0;
-  uint32_t count = 0, ties = 0;
-  for (int i = from + lane; i < to; i += 32) {
-    const uint32_t k = keys[i];
-    ties += limited && k == cut;
-    if (k <= cut) continue;
-    const unsigned long long w = samp_weight(K::value(k), top, c);
-    if (w < least) continue;
-    mass += w;
-    count++;
-  }
+  uint32_t ties = 0;
+  if (!by_list) {
+    for (int i = from + lane; i < to; i += 32) {
+      const uint32_t k = keys[i];
+      ties += limited && k == cut;
+      if (k <= cut) continue;
+      const u64 w = weight(k);
+      if (w < least) continue;
+      mass += w;
+      count++;
+    }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(~0u, mass, o);
-  count = __reduce_add_sync(~0u, count);
-  ties = __reduce_add_sync(~0u, ties);
+    for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(~0u, mass, o);
+    count = __reduce_add_sync(~0u, count);
+    ties = __reduce_add_sync(~0u, ties);
+  }
   __syncthreads();
   if (lane == 0) {
     warp_mass[warp] = mass;
@@ -278,24 +772,40 @@ __global__ void __launch_bounds__(kSampThreads) sample_kernel(const __grid_const
     warp_b[warp] = ties;
   }
   __syncthreads();
+  if (by_list) {
+    // of the bins that did not stay whole: the listed ones
+    for (uint32_t i = tid; i < own_n; i += T) {
+      const uint32_t k = own[i], of = own_warp[i];
+      if (k < cut) continue;
+      if (k == cut && limited) {
+        atomicAdd(&warp_b[of], 1u);
+        continue;
+      }
+      const u64 w = weight(k);
+      if (w < least) continue;
+      atomicAdd(&warp_mass[of], w);
+      atomicAdd(&warp_a[of], 1u);
+    }
+    __syncthreads();
+  }
   // lane i: warp i's
-  mass = warp_mass[lane];
-  ties = warp_b[lane];
-  unsigned long long cta_mass = mass;
+  mass = lane < kWarps ? warp_mass[lane] : 0;
+  ties = lane < kWarps ? warp_b[lane] : 0;
+  u64 cta_mass = mass;
 #pragma unroll
   for (int o = 16; o; o >>= 1) cta_mass += __shfl_xor_sync(~0u, cta_mass, o);
-  tell(1, {cta_mass, __reduce_add_sync(~0u, warp_a[lane]), __reduce_add_sync(~0u, ties)});
+  tell(1, {cta_mass, 0, __reduce_add_sync(~0u, lane < kWarps ? warp_a[lane] : 0), __reduce_add_sync(~0u, ties)});
   unsigned long long total = 0, start = 0;           // of the row; before this CTA
-  uint32_t all = 0, tie_at = 0, tie_start = 0;
+  uint32_t all = 0, ties_at = 0, tie_start = 0;
   for (int q = 0; q < split; q++) {
     if (q == rank) {
       start = total;
-      tie_start = tie_at;
+      tie_start = ties_at;
     }
-    const uint32_t stay = min(part[1][q].ties, take - min(take, tie_at));
+    const uint32_t stay = min(part[1][q].ties, take - min(take, ties_at));
     total += part[1][q].mass + stay * cut_w;
     all += part[1][q].count + stay;
-    tie_at += part[1][q].ties;
+    ties_at += part[1][q].ties;
   }
   const float u = p.u[row];
   unsigned long long target = u > 0.f ? (unsigned long long)fmin((double)u * (double)total, 9e18) : 0;
@@ -316,36 +826,53 @@ __global__ void __launch_bounds__(kSampThreads) sample_kernel(const __grid_const
     if (lane >= o) end += b;
   }
   end += start;
-  const bool mine = target < end && target >= end - mass;
-  if (!(__ballot_sync(~0u, mine) >> warp & 1)) return;
-  unsigned long long at = __shfl_sync(~0u, end - mass, warp);
-  uint32_t tie = __shfl_sync(~0u, tie_before, warp);
-  for (int i0 = from; i0 < to; i0 += 32) {
-    const uint32_t k = i0 + lane < to ? keys[i0 + lane] : 0;
+  const uint32_t has = __ballot_sync(~0u, lane < kWarps && target < end && target >= end - mass);
+  if (!has) return;                                  // another CTA's (all of this one's warps see the same)
+  const int who = __ffs(has) - 1;
+  u64 at = __shfl_sync(~0u, end - mass, who);
+  uint32_t tie = __shfl_sync(~0u, tie_before, who);
+  // that warp's run, a score a thread and turn
+  const int run_at = who * run, run_end = min(size, run_at + run);
+  for (int i0 = run_at; i0 < run_end; i0 += T) {
+    const uint32_t k = i0 + tid < run_end ? keys[i0 + tid] : 0;
     const bool same = limited && k == cut;
     const uint32_t sames = __ballot_sync(~0u, same);
-    unsigned long long w = 0;
-    if (k > cut) w = samp_weight(K::value(k), top, c);
+    u64 w = k > cut ? weight(k) : 0;
     if (w < least) w = 0;
-    if (same && tie + __popc(sames & ((1u << lane) - 1)) < take) w = cut_w;
-    unsigned long long s = w;
+    __syncthreads();                                 // the last turn's sums have been read
+    if (lane == 0) warp_b[warp] = __popc(sames);
+    __syncthreads();
+    if (same) {
+      const uint32_t ahead = tie + __popc(sames & ((1u << lane) - 1));
+      uint32_t more = 0;
+      for (int i = 0; i < warp; i++) more += warp_b[i];
+      w = ahead + more < take ? cut_w : 0;
+    }
+    u64 s = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long b = __shfl_up_sync(~0u, s, o);
+      const u64 b = __shfl_up_sync(~0u, s, o);
       if (lane >= o) s += b;
     }
-    const uint32_t past = __ballot_sync(~0u, at + s > target);
-    if (past) {
-      if (lane == __ffs(past) - 1) {
-        const float l = K::value(k);
-        p.token[row] = first + i0 + lane;
-        if (p.logprob) p.logprob[row] = (float)((l == top ? 0.0 : ((double)l - (double)top) / (double)temperature) - log((double)total / kSampOne));
-        if (p.kept) p.kept[row] = (int)all;
-      }
-      return;
+    if (lane == 31) warp_mass[warp] = s;
+    __syncthreads();
+    u64 sums = lane < kWarps ? warp_mass[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 b = __shfl_up_sync(~0u, sums, o);
+      if (lane >= o) sums += b;
     }
-    at += __shfl_sync(~0u, s, 31);
-    tie += __popc(sames);
+    const u64 ahead = __shfl_sync(~0u, sums, max(warp - 1, 0)), turn = __shfl_sync(~0u, sums, 31);
+    s += at + (warp ? ahead : 0);
+    if (s > target && s - w <= target) {             // one score of the row
+      const float l = K::value(k);
+      p.token[row] = first + i0 + tid;
+      if (p.logprob) p.logprob[row] = (float)((l == top ? 0.0 : ((double)l - (double)top) / (double)temperature) - log((double)total / kSampOne));
+      if (p.kept) p.kept[row] = (int)all;
+    }
+    at += turn;
+    if (at > target) return;
+    tie += __reduce_add_sync(~0u, lane < kWarps ? warp_b[lane] : 0);
   }
 }
 
