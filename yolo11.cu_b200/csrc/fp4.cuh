@@ -20,14 +20,21 @@ __device__ __forceinline__ uint32_t floats_to_e2m1x8(const float (&v)[8]) {
       : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
-// Eight codes as half2 pairs of 2^-14 times their values; exact (a code's three low bits are the low end of fp16's
-// exponent and the first bit of its fraction).
+// Eight codes as half2 pairs; exact.  (A byte register has to be the low one of its word: the upper ones of an unpacked
+// word read as the low one.)
 __device__ __forceinline__ void e2m1x8_to_half2x4(uint32_t codes, uint32_t (&h)[4]) {
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const uint32_t c = codes >> (8 * e);
-    h[e] = (c & 7u) << 9 | (c & 8u) << 12 | (c & 0x70u) << 21 | (c & 0x80u) << 24;
-  }
+  for (int e = 0; e < 4; e++)
+    asm("{\n\t.reg .b8 a, b;\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tmov.b16 {a, b}, lo;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}"
+        : "=r"(h[e]) : "r"(codes >> (8 * e)));
+}
+// Packed 16-bit maximum of |a| and |b|; a NaN stays.
+template <bool BF16>
+__device__ __forceinline__ uint32_t amax_nan_pair(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
+  return r;
 }
 
 // D[tmem] (+)= A[smem] * B[smem]^T over 64 columns of e2m1 codes with scales in TMEM, fp32 sums.

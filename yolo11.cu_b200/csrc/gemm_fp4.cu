@@ -14,7 +14,7 @@ struct GemmFp4Args {
 
 constexpr int kFp4Cols = 256;              // columns of a stage: 128 bytes of codes a row, four MMAs
 constexpr int kFp4Codes = 128 * 128;       // codes of 128 rows
-constexpr int kFp4Threads = 192;           // loads, MMAs, four warps of sums
+constexpr int kFp4Threads = 256;           // of a split product: loads, MMAs, four warps for scales and sums, two that join them
 template <bool NV>
 constexpr int kFp4Bpc = NV ? 4 : 2;        // scale blocks of 256 columns
 
@@ -48,16 +48,17 @@ __device__ __forceinline__ void fp4_put_scales(uint32_t taddr, const uint32_t* v
 //  * warps 2-5 and 6-9: scales from shared memory to TMEM (x's of the CTA's own rows, w's of all) for every other stage,
 //    each four warps with a place of their own there.
 //  * warp 1 of the leader: the MMAs.
-//  * warps 10-13: sums out of TMEM, factor, bias or gate, rounding, through shared memory to rows of 64 bytes.
+//  * warps 10-17: sums out of TMEM, factor, bias or gate, rounding, through shared memory to rows of 64 bytes; of the two
+//    warps that can read a lane each takes every other unit.
 // TMEM: two accumulators of 256 columns and two places of 48 for scales are 96 columns too many.  So the
 // accumulators share 96 columns (0-255 and 160-415): a tile's shared ones are drained first, and the next tile
 // may begin.
-constexpr int kFp4PairThreads = 448;
+constexpr int kFp4PairThreads = 576;
 template <bool NV>
 struct Fp4Pair {
   static constexpr int kStages = 5;
   static constexpr int kStage = 2 * kFp4Codes + 3 * 2048;
-  static constexpr int kStaging = 4 * 32 * 64;
+  static constexpr int kStaging = 8 * 32 * 64;
   static constexpr int kSmem = kStages * kStage + kStaging + 1024;
   static constexpr int kD1 = 160, kSf = 416, kSfSet = 48;
 };
@@ -95,7 +96,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ GemmFp4Args a, const __grid_constan
     mbar_init(sready, 8);
     mbar_init(sready + 8, 8);
     mbar_init(done, 1);
-    mbar_init(shared_free, 8);
+    mbar_init(shared_free, 16);
     mbar_fence_init();
   }
   pdl_wait();
@@ -222,7 +223,8 @@ gemm_fp4_pair_kernel(const __grid_constant__ GemmFp4Args a, const __grid_constan
   } else {
     const int sub = warp & 3;
     const uint32_t lanes = (uint32_t)(sub * 32) << 16, lead_free = cluster_map(shared_free, 0);
-    const uint32_t stage = base + S::kStages * S::kStage + sub * 2048;
+    const int half = warp >= 14;
+    const uint32_t stage = base + S::kStages * S::kStage + (warp - 10) * 2048;
     const uint8_t* stage_p = fp4_raw + (stage - smem_u32(fp4_raw));
     const float alpha = p.alpha, alpha2 = p.alpha2;
     // 32 outputs of the warp's 32 rows, from column c0 on: rounded ..
@@ -248,24 +250,42 @@ gemm_fp4_pair_kernel(const __grid_constant__ GemmFp4Args a, const __grid_constan
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((h ^ ((lane >> 1) & 3)) << 4)),
                      "r"(o[4 * h]), "r"(o[4 * h + 1]), "r"(o[4 * h + 2]), "r"(o[4 * h + 3]) : "memory");
       __syncwarp();
-      uint4 v[4];
+      if (a.y_vec && c0 + 32 <= p.n) {
+        uint4 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int row = j * 8 + (lane >> 2), h = lane & 3;
-        v[j] = *(const uint4*)(stage_p + row * 64 + ((h ^ ((row >> 1) & 3)) << 4));
-      }
+        for (int j = 0; j < 4; j++) {
+          const int row = j * 8 + (lane >> 2), h = lane & 3;
+          v[j] = *(const uint4*)(stage_p + row * 64 + ((h ^ ((row >> 1) & 3)) << 4));
+        }
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int row = j * 8 + (lane >> 2), c = c0 + (lane & 3) * 8;
-        if (m0 + row >= p.rows || c >= p.n) continue;
-        uint16_t* y = (uint16_t*)p.y + (long long)(m0 + row) * p.y_row + c;
-        if (a.y_vec && c + 8 <= p.n) {
-          *(uint4*)y = v[j];
-        } else {
-          const uint32_t* w = (const uint32_t*)&v[j];
+        for (int j = 0; j < 4; j++) {
+          const int row = j * 8 + (lane >> 2);
+          if (m0 + row < p.rows) *(uint4*)((uint16_t*)p.y + (long long)(m0 + row) * p.y_row + c0 + (lane & 3) * 8) = v[j];
+        }
+      } else {
+        // two rows at once, a pair a lane; where a row starts between two words, the pairs from its second element on,
+        // and the first and last by themselves
+        const int q = lane & 15, left = min(32, p.n - c0), here = p.rows - m0;
+        uint16_t* y = (uint16_t*)p.y + (long long)(m0 + (lane >> 4)) * p.y_row + c0;
+#pragma unroll 1
+        for (int j0 = 0; j0 < 16; j0 += 4) {
+          uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (c + e < p.n) y[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+          for (int j = 0; j < 4; j++) {
+            const int row = (j0 + j) * 2 + (lane >> 4);
+            w[j] = *(const uint32_t*)(stage_p + row * 64 + (((q >> 2) ^ ((row >> 1) & 3)) << 4) + (q & 3) * 4);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const uint32_t next = __shfl_down_sync(~0u, w[j], 1, 16);
+            const bool there = (j0 + j) * 2 + (lane >> 4) < here, odd = ((uintptr_t)y & 2) != 0;
+            const int e = 2 * q + odd;
+            const uint32_t v = odd ? __byte_perm(w[j], next, 0x5432) : w[j];
+            if (there && e + 1 < left) *(uint32_t*)(y + e) = v;
+            else if (there && e < left) y[e] = (uint16_t)v;
+            if (there && odd && q == 0) y[0] = (uint16_t)w[j];
+            y += 2 * p.y_row;
+          }
         }
       }
     };
@@ -278,31 +298,29 @@ gemm_fp4_pair_kernel(const __grid_constant__ GemmFp4Args a, const __grid_constan
       const int m0 = tm * 256 + (int)rank * 128 + sub * 32, n0 = tn * kOut;
       const uint32_t d = tmem + (li & 1) * S::kD1 + lanes;
       // 32 outputs are a unit of 32 columns (gated: and as many 64 further on, for the other factor).  The ones that hold shared columns
-      // first and together (a load takes 600 cycles beside the MMAs, however much it brings); then the next tile may begin
-      constexpr int kUnits = kOut / 32, kCols = GATED ? 64 : 32, kFirst = GATED ? 2 : 3;
+      // (three; gated two) first and together (a load takes 600 cycles beside the MMAs, however much it brings); then the
+      // next tile may begin.  (Not unrolled: the code of all units would be fetched once a tile.)
+      constexpr int kUnits = kOut / 32, kFirst = GATED ? 2 : 3, kOnce = GATED ? 1 : 2, kCols = GATED ? 64 : 32;
       const auto unit = [&](int i) { return (li & 1) ? i : (i + kUnits - kFirst) % kUnits; };
-      uint32_t o[16];
+#pragma unroll 1
+      for (int i0 = half; i0 < kUnits; i0 += 2 * kOnce) {
+        uint32_t r[kOnce][kCols], o[16];
 #pragma unroll
-      for (int i0 = 0; i0 < kUnits; i0 += kFirst) {
-        uint32_t r[kFirst][kCols];
-#pragma unroll
-        for (int i = 0; i < kFirst; i++) {
-          if (i0 + i >= kUnits) break;
-          const int u = unit(i0 + i), at = GATED ? (u >> 1) * 128 + (u & 1) * 32 : u * 32;
+        for (int i = 0; i < kOnce; i++) {
+          const int u = unit(i0 + 2 * i), at = GATED ? (u >> 1) * 128 + (u & 1) * 32 : u * 32;
           tmem_ld32(d + at, r[i]);
           if (GATED) tmem_ld32(d + at + 64, r[i] + 32);
         }
         tmem_ld_wait();
-        if (i0 == 0) {
+        if (i0 == half) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(lead_free);
         }
 #pragma unroll
-        for (int i = 0; i < kFirst; i++) {
-          if (i0 + i >= kUnits) break;
-          finish(r[i], r[i] + (GATED ? 32 : 0), n0 + unit(i0 + i) * 32, o);
-          emit(o, m0, n0 + unit(i0 + i) * 32);
+        for (int i = 0; i < kOnce; i++) {
+          finish(r[i], r[i] + (GATED ? 32 : 0), n0 + unit(i0 + 2 * i) * 32, o);
+          emit(o, m0, n0 + unit(i0 + 2 * i) * 32);
         }
       }
     }
@@ -431,7 +449,7 @@ gemm_fp4_split_kernel(const __grid_constant__ GemmFp4Args a, const __grid_consta
   }
   const int rows = min(NT, p.rows - m0);
   float* const part = (float*)(fp4_raw + (base - smem_u32(fp4_raw)));     // [matrix][row][128 outputs], in the ring
-  if (warp >= 2) {
+  if (warp >= 2 && warp < 6) {
     const int sub = warp & 3;
     const uint32_t lanes = (uint32_t)(sub * 32) << 16;
     constexpr int kWords = 4 * kBpc * (S::kA + 1);   // weights', second weights', x's
@@ -459,12 +477,12 @@ gemm_fp4_split_kernel(const __grid_constant__ GemmFp4Args a, const __grid_consta
 #pragma unroll 1
       for (int x = 0; x < S::kA; x++) {
 #pragma unroll 1
-        for (int m = 0; m < rows; m += 16) {
-          uint32_t r[16];
-          tmem_ld16p(tmem + lanes + x * NT + m, r);
+        for (int m = 0; m < rows; m += 32) {
+          uint32_t r[32];
+          tmem_ld32(tmem + lanes + x * NT + m, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 16; e++) part[(x * NT + m + e) * 128 + sub * 32 + lane] = __uint_as_float(r[e]);
+          for (int e = 0; e < 32; e++) part[(x * NT + m + e) * 128 + sub * 32 + lane] = __uint_as_float(r[e]);
         }
       }
     }
@@ -474,39 +492,63 @@ gemm_fp4_split_kernel(const __grid_constant__ GemmFp4Args a, const __grid_consta
   if (split > 1) cluster_barrier();
   else __syncthreads();
   const uint32_t part_sm = smem_u32(part);
-  // two outputs a thread and turn; rows rank, rank + split, ..
-  for (int i = tid; i < ((rows - rank + split - 1) / split) * 64; i += kFp4Threads) {
-    const int m = rank + i / 64 * split, j = i % 64 * 2;
-    if (n0 + j >= p.n) continue;
-    float v[S::kA][2];
+  // two outputs a thread, four rows a turn, of rows rank, rank + split, ..
+  const int j = tid % 64 * 2, step = kFp4Threads / 64 * split;
+  if (n0 + j < p.n) {
+    const bool two = n0 + j + 1 < p.n;
+    const float bias0 = p.bias ? p.bias[n0 + j] : 0.f, bias1 = p.bias && two ? p.bias[n0 + j + 1] : 0.f;
+#pragma unroll 1
+    for (int m = rank + tid / 64 * split; m < rows; m += 4 * step) {
+      float2 v[S::kA][4];
 #pragma unroll
-    for (int x = 0; x < S::kA; x++) {
-      v[x][0] = v[x][1] = 0.f;
-      const uint32_t at = part_sm + ((x * NT + m) * 128 + j) * 4;
-      for (int q = 0; q < split; q++) {
-        float b0, b1;
-        if (split > 1)
-          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(b0), "=f"(b1) : "r"(cluster_map(at, q)) : "memory");
-        else
-          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(b0), "=f"(b1) : "r"(at) : "memory");
-        v[x][0] += b0;
-        v[x][1] += b1;
+      for (int x = 0; x < S::kA; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[x][i] = make_float2(0.f, 0.f);
+      // four CTAs' at a time, added in the CTAs' order
+#pragma unroll 1
+      for (int q0 = 0; q0 < split; q0 += 4) {
+        float2 b[4][S::kA][4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const uint32_t from = split > 1 ? cluster_map(part_sm, min(q0 + q, split - 1)) : part_sm;
+#pragma unroll
+          for (int x = 0; x < S::kA; x++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              b[q][x][i] = make_float2(0.f, 0.f);
+              if (q0 + q < split && m + i * step < rows) {
+                const uint32_t at = from + ((x * NT + m + i * step) * 128 + j) * 4;
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(b[q][x][i].x), "=f"(b[q][x][i].y) : "r"(at) : "memory");
+              }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+          for (int x = 0; x < S::kA; x++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              v[x][i].x += b[q][x][i].x;
+              v[x][i].y += b[q][x][i].y;
+            }
       }
-    }
-    float o[2];
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-      o[e] = v[0][e] * p.alpha;
-      if (GATED) o[e] = fp4_silu(o[e]) * (v[S::kA - 1][e] * p.alpha2);
-      else if (p.bias && n0 + j + e < p.n) o[e] = fmaf(v[0][e], p.alpha, p.bias[n0 + j + e]);
-    }
-    uint16_t* y = (uint16_t*)p.y + (long long)(m0 + m) * p.y_row + n0 + j;
-    const uint32_t w = p.dtype == YK_BF16 ? float2_to_pair<true>(o[0], o[1]) : float2_to_pair<false>(o[0], o[1]);
-    if (a.y_pair && n0 + j + 1 < p.n) {
-      *(uint32_t*)y = w;
-    } else {
-      y[0] = (uint16_t)w;
-      if (n0 + j + 1 < p.n) y[1] = (uint16_t)(w >> 16);
+      for (int i = 0; i < 4; i++) {
+        if (m + i * step >= rows) break;
+        float2 o = make_float2(fmaf(v[0][i].x, p.alpha, bias0), fmaf(v[0][i].y, p.alpha, bias1));
+        if (GATED) {
+          const float2 u = v[S::kA - 1][i];
+          o = make_float2(fp4_silu(o.x) * (u.x * p.alpha2), fp4_silu(o.y) * (u.y * p.alpha2));
+        }
+        uint16_t* y = (uint16_t*)p.y + (long long)(m0 + m + i * step) * p.y_row + n0 + j;
+        const uint32_t w = p.dtype == YK_BF16 ? float2_to_pair<true>(o.x, o.y) : float2_to_pair<false>(o.x, o.y);
+        if (a.y_pair && two) {
+          *(uint32_t*)y = w;
+        } else {
+          y[0] = (uint16_t)w;
+          if (two) y[1] = (uint16_t)(w >> 16);
+        }
+      }
     }
   }
   if (warp == 1) {
@@ -588,12 +630,19 @@ static int launch_fp4(GemmFp4Args& a, cudaStream_t st) {
   a.tiles_n = (p.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
   const long long tiles = (long long)a.tiles_m * a.tiles_n;
   if (tiles > 0x7fffffffll) return refuse(YK_EUNSUP, "gemm_fp4: rows * n too large");
+  // One round of CTAs, with at least two stages of columns each: as many CTAs share a tile's columns as the SMs have room
+  // for (measured, 16 x 4096 outputs x 8192 columns: 1, 2, 4, 8 give 12.3, 8.9, 6.5, 7.9 us; 16 x 12000 x 4096: 8.0,
+  // 8.4, 10.7, 16.8; 16 x 2000 x 2000, 8 stages: 5.6, 5.2, 4.7, 5.6).
   const int nt = p.rows <= 32 ? 32 : 128;
   const long long small = (long long)((p.n + 127) / 128) * ((p.rows + nt - 1) / nt);
   int split = 1;
-  while (split < 8 && small * split * 2 <= sms * (GATED ? 1 : 2) && a.chunks >= 2 * split) split *= 2;
+  while (split < 8 && small * split * 2 <= sms && a.chunks >= 4 * split) split *= 2;
   if (g_fp4_split && g_fp4_split <= a.chunks) split = g_fp4_split;
-  if (g_fp4_kernel ? g_fp4_kernel == 1 : p.rows > 128 && tiles * 4 >= sms)
+  // Pairs beyond that round: their tiles are four times as large (measured, split by the rule against pairs: 400 x 4096 x
+  // 8192, 128 tiles, 18.2 and 18.6 us; 400 x 12000 x 4096, 376 tiles, 25.0 and 21.3; 800 x 12000 x 4096 40.9 and 28.6).  Gated
+  // tiles leave room for one CTA an SM and take twice the work: half a round (800 x 2000 x 2000, 112 tiles, 17.0 and 11.3 us;
+  // 100 x 12000 x 1000 12.7 and 11.2; 400 x 2000 x 2000, 64 tiles, 11.8 and 11.0).
+  if (g_fp4_kernel ? g_fp4_kernel == 1 : p.rows > (GATED ? 64 : 128) && small > (GATED ? sms / 2 : sms))
     return p.dtype == YK_BF16 ? launch_fp4_pair<NV, GATED, true>(a, st) : launch_fp4_pair<NV, GATED, false>(a, st);
   if ((p.rows + nt - 1) / nt > 65535 || small * split > 0x7fffffffll) return refuse(YK_EUNSUP, "gemm_fp4: rows * n too large");
   return nt == 32 ? launch_fp4_split<NV, GATED, 32>(a, split, st) : launch_fp4_split<NV, GATED, 128>(a, split, st);

@@ -1,111 +1,163 @@
 // Rows to 4-bit floats with a scale for each group of columns (yk_quant_fp4).
+#include <math.h>
+
 #include "fp4.cuh"
 
 namespace yk {
 
 struct QuantFp4Args {
   YkQuantFp4 p;
-  int blocks;       // scale blocks along a row
-  int x_vec, v_vec; // x, values allow 16-byte accesses
+  int blocks;        // scale blocks along a row
+  int x_align, v_align;   // 16 where rows of x, of values allow such accesses, else 2
+  int exact;         // the matrix's scale is a power of two
+  float six, over_six, over_scale;     // 6 scale, 1 / (6 scale), 1 / scale
 };
 
-// HBM bound: x is read once, everything else written once.  A CTA has 128 rows (a scale block's) of 256
-// columns: a warp takes a row's 256 at a time, a lane 8 of them, so that a group is 2 or 4 neighbouring
-// lanes and its maximum one or two shuffles; four rows are in flight.  Scales meet in shared memory and
-// leave as whole blocks, as a group's own byte would be a 32-byte sector of its own.
-// The division is x * r with r = 1 / S rounded, then one correction by the remainder x - q S (Markstein,
-// 1990): it rounds as x / S does, so that values halfway between two codes go the way that the definition says, at two
-// packed FMAs for two columns.  Groups with infinities or NaN, tiny or clamped scales divide plainly.
+// HBM bound: x is read once, everything else written once.  A CTA has 32 rows of 256 columns: a warp takes four rows'
+// 256 at once, a lane 8 of each, so that a group is 2 or 4 neighbouring lanes and its maximum one or two shuffles.
+// The rows are 8 behind one another and the ones 32, 64 and 96 further on, as their scales lie together
+// (128 bytes of each block): they meet in shared memory, as a group's own byte would be a 32-byte sector of its own.
+// The arithmetic would take longer than the memory if it divided:
+//  * a / b is a * r with r = 1 / b rounded, then one correction by the remainder a - q b (Markstein, 1990): it rounds as
+//    a / b does, so that values halfway between two codes go the way that the definition says.
+//  * r comes from the 8 fractions that an e4m3 scale can have, times the matrix's scale, in a table; powers of two
+//    move its exponent.  Where S is a power of two, the product alone is exact.
+// Groups with infinities or NaN, tiny or clamped scales divide plainly.
 constexpr int kQuantCols = 256, kQuantThreads = 256;
+
+// Eight 16-bit elements (two where there are fewer columns) at any even address, as pairs.
+__device__ __forceinline__ uint4 quant_load8(const uint16_t* x, int align, int cols, bool first) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  uint32_t* u = (uint32_t*)&v;
+  if (cols >= 8 && align == 16) return __ldcs((const uint4*)x);
+  if (cols >= 8 && ((uintptr_t)x & 2) == 0) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) u[e] = ((const uint32_t*)x)[e];
+  } else if (cols >= 9 && !first) {
+    // the pairs around them, from the element before to the one behind
+    const uint32_t* w = (const uint32_t*)(x - 1);
+    uint32_t last = w[0];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t next = w[e + 1];
+      u[e] = __byte_perm(last, next, 0x5432);
+      last = next;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (e < cols) u[e >> 1] |= (uint32_t)x[e] << (16 * (e & 1));
+  }
+  return v;
+}
+__device__ __forceinline__ void quant_store8(uint16_t* y, int align, int cols, const uint32_t (&o)[4]) {
+  if (cols >= 8 && align == 16) {
+    __stcs((uint4*)y, make_uint4(o[0], o[1], o[2], o[3]));
+  } else if (cols >= 8 && ((uintptr_t)y & 2) == 0) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) ((uint32_t*)y)[e] = o[e];
+  } else if (cols >= 8) {
+    y[0] = (uint16_t)o[0];
+#pragma unroll
+    for (int e = 0; e < 3; e++) ((uint32_t*)(y + 1))[e] = __byte_perm(o[e], o[e + 1], 0x5432);
+    y[7] = (uint16_t)(o[3] >> 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (e < cols) y[e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
+  }
+}
 
 template <bool BF16, bool NV>
 __global__ void __launch_bounds__(kQuantThreads) quant_fp4_kernel(const __grid_constant__ QuantFp4Args a) {
   constexpr int kLanes = NV ? 2 : 4;                 // of a group
   constexpr int kBlocks = NV ? 4 : 2;                // scale blocks of 256 columns
-  constexpr int kRows = 4;                           // of a warp in flight
-  __shared__ __align__(16) uint8_t sc[kBlocks * kFp4Block];
+  constexpr int kRows = 4;                           // of a warp
+  __shared__ __align__(16) uint8_t sc[kBlocks * 128];
+  __shared__ float2 fraction[8];                     // scale * (1 + i / 8), and 1 / that
   const YkQuantFp4& p = a.p;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row0 = blockIdx.y * 128, c = blockIdx.x * kQuantCols + lane * 8;
+  const int part = blockIdx.y & 3, row0 = (blockIdx.y >> 2) * 128;  // rows part * 8 + warp, and 32, 64, 96 on
+  const int c = blockIdx.x * kQuantCols + lane * 8;
   const int rows = min(128, p.rows - row0), cols = p.cols - c;      // columns from the lane's first on
-  for (int i = threadIdx.x; i < kBlocks * kFp4Block / 4; i += kQuantThreads) ((uint32_t*)sc)[i] = 0;
+  if (threadIdx.x < kBlocks * 32) ((uint32_t*)sc)[threadIdx.x] = 0;
+  if (NV && threadIdx.x >= 128 && threadIdx.x < 136) {
+    const float m = p.scale * (1.f + 0.125f * (threadIdx.x - 128));
+    fraction[threadIdx.x - 128] = make_float2(m, 1.f / m);
+  }
   __syncthreads();
   pdl_wait();
   pdl_trigger();
   const int g = lane / kLanes;                       // group of the CTA's columns
-  uint8_t* const sc_at = sc + g / 4 * kFp4Block + g % 4;
-  for (int r0 = warp; r0 < rows; r0 += 8 * kRows) {
+  uint8_t* const sc_at = sc + g / 4 * 128 + warp * 16 + g % 4;
+  {
+    const int r0 = part * 8 + warp;
     uint4 raw[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
-      const int r = r0 + 8 * i;
-      const uint16_t* x = (const uint16_t*)p.x + (long long)(row0 + r) * p.x_row + c;
+      const int r = r0 + 32 * i;
       raw[i] = make_uint4(0, 0, 0, 0);
-      if (r >= rows || cols <= 0) continue;
-      if (a.x_vec && cols >= 8) {
-        raw[i] = __ldcs((const uint4*)x);
-      } else {
-        uint32_t* u = (uint32_t*)&raw[i];
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (e < cols) u[e >> 1] |= (uint32_t)x[e] << (16 * (e & 1));
-      }
+      if (r < rows && cols > 0) raw[i] = quant_load8((const uint16_t*)p.x + (long long)(row0 + r) * p.x_row + c, a.x_align, cols, c == 0);
     }
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
-      const int r = r0 + 8 * i;
+      const int r = r0 + 32 * i;
       if (r >= rows) break;                          // (the whole warp)
       const uint32_t* u = (const uint32_t*)&raw[i];
-      float2 v[4];
-      uint32_t top = 0;                              // largest |x| as bits: a NaN is above infinity
+      // largest |x|, NaN above infinity
+      uint32_t top = amax_nan_pair<BF16>(amax_nan_pair<BF16>(u[0], u[1]), amax_nan_pair<BF16>(u[2], u[3]));
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        v[e] = pair_to_float2<BF16>(u[e]);
-        top = max(top, max(__float_as_uint(v[e].x) & 0x7fffffffu, __float_as_uint(v[e].y) & 0x7fffffffu));
-      }
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
-      const bool nan = top > 0x7f800000u;
-      float amax = __uint_as_float(top);
-      if (__any_sync(~0u, top >= 0x7f800000u)) {     // rare: finite values only
+      for (int o = 1; o < kLanes; o <<= 1) top = amax_nan_pair<BF16>(top, __shfl_xor_sync(~0u, top, o));
+      top = amax_nan_pair<BF16>(top, top >> 16);
+      float amax = elem_to_float<BF16>((uint16_t)top);
+      const bool odd = !(amax < INFINITY), nan = amax != amax;
+      if (__any_sync(~0u, odd)) {                    // rare: finite values only
         float m = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) m = fmaxf(m, fmaxf(finite_abs(v[e].x), finite_abs(v[e].y)));
+        for (int e = 0; e < 4; e++) {
+          const float2 v = pair_to_float2<BF16>(u[e]);
+          m = fmaxf(m, fmaxf(finite_abs(v.x), finite_abs(v.y)));
+        }
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
         amax = m;
       }
-      const float t = amax / (6.f * p.scale);
-      float s;
+      float S, inv;                                  // the group's scale * the matrix's, and its inverse
       uint32_t byte;
-      bool plain = top >= 0x7f800000u;
+      bool plain = odd;
       if (NV) {
+        const float q = amax * a.over_six, t = q < 512.f ? fmaf(fmaf(-q, a.six, amax), a.over_six, q) : q;   // (clamped beyond)
         byte = float2_to_e4m3x2(fminf(fmaxf(t, 0.001953125f), 448.f), 0.f) & 0xffu;
-        s = e4m3x2_to_float2(byte).x;
-        plain |= t > 448.f;
+        plain |= !(t <= 448.f);
+        const uint32_t s = __float_as_uint(e4m3x2_to_float2(byte).x), power = (s & 0x7f800000u) - 0x3f800000u;
+        const float2 f = fraction[(s >> 20) & 7];
+        S = __uint_as_float(__float_as_uint(f.x) + power);
+        inv = __uint_as_float(__float_as_uint(f.y) - power);
       } else {
-        // the exponent of the smallest power of two >= t, as a float's biased one
-        const uint32_t b = __float_as_uint(t);
-        byte = min(max((b >> 23) + ((b & 0x7fffffu) != 0), 127u - 96u), 127u + 96u);
-        s = __uint_as_float(byte << 23);
-        plain |= t > 7.9228162514264338e28f;         // 2^96
+        // the smallest power of two >= amax / (6 scale): difference of the exponents, and one more if the fraction is larger
+        const int e = ((int)(__float_as_uint(amax) - __float_as_uint(a.six)) + 0x7fffff) >> 23, k = min(max(e, -96), 96);
+        plain |= e > 96;
+        byte = k + 127;
+        S = __uint_as_float(__float_as_uint(p.scale) + k * 0x800000);
+        inv = __uint_as_float(__float_as_uint(a.over_scale) - k * 0x800000);
       }
-      const float S = s * p.scale;
-      plain |= S < 8.6736174e-19f;                   // 2^-60: the remainder below would lose bits
       if (nan) byte = NV ? 0x7fu : 0xffu;
+      plain |= S < 8.6736174e-19f;                   // 2^-60: the remainder below would lose bits
       float q[8];
       if (plain) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float d = (e & 1 ? v[e >> 1].y : v[e >> 1].x) / S;
-          q[e] = nan ? 0.f : fminf(fmaxf(d, -6.f), 6.f);
+        for (int e = 0; e < 4; e++) {
+          const float2 v = pair_to_float2<BF16>(u[e]);
+          q[2 * e] = nan ? 0.f : fminf(fmaxf(v.x / S, -6.f), 6.f);
+          q[2 * e + 1] = nan ? 0.f : fminf(fmaxf(v.y / S, -6.f), 6.f);
         }
       } else {
-        const float inv = 1.f / S;
         const float2 r2 = make_float2(inv, inv), s2 = make_float2(-S, -S);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float2 q0 = mul2(v[e], r2), d = ffma2(ffma2(q0, s2, v[e]), r2, q0);
+          const float2 v = pair_to_float2<BF16>(u[e]);
+          float2 d = mul2(v, r2);
+          if (NV || !a.exact) d = ffma2(ffma2(d, s2, v), r2, d);
           q[2 * e] = d.x;
           q[2 * e + 1] = d.y;
         }
@@ -114,7 +166,7 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp4_kernel(const __grid_c
       const uint32_t s01 = __byte_perm(u[0], u[1], 0x7531), s23 = __byte_perm(u[2], u[3], 0x7531);
       const uint32_t signs = (__byte_perm(s01, s23, 0x6420) & 0x80808080u) >> 4 | (__byte_perm(s01, s23, 0x7531) & 0x80808080u);
       const uint32_t codes = floats_to_e2m1x8(q) | (nan ? 0u : signs);
-      if (lane % kLanes == 0 && cols > 0) sc_at[r % 32 * 16 + r / 32 * 4] = (uint8_t)byte;
+      if (lane % kLanes == 0 && cols > 0) sc_at[i * 4] = (uint8_t)byte;
       if (cols <= 0) continue;
       *(uint32_t*)((uint8_t*)p.codes + (long long)(row0 + r) * p.codes_row + c / 2) = codes;
       if (p.values) {
@@ -123,25 +175,18 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp4_kernel(const __grid_c
         const float f = nan ? __uint_as_float(0x7fc00000u) : S;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float2 w = mul2(mul2(__half22float2(*(const __half2*)&h[e]), make_float2(16384.f, 16384.f)), make_float2(f, f));
+          const float2 w = mul2(__half22float2(*(const __half2*)&h[e]), make_float2(f, f));
           o[e] = float2_to_pair<BF16>(w.x, w.y);
         }
-        uint16_t* to = (uint16_t*)p.values + (long long)(row0 + r) * p.values_row + c;
-        if (a.v_vec && cols >= 8) {
-          *(uint4*)to = make_uint4(o[0], o[1], o[2], o[3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (e < cols) to[e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
-        }
+        quant_store8((uint16_t*)p.values + (long long)(row0 + r) * p.values_row + c, a.v_align, cols, o);
       }
     }
   }
   __syncthreads();
-  // this CTA's blocks lie behind one another
+  // this CTA's part of its blocks, which lie behind one another
   const int b0 = blockIdx.x * kBlocks, nb = min(kBlocks, a.blocks - b0);
-  uint4* to = (uint4*)((uint8_t*)p.scales + ((long long)blockIdx.y * a.blocks + b0) * kFp4Block);
-  for (int i = threadIdx.x; i < nb * kFp4Block / 16; i += kQuantThreads) to[i] = ((const uint4*)sc)[i];
+  uint8_t* to = (uint8_t*)p.scales + ((long long)(blockIdx.y >> 2) * a.blocks + b0) * kFp4Block + part * 128;
+  if (threadIdx.x < nb * 8) ((uint4*)(to + threadIdx.x / 8 * kFp4Block))[threadIdx.x % 8] = ((const uint4*)sc)[threadIdx.x];
 }
 
 }  // namespace yk
@@ -158,7 +203,7 @@ extern "C" int yk_quant_fp4(const YkQuantFp4* p, yk_stream_t st) {
   if (!fp4_format(p->format)) return refuse(YK_EUNSUP, "quant_fp4: format must be YK_NVFP4 or YK_MXFP4");
   if (p->dtype != YK_F16 && p->dtype != YK_BF16) return refuse(YK_EUNSUP, "quant_fp4: dtype must be fp16 or bf16");
   if (p->rows < 0 || p->cols < 1) return refuse(YK_EINVAL, "quant_fp4: bad rows or cols");
-  if (p->rows > 65535 * 128 || p->cols > 1 << 30) return refuse(YK_EUNSUP, "quant_fp4: at most 8388480 rows and 2^30 columns");
+  if (p->rows > 1 << 20 || p->cols > 1 << 30) return refuse(YK_EUNSUP, "quant_fp4: at most 2^20 rows and 2^30 columns");
   if (p->scale != 0.f && !(p->scale >= 9.3132257e-10f && p->scale <= 1073741824.f))
     return refuse(YK_EINVAL, "quant_fp4: scale must be 0 or between 2^-30 and 2^30");
   if (!aligned16(p->codes) || !aligned16(p->scales) || p->codes_row % 16 || p->codes_row < (p->cols + 1ll) / 2)
@@ -169,13 +214,18 @@ extern "C" int yk_quant_fp4(const YkQuantFp4* p, yk_stream_t st) {
   if (p->rows == 0) return YK_OK;
   QuantFp4Args a{*p};
   if (a.p.scale == 0.f) a.p.scale = 1.f;
+  a.six = 6.f * a.p.scale;
+  a.over_six = 1.f / a.six;
+  a.over_scale = 1.f / a.p.scale;
+  int power;
+  a.exact = frexpf(a.p.scale, &power) == 0.5f;
   a.blocks = fp4_blocks(p->cols, p->format);
-  a.x_vec = aligned16(p->x) && p->x_row % 8 == 0;
-  a.v_vec = aligned16(p->values) && p->values_row % 8 == 0;
+  a.x_align = aligned16(p->x) && p->x_row % 8 == 0 ? 16 : 2;
+  a.v_align = aligned16(p->values) && p->values_row % 8 == 0 ? 16 : 2;
   const bool bf = p->dtype == YK_BF16, nv = p->format == YK_NVFP4;
   const auto kern = nv ? bf ? quant_fp4_kernel<true, true> : quant_fp4_kernel<false, true>
                        : bf ? quant_fp4_kernel<true, false> : quant_fp4_kernel<false, false>;
-  launch_k(kern, dim3((unsigned)((p->cols + (long long)kQuantCols - 1) / kQuantCols), (unsigned)((p->rows + 127) / 128)),
+  launch_k(kern, dim3((unsigned)((p->cols + (long long)kQuantCols - 1) / kQuantCols), (unsigned)((p->rows + 127) / 128 * 4)),
            kQuantThreads, 0, (cudaStream_t)st, a);
   note_launch();
   return check_launch("quant_fp4");

@@ -6,8 +6,7 @@ namespace yk {
 struct SampleArgs {
   YkSample p;
   int split;         // CTAs of a row: a cluster
-  int slice;         // scores of a CTA, a multiple of 8
-  int vec;           // rows allow 16-byte loads
+  int slice;         // scores of a CTA, a multiple of 256
 };
 
 // A row's scores are read once, into the shared memory of a cluster, as keys whose order is that of the
@@ -138,7 +137,9 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
   const YkSample& p = a.p;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, split = a.split;
   const int row = blockIdx.x / split, rank = split > 1 ? (int)cluster_rank() : 0;
-  const int first = rank * a.slice, size = max(0, min(a.slice, p.n - first));
+  // the row begins `lead` scores behind a 16-byte boundary; a CTA's slices begin on one, so `first` may be negative
+  const int lead = (int)((uintptr_t)((const key_t*)p.logits + row * p.row) / sizeof(key_t) % kVec);
+  const int first = rank * a.slice - lead, size = max(0, min(a.slice, p.n - first)), begin = max(0, -first);
   const auto meet = [&] { if (split > 1) cluster_barrier(); else __syncthreads(); };
   // this CTA's part to all of the row's, in turn `which`
   const auto tell = [&](int which, SampPart v) {
@@ -160,36 +161,29 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
   // ---- scores into shared memory, the largest
   uint32_t top_key = K::kNone;
   {
+    // 16 bytes a load, from the boundary before the row on: what comes before it there counts as NaN
     const key_t* from = (const key_t*)p.logits + row * p.row + first;
-    if (a.vec) {
-      constexpr int kAhead = 4;                      // loads on their way
-      for (int i0 = tid * kVec; i0 < a.slice; i0 += T * kVec * kAhead) {
-        uint4 raw[kAhead];
+    constexpr int kAhead = 4;                        // loads on their way
+    for (int i0 = tid * kVec; i0 < a.slice; i0 += T * kVec * kAhead) {
+      uint4 raw[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; j++) {
-          const int i = i0 + j * T * kVec;
-          if (i + kVec <= size) raw[j] = __ldcs((const uint4*)(from + i));
-        }
-#pragma unroll
-        for (int j = 0; j < kAhead; j++) {
-          const int i = i0 + j * T * kVec;
-          if (i >= a.slice) break;
-          key_t* k = (key_t*)&raw[j];
-          if (i + kVec > size)
-            for (int e = 0; e < kVec; e++) k[e] = i + e < size ? from[i + e] : (key_t)~0u;   // (NaN)
-#pragma unroll
-          for (int e = 0; e < kVec; e++) {
-            k[e] = (key_t)K::of(k[e]);
-            top_key = max(top_key, (uint32_t)k[e]);
-          }
-          *(uint4*)(keys + i) = raw[j];
-        }
+      for (int j = 0; j < kAhead; j++) {
+        const int i = i0 + j * T * kVec;
+        if (i >= begin && i + kVec <= size) raw[j] = __ldcs((const uint4*)(from + i));
       }
-    } else {
-      for (int i = tid; i < a.slice; i += T) {
-        const key_t k = (key_t)(i < size ? K::of(from[i]) : K::kNone);
-        top_key = max(top_key, (uint32_t)k);
-        keys[i] = k;
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) {
+        const int i = i0 + j * T * kVec;
+        if (i >= a.slice) break;
+        key_t* k = (key_t*)&raw[j];
+        if (i < begin || i + kVec > size)
+          for (int e = 0; e < kVec; e++) k[e] = i + e >= begin && i + e < size ? from[i + e] : (key_t)~0u;
+#pragma unroll
+        for (int e = 0; e < kVec; e++) {
+          k[e] = (key_t)K::of(k[e]);
+          top_key = max(top_key, (uint32_t)k[e]);
+        }
+        *(uint4*)(keys + i) = raw[j];
       }
     }
   }
@@ -882,13 +876,14 @@ template <int DT>
 static int launch_sample(SampleArgs& a, cudaStream_t st) {
   const YkSample& p = a.p;
   // CTAs of a row: as many as the SMs have room for, each with scores for two a thread; and what shared memory asks for
+  constexpr int kVec = 16 / (DT == YK_F32 ? 4 : 2);
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   a.split = 1;
   while (a.split < 8 && (p.n > kSampSlice * a.split || ((long long)p.rows * a.split * 2 <= sms && p.n >= 4096 * a.split))) a.split *= 2;
   if (g_samp_split && p.n <= kSampSlice * g_samp_split) a.split = g_samp_split;
-  a.slice = ((p.n + a.split - 1) / a.split + 255) / 256 * 256;
-  a.vec = aligned16(p.logits) && p.row % (16 / (DT == YK_F32 ? 4 : 2)) == 0;
+  const int width = p.n + (aligned16(p.logits) && p.row % kVec == 0 ? 0 : kVec - 1);   // with what may come before the row
+  a.slice = ((width + a.split - 1) / a.split + 255) / 256 * 256;
   const int smem = a.slice * (DT == YK_F32 ? 4 : 2);
   const auto kern = sample_kernel<DT>;
   if (smem_attr(kern, smem) != cudaSuccess) return check_launch("sample attr");
