@@ -459,6 +459,8 @@ int yk_test_gemm_fp4(int kernel, int split);
 // Test hook: CTAs of a row in yk_sample (1, 2, 4 or 8; 0: the library's rule, as where a row needs more).
 // Results do not depend on it; tests compare all bit for bit.
 int yk_test_sample(int split);
+// Test hook: 16-bit scores in yk_sample counted by bins of weight (1) or by place (2); 0: the library's rule.
+int yk_test_sample_kernel(int kernel);
 const char* yk_last_cuda_error(void);
 // Number of kernels this library launched since load (all devices) — a host-side counter.
 long long yk_launch_count(void);

@@ -443,6 +443,72 @@ def test_sample_special_parameters(lib, cuda):
     assert got[2] == [2000] * 6
 
 
+@pytest.fixture
+def by_place(lib, cuda):
+    """16-bit scores counted by place whatever their number, which only long rows are by themselves."""
+    ok(lib, lib.yk_test_sample_kernel(2))
+    yield
+    ok(lib, lib.yk_test_sample_kernel(0))
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("split", [1, 2, 8])
+@pytest.mark.parametrize("n", [1, 7, 1000, 5003, 40001])
+def test_sample_by_place(lib, cuda, by_place, n, split, t):
+    test_sample(lib, cuda, n, split, t)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_sample_by_place_ties(lib, cuda, by_place, t):
+    test_sample_ties(lib, cuda, t)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_sample_by_place_special_scores(lib, cuda, by_place, t):
+    test_sample_special_scores(lib, cuda, t)
+
+
+def test_sample_by_place_special_parameters(lib, cuda, by_place):
+    test_sample_special_parameters(lib, cuda)
+
+
+@pytest.mark.parametrize("scale", [0.01, 3.0, 300.0])
+def test_sample_kernels_agree(lib, cuda, scale):
+    """Bins and places give the same bits: scores around zero (both zeros among them), far from it, in strided rows."""
+    from yolo11_cu_b200 import runtime as rt
+    g = torch.Generator().manual_seed(8)
+    for dt in (torch.float16, torch.bfloat16):
+        x = torch.randn(9, 20011, generator=g) * scale
+        x[:, ::5] = 0
+        x[:, 1::10] = -0.0
+        x[3, 7:20000] = -math.inf
+        x[4, :19000] = torch.finfo(dt).min
+        x[5, 100:] = math.nan
+        x = x.to(dt).cuda()
+        kw = dict(temperature=[1.0, 0.2, 5.0] * 3, u=torch.rand(9, generator=g).tolist())
+        for more in ({}, dict(top_p=[0.9] * 9), dict(top_k=[0, 3, 4000] * 3), dict(top_k=[6000] * 9, top_p=[0.4, 0.99, 1.0] * 3, min_p=[0.0, 0.1, 0.01] * 3)):
+            runs = []
+            for kernel, split in ((1, 0), (2, 0), (2, 1), (2, 4), (2, 8)):
+                ok(lib, lib.yk_test_sample_kernel(kernel))
+                ok(lib, lib.yk_test_sample(split))
+                runs.append(run_sample(lib, rt, x[:, 2:], **kw, **more, check=False))
+            ok(lib, lib.yk_test_sample_kernel(0))
+            ok(lib, lib.yk_test_sample(0))
+            assert all(r == runs[0] for r in runs), more
+
+
+def test_sample_counts_of_one_place(lib, cuda):
+    """As many equal scores as a CTA can have: a 16-bit count by place stays in its half of a word."""
+    from yolo11_cu_b200 import runtime as rt
+    for n in (64000, 128000, 262144):
+        x = torch.zeros(2, n, dtype=torch.bfloat16, device="cuda")
+        x[1] = 1.0078125                          # (an odd place: the upper half)
+        for kw in (dict(top_k=[n - 1] * 2), dict(top_p=[0.75] * 2)):
+            got = run_sample(lib, rt, x, u=[0.5] * 2, check=False, **kw)
+            stay = n - 1 if "top_k" in kw else math.ceil(0.75 * n)
+            assert got[2] == [stay] * 2 and got[0] == [stay // 2] * 2
+
+
 def test_sample_long_rows(lib, cuda):
     from yolo11_cu_b200 import runtime as rt
     g = torch.Generator().manual_seed(9)

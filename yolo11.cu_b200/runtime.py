@@ -189,6 +189,7 @@ _SIGS = {
     "yk_test_attn_kv8": (C.c_int, [C.c_int]),
     "yk_test_gemm_fp4": (C.c_int, [C.c_int, C.c_int]),
     "yk_test_sample": (C.c_int, [C.c_int]),
+    "yk_test_sample_kernel": (C.c_int, [C.c_int]),
     "yk_last_cuda_error": (C.c_char_p, []),
     "yk_launch_count": (C.c_longlong, []),
     # engine ABI (include/yolo.h)
