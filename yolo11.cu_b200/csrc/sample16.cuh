@@ -10,15 +10,16 @@ namespace yk {
 //  * The warps of the row's cluster sum the places in reach of the largest score (2^-46 of its weight) in steps of 256,
 //    over the counts of all CTAs, and tell all CTAs.
 //  * Each CTA finds the step that holds a border, and goes through its places.
-//  * Each CTA sums what stays of its own scores, and the one that holds the token reads its scores once more: first
-//    by warp, then the run of the warp that it is in.  Weights come from a table there, if the places that stay are
-//    fewer than kSamp16Table.
+//  * Each CTA sums what stays of its own scores over the places that stay, which fills a table of their weights; the CTA
+//    that holds the token then reads its scores once more, by warp.  Where more places stay than the table holds (scores
+//    of both signs, for most magnitudes lie near 0), or without a limit, a CTA sums them score by score and by warp at once.
 // An addition in shared memory takes a warp about 5 clocks, an exact weight about 50.  64 rows of 128000: 31 us (0.5 TB/s;
 // by bins, with an exact weight for each score, 62), of which the counts take 5, the sums by step 6, a border 3, the pass
-// through the token's CTA 7; the rest are some ten waits of the whole cluster or CTA for one another.
+// through the token's CTA 7; the rest are some ten waits of the whole cluster or CTA for one another.  47 us if a row keeps
+// scores of both signs; 35 without limits.
 constexpr int kSamp16Slice = 64000;             // scores of a CTA at most: a count stays below 2^16
 constexpr int kSamp16Threads = 1024;
-constexpr int kSamp16Table = 8192;
+constexpr int kSamp16Table = 11264;            // places that stay, and one for all others
 constexpr int kSamp16Smem = 65536 * 2 + kSamp16Table * 8;
 
 
@@ -89,10 +90,17 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
     asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(below) : "r"(w));
     return w ^ (0x7fff7fffu & ~below);
   };
+  // the place of one of eight scores
+  const auto place_of = [&](const uint4& raw, int e) {
+    const uint32_t place = places(((const uint32_t*)&raw)[e >> 1]) >> (e & 1) * 16 & 0xffffu;
+    return place - (place == 0x8000u);
+  };
   // parameters, on their way meanwhile
   const float temperature = p.temperature ? p.temperature[row] : 1.f, u = p.u ? p.u[row] : 0.f;
   const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
   int top_k = p.top_k ? p.top_k[row] : 0;
+  if (top_k <= 0 || top_k >= p.n) top_k = 0;
+  const bool by_p = top_p < 1.f, limits = top_k || by_p;
 
   // ---- counts by place, the largest key
   uint32_t largest = DT == YK_BF16 ? 0xff80ff80u : 0xfc00fc00u;      // -infinity twice
@@ -109,6 +117,7 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
         const uint32_t w = ((const uint32_t*)&raw[j])[e], q = places(w);
         if (DT == YK_BF16) asm("max.bf16x2 %0, %1, %2;" : "=r"(largest) : "r"(largest), "r"(w));
         else asm("max.f16x2 %0, %1, %2;" : "=r"(largest) : "r"(largest), "r"(w));
+        if (!limits) continue;
         atomicAdd((uint32_t*)(samp_raw + (q & 0xfffeu) * 2), q & 1 ? 0x10000u : 1u);
         atomicAdd((uint32_t*)(samp_raw + (q >> 17) * 4), q & 0x10000u ? 0x10000u : 1u);
       }
@@ -159,8 +168,6 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
   };
   const int top_place = 65535 - (int)top_key;
   const u64 least = min_p > 0.f ? min((u64)ceil(fmin((double)min_p, 1.0) * kSampOne), weight(top_place)) : 1ull;
-  const bool by_p = top_p < 1.f;
-  if (top_k <= 0 || top_k >= p.n) top_k = 0;
   // places from `end` on have no weight: scores more than 46 ln 2 temperatures below the top
   int end = top_place + 1;
   if (top < INFINITY) {
@@ -172,7 +179,7 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
   // Places before `cut` stay, and of the scores at it the first `take`.
   int cut = end;
   uint32_t take = 0;
-  if (top_k || by_p) {
+  if (limits) {
     // sums by step of kStep places, from a multiple of 8 on, each by one warp of the row's
     const int start = top_place & ~7, steps = (end - start + kStep - 1) / kStep;
 #pragma unroll 1
@@ -316,18 +323,43 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
   // ---- what stays of this CTA's scores, by place
   const u64 cut_w = take ? weight(cut) : 0;
   if (cut_w < least) take = 0;
-  const bool listed = cut - top_place < kSamp16Table;
+  const uint32_t kept = cut - top_place, cut_place = take ? cut : ~0u;
+  const int run = a.slice / kWarps, run_from = warp * run, run_to = min(size, run_from + run);   // of consecutive scores, a warp's
+  const auto weight_at = [&](uint32_t place) {  // 0 at the cut
+    const u64 w = place - (uint32_t)top_place < kept ? weight((int)place) : 0;
+    return w < least ? 0 : w;
+  };
+  const bool listed = limits && kept < kSamp16Table;
   u64 mass = 0;
-  uint32_t count = 0;
-  for (int i0 = top_place; i0 <= cut; i0 += T) {
-    const int i = i0 + tid;
-    const uint32_t c = i < cut ? count_at(i) : 0;
-    u64 w = 0;
-    if (__any_sync(~0u, c != 0 || i == 0x8000)) w = weight(min(i, 65535));   // (0x8000: -0, counted at 0)
-    if (w < least) w = 0;
-    if (listed && i <= cut) found_weight[i - top_place] = i < cut ? w : 0;   // (the last one: all that do not stay)
-    mass += c * w;
-    count += w ? c : 0;
+  uint32_t count = 0, ties = 0;
+  if (listed) {
+    for (int i0 = top_place; i0 <= cut; i0 += T) {
+      const int i = i0 + tid;
+      const uint32_t c = i < cut ? count_at(i) : 0;
+      u64 w = 0;
+      if (__any_sync(~0u, c != 0)) w = weight(min(i, 65535));
+      if (w < least) w = 0;
+      if (i <= cut) found_weight[i - top_place] = i < cut ? w : 0;   // (the last one: all others)
+      mass += c * w;
+      count += w ? c : 0;
+    }
+  } else {
+    // without a limit, or where too many places stay for the table: each score by itself
+#pragma unroll 1
+    for (int i = run_from + lane * 8; i < run_to; i += 256) {
+      const uint4 raw = load8(i);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const uint32_t place = place_of(raw, e);
+        u64 w = weights.of(K::value(65535u - place), table);
+        if (place - (uint32_t)top_place >= kept || w < least) w = 0;
+        mass += w;
+        count += w != 0;
+        ties += place == cut_place;
+      }
+    }
+    ties = __reduce_add_sync(~0u, ties);
+    if (lane == 0) warp_a[warp] = ties;
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(~0u, mass, o);
@@ -359,55 +391,34 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
   u64 target = u > 0.f ? (u64)fmin((double)u * (double)total, 9e18) : 0;
   target = min(target, total - 1);
   if (target < at || target - at >= mine) return;   // another CTA's
-  // weight of a score by its place, but for those at the cut
-  const uint32_t kept = cut - top_place;
-  const auto weight_at = [&](uint32_t place) {
-    const u64 w = place - top_place < kept ? weight((int)place) : 0;
-    return w < least ? 0 : w;
-  };
-  const uint32_t cut_place = take ? cut : ~0u;
-  // ---- by warp: a warp has a run of consecutive scores
-  const int run = a.slice / kWarps;             // (a multiple of 8)
-  {
-    u64 sum = 0;
-    uint32_t ties = 0;
-    const int run_end = min(size, (warp + 1) * run);
+  // ---- by warp
+  if (listed) {
+    mass = 0;
 #pragma unroll 1
-    for (int i0 = warp * run + lane * 8; i0 < run_end; i0 += 512) {
+    for (int i0 = run_from + lane * 8; i0 < run_to; i0 += 512) {
       uint4 raw[2];
 #pragma unroll
-      for (int j = 0; j < 2; j++) raw[j] = i0 + j * 256 < run_end ? load8(i0 + j * 256) : make_uint4(~0u, ~0u, ~0u, ~0u);
-      const auto place_of = [&](int e) {
-        const uint32_t place = places(((const uint32_t*)&raw[e >> 3])[e >> 1 & 3]) >> (e & 1) * 16 & 0xffffu;
-        return place - (place == 0x8000u);
-      };
-      if (listed) {
+      for (int j = 0; j < 2; j++) raw[j] = i0 + j * 256 < run_to ? load8(i0 + j * 256) : make_uint4(~0u, ~0u, ~0u, ~0u);
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const uint32_t place = place_of(e);
-          sum += found_weight[min(place - top_place, kept)];
-          ties += place == cut_place;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const uint32_t place = place_of(e);
-          sum += weight_at(place);
-          ties += place == cut_place;
-        }
+      for (int e = 0; e < 16; e++) {
+        const uint32_t place = place_of(raw[e >> 3], e & 7);
+        mass += found_weight[min(place - top_place, kept)];
+        ties += place == cut_place;
       }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(~0u, mass, o);
     ties = __reduce_add_sync(~0u, ties);
     __syncthreads();
     if (lane == 0) {
-      warp_mass[warp] = sum;
+      warp_mass[warp] = mass;
       warp_a[warp] = ties;
     }
     __syncthreads();
   }
-  uint32_t ties = warp_a[lane], tie_before = ties;
+  // lane i: warp i's
+  ties = warp_a[lane];
+  uint32_t tie_before = ties;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t b = __shfl_up_sync(~0u, tie_before, o);
@@ -433,7 +444,7 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
     const uint32_t k = i >= begin && i < run_end ? K::of(scores[first + i]) : K::kNone, place = 65535u - k;
     const bool same = place == cut_place;
     const uint32_t sames = __ballot_sync(~0u, same);
-    u64 w = listed ? found_weight[min(place - top_place, kept)] : weight_at(place);
+    u64 w = weight_at(place);
     __syncthreads();                            // the last turn's sums have been read
     if (lane == 0) warp_b[warp] = __popc(sames);
     __syncthreads();
