@@ -336,7 +336,7 @@ int yk_gemv4(const YkGemv4* p, yk_stream_t st);
 // the angle pos[axis of i][n] * freqs[i]: (a, b) -> (a cos - b sin, b cos + a sin), rounded once to dtype.
 // The pair is channels (i, i + rot/2), or (2i, 2i + 1) if interleaved; channels from rot on do not turn.
 // The first sections[0] pairs follow axis 0, the next sections[1] axis 1, and so on (time, row, column of
-// an image's tokens).  Angles are products in 64 bits, so far positions lose nothing.  Rows whose pos on
+// an image's tokens).  Whole turns are taken off in 64 bits, so far positions lose nothing.  Rows whose pos on
 // axis 0 is negative are left as they are.  Outputs may be the inputs themselves.
 typedef struct {
   const void* q;           // head h of row n at n*q_row + h*dim; fp16 or bf16, 16-byte aligned
@@ -346,7 +346,7 @@ typedef struct {
   const void* q_weight;    // [dim] of dtype, or NULL: no norm
   const void* k_weight;
   const int* pos;          // axis a of row n at a*pos_axis + n
-  const float* freqs;      // [rot / 2] radians a position
+  const float* freqs;      // [rot / 2] radians a position, finite
   long long q_row, k_row, q_out_row, k_out_row;   // elements, multiples of 8
   long long pos_axis;
   int rows;

@@ -571,3 +571,66 @@ def test_captured_and_on_another_stream(lib, cuda):
     side.synchronize()
     for a, b in zip((qkv, y, token, lp), want[2]):
         assert torch.equal(a, b)
+
+
+def test_two_graphs_at_once(lib, cuda):
+    """Two captured graphs of the large forms (whole tiles by pairs, split columns, scores by place and by bin, rows in
+    several turns) replayed side by side on two streams: what each gives alone."""
+    from yolo11_cu_b200 import runtime as rt
+    gen = torch.Generator().manual_seed(12)
+    new = lambda *s, dtype=torch.half: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+
+    def program(m, n, k):
+        qkv = torch.randn(4000, 24, 64, generator=gen).half().cuda()
+        out, pos, freqs = torch.zeros_like(qkv), torch.arange(4000, dtype=torch.int32, device="cuda"), torch.rand(32, generator=gen).cuda()
+        x, codes, scales = torch.randn(m, k, generator=gen).half().cuda(), new(m, k // 2, dtype=torch.uint8), \
+            new(lib.yk_fp4_scale_bytes(m, k, 0), dtype=torch.uint8)
+        w, y, small = random_matrix(n, k, 0, gen, torch.half, 0.1), new(m, n), new(8, n)
+        logits, u = torch.randn(9, 40000, generator=gen).half().cuda(), torch.rand(9, generator=gen).cuda()
+        top_p = torch.full((9,), 0.9, device="cuda")
+        token, other = new(9, dtype=torch.int32), new(9, dtype=torch.int32)
+        rot = rt.YkQkRotate(q=qkv.data_ptr(), k=qkv.data_ptr() + 2 * 64 * 16, q_out=out.data_ptr(), k_out=out.data_ptr() + 2 * 64 * 16,
+                            pos=pos.data_ptr(), freqs=freqs.data_ptr(), q_row=24 * 64, k_row=24 * 64, q_out_row=24 * 64, k_out_row=24 * 64,
+                            rows=4000, heads=16, kv_heads=8, dim=64, rot=64, axes=1)
+        qu = rt.YkQuantFp4(x=x.data_ptr(), codes=codes.data_ptr(), scales=scales.data_ptr(), x_row=k, codes_row=k // 2, rows=m, cols=k)
+        ge = [rt.YkGemmFp4(x=codes.data_ptr(), xscale=scales.data_ptr(), w=w[0].data_ptr(), wscale=w[1].data_ptr(), y=o.data_ptr(),
+                           x_row=k // 2, w_row=w[0].stride(0), y_row=n, rows=len(o), n=n, k=k) for o in (y, small)]
+        sa = [rt.YkSample(logits=logits.data_ptr(), u=u.data_ptr(), top_p=top_p.data_ptr(), token=o.data_ptr(), row=40000, rows=9, n=c)
+              for o, c in ((token, 40000), (other, 20000))]
+
+        def step():
+            ok(lib, lib.yk_qk_rotate(C.byref(rot), stream()))
+            ok(lib, lib.yk_quant_fp4(C.byref(qu), stream()))
+            for a in ge:
+                ok(lib, lib.yk_gemm_fp4(C.byref(a), stream()))
+            for a, kernel in zip(sa, (2, 1)):
+                ok(lib, lib.yk_test_sample_kernel(kernel))
+                ok(lib, lib.yk_sample(C.byref(a), stream()))
+            ok(lib, lib.yk_test_sample_kernel(0))
+
+        return step, (out, codes, scales, y, small, token, other), (qkv, x, w, logits, u, top_p, pos, freqs, rot, qu, ge, sa)
+
+    graphs, wants, outs, keep = [], [], [], []
+    for size in ((600, 5000, 1024), (1300, 2100, 2016)):
+        step, out, held = program(*size)
+        step()
+        torch.cuda.synchronize()
+        wants.append([o.clone() for o in out])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        graphs.append(graph)
+        outs.append(out)
+        keep.append((step, held))
+    for o in outs[0] + outs[1]:
+        o.zero_()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for out, want in zip(outs, wants):
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)

@@ -1,5 +1,5 @@
-// Helpers shared by the text-decoder operators (kv.cu, attn8.cu, norm8.cu, gemv4.cu): e4m3
-// conversion, 16-bit type selection, refusals with a reason.
+// Helpers shared by the text-decoder operators (kv.cu, attn8.cu, norm8.cu, gemv4.cu, rotate.cu,
+// quant_fp4.cu, gemm_fp4.cu, sample.cu): e4m3 conversion, 16-bit type selection, refusals with a reason.
 #pragma once
 #include <cuda_bf16.h>
 
