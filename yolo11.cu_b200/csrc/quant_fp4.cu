@@ -23,10 +23,17 @@ struct QuantFp4Args {
 //  * r comes from the 8 fractions that an e4m3 scale can have, times the matrix's scale, in a table; powers of two
 //    move its exponent.  Where S is a power of two, the product alone is exact.
 // Groups with infinities or NaN, tiny or clamped scales divide plainly.
-// 12000 x 5120 to codes, scales and values: 57 us, 4.9 TB/s (63 with a division and a byte store for each group); 190
-// instructions for a lane's 8 elements keep the issue slots 74 % busy.  16 x 4096: 2.8 us, the launch.
+// 12000 x 5120 to codes, scales and values: 55 us, 5.1 TB/s (63 with a division and a byte store for each group; the same
+// loads and stores without arithmetic 42.5, without that of the values 49; 4 or 6 CTAs an SM instead of 5 take 2 us more).
+// 16 x 4096: 2.8 us, the launch.
 constexpr int kQuantCols = 256, kQuantThreads = 256;
 
+__device__ __forceinline__ float2 quant_mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 // Eight 16-bit elements (two where there are fewer columns) at any even address, as pairs.
 __device__ __forceinline__ uint4 quant_load8(const uint16_t* x, int align, int cols, bool first) {
   uint4 v = make_uint4(0, 0, 0, 0);
@@ -70,8 +77,34 @@ __device__ __forceinline__ void quant_store8(uint16_t* y, int align, int cols, c
   }
 }
 
+// The rare cases, out of line so that the others' code stays together: the largest finite |x| of a group's eight, and the
+// codes (without signs) by division, 0 in a group with a NaN.
+template <bool BF16>
+__device__ __noinline__ float quant_finite_max(uint4 raw) {
+  const uint32_t* u = (const uint32_t*)&raw;
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float2 v = pair_to_float2<BF16>(u[e]);
+    m = fmaxf(m, fmaxf(finite_abs(v.x), finite_abs(v.y)));
+  }
+  return m;
+}
+template <bool BF16>
+__device__ __noinline__ uint32_t quant_plain(uint4 raw, float S, bool nan) {
+  const uint32_t* u = (const uint32_t*)&raw;
+  float q[8];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float2 v = pair_to_float2<BF16>(u[e]);
+    q[2 * e] = nan ? 0.f : fminf(fmaxf(v.x / S, -6.f), 6.f);
+    q[2 * e + 1] = nan ? 0.f : fminf(fmaxf(v.y / S, -6.f), 6.f);
+  }
+  return floats_to_e2m1x8(q);
+}
+
 template <bool BF16, bool NV>
-__global__ void __launch_bounds__(kQuantThreads) quant_fp4_kernel(const __grid_constant__ QuantFp4Args a) {
+__global__ void __launch_bounds__(kQuantThreads, 5) quant_fp4_kernel(const __grid_constant__ QuantFp4Args a) {
   constexpr int kLanes = NV ? 2 : 4;                 // of a group
   constexpr int kBlocks = NV ? 4 : 2;                // scale blocks of 256 columns
   constexpr int kRows = 4;                           // of a warp
@@ -114,12 +147,7 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp4_kernel(const __grid_c
       float amax = elem_to_float<BF16>((uint16_t)top);
       const bool odd = !(amax < INFINITY), nan = amax != amax;
       if (__any_sync(~0u, odd)) {                    // rare: finite values only
-        float m = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float2 v = pair_to_float2<BF16>(u[e]);
-          m = fmaxf(m, fmaxf(finite_abs(v.x), finite_abs(v.y)));
-        }
+        float m = quant_finite_max<BF16>(raw[i]);
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
         amax = m;
@@ -145,29 +173,26 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp4_kernel(const __grid_c
       }
       if (nan) byte = NV ? 0x7fu : 0xffu;
       plain |= S < 8.6736174e-19f;                   // 2^-60: the remainder below would lose bits
-      float q[8];
+      uint32_t codes;
       if (plain) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float2 v = pair_to_float2<BF16>(u[e]);
-          q[2 * e] = nan ? 0.f : fminf(fmaxf(v.x / S, -6.f), 6.f);
-          q[2 * e + 1] = nan ? 0.f : fminf(fmaxf(v.y / S, -6.f), 6.f);
-        }
+        codes = quant_plain<BF16>(raw[i], S, nan);
       } else {
+        float q[8];
         const float2 r2 = make_float2(inv, inv), s2 = make_float2(-S, -S);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const float2 v = pair_to_float2<BF16>(u[e]);
-          float2 d = mul2(v, r2);
+          float2 d = quant_mul2(v, r2);
           if (NV || !a.exact) d = ffma2(ffma2(d, s2, v), r2, d);
           q[2 * e] = d.x;
           q[2 * e + 1] = d.y;
         }
+        codes = floats_to_e2m1x8(q);
       }
       // signs come from x itself: those of zeros and of quotients that underflow would be lost
       const uint32_t s01 = __byte_perm(u[0], u[1], 0x7531), s23 = __byte_perm(u[2], u[3], 0x7531);
       const uint32_t signs = (__byte_perm(s01, s23, 0x6420) & 0x80808080u) >> 4 | (__byte_perm(s01, s23, 0x7531) & 0x80808080u);
-      const uint32_t codes = floats_to_e2m1x8(q) | (nan ? 0u : signs);
+      codes |= nan ? 0u : signs;
       if (lane % kLanes == 0 && cols > 0) sc_at[i * 4] = (uint8_t)byte;
       if (cols <= 0) continue;
       *(uint32_t*)((uint8_t*)p.codes + (long long)(row0 + r) * p.codes_row + c / 2) = codes;
@@ -177,7 +202,7 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp4_kernel(const __grid_c
         const float f = nan ? __uint_as_float(0x7fc00000u) : S;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float2 w = mul2(__half22float2(*(const __half2*)&h[e]), make_float2(f, f));
+          const float2 w = quant_mul2(__half22float2(*(const __half2*)&h[e]), make_float2(f, f));
           o[e] = float2_to_pair<BF16>(w.x, w.y);
         }
         quant_store8((uint16_t*)p.values + (long long)(row0 + r) * p.values_row + c, a.v_align, cols, o);
