@@ -94,3 +94,10 @@ def test_hooks_refuse(lib):
     assert lib.yk_test_gemm_fp4(3, 0) == EINVAL and lib.yk_test_gemm_fp4(1, 3) == EINVAL
     assert lib.yk_test_sample(16) == EINVAL and lib.yk_test_sample(-1) == EINVAL
     assert lib.yk_test_gemm_fp4(0, 0) == 0 and lib.yk_test_sample(0) == 0
+
+
+def test_kernel_hook_of_sampling():
+    from yolo11_cu_b200 import runtime as rt
+    lib = rt.load()
+    assert lib.yk_test_sample_kernel(-1) == EINVAL and lib.yk_test_sample_kernel(3) == EINVAL
+    assert lib.yk_test_sample_kernel(2) == 0 and lib.yk_test_sample_kernel(0) == 0

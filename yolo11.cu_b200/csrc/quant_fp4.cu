@@ -23,8 +23,9 @@ struct QuantFp4Args {
 //  * r comes from the 8 fractions that an e4m3 scale can have, times the matrix's scale, in a table; powers of two
 //    move its exponent.  Where S is a power of two, the product alone is exact.
 // Groups with infinities or NaN, tiny or clamped scales divide plainly.
-// 12000 x 5120 to codes, scales and values: 55 us, 5.1 TB/s (63 with a division and a byte store for each group; the same
-// loads and stores without arithmetic 42.5, without that of the values 49; 4 or 6 CTAs an SM instead of 5 take 2 us more).
+// 12000 x 5120 to codes, scales and values: 53 us back to back, 5.2 TB/s, 57 with inputs that change (63 with a division and a
+// byte store for each group; the same loads and stores without arithmetic 42.5, without that of the values 49; 4 or 6 CTAs
+// an SM instead of 5 take 2 us more).
 // 16 x 4096: 2.8 us, the launch.
 constexpr int kQuantCols = 256, kQuantThreads = 256;
 

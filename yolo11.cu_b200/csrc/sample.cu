@@ -66,6 +66,12 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
   pdl_wait();
   pdl_trigger();
 
+  // parameters, on their way meanwhile
+  const float temperature = p.temperature ? p.temperature[row] : 1.f, u = p.u ? p.u[row] : 0.f;
+  const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
+  int top_k = p.top_k ? p.top_k[row] : 0;
+  if (top_k <= 0 || top_k >= p.n) top_k = 0;
+
   // ---- scores into shared memory, the largest
   uint32_t top_key = K::kNone;
   {
@@ -104,7 +110,6 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
   };
   tell(0, {0, 0, block_max(top_key), 0});
   for (int i = 0; i < split; i++) top_key = max(top_key, part[0][i].count);
-  const float temperature = p.temperature ? p.temperature[row] : 1.f;
   const bool greedy = !(temperature > 0.f) || !p.u;
   const bool any = top_key > K::kNone;
   if (!any || greedy) {
@@ -127,11 +132,8 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
   SampWeights weights;
   weights.set(top, temperature);
   const auto weight = [&](uint32_t k) { return weights.of(K::value(k), table); };
-  const u64 least = p.min_p && p.min_p[row] > 0.f ? min((u64)ceil(fmin((double)p.min_p[row], 1.0) * kSampOne), weight(top_key)) : 1ull;
-  const float top_p = p.top_p ? p.top_p[row] : 1.f;
+  const u64 least = min_p > 0.f ? min((u64)ceil(fmin((double)min_p, 1.0) * kSampOne), weight(top_key)) : 1ull;
   const bool by_p = top_p < 1.f;
-  int top_k = p.top_k ? p.top_k[row] : 0;
-  if (top_k <= 0 || top_k >= p.n) top_k = 0;
 
   // Keys above `cut` stay, and of those that equal it the first `take`.
   uint32_t cut = K::kNone, take = 0;
@@ -170,8 +172,11 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
       for (int i = tid; i < (by_p ? 2 : 1) * share; i += T) {
         const int b = i < share ? rank * share + i : kSampBins + rank * share + i - share;
         const uint32_t at = smem_u32(&hist[b]);
-        uint32_t v = 0;
-        for (int q = 0; q < split; q++) v += ld_cluster_u32(cluster_map(at, q));
+        uint32_t v = 0, part_of[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) part_of[q] = q < split ? ld_cluster_u32(cluster_map(at, q)) : 0;   // (on their way together)
+#pragma unroll
+        for (int q = 0; q < 8; q++) v += part_of[q];
         for (int q = 0; q < split; q++) st_cluster_u32(cluster_map(at, q), v);
       }
       meet();
@@ -709,7 +714,6 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
     all += part[1][q].count + stay;
     ties_at += part[1][q].ties;
   }
-  const float u = p.u[row];
   unsigned long long target = u > 0.f ? (unsigned long long)fmin((double)u * (double)total, 9e18) : 0;
   target = min(target, total - 1);
   // the first score at which the sum passes the target: its warp, then itself
