@@ -404,7 +404,7 @@ typedef struct {
   const void* w2scale;
   const float* bias;       // [n] or NULL; not with w2
   void* y;                 // [rows][y_row]
-  long long x_row, w_row;  // bytes, multiples of 16
+  long long x_row, w_row;  // bytes, multiples of 16 (of 128: up to a fifth faster)
   long long y_row;         // elements
   int rows, n, k;
   int format;              // YK_NVFP4 or YK_MXFP4

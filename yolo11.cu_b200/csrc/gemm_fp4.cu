@@ -55,7 +55,8 @@ __device__ __forceinline__ void fp4_put_scales(uint32_t taddr, const uint32_t* v
 // may begin.
 // 2048 x 8192 x 8192: 55 us in a burst (5.0 PFLOP/s; 66 us back to back for long, at the power limit's clocks).  The MMAs
 // take 550 of at least 512 cycles a stage; 256 tiles on 74 pairs are 3.5 rounds, of which the last half runs on half the
-// SMs, and one epilogue stands alone.  Gated 777 x 11000 x 4000: 45 and 51 us, 301 tiles, each with the epilogue of two.
+// SMs, and one epilogue stands alone.  Gated 1024 x 9472 x 4096: 31 us (5.1 PFLOP/s); 777 x 11000 x 4000: 45 us, as rows of
+// 2000 bytes put each 128-byte piece of a row into two L2 lines (37 us for 4096 columns) and 9 rows take a quarter of the tiles.
 constexpr int kFp4PairThreads = 576;
 template <bool NV>
 struct Fp4Pair {

@@ -58,7 +58,7 @@ class Fp4:
 
     def __init__(self, lib, rows, cols, fmt, device, scale=1.0):
         self.rows, self.cols, self.fmt, self.scale = rows, cols, fmt, scale
-        self.codes = torch.zeros(rows, -(-cols // 32) * 16, dtype=torch.uint8, device=device)
+        self.codes = torch.zeros(rows, -(-cols // 256) * 128, dtype=torch.uint8, device=device)   # (rows on L2 lines)
         self.scales = torch.zeros(lib.yk_fp4_scale_bytes(rows, cols, fmt), dtype=torch.uint8, device=device)
 
     def fill(self, lib, x, n, cols=None):
