@@ -22,7 +22,8 @@ struct QuantFp4Args {
 //    a / b does, so that values halfway between two codes go the way that the definition says.
 //  * r comes from the 8 fractions that an e4m3 scale can have, times the matrix's scale, in a table; powers of two
 //    move its exponent.  Where S is a power of two, the product alone is exact.
-// Groups with infinities or NaN, tiny or clamped scales divide plainly.
+// Groups with infinities or NaN, tiny or clamped scales divide plainly; groups of zeros, which edges are full of, do not (460 x 429
+// MXFP4: 10.9 -> 5.2 us).
 // 12000 x 5120 to codes, scales and values: 53 us back to back, 5.2 TB/s, 57 with inputs that change (63 with a division and a
 // byte store for each group; the same loads and stores without arithmetic 42.5, without that of the values 49; 4 or 6 CTAs
 // an SM instead of 5 take 2 us more).
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(kQuantThreads, 5) quant_fp4_kernel(const __gri
         inv = __uint_as_float(__float_as_uint(a.over_scale) - k * 0x800000);
       }
       if (nan) byte = NV ? 0x7fu : 0xffu;
-      plain |= S < 8.6736174e-19f;                   // 2^-60: the remainder below would lose bits
+      plain |= S < 8.6736174e-19f && amax > 0.f;     // 2^-60: the remainder below would lose bits
       uint32_t codes;
       if (plain) {
         codes = quant_plain<BF16>(raw[i], S, nan);
