@@ -43,12 +43,16 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
   __shared__ uint32_t border_key[5];
   __shared__ uint32_t found_bin, found_above, found_first, found_last, own_n;
   const YkSample& p = a.p;
+  if (a.split > 1) cluster_arrive();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, split = a.split;
   const int row = blockIdx.x / split, rank = split > 1 ? (int)cluster_rank() : 0;
   // the row begins `lead` scores behind a 16-byte boundary; a CTA's slices begin on one, so `first` may be negative
   const int lead = (int)((uintptr_t)((const key_t*)p.logits + row * p.row) / sizeof(key_t) % kVec);
   const int first = rank * a.slice - lead, size = max(0, min(a.slice, p.n - first)), begin = max(0, -first);
-  const auto meet = [&] { if (split > 1) cluster_barrier(); else __syncthreads(); };
+  const auto meet = [&] {
+    __syncwarp();                                    // (the cluster's barrier takes whole warps)
+    if (split > 1) cluster_barrier(); else __syncthreads();
+  };
   // this CTA's part to all of the row's, in turn `which`
   const auto tell = [&](int which, SampPart v) {
     if (tid < split) {
@@ -108,7 +112,12 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
     __syncthreads();
     return __reduce_max_sync(~0u, lane < kWarps ? warp_a[lane] : 0);
   };
-  tell(0, {0, 0, block_max(top_key), 0});
+  top_key = block_max(top_key);
+  if (split > 1) {                                   // every CTA of the row has started: its shared memory may be written
+    __syncwarp();
+    cluster_wait();
+  }
+  tell(0, {0, 0, top_key, 0});
   for (int i = 0; i < split; i++) top_key = max(top_key, part[0][i].count);
   const bool greedy = !(temperature > 0.f) || !p.u;
   const bool any = top_key > K::kNone;

@@ -50,13 +50,17 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
   __shared__ u64 found_mass;
   __shared__ uint32_t found_place, found_take;
   const YkSample& p = a.p;
+  if (a.split > 1) cluster_arrive();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, split = a.split;
   const int row = blockIdx.x / split, rank = split > 1 ? (int)cluster_rank() : 0;
   // the row begins `lead` scores behind a 16-byte boundary; a CTA's slices begin on one, so `first` may be negative
   const uint16_t* const scores = (const uint16_t*)p.logits + row * p.row;
   const int lead = (int)((uintptr_t)scores / 2 % 8);
   const int first = rank * a.slice - lead, size = max(0, min(a.slice, p.n - first)), begin = max(0, -first);
-  const auto meet = [&] { if (split > 1) cluster_barrier(); else __syncthreads(); };
+  const auto meet = [&] {
+    __syncwarp();                               // (the cluster's barrier takes whole warps)
+    if (split > 1) cluster_barrier(); else __syncthreads();
+  };
   const auto tell = [&](int which, SampPart v) {
     if (tid < split) {
       const uint32_t to = smem_u32(&part[which][rank]), at = split > 1 ? cluster_map(to, tid) : to;
@@ -135,6 +139,10 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
   if (tid == 0) {                               // both zeros at one place
     counts[0x3fff] += counts[0x4000] << 16;
     counts[0x4000] &= 0xffff0000u;
+  }
+  if (split > 1) {                              // every CTA of the row has started: its shared memory may be written
+    __syncwarp();
+    cluster_wait();
   }
   tell(0, {0, 0, top_key, 0});
   for (int i = 0; i < split; i++) top_key = max(top_key, part[0][i].count);
