@@ -48,6 +48,23 @@ def lib(pkg):
     return runtime.load()
 
 
+def release_hooks(lib):
+    """The library's own rules again, whatever a test forced (yk_test_inject, which takes a GPU, is its test's own to release)."""
+    lib.yk_test_nms_cluster(0)
+    lib.yk_test_attn_kv8(0)
+    lib.yk_test_gemm_fp4(0, 0)
+    lib.yk_test_sample(0)
+    lib.yk_test_sample_kernel(0)
+
+
+@pytest.fixture(autouse=True)
+def hooks_end_with_their_test():
+    yield
+    from yolo11_cu_b200 import runtime
+    if runtime._lib is not None:
+        release_hooks(runtime._lib)
+
+
 @pytest.fixture(scope="session")
 def cuda():
     import torch
