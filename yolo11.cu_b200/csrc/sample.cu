@@ -11,9 +11,9 @@ namespace yk {
 //    within 10^-4: the bins in which the sum may reach top_p.
 //  * One pass adds up the exact weights of all others, and lists the scores of those bins (some hundreds).
 //  * Every CTA sorts the list and finds both borders in it.
-//  * Where the list would be too long (thousands of equal scores, temperature infinity) the borders are
-//    found digit by digit of the key instead: sums by digit of the keys that share the digits so far, two or
-//    three turns a border.
+//  * Where the list would be too long (thousands of equal scores), or a temperature so high that the ends of the floats weigh
+//    alike (infinity), the borders are found digit by digit of the key instead: sums by digit of the keys that share the
+//    digits so far, two or three turns a border.
 // A chain of some twelve stages of 1 to 4 us, each the wait of a cluster for its slowest CTA: 1 x 32000 15 us; 200 x 151000
 // of fp32 183 us, 5.4 rounds of two CTAs an SM (12 % of the copy rate; issue slots 55 % busy).
 constexpr int kSampSlice = 32768;          // scores of a CTA at most
@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
   };
   const auto bin_of = [&](uint32_t k) { return (int)(place(k) >> 8); };
   bool open = top_k || by_p;                         // borders to find
-  if (open && top < INFINITY) {
+  // (bins take differences of floats and count -infinity, the padding's too, as a score far below: not at flat temperatures)
+  if (open && top < INFINITY && weights.steep()) {
     // ---- counts by bin
     for (int i = tid * kVec; i < a.slice; i += T * kVec) {     // (keys behind the last score are kNone: beyond the bins)
       const uint4 raw = *(const uint4*)(keys + i);

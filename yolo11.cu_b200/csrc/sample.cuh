@@ -86,6 +86,9 @@ struct SampWeights {
     const unsigned long long v = (unsigned long long)__double_as_longlong(fma(s, p, s) + 4503599627370496.0) & 0xfffffffffffffull;
     return (uint32_t)__double2hiint(z) < 0xc0470000u ? v : 0ull;     // z > -46
   }
+  // Neither -2^128, which of_near takes for -infinity, nor 2^128 below the top, where the difference of two floats ends, weighs
+  // anything (2^-64 of the top at most).  Not so at flat temperatures (above 7.6 10^36; a top near -2^128: above 4 10^29).
+  __device__ bool steep() const { return (340282366920938463463374607431768211456.0 + fmin((double)top, 0.0)) * c >= 64.; }
   // mode 0 (of 0 and subnormal numbers 10^-38 off; a NaN gives anything)
   __device__ __forceinline__ unsigned long long of_near(float l, const double* table) const {
     const uint32_t b = __float_as_uint(l);
