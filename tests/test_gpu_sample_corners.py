@@ -3,6 +3,7 @@ Tokens and counts are exact (the inputs keep sums 10^-9 of the total away from b
 probabilities have run_sample's bound."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -77,3 +78,26 @@ def test_lowest_scores_lead(lib, cuda, temperature, t):
     x = x.to(TYPES[t][0]).cuda()
     for kw in (dict(top_p=[0.9] * 4), dict(top_p=[0.31] * 4, top_k=[0, 70, 0, 55]), dict(top_k=[90, 89, 1, 60])):
         everywhere(lib, x, t, temperature=[temperature] * 4, u=[0.93, 0.41, 0.0731, 0.62], **kw)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_infinite_scores_beside_every_nan(lib, cuda, t):
+    """The NaN next to infinity in the order of codes (and all others) are scores of no weight, also where infinity leads."""
+    inf = {"f16": 0x7c00, "bf16": 0x7f80}[t]
+    nans = np.concatenate([inf + np.arange(1, 12), 0x8000 + inf + np.arange(1, 12), [0x7fff, 0xffff, inf + 0x40]]).astype(np.uint16)
+    rows = []
+    for lead in ([inf] * 3, [inf], [0x3c00, 0x3c00, 0x2000], [0x8000 + inf - 1] * 2):
+        row = np.zeros(100, np.uint16)
+        row[:nans.size] = nans
+        row[nans.size:] = 0x8000 + inf                      # -infinity
+        row[60:60 + len(lead)] = lead
+        row[2:5], row[80:83] = row[80:83].copy(), row[2:5].copy()
+        rows.append(row)
+    x = torch.from_numpy(np.stack(rows).view(np.int16)).view(TYPES[t][0]).cuda()
+    m = len(rows)
+    for u in (0.0, 0.4, 0.9):
+        for k in (1, 2, 3, 5, 99):
+            everywhere(lib, x, t, u=[u] * m, top_k=[k] * m)
+            everywhere(lib, x, t, splits=(1, 8), u=[u] * m, top_k=[k] * m, top_p=[0.55] * m)
+        everywhere(lib, x, t, splits=(1, 8), u=[u] * m, top_p=[0.3] * m)
+        everywhere(lib, x, t, splits=(1, 8), u=[u] * m, min_p=[0.5] * m)

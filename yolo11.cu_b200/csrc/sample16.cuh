@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
       uint32_t count = 0, some = 0;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        if (place + e >= end) c[e] = 0;
+        if (place + e < top_place || place + e >= end) c[e] = 0;   // (NaN are before infinity)
         count += c[e];
         some |= (c[e] != 0) << e;
       }
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kSamp16Threads, 1) sample16_kernel(const __gri
       u64 one = 0, n = 0, m = 0, n_to = 0, m_to = 0;   // of a score there, of all of them, with those before
       if (tid < kStep) {
         uint32_t c = 0;
-        if (place < end) {
+        if (place >= top_place && place < end) {
           const uint32_t l = smem_u32(counts) + (place >> 1) * 4;
 #pragma unroll 4
           for (int q = 0; q < split; q++) c += ld_cluster_u32(split > 1 ? cluster_map(l, q) : l) >> (place & 1) * 16 & 0xffffu;
