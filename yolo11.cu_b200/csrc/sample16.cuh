@@ -17,7 +17,9 @@ namespace yk {
 // by bins, with an exact weight for each score, 62), of which the counts take 5, the sums by step 6, a border 3, the pass
 // through the token's CTA 7; the rest are some ten waits of the whole cluster or CTA for one another.  47 us if a row keeps
 // scores of both signs; 35 without limits.
-constexpr int kSamp16Slice = 64000;             // scores of a CTA at most: a count stays below 2^16
+// Scores of a CTA at most: a count stays below 2^16, also where the start of the row moves a CTA's part by 256.  (64 rows of 128256 or
+// 130048: 32 us by two CTAs each, which fill the SMs; 50 by four, two rounds, as from 130049 on.)
+constexpr int kSamp16Slice = 65024;
 constexpr int kSamp16Threads = 1024;
 constexpr int kSamp16Table = 11264;            // places that stay, and one for all others
 constexpr int kSamp16Smem = 65536 * 2 + kSamp16Table * 8;
