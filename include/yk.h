@@ -336,8 +336,8 @@ int yk_gemv4(const YkGemv4* p, yk_stream_t st);
 // the angle pos[axis of i][n] * freqs[i]: (a, b) -> (a cos - b sin, b cos + a sin), rounded once to dtype.
 // The pair is channels (i, i + rot/2), or (2i, 2i + 1) if interleaved; channels from rot on do not turn.
 // The first sections[0] pairs follow axis 0, the next sections[1] axis 1, and so on (time, row, column of
-// an image's tokens).  Whole turns are taken off in 64 bits, so far positions lose nothing.  Rows whose pos on
-// axis 0 is negative are left as they are.  Outputs may be the inputs themselves.
+// an image's tokens).  Whole turns are taken off in whole numbers: an angle is within 2^-31 of a turn at any position, with
+// frequencies up to 2^40.  Rows whose pos on axis 0 is negative are left as they are.  Outputs may be the inputs themselves.
 typedef struct {
   const void* q;           // head h of row n at n*q_row + h*dim; fp16 or bf16, 16-byte aligned
   const void* k;           // likewise with k_row; NULL with kv_heads 0

@@ -22,8 +22,9 @@ struct RotateArgs {
 // The work is cut into steps of kRotV heads a lane.  Warps stay and take equal runs of steps, from any head of
 // any row on, as a grid of whole rows leaves its last wave half empty (54 us); the next steps are loaded into shared
 // memory meanwhile, kRotStages - 1 ahead.  A call of few steps has a warp for each (64 rows of the same: 3.7 us).
-// Angles: the turns of a position are held modulo one in units of 2^-64, so a product with a position of 31 bits keeps
-// 2^-33 of a turn and needs no 64-bit floats for each row.  A cosine is rounded to 32 bits, and w c again.
+// Angles: the turns of a position are held modulo one in units of 2^-64, good to the last of them for frequencies up to 2^40 (1 / 2 pi
+// comes in two doubles), so an angle is within 2^-31 of a turn at any position of 31 bits and needs no 64-bit floats for each
+// row.  A cosine is rounded to 32 bits, and w c again.
 constexpr int kRotWarps = 4, kRotBlocks = 5;    // of a CTA; CTAs an SM
 constexpr int kRotV = 2, kRotStages = 3;
 constexpr int kRotStage = kRotV * 1024 + 256;   // a step's data, and the positions of a warp's rows: [4][16]
@@ -38,7 +39,7 @@ __device__ __forceinline__ float2 rot_mul(float2 a, float2 b) {
 template <bool BF16, int L, bool INTER>
 __global__ void __launch_bounds__(kRotWarps * 32, kRotBlocks) rotate_kernel(const __grid_constant__ RotateArgs a) {
   extern __shared__ __align__(16) uint8_t rot_smem[];
-  __shared__ long long freq[128];                    // of each pair: turns a position, in units of 2^-64, less whole turns
+  __shared__ unsigned long long freq[128];           // of each pair: turns a position, in units of 2^-64, less whole turns
   __shared__ __align__(16) float weights[2][L * 16];
   const YkQkRotate& p = a.p;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -89,9 +90,10 @@ __global__ void __launch_bounds__(kRotWarps * 32, kRotBlocks) rotate_kernel(cons
 #pragma unroll 1
   for (int i = 0; i < kRotStages - 1; i++) issue();
   for (int i = threadIdx.x; i < half; i += kRotWarps * 32) {
-    double d = (double)p.freqs[i] * 0.15915494309189533577;   // 1 / 2 pi
-    d -= rint(d);
-    freq[i] = __double2ll_rn(d * 18446744073709551616.);
+    // 1 / 2 pi in two doubles: the product's rounding error and the second one's share are a part of their own, far below a turn
+    const double f = p.freqs[i], h = f * 0.15915494309189533577, e = fma(f, 0.15915494309189533577, -h) + f * -9.839338337591243e-18;
+    freq[i] = (unsigned long long)__double2ll_rn((h - rint(h)) * 18446744073709551616.) +
+              (unsigned long long)__double2ll_rn(e * 18446744073709551616.);
   }
   for (int i = threadIdx.x; i < 2 * L * 16; i += kRotWarps * 32) {
     const uint16_t* weight = (const uint16_t*)(i < L * 16 ? p.q_weight : p.k_weight);
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(kRotWarps * 32, kRotBlocks) rotate_kernel(cons
       for (int i = lane; i < rows * half; i += 32) {
         const int tr = i / half, pair = i - tr * half;
         const int axis = (pair >= a.after[0]) + (pair >= a.after[1]) + (pair >= a.after[2]);
-        const int t = (int)(((unsigned long long)freq[pair] * (unsigned long long)pos[axis * 16 + tr]) >> 32);
+        const int t = (int)((freq[pair] * (unsigned long long)pos[axis * 16 + tr]) >> 32);
         float s, c;
         sincospif((float)t * 4.656612873e-10f, &s, &c);   // 2^-31
         turn[i] = make_float2(c, s);
