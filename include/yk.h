@@ -341,7 +341,7 @@ int yk_gemv4(const YkGemv4* p, yk_stream_t st);
 typedef struct {
   const void* q;           // head h of row n at n*q_row + h*dim; fp16 or bf16, 16-byte aligned
   const void* k;           // likewise with k_row; NULL with kv_heads 0
-  void* q_out;             // likewise with q_out_row; q itself, or apart from it
+  void* q_out;             // likewise with q_out_row; q itself with its stride, or apart from it
   void* k_out;
   const void* q_weight;    // [dim] of dtype, or NULL: no norm
   const void* k_weight;

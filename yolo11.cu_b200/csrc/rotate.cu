@@ -283,6 +283,8 @@ extern "C" int yk_qk_rotate(const YkQkRotate* p, yk_stream_t st) {
   if ((p->q_row | p->q_out_row) % 8 || p->q_row < qw || p->q_out_row < qw || (p->axes > 1 && p->pos_axis < p->rows) ||
       (kw && ((p->k_row | p->k_out_row) % 8 || p->k_row < kw || p->k_out_row < kw)))
     return refuse(YK_EINVAL, "qk_rotate: row strides are multiples of 8 that hold a row, pos_axis at least rows");
+  if (p->rows > 1 && ((p->q_out == p->q && p->q_out_row != p->q_row) || (kw && p->k_out == p->k && p->k_out_row != p->k_row)))
+    return refuse(YK_EINVAL, "qk_rotate: rows in place have one stride");
   if (!aligned16(p->q) || !aligned16(p->q_out) || !aligned16(p->q_weight) || !aligned16(p->k_weight) ||
       (kw && (!aligned16(p->k) || !aligned16(p->k_out))))
     return refuse(YK_EINVAL, "qk_rotate: q, k, outputs and weights need 16-byte alignment");
