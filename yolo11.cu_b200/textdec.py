@@ -301,14 +301,16 @@ class TextDecoder:
             return
         want = dict(temperature=(temperature, torch.float32), top_k=(top_k, torch.int32), top_p=(top_p, torch.float32),
                     min_p=(min_p, torch.float32))
-        if not hasattr(self, "_settings"):
-            self._settings = {k: torch.zeros(self.requests, dtype=t, device=self.device) for k, (_, t) in want.items()}
-            self.gen = torch.Generator(device=self.device)
         for k, (v, t) in want.items():
             v = torch.as_tensor(v, dtype=t)
             if v.dim() and v.shape != (self.requests,):
                 raise ValueError(f"{k}: one value, or one for each of {self.requests} requests")
-            self._settings[k].copy_(v.expand(self.requests))
+            want[k] = v.expand(self.requests)
+        if not hasattr(self, "_settings"):
+            self._settings = {k: torch.zeros(self.requests, dtype=v.dtype, device=self.device) for k, v in want.items()}
+            self.gen = torch.Generator(device=self.device)
+        for k, v in want.items():
+            self._settings[k].copy_(v)
         self.sampling = self._settings
         self.gen.manual_seed(seed)
 
