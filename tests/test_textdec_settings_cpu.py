@@ -27,3 +27,16 @@ def test_refused_settings_change_nothing(dec):
     with pytest.raises(ValueError):
         dec.set_sampling([1.0, 2.0])
     assert dec.sampling is None
+
+
+def test_the_captured_step_can_be_let_go(dec):
+    dec.graphs = {False: "greedy", True: "drawn"}
+    assert dec.graph == "greedy"
+    dec.set_sampling(1.0)
+    assert dec.graph == "drawn"
+    dec.graph = None                                 # what was captured is out of date, in both ways
+    assert dec.graph is None and dec.graphs == {}
+    dec.set_sampling(None)
+    assert dec.graph is None
+    dec.graph = "another"
+    assert dec.graphs == {False: "another"}

@@ -141,6 +141,14 @@ class TextDecoder:
         """The captured step of the present way to choose tokens, if there is one."""
         return self.graphs.get(self.sampling is not None)
 
+    @graph.setter
+    def graph(self, captured):
+        """None lets go of what was captured, in every way to choose tokens: the next step is captured anew."""
+        if captured is None:
+            self.graphs.clear()
+        else:
+            self.graphs[self.sampling is not None] = captured
+
     def _weight(self, w):
         """A weight matrix in the decoder's format."""
         if self.fp4 is None:
@@ -377,7 +385,7 @@ class TextDecoder:
     def decode(self, steps: int, graph: bool = True):
         """`steps` tokens for every request, the best ones or as set_sampling says; [steps, requests].  Where the plan
         refuses a request a step (no free block, or its table is full) it gives -1, and its token waits for the next step.
-        The first call (of each way to choose tokens) captures the step."""
+        The first call (of each way to choose tokens), and the first after `graph` was set to None, captures the step."""
         out = torch.empty(steps, self.requests, dtype=torch.long, device=self.device)
         self.fresh.fill_(1)
         for i in range(steps):
