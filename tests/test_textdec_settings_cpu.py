@@ -10,6 +10,7 @@ def dec(pkg):
     from yolo11_cu_b200 import textdec
     d = textdec.TextDecoder.__new__(textdec.TextDecoder)
     d.requests, d.device, d.sampling, d.gen, d.graphs = 3, "cpu", None, None, {}
+    d.unscored = torch.zeros(3, dtype=torch.bool)
     d.lens, d.shift = torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
     return d
 

@@ -133,6 +133,7 @@ class TextDecoder:
             self.at, self.shift = torch.full((3, n), -1, dtype=i32, device=device), new(requests, dtype=i32)
         # sampling: None (the best token), or the requests' settings; `u` is drawn before each step
         self.sampling, self.gen = None, None
+        self.unscored = new(requests, dtype=torch.bool)       # requests that had no score to draw from in the last step
         self.u, self.picked, self.logprob = new(requests, dtype=torch.float32), new(requests, dtype=i32), new(requests, dtype=torch.float32)
         self.graphs = {}
 
@@ -211,7 +212,10 @@ class TextDecoder:
                         top_p=s["top_p"].data_ptr(), min_p=s["min_p"].data_ptr(), u=self.u.data_ptr(), token=self.picked.data_ptr(),
                         logprob=self.logprob.data_ptr(), row=self.vocab, rows=self.requests, n=self.vocab, dtype=rt.YK_F16)
         self._ok(self.lib.yk_sample(C.byref(a), self._stream))
-        return self.picked.long()
+        # a row without any weight (all NaN or -infinity) gives -1, which is no row of the embedding: the token stays
+        none = self.picked < 0
+        torch.logical_and(none, self.placed, out=self.unscored)
+        return torch.where(none, self.next, self.picked)
 
     def _matmul(self, x, w, y, n, scales=None):
         """y = x w^T; 64 rows a call.  scales: x is e4m3 codes."""
@@ -306,6 +310,7 @@ class TextDecoder:
         settings are written where a captured step reads them."""
         if temperature is None:
             self.sampling = None
+            self.unscored.zero_()
             return
         want = dict(temperature=(temperature, torch.float32), top_k=(top_k, torch.int32), top_p=(top_p, torch.float32),
                     min_p=(min_p, torch.float32))
@@ -385,6 +390,8 @@ class TextDecoder:
     def decode(self, steps: int, graph: bool = True):
         """`steps` tokens for every request, the best ones or as set_sampling says; [steps, requests].  Where the plan
         refuses a request a step (no free block, or its table is full) it gives -1, and its token waits for the next step.
+        A request whose scores leave nothing to draw (all NaN or -infinity) keeps its token, which goes in again, and is true in
+        `unscored` until a step draws one for it.
         The first call (of each way to choose tokens), and the first after `graph` was set to None, captures the step."""
         out = torch.empty(steps, self.requests, dtype=torch.long, device=self.device)
         self.fresh.fill_(1)
