@@ -1,10 +1,18 @@
-"""TextDecoder at its ends: a new capture on request, scores without a choice."""
+"""TextDecoder at its ends: scores without a choice, a new capture on request, 4-bit rows of every size, 4-bit weights beside the
+16-bit ones.
+
+Bounds.  A scale of e4m3 is within 2^-4 of a group's largest value over 6, so it is at most 17/96 of that value, and a code is off by
+at most one unit of it (between 4 and 6; what exceeds 6 exceeds it by 0.4).  A power-of-two scale is at most twice a sixth: 1/3.  The
+16-bit weights are 2^-11 off the seed's."""
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_textdec_modes import make, rows_of
+import decode_ref as ref
+from test_gpu_textdec_modes import f64, make, matrix, rows_of
 
 pytestmark = pytest.mark.gpu
+UNIT = {"nvfp4": 17 / 96, "mxfp4": 1 / 3}
 
 
 def test_a_new_capture_on_request(lib, cuda, pkg):
@@ -47,3 +55,37 @@ def test_scores_without_a_choice(lib, cuda, pkg, weights, graph):
         assert a[1] == mine                          # it went in (-1 would say that the plan refused it)
         assert a[4:] == [False, True, False, False] and b[4:] == [False] * 4
     assert int(dec.next[1]) == mine and dec.placed.all()
+
+
+@pytest.mark.parametrize("weights", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("size", [2.0 ** -6, 0.1, 1.0, 16.0])
+def test_rows_of_every_size_in_four_bits(lib, cuda, pkg, weights, size):
+    """Attention over a long cache is small, a norm's rows are about one, a gate's product may be large."""
+    dec = make(pkg, weights=weights)
+    for cols, m in dec.x4.items():
+        x = (torch.randn(40, cols, generator=torch.Generator().manual_seed(cols)).cuda() * size).half()
+        dec._ok(m.fill(dec.lib, x, 40))
+        v = f64(x)
+        g = ref.GROUP[dec.fp4]
+        largest = np.repeat(np.abs(v).reshape(40, -1, g).max(-1), g, 1)
+        assert largest.min() >= 6 * 2.0 ** -6 * m.scale or weights == "mxfp4", "below the scale's normal range"
+        assert (np.abs(matrix(m)[:40] - v) <= UNIT[weights] * largest).all()
+
+
+@pytest.mark.parametrize("weights", ["nvfp4", "mxfp4"])
+def test_weights_are_the_seeds_in_four_bits(lib, cuda, pkg, weights):
+    dec = make(pkg, weights=weights)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    wide = (dec.heads + 2 * dec.kv_heads) * dec.dim
+    sizes = dict(qkv=(wide, dec.width), out=(dec.width, dec.heads * dec.dim), up=(dec.hidden, dec.width),
+                 down=(dec.width, dec.hidden), gate=(dec.hidden, dec.width))
+    seen = [(w[k], torch.randn(*s, generator=g, device="cuda") * s[1] ** -0.5) for w in dec.w for k, s in sizes.items()]
+    for _ in dec.norms:                              # (drawn whole for each of them)
+        torch.randn(2 * dec.layers + 1, dec.width, generator=g, device="cuda")
+    seen.append((dec.head, torch.randn(dec.vocab, dec.width, generator=g, device="cuda") * dec.width ** -0.5))
+    for m, w in seen:
+        v = f64(w)
+        n = ref.GROUP[dec.fp4]
+        largest = np.repeat(np.abs(v).reshape(m.rows, -1, n).max(-1), n, 1)
+        # (the group's largest is rounded to 16 bits, too)
+        assert (np.abs(matrix(m) - v) <= (UNIT[weights] + 2.0 ** -10) * largest + 2.0 ** -25).all()

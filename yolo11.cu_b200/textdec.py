@@ -123,7 +123,11 @@ class TextDecoder:
         self.ws = new(size, dtype=torch.uint8)
         if self.fp4 is not None:
             self.x16, self.last16 = new(n, width), new(requests, width)
-            self.x4 = {c: Fp4(self.lib, n, c, self.fp4, device) for c in {width, heads * dim, hidden}}
+            # e4m3 scales keep their three bits from 2^-6 to 448, so that groups of rows do whose largest value lies between 6 / 64
+            # and 2688 of the whole matrix's scale: 0.003 to 84 with 2^-5.  A norm's rows are about one (at most the square root of
+            # their width), an average over a long cache is small.  Powers of two have the whole range.
+            scale = 2.0 ** -5 if self.fp4 == rt.YK_NVFP4 else 1.0
+            self.x4 = {c: Fp4(self.lib, n, c, self.fp4, device, scale) for c in {width, heads * dim, hidden}}
         if rotary:
             self.head_norms = [(1 + 0.1 * rand(2, dim)).half() for _ in range(layers)]       # of queries, of keys
             pairs = torch.arange(dim // 2, dtype=torch.float64)
