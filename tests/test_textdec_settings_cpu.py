@@ -41,3 +41,32 @@ def test_the_captured_step_can_be_let_go(dec):
     assert dec.graph is None
     dec.graph = "another"
     assert dec.graphs == {False: "another"}
+
+
+def behind(dec, places, lens):
+    counts = torch.tensor(lens)
+    owner = torch.repeat_interleave(torch.arange(3), counts)
+    return dec._behind(torch.tensor(places, dtype=torch.int32).reshape(3, -1), owner, counts, sum(lens)).tolist(), dec._shift.tolist()
+
+
+def test_places_behind_an_image(dec):
+    """Text follows the image rows before it in the call by one place; where there are none, its token's number and its request's
+    shift.  Image rows lie where the caller puts them."""
+    dec.lens.copy_(torch.tensor([0, 5, 9]))
+    dec.shift.copy_(torch.tensor([0, 0, -4]))
+    t, r, c = [-1, 2, 2, -1, -1, -1], [-1, 2, 3, -1, -1, -1], [-1, 2, 6, -1, -1, -1]
+    got, shift = behind(dec, [t, r, c], [5, 0, 1])
+    assert got == [[0, 2, 2, 7, 8, 5], [0, 2, 3, 7, 8, 5], [0, 2, 6, 7, 8, 5]]
+    assert shift == [7 - 3, 0, -4]                   # the next token, number 5, lies at 9
+    # an image that the caller puts before earlier places: text follows that image
+    got, shift = behind(dec, [[-1, 0, 1, -1], [-1, 0, 0, -1], [-1, 1, 0, -1]], [0, 4, 0])
+    assert got[0] == [5, 0, 1, 2] and shift == [0, 2 - 8, -4]
+    # two images in one call: the larger places count
+    got, shift = behind(dec, [[10, 3, -1]] * 3, [0, 0, 3])
+    assert got[0] == [10, 3, 11] and shift == [0, 0, 11 - 11]
+
+
+def test_places_of_no_rows(dec):
+    dec.shift.copy_(torch.tensor([1, 2, 3]))
+    got, shift = behind(dec, [], [0, 0, 0])
+    assert got == [[], [], []] and shift == [1, 2, 3]

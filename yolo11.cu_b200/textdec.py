@@ -124,7 +124,8 @@ class TextDecoder:
         if self.fp4 is not None:
             self.x16, self.last16 = new(n, width), new(requests, width)
             # e4m3 scales keep their three bits from 2^-6 to 448, so that groups of rows do whose largest value lies between 6 / 64
-            # and 2688 of the whole matrix's scale: 0.003 to 84 with 2^-5.  A norm's rows are about one (at most the square root of
+            # and 2688 of the whole matrix's scale: 0.003 to 84 with 2^-5 (rows of deviation 1/64: a value
+            # is off by up to 0.17 of its group's largest one; 0.33 with 1).  A norm's rows are about one (at most the square root of
             # their width), an average over a long cache is small.  Powers of two have the whole range.
             scale = 2.0 ** -5 if self.fp4 == rt.YK_NVFP4 else 1.0
             self.x4 = {c: Fp4(self.lib, n, c, self.fp4, device, scale) for c in {width, heads * dim, hidden}}
@@ -335,8 +336,10 @@ class TextDecoder:
         """rows [sum(lens), width]: each request's new rows one after another (embeddings of prompt
         tokens, image tokens); lens[r] may be 0.  Fills the cache and picks the next token of each request
         whose rows went in (`placed`); the others, without rows or refused, keep theirs.
-        places [3][sum(lens)] (rotary): time, row and column of each row, or -1 for rows that follow their request's
-        last place, as text does; later tokens go on behind the largest place that a request was given here."""
+        places [3][sum(lens)] (rotary): time, row and column of each row, which lies there whatever came before it, or -1 for
+        rows of text.  Text behind such rows, and every later token, goes on from one place behind the largest place given
+        in this call before it; without any it goes on as before.  So an image given places below those that its request has
+        had takes the text behind it back there, too: the next token of request r lies at lens[r] + shift[r]."""
         n = sum(lens)
         if n > self.rows or n != rows.shape[0] or len(lens) != self.requests:
             raise ValueError(f"{n} rows in {len(lens)} requests, {rows.shape[0]} given: at most {self.rows} "
@@ -365,11 +368,11 @@ class TextDecoder:
         return self.next
 
     def _behind(self, places, owner, counts, n):
-        """places with text rows (-1) put behind the largest place before them in their request; the requests' shifts after it
-        go to self._shift."""
+        """places with rows of text (-1) put behind the largest place given before them in their request's rows here (text rows
+        themselves do not count), or by their request's shift; the requests' shifts after it go to self._shift."""
         start = self.lens.long()[owner] + torch.arange(n, device=self.device) - (counts.cumsum(0) - counts)[owner]   # token numbers
         text = places[0] < 0
-        # a text row lies at its token's number + shift; the shift is that of the image rows before it: one behind their
+        # a row of text lies at its token's number + shift; the shift is that of the image rows before it: one behind their
         # largest place, less the number of the token that follows the last of them
         big = torch.where(text, torch.full_like(places[0], -1), places.amax(0)).long()
         key = owner * (1 << 32)
