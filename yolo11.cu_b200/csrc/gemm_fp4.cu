@@ -598,12 +598,6 @@ static bool encode_fp4(CUtensorMap* m, const void* base, int rows, int k, long l
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static int fp4_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
-}
-
 template <bool NV, bool GATED, bool BF16>
 static int launch_fp4_pair(const GemmFp4Args& a, cudaStream_t st) {
   using S = Fp4Pair<NV>;
@@ -614,7 +608,7 @@ static int launch_fp4_pair(const GemmFp4Args& a, cudaStream_t st) {
       !encode_fp4(&tw2, GATED ? p.w2 : p.w, p.n, p.k, p.w_row, GATED ? 64 : 128))
     return refuse(YK_EUNSUP, "gemm_fp4: no tensor map for these sizes");
   if (smem_attr(kern, S::kSmem) != cudaSuccess) return check_launch("gemm_fp4 attr");
-  const int tiles = a.tiles_m * a.tiles_n, pairs = fp4_sms() / 2;
+  const int tiles = a.tiles_m * a.tiles_n, pairs = sm_count() / 2;
   launch_kc(kern, 2 * (tiles < pairs ? tiles : pairs), kFp4PairThreads, S::kSmem, 2, st, a, tx, tw, tw2);
   note_launch();
   return check_launch("gemm_fp4");
@@ -641,7 +635,7 @@ static int g_fp4_kernel = 0, g_fp4_split = 0;
 template <bool NV, bool GATED>
 static int launch_fp4(GemmFp4Args& a, cudaStream_t st) {
   const YkGemmFp4& p = a.p;
-  const int sms = fp4_sms();
+  const int sms = sm_count();
   a.tiles_m = (p.rows + 255) / 256;
   a.tiles_n = (p.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
   const long long tiles = (long long)a.tiles_m * a.tiles_n;

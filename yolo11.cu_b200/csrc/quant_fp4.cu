@@ -30,12 +30,6 @@ struct QuantFp4Args {
 // 16 x 4096: 2.8 us, the launch.
 constexpr int kQuantCols = 256, kQuantThreads = 256;
 
-__device__ __forceinline__ float2 quant_mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
 // Eight 16-bit elements (two where there are fewer columns) at any even address, as pairs.
 __device__ __forceinline__ uint4 quant_load8(const uint16_t* x, int align, int cols, bool first) {
   uint4 v = make_uint4(0, 0, 0, 0);
@@ -184,7 +178,7 @@ __global__ void __launch_bounds__(kQuantThreads, 5) quant_fp4_kernel(const __gri
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const float2 v = pair_to_float2<BF16>(u[e]);
-          float2 d = quant_mul2(v, r2);
+          float2 d = fmul2(v, r2);
           if (NV || !a.exact) d = ffma2(ffma2(d, s2, v), r2, d);
           q[2 * e] = d.x;
           q[2 * e + 1] = d.y;
@@ -204,7 +198,7 @@ __global__ void __launch_bounds__(kQuantThreads, 5) quant_fp4_kernel(const __gri
         const float f = nan ? __uint_as_float(0x7fc00000u) : S;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float2 w = quant_mul2(__half22float2(*(const __half2*)&h[e]), make_float2(f, f));
+          const float2 w = fmul2(__half22float2(*(const __half2*)&h[e]), make_float2(f, f));
           o[e] = float2_to_pair<BF16>(w.x, w.y);
         }
         quant_store8((uint16_t*)p.values + (long long)(row0 + r) * p.values_row + c, a.v_align, cols, o);

@@ -29,13 +29,6 @@ constexpr int kRotWarps = 4, kRotBlocks = 5;    // of a CTA; CTAs an SM
 constexpr int kRotV = 2, kRotStages = 3;
 constexpr int kRotStage = kRotV * 1024 + 256;   // a step's data, and the positions of a warp's rows: [4][16]
 
-__device__ __forceinline__ float2 rot_mul(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-
 template <bool BF16, int L, bool INTER>
 __global__ void __launch_bounds__(kRotWarps * 32, kRotBlocks) rotate_kernel(const __grid_constant__ RotateArgs a) {
   extern __shared__ __align__(16) uint8_t rot_smem[];
@@ -146,10 +139,10 @@ __global__ void __launch_bounds__(kRotWarps * 32, kRotBlocks) rotate_kernel(cons
           } else {
             const float4 u = *(const float4*)(t + l * 8 + 2 * e);
             const float2 c = make_float2(u.x, u.z), s = make_float2(u.y, u.w), w0 = A[0][e], w1 = A[1][e];
-            A[0][e] = rot_mul(w0, c);
-            A[1][e] = rot_mul(w1, c);
-            B[0][e] = rot_mul(w1, make_float2(-s.x, -s.y));
-            B[1][e] = rot_mul(w0, s);
+            A[0][e] = fmul2(w0, c);
+            A[1][e] = fmul2(w1, c);
+            B[0][e] = fmul2(w1, make_float2(-s.x, -s.y));
+            B[1][e] = fmul2(w0, s);
           }
         }
       }
@@ -180,12 +173,12 @@ __global__ void __launch_bounds__(kRotWarps * 32, kRotBlocks) rotate_kernel(cons
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) y[c][e] = rot_mul(y[c][e], make_float2(inv, inv));
+          for (int e = 0; e < 4; e++) y[c][e] = fmul2(y[c][e], make_float2(inv, inv));
       }
 #pragma unroll
       for (int c = 0; c < 2; c++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) z[c][e] = rot_mul(y[c][e], A[c][e]);
+        for (int e = 0; e < 4; e++) z[c][e] = fmul2(y[c][e], A[c][e]);
       if (turns) {
 #pragma unroll
         for (int c = 0; c < 2; c++)
@@ -209,12 +202,6 @@ __global__ void __launch_bounds__(kRotWarps * 32, kRotBlocks) rotate_kernel(cons
   }
 }
 
-static int rotate_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
-}
-
 template <bool BF16, int L, bool INTER>
 static int launch_rotate(const RotateArgs& in, cudaStream_t st) {
   RotateArgs a = in;
@@ -232,7 +219,7 @@ static int launch_rotate(const RotateArgs& in, cudaStream_t st) {
   a.warp_bytes = kRotStages * kRotStage + (rows * p.rot * 4 + 15) / 16 * 16;
   const int bytes = kRotWarps * a.warp_bytes;
   const int fit = (227 << 10) / (bytes + 2048 + L * 128), blocks = fit < kRotBlocks ? fit : kRotBlocks;
-  const long long want = (all + kRotWarps - 1) / kRotWarps, most = (long long)blocks * rotate_sms();
+  const long long want = (all + kRotWarps - 1) / kRotWarps, most = (long long)blocks * sm_count();
   const unsigned grid = (unsigned)(want < most ? want : most);
   a.each = all / (grid * kRotWarps);
   a.more = (int)(all % (grid * kRotWarps));

@@ -798,8 +798,7 @@ template <int DT>
 static int launch_sample(SampleArgs& a, cudaStream_t st) {
   const YkSample& p = a.p;
   constexpr int kVec = 16 / (DT == YK_F32 ? 4 : 2);
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = sm_count();
   // CTAs of a row: as many as the SMs have room for, each with scores for two a thread or more; and what one can hold.
   const auto split_for = [&](int most, bool whole) {
     int split = 1;

@@ -15,6 +15,12 @@ static int refuse(int code, const char* what) {
   snprintf(g_cuda_err, sizeof g_cuda_err, "%s", what);
   return code;
 }
+// SMs of the current device.
+static int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
+}
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Two e4m3 codes (low and high byte) as a half2; exact.
@@ -78,6 +84,13 @@ __device__ __forceinline__ float finite_abs(float v) {
 __device__ __forceinline__ float rcp_fast(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Both products, rounded each; the sign of a zero stays (mul2 adds 0 to it).
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return ffma2(a, b, make_float2(0.f, 0.f)); }
