@@ -15,7 +15,7 @@ namespace yk {
 //    alike (infinity), the borders are found digit by digit of the key instead: sums by digit of the keys that share the
 //    digits so far, two or three turns a border.
 // A chain of some twelve stages of 1 to 4 us, each the wait of a cluster for its slowest CTA: 1 x 32000 15 us; 200 x 151000
-// of fp32 183 us, 5.4 rounds of two CTAs an SM (12 % of the copy rate; issue slots 55 % busy).
+// of fp32 185 us, 5.4 rounds of two CTAs an SM (12 % of the copy rate; issue slots 55 % busy).
 constexpr int kSampSlice = 32768;          // scores of a CTA at most
 constexpr int kSampBins = 46 * 64;         // weights below 2^-46 count nothing
 constexpr int kSampDigits = 2048;
